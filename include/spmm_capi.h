@@ -359,6 +359,56 @@ int spmm_c_hybrid_run(const spmm_hybrid_plan_t* plan, const spmm_csr_t* h_A,
                       const float* h_B, float* h_C, int N, int warmup, int iters,
                       float* ms_out);                            /* spmm_hybrid.h:62 */
 
+/* ---- mixture-of-experts routing (no reference counterpart) -------------
+ * The routing matrix of `tokens` x `experts` with k entries a row: entry
+ * i = t * k + j is token t's choice j.  In expert order the entries are sorted
+ * by expert, those of one expert in the order of the entries; slot s of that
+ * order is row s of the expert-ordered operands (tokens * k rows).
+ *   d_experts [tokens, k]  the chosen experts, -1 for none
+ *   d_weights [tokens, k]  fp32, 0 for none
+ *   d_offsets [experts+1]  first slot of each expert; d_offsets[experts] slots are taken
+ *   d_entries [tokens*k]   the entry in each slot, -1 behind the last taken one
+ *   d_slots   [tokens, k]  the slot of each entry, -1 for none
+ * `type`: SPMM_F32, SPMM_F16 or SPMM_BF16, of every void* operand of a call.
+ * All operands are contiguous device arrays, aligned for their elements; sums
+ * are fp32 and rounded once; every launch is deterministic.
+ * route: d_logits [tokens, experts].  The k largest, ties to the lowest expert;
+ *   -inf is never chosen (a token of only -inf has no expert), NaN is above all
+ *   numbers and makes the token's weights NaN.  over: the softmax over the
+ *   chosen experts, or over all.  d_workspace: spmm_c_route_workspace bytes.
+ *   experts <= 1024, k <= 64, k <= experts (SPMM_UNSUPPORTED, SPMM_INVALID).
+ * route_backward: d_dlogits of the logits' type; d_logits is read for
+ *   SPMM_OVER_ALL only.
+ * group_entries: the order alone, for ids of the caller's own (any id outside
+ *   [0, groups) has no slot); spmm_c_group_workspace bytes.
+ * dispatch: d_x [tokens, features] -> d_xs [tokens*k, features] in expert
+ *   order, rows without an entry zero.
+ * combine: d_y[t] = sum over j of d_weights[t,j] * d_ys[slot of (t,j)];
+ *   d_weights null: unweighted, the gradient of dispatch.
+ * combine_backward: d_dys [tokens*k, features] (rows without an entry zero) and
+ *   d_dweights [tokens, k] fp32. */
+enum { SPMM_F32 = 0, SPMM_F16 = 1, SPMM_BF16 = 2 };
+enum { SPMM_OVER_CHOSEN = 0, SPMM_OVER_ALL = 1 };
+long long spmm_c_route_workspace(int tokens, int experts, int k);
+long long spmm_c_group_workspace(int entries, int groups);
+int spmm_c_route(const void* d_logits, int type, int tokens, int experts, int k, int over,
+                 int* d_experts, float* d_weights, int* d_offsets, int* d_entries, int* d_slots,
+                 void* d_workspace, void* stream);
+int spmm_c_route_backward(const void* d_logits, int type, int tokens, int experts, int k,
+                          int over, const int* d_experts, const float* d_weights,
+                          const float* d_dweights, void* d_dlogits, void* stream);
+int spmm_c_group_entries(const int* d_ids, int entries, int groups, int* d_offsets,
+                         int* d_entries, int* d_slots, void* d_workspace, void* stream);
+int spmm_c_dispatch(const void* d_x, int type, int tokens, int k, int features,
+                    const int* d_slots, const int* d_offsets, int experts, void* d_xs,
+                    void* stream);
+int spmm_c_combine(const void* d_ys, int type, int tokens, int k, int features,
+                   const int* d_slots, const float* d_weights, void* d_y, void* stream);
+int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int tokens, int k,
+                            int features, const int* d_slots, const float* d_weights,
+                            const int* d_offsets, int experts, void* d_dys, float* d_dweights,
+                            void* stream);
+
 /* ---- measurement helpers (no reference counterpart) -------------------
  * Launch one entry point `reps` times back to back on `stream` without
  * synchronising, so a caller's events can bracket a batch.  kernel ids:

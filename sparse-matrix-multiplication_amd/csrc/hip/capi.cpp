@@ -122,6 +122,12 @@ int guarded(F f) {
     }
 }
 
+bool element_type(int type, spmm::engine::ElementType* out) {
+    if (type != SPMM_F32 && type != SPMM_F16 && type != SPMM_BF16) return false;
+    *out = static_cast<spmm::engine::ElementType>(type);
+    return true;
+}
+
 spmm::engine::CsrRole role_of(int id) { return static_cast<spmm::engine::CsrRole>(id); }
 
 int launch_id(int kernel_id, const void* d_A_any, const void* d_B, float* d_C, int N,
@@ -983,5 +989,87 @@ int spmm_c_time_repeat(int kernel_id, const void* d_A_any, const void* d_B, floa
 }
 
 int spmm_c_device_synchronize(void) { return from_hip(hipDeviceSynchronize(), "hipDeviceSynchronize"); }
+
+long long spmm_c_route_workspace(int tokens, int experts, int k) {
+    return spmm::engine::route_workspace(tokens, experts, k);
+}
+
+long long spmm_c_group_workspace(int entries, int groups) {
+    return spmm::engine::group_workspace(entries, groups);
+}
+
+int spmm_c_group_entries(const int* d_ids, int entries, int groups, int* d_offsets,
+                         int* d_entries, int* d_slots, void* d_workspace, void* stream) {
+    return guarded([&] {
+        return from_engine(spmm::engine::launch_group_entries(d_ids, entries, groups, d_offsets,
+                                                              d_entries, d_slots, d_workspace,
+                                                              as_stream(stream)));
+    });
+}
+
+int spmm_c_route(const void* d_logits, int type, int tokens, int experts, int k, int over,
+                 int* d_experts, float* d_weights, int* d_offsets, int* d_entries, int* d_slots,
+                 void* d_workspace, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        if (over != SPMM_OVER_CHOSEN && over != SPMM_OVER_ALL) {
+            return set_error(SPMM_INVALID, "route: unknown softmax range");
+        }
+        return from_engine(spmm::engine::launch_route(
+            d_logits, t, tokens, experts, k, over == SPMM_OVER_ALL, d_experts, d_weights,
+            d_offsets, d_entries, d_slots, d_workspace, as_stream(stream)));
+    });
+}
+
+int spmm_c_route_backward(const void* d_logits, int type, int tokens, int experts, int k, int over,
+                          const int* d_experts, const float* d_weights, const float* d_dweights,
+                          void* d_dlogits, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        if (over != SPMM_OVER_CHOSEN && over != SPMM_OVER_ALL) {
+            return set_error(SPMM_INVALID, "route_backward: unknown softmax range");
+        }
+        return from_engine(spmm::engine::launch_route_backward(
+            d_logits, t, tokens, experts, k, over == SPMM_OVER_ALL, d_experts, d_weights,
+            d_dweights, d_dlogits, as_stream(stream)));
+    });
+}
+
+int spmm_c_dispatch(const void* d_x, int type, int tokens, int k, int features,
+                    const int* d_slots, const int* d_offsets, int experts, void* d_xs,
+                    void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_dispatch(d_x, t, tokens, k, features, d_slots,
+                                                         d_offsets, experts, d_xs,
+                                                         as_stream(stream)));
+    });
+}
+
+int spmm_c_combine(const void* d_ys, int type, int tokens, int k, int features,
+                   const int* d_slots, const float* d_weights, void* d_y, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_combine(d_ys, t, tokens, k, features, d_slots,
+                                                        d_weights, d_y, as_stream(stream)));
+    });
+}
+
+int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int tokens, int k,
+                            int features, const int* d_slots, const float* d_weights,
+                            const int* d_offsets, int experts, void* d_dys, float* d_dweights,
+                            void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_combine_backward(
+            d_dy, d_ys, t, tokens, k, features, d_slots, d_weights, d_offsets, experts, d_dys,
+            d_dweights, as_stream(stream)));
+    });
+}
 
 }  // extern "C"

@@ -280,5 +280,37 @@ struct CsrChoice {
 CsrChoice choose_csr_form(const CSR& h_A, int N);
 const char* csr_form_name(CsrForm f);  // "rowgroups", "engine", "split", "khalf"
 
+// ---- mixture-of-experts routing (route.hip, tokens.hip) -----------------
+enum class ElementType : int { F32 = 0, F16 = 1, BF16 = 2 };
+
+// Bytes of workspace that launch_route / launch_group_entries need (0 for no
+// entries).
+long long route_workspace(long long tokens, int experts, int k);
+long long group_workspace(long long entries, int groups);
+// Stable counting sort of n entries by id: offsets (groups + 1) the first
+// place of each group, entries[place] the entry there, slots[entry] its place;
+// -1 behind the last group and for ids outside [0, groups).
+Error launch_group_entries(const int* ids, int n, int groups, int* offsets, int* entries,
+                           int* slots, void* workspace, hipStream_t stream);
+// The k largest logits of each token, their softmax weights (over the chosen
+// or over all experts), and the order of the tokens * k entries by expert.
+Error launch_route(const void* logits, ElementType type, int tokens, int experts, int k, bool all,
+                   int* out_experts, float* out_weights, int* offsets, int* entries, int* slots,
+                   void* workspace, hipStream_t stream);
+Error launch_route_backward(const void* logits, ElementType type, int tokens, int experts, int k,
+                            bool all, const int* chosen, const float* weights,
+                            const float* dweights, void* dlogits, hipStream_t stream);
+// Rows of tokens into expert order and back (weights null: unweighted), and
+// the gradients of the weighted way back.
+Error launch_dispatch(const void* x, ElementType type, int tokens, int k, int features,
+                      const int* slots, const int* offsets, int experts, void* xs,
+                      hipStream_t stream);
+Error launch_combine(const void* ys, ElementType type, int tokens, int k, int features,
+                     const int* slots, const float* weights, void* y, hipStream_t stream);
+Error launch_combine_backward(const void* dy, const void* ys, ElementType type, int tokens, int k,
+                              int features, const int* slots, const float* weights,
+                              const int* offsets, int experts, void* dys, float* dweights,
+                              hipStream_t stream);
+
 }  // namespace engine
 }  // namespace spmm

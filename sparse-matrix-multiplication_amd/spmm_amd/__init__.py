@@ -163,6 +163,14 @@ _SIGNATURES = {
     "spmm_c_time_repeat": (_int, [_int, _vp, _vp, _vp, _int, _int, _vp, _P(_float)]),
     "spmm_c_device_synchronize": (_int, []),
     "spmm_c_shader_clock_trace": (_int, [_vp, _int, _int, _vp]),
+    "spmm_c_route_workspace": (ctypes.c_longlong, [_int] * 3),
+    "spmm_c_group_workspace": (ctypes.c_longlong, [_int] * 2),
+    "spmm_c_route": (_int, [_vp] + [_int] * 5 + [_vp] * 7),
+    "spmm_c_route_backward": (_int, [_vp] + [_int] * 5 + [_vp] * 5),
+    "spmm_c_group_entries": (_int, [_vp, _int, _int] + [_vp] * 5),
+    "spmm_c_dispatch": (_int, [_vp] + [_int] * 4 + [_vp, _vp, _int, _vp, _vp]),
+    "spmm_c_combine": (_int, [_vp] + [_int] * 4 + [_vp] * 4),
+    "spmm_c_combine_backward": (_int, [_vp, _vp] + [_int] * 4 + [_vp] * 3 + [_int] + [_vp] * 3),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -1035,3 +1043,18 @@ def time_repeat(kernel: str, A, B, C, reps: int, stream=None) -> float:
                                     C.data_ptr(), int(B.shape[1]), reps, _stream_handle(stream),
                                     ctypes.byref(ms)))
     return ms.value
+
+
+# Mixture-of-experts routing and products, low-rank adapters (experts.py needs
+# torch, which host-only users of this module never import).
+_EXPERTS = ("Routing", "route", "route_backward", "group_entries", "dispatch", "dispatch_backward",
+            "combine", "combine_backward")
+
+
+def __getattr__(name: str):
+    if name in _EXPERTS:
+        from . import experts
+        for n in _EXPERTS:
+            globals()[n] = getattr(experts, n)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -1,0 +1,238 @@
+"""Mixture-of-experts routing and products over libspmm_amd.so.
+
+The routing of T tokens to E experts, k of them a token, is a sparse T x E
+matrix with k entries a row.  ``route`` finds it and the order of its entries
+by expert, ``dispatch`` and ``combine`` multiply by it (tokens into expert
+order and back, weighted).  Every call has its gradient beside it.
+
+Operands are contiguous cuda tensors on the current device; outputs are
+allocated where none is given, on the stream that the launch goes to (`stream`
+or the current one).  Nothing synchronises.
+"""
+from __future__ import annotations
+
+import contextlib
+from dataclasses import dataclass
+from typing import Any
+
+import torch
+
+from . import SPMM_INVALID, SpmmError, _check, lib
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_OVER = {"chosen": 0, "all": 1}
+_INT = (torch.int32,)
+_FLOAT = (torch.float32,)
+
+
+def _operand(t, name: str, dtypes, shape, device=None) -> None:
+    """One contiguous operand of the given type and shape (None: any size) on
+    the current device, and on `device` where that is given."""
+    if not isinstance(t, torch.Tensor):
+        raise SpmmError(SPMM_INVALID, f"{name}: expected a torch tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise SpmmError(SPMM_INVALID, f"{name}: must be a cuda tensor (got {t.device})")
+    where = t.device
+    if device is None:
+        if where.index != torch.cuda.current_device():
+            raise SpmmError(SPMM_INVALID, f"{name}: on {where}, the current device is "
+                                          f"cuda:{torch.cuda.current_device()}")
+    elif where != device:
+        raise SpmmError(SPMM_INVALID, f"{name}: on {where}, expected {device}")
+    if t.dtype not in dtypes:
+        want = " or ".join(str(d) for d in dtypes)
+        raise SpmmError(SPMM_INVALID, f"{name}: dtype {t.dtype}, expected {want}")
+    got = t.shape
+    if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
+        want = ", ".join("any" if w is None else str(w) for w in shape)
+        raise SpmmError(SPMM_INVALID, f"{name}: shape {tuple(got)}, expected ({want})")
+    if not t.is_contiguous():
+        raise SpmmError(SPMM_INVALID, f"{name}: must be contiguous (row-major)")
+
+
+def _out(t, name: str, dtype, shape, device):
+    """The output given, checked, or a new one."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _operand(t, name, (dtype,), shape, device)
+    return t
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(stream):
+    """Allocations inside belong to the stream that the launch goes to, so that
+    freeing them needs no wait of another stream's."""
+    return _here if stream is None else torch.cuda.stream(stream)
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+@dataclass
+class Routing:
+    """Tokens' experts and the order of the (token, choice) entries by expert.
+
+    experts  int32 [T, k]   chosen experts, -1 for none
+    weights  fp32  [T, k]   their softmax weights, 0 for none
+    offsets  int32 [E + 1]  each expert's first row in expert order
+    entries  int32 [T * k]  the entry t * k + j in each row, -1 behind the last
+    slots    int32 [T, k]   the row of each entry, -1 for none
+    over     "chosen" or "all": what the softmax runs over
+    """
+    experts: Any
+    weights: Any
+    offsets: Any
+    entries: Any
+    slots: Any
+    over: str = "chosen"
+
+    def _sizes(self):
+        """(tokens, k, experts), after a look at the fields that every call reads."""
+        if not isinstance(self.slots, torch.Tensor) or self.slots.dim() != 2 \
+                or not isinstance(self.offsets, torch.Tensor) or self.offsets.dim() != 1 \
+                or self.offsets.shape[0] < 2:
+            raise SpmmError(SPMM_INVALID, "routing: slots [T, k] and offsets [E + 1] are needed")
+        T, k = self.slots.shape
+        if k < 1:
+            raise SpmmError(SPMM_INVALID, "routing: no choice a token")
+        return T, k, self.offsets.shape[0] - 1
+
+
+def _over_id(over) -> int:
+    if over not in _OVER:
+        raise SpmmError(SPMM_INVALID, f"over: {over!r}, expected 'chosen' or 'all'")
+    return _OVER[over]
+
+
+def route(logits, k: int, over: str = "chosen", stream=None) -> Routing:
+    """The k largest of each token's logits [T, E] (float32, float16 or
+    bfloat16), their softmax weights over the chosen experts or over "all", and
+    the entries' order by expert.  Ties go to the lowest expert; -inf is never
+    chosen; a NaN is above all numbers and makes its token's weights NaN."""
+    over_id = _over_id(over)
+    _operand(logits, "logits", _TYPES, (None, None))
+    T, E = logits.shape
+    k = int(k)
+    if not 1 <= k <= E:
+        raise SpmmError(SPMM_INVALID, f"k: {k}, expected 1 to {E} experts")
+    L = lib()
+    device = logits.device
+    with _on(stream):
+        experts = torch.empty((T, k), dtype=torch.int32, device=device)
+        slots = torch.empty((T, k), dtype=torch.int32, device=device)
+        entries = torch.empty(T * k, dtype=torch.int32, device=device)
+        offsets = torch.empty(E + 1, dtype=torch.int32, device=device)
+        weights = torch.empty((T, k), dtype=torch.float32, device=device)
+        room = L.spmm_c_route_workspace(T, E, k)
+        work = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+        _check(L.spmm_c_route(logits.data_ptr(), _TYPES[logits.dtype], T, E, k, over_id,
+                              experts.data_ptr(), weights.data_ptr(), offsets.data_ptr(),
+                              entries.data_ptr(), slots.data_ptr(),
+                              work.data_ptr() if room else None, _stream()))
+    return Routing(experts, weights, offsets, entries, slots, over)
+
+
+def route_backward(logits, routing: Routing, dweights, out=None, stream=None):
+    """The gradient of ``route``'s weights with respect to the logits, of the
+    logits' type: [T, E]."""
+    over_id = _over_id(routing.over)
+    _operand(logits, "logits", _TYPES, (None, None))
+    T, E = logits.shape
+    device = logits.device
+    _operand(routing.weights, "routing.weights", _FLOAT, (T, None), device)
+    k = routing.weights.shape[1]
+    _operand(routing.experts, "routing.experts", _INT, (T, k), device)
+    _operand(dweights, "dweights", _FLOAT, (T, k), device)
+    with _on(stream):
+        out = _out(out, "out", logits.dtype, (T, E), device)
+        _check(lib().spmm_c_route_backward(
+            logits.data_ptr(), _TYPES[logits.dtype], T, E, k, over_id, routing.experts.data_ptr(),
+            routing.weights.data_ptr(), dweights.data_ptr(), out.data_ptr(), _stream()))
+    return out
+
+
+def group_entries(ids, groups: int, stream=None):
+    """The stable order of entries by group, for ids int32 of any shape: (offsets
+    [groups + 1], entries [n], slots like ids).  An id outside [0, groups) has no
+    place: slot -1, and -1 fills the entries behind the last group."""
+    if not isinstance(ids, torch.Tensor):
+        raise SpmmError(SPMM_INVALID, f"ids: expected a torch tensor, got {type(ids).__name__}")
+    _operand(ids, "ids", _INT, ids.shape)
+    n, device = ids.numel(), ids.device
+    groups = int(groups)
+    if groups < 1:
+        raise SpmmError(SPMM_INVALID, f"groups: {groups}, expected at least 1")
+    L = lib()
+    with _on(stream):
+        offsets = torch.empty(groups + 1, dtype=torch.int32, device=device)
+        entries = torch.empty(n, dtype=torch.int32, device=device)
+        slots = torch.empty_like(ids)
+        room = L.spmm_c_group_workspace(n, groups)
+        work = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+        _check(L.spmm_c_group_entries(ids.data_ptr(), n, groups, offsets.data_ptr(),
+                                      entries.data_ptr(), slots.data_ptr(),
+                                      work.data_ptr() if room else None, _stream()))
+    return offsets, entries, slots
+
+
+def dispatch(x, routing: Routing, out=None, stream=None):
+    """Rows of x [T, D] into expert order: [T * k, D]; rows without an entry are zero."""
+    T, k, E = routing._sizes()
+    _operand(x, "x", _TYPES, (T, None))
+    D, device = x.shape[1], x.device
+    _operand(routing.slots, "routing.slots", _INT, (T, k), device)
+    _operand(routing.offsets, "routing.offsets", _INT, (E + 1,), device)
+    with _on(stream):
+        out = _out(out, "out", x.dtype, (T * k, D), device)
+        _check(lib().spmm_c_dispatch(x.data_ptr(), _TYPES[x.dtype], T, k, D,
+                                     routing.slots.data_ptr(), routing.offsets.data_ptr(), E,
+                                     out.data_ptr(), _stream()))
+    return out
+
+
+def _gather(ys, name: str, routing: Routing, weighted: bool, out, stream):
+    T, k, _ = routing._sizes()
+    _operand(ys, name, _TYPES, (T * k, None))
+    D, device = ys.shape[1], ys.device
+    _operand(routing.slots, "routing.slots", _INT, (T, k), device)
+    if weighted:
+        _operand(routing.weights, "routing.weights", _FLOAT, (T, k), device)
+    with _on(stream):
+        out = _out(out, "out", ys.dtype, (T, D), device)
+        _check(lib().spmm_c_combine(ys.data_ptr(), _TYPES[ys.dtype], T, k, D,
+                                    routing.slots.data_ptr(),
+                                    routing.weights.data_ptr() if weighted else None,
+                                    out.data_ptr(), _stream()))
+    return out
+
+
+def dispatch_backward(dxs, routing: Routing, out=None, stream=None):
+    """The gradient of ``dispatch``: each token's rows of dxs [T * k, D] added up: [T, D]."""
+    return _gather(dxs, "dxs", routing, False, out, stream)
+
+
+def combine(ys, routing: Routing, out=None, stream=None):
+    """Each token's rows of ys [T * k, D] in expert order, weighted and added up: [T, D]."""
+    return _gather(ys, "ys", routing, True, out, stream)
+
+
+def combine_backward(dy, ys, routing: Routing, stream=None):
+    """The gradients of ``combine`` for dy [T, D]: (dys [T * k, D], dweights fp32 [T, k])."""
+    T, k, E = routing._sizes()
+    _operand(ys, "ys", _TYPES, (T * k, None))
+    D, device = ys.shape[1], ys.device
+    _operand(dy, "dy", (ys.dtype,), (T, D), device)
+    _operand(routing.slots, "routing.slots", _INT, (T, k), device)
+    _operand(routing.weights, "routing.weights", _FLOAT, (T, k), device)
+    _operand(routing.offsets, "routing.offsets", _INT, (E + 1,), device)
+    with _on(stream):
+        dys = torch.empty_like(ys)
+        dweights = torch.empty((T, k), dtype=torch.float32, device=device)
+        _check(lib().spmm_c_combine_backward(
+            dy.data_ptr(), ys.data_ptr(), _TYPES[ys.dtype], T, k, D, routing.slots.data_ptr(),
+            routing.weights.data_ptr(), routing.offsets.data_ptr(), E, dys.data_ptr(),
+            dweights.data_ptr(), _stream()))
+    return dys, dweights
