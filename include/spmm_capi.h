@@ -409,6 +409,34 @@ int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int to
                             const int* d_offsets, int experts, void* d_dys, float* d_dweights,
                             void* stream);
 
+/* ---- grouped products and low-rank adapters (no reference counterpart) --
+ * Matrix-core products of SPMM_F16 or SPMM_BF16 operands (SPMM_UNSUPPORTED for
+ * SPMM_F32), fp32 sums rounded once; contiguous device arrays, any sizes.
+ * grouped_mm: the block-diagonal product of rows in group order with their
+ *   group's weights.  Group g has rows [d_offsets[g], d_offsets[g+1]) of d_x
+ *   [rows, depth]; d_w is [groups, width, depth], or [groups, depth, width]
+ *   with w_in_rows; d_out [rows, width], rows in no group zero.  The gradient
+ *   for x is the same call on dout with w_in_rows the other way round.
+ * grouped_outer: d_out[g] [height, width] = the sum over the group's rows of
+ *   p[s]^T q[s], zero for an empty group: the gradient of the weights (p = dout,
+ *   q = x, or the other way round for w_in_rows).
+ * adapter_mm: d_out[s] = x[s] w^T + scale[a] (x[s] A_a^T) B_a^T with a =
+ *   d_ids[s], d_w [width, depth], d_a [adapters, rank, depth], d_b [adapters,
+ *   width, rank], d_scale [adapters] fp32 or null; rows whose id is outside
+ *   [0, adapters) take the projection alone.  x A_a^T is rounded to the
+ *   operands' type.  d_workspace: spmm_c_adapter_workspace bytes; calls that
+ *   share one must not overlap.  rank <= 1024. */
+int spmm_c_grouped_mm(const void* d_x, const void* d_w, int type, const int* d_offsets,
+                      int groups, int rows, int width, int depth, int w_in_rows, void* d_out,
+                      void* stream);
+int spmm_c_grouped_outer(const void* d_p, const void* d_q, int type, const int* d_offsets,
+                         int groups, int rows, int height, int width, void* d_out, void* stream);
+long long spmm_c_adapter_workspace(int rows, int rank);
+int spmm_c_adapter_mm(const void* d_x, const void* d_w, const void* d_a, const void* d_b,
+                      const int* d_ids, const float* d_scale, int type, int rows, int width,
+                      int depth, int adapters, int rank, void* d_out, void* d_workspace,
+                      void* stream);
+
 /* ---- measurement helpers (no reference counterpart) -------------------
  * Launch one entry point `reps` times back to back on `stream` without
  * synchronising, so a caller's events can bracket a batch.  kernel ids:

@@ -1072,4 +1072,43 @@ int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int to
     });
 }
 
+int spmm_c_grouped_mm(const void* d_x, const void* d_w, int type, const int* d_offsets, int groups,
+                      int rows, int width, int depth, int w_in_rows, void* d_out, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_grouped_mm(d_x, d_w, t, d_offsets, groups, rows,
+                                                           width, depth, w_in_rows != 0, d_out,
+                                                           as_stream(stream)));
+    });
+}
+
+int spmm_c_grouped_outer(const void* d_p, const void* d_q, int type, const int* d_offsets,
+                         int groups, int rows, int height, int width, void* d_out, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_grouped_outer(d_p, d_q, t, d_offsets, groups, rows,
+                                                              height, width, d_out,
+                                                              as_stream(stream)));
+    });
+}
+
+long long spmm_c_adapter_workspace(int rows, int rank) {
+    return spmm::engine::adapter_workspace(rows, rank);
+}
+
+int spmm_c_adapter_mm(const void* d_x, const void* d_w, const void* d_a, const void* d_b,
+                      const int* d_ids, const float* d_scale, int type, int rows, int width,
+                      int depth, int adapters, int rank, void* d_out, void* d_workspace,
+                      void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_adapter_mm(
+            d_x, d_w, d_a, d_b, d_ids, d_scale, t, rows, width, depth, adapters, rank, d_out,
+            d_workspace, as_stream(stream)));
+    });
+}
+
 }  // extern "C"

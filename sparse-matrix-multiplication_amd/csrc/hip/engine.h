@@ -312,5 +312,24 @@ Error launch_combine_backward(const void* dy, const void* ys, ElementType type, 
                               const int* offsets, int experts, void* dys, float* dweights,
                               hipStream_t stream);
 
+// ---- grouped products and adapters (grouped_mm.hip), fp16 and bf16 ------
+// out[s] = x[s] W_g^T for the rows offsets[g] <= s < offsets[g + 1] of group g;
+// rows in no group are zeroed.  W is [groups, width, depth], or with w_in_rows
+// [groups, depth, width].
+Error launch_grouped_mm(const void* x, const void* w, ElementType type, const int* offsets,
+                        int groups, int total, int width, int depth, bool w_in_rows, void* out,
+                        hipStream_t stream);
+// out[g] = sum over the group's rows of p[s]^T q[s]: [groups, height, width].
+Error launch_grouped_outer(const void* p, const void* q, ElementType type, const int* offsets,
+                           int groups, int total, int height, int width, void* out,
+                           hipStream_t stream);
+// out[s] = x[s] w^T + scale[a] (x[s] down[a]^T) up[a]^T, a = ids[s]; the
+// projection alone where a is outside [0, adapters).  scale null: 1.
+long long adapter_workspace(long long total, int rank);
+Error launch_adapter_mm(const void* x, const void* w, const void* down, const void* up,
+                        const int* ids, const float* scale, ElementType type, int total, int width,
+                        int depth, int adapters, int rank, void* out, void* workspace,
+                        hipStream_t stream);
+
 }  // namespace engine
 }  // namespace spmm

@@ -163,6 +163,10 @@ _SIGNATURES = {
     "spmm_c_time_repeat": (_int, [_int, _vp, _vp, _vp, _int, _int, _vp, _P(_float)]),
     "spmm_c_device_synchronize": (_int, []),
     "spmm_c_shader_clock_trace": (_int, [_vp, _int, _int, _vp]),
+    "spmm_c_grouped_mm": (_int, [_vp, _vp, _int, _vp] + [_int] * 5 + [_vp, _vp]),
+    "spmm_c_grouped_outer": (_int, [_vp, _vp, _int, _vp] + [_int] * 4 + [_vp, _vp]),
+    "spmm_c_adapter_workspace": (ctypes.c_longlong, [_int] * 2),
+    "spmm_c_adapter_mm": (_int, [_vp] * 6 + [_int] * 6 + [_vp] * 3),
     "spmm_c_route_workspace": (ctypes.c_longlong, [_int] * 3),
     "spmm_c_group_workspace": (ctypes.c_longlong, [_int] * 2),
     "spmm_c_route": (_int, [_vp] + [_int] * 5 + [_vp] * 7),
@@ -1048,7 +1052,7 @@ def time_repeat(kernel: str, A, B, C, reps: int, stream=None) -> float:
 # Mixture-of-experts routing and products, low-rank adapters (experts.py needs
 # torch, which host-only users of this module never import).
 _EXPERTS = ("Routing", "route", "route_backward", "group_entries", "dispatch", "dispatch_backward",
-            "combine", "combine_backward")
+            "combine", "combine_backward", "grouped_mm", "grouped_mm_backward", "adapter_mm")
 
 
 def __getattr__(name: str):

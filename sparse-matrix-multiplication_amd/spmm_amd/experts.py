@@ -1,9 +1,13 @@
-"""Mixture-of-experts routing and products over libspmm_amd.so.
+"""Mixture-of-experts routing and products, and low-rank adapters, over
+libspmm_amd.so.
 
 The routing of T tokens to E experts, k of them a token, is a sparse T x E
 matrix with k entries a row.  ``route`` finds it and the order of its entries
 by expert, ``dispatch`` and ``combine`` multiply by it (tokens into expert
-order and back, weighted).  Every call has its gradient beside it.
+order and back, weighted).  ``grouped_mm`` is the block-diagonal product of the
+rows in expert order with their experts' weights.  Every one of these has its
+gradient beside it.  ``adapter_mm`` is a shared projection with each row's own
+low-rank adapter.
 
 Operands are contiguous cuda tensors on the current device; outputs are
 allocated where none is given, on the stream that the launch goes to (`stream`
@@ -17,7 +21,7 @@ from typing import Any
 
 import torch
 
-from . import SPMM_INVALID, SpmmError, _check, lib
+from . import SPMM_INVALID, SPMM_UNSUPPORTED, SpmmError, _check, lib
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _OVER = {"chosen": 0, "all": 1}
@@ -236,3 +240,83 @@ def combine_backward(dy, ys, routing: Routing, stream=None):
             routing.weights.data_ptr(), routing.offsets.data_ptr(), E, dys.data_ptr(),
             dweights.data_ptr(), _stream()))
     return dys, dweights
+
+
+_HALF = (torch.float16, torch.bfloat16)
+
+
+def _half(t, name: str, shape) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype == torch.float32:
+        raise SpmmError(SPMM_UNSUPPORTED, f"{name}: float16 or bfloat16 (matrix cores)")
+    _operand(t, name, _HALF, shape)
+
+
+def grouped_mm(x, w, offsets, w_in_rows: bool = False, out=None, stream=None):
+    """Rows of x [S, K] times their group's weights: [S, N].  Group g has rows
+    offsets[g] to offsets[g + 1] (int32 [G + 1]); w is [G, N, K], or [G, K, N] with
+    w_in_rows.  Rows in no group are zero."""
+    _half(x, "x", (None, None))
+    S, K = x.shape
+    device = x.device
+    _operand(w, "w", (x.dtype,), (None, K, None) if w_in_rows else (None, None, K), device)
+    G, N = w.shape[0], w.shape[2 if w_in_rows else 1]
+    _operand(offsets, "offsets", _INT, (G + 1,), device)
+    with _on(stream):
+        out = _out(out, "out", x.dtype, (S, N), device)
+        _check(lib().spmm_c_grouped_mm(x.data_ptr(), w.data_ptr(), _TYPES[x.dtype],
+                                       offsets.data_ptr(), G, S, N, K, int(bool(w_in_rows)),
+                                       out.data_ptr(), _stream()))
+    return out
+
+
+def grouped_mm_backward(dy, x, w, offsets, w_in_rows: bool = False, stream=None):
+    """The gradients of ``grouped_mm`` for dy [S, N]: (dx [S, K], dw like w)."""
+    _half(x, "x", (None, None))
+    S, K = x.shape
+    device = x.device
+    _operand(w, "w", (x.dtype,), (None, K, None) if w_in_rows else (None, None, K), device)
+    G, N = w.shape[0], w.shape[2 if w_in_rows else 1]
+    _operand(dy, "dy", (x.dtype,), (S, N), device)
+    _operand(offsets, "offsets", _INT, (G + 1,), device)
+    p, q, height, width = (x, dy, K, N) if w_in_rows else (dy, x, N, K)
+    with _on(stream):
+        dw = torch.empty_like(w)
+        dx = torch.empty_like(x)
+        L, s = lib(), _stream()
+        _check(L.spmm_c_grouped_mm(dy.data_ptr(), w.data_ptr(), _TYPES[x.dtype],
+                                   offsets.data_ptr(), G, S, K, N, int(not w_in_rows),
+                                   dx.data_ptr(), s))
+        _check(L.spmm_c_grouped_outer(p.data_ptr(), q.data_ptr(), _TYPES[x.dtype],
+                                      offsets.data_ptr(), G, S, height, width, dw.data_ptr(), s))
+    return dx, dw
+
+
+def adapter_mm(x, w, a, b, ids, scale=None, out=None, stream=None):
+    """A shared projection with low-rank adapters of many requests at once: row s of
+    the result is x[s] w^T + scale[i] (x[s] a[i]^T) b[i]^T with i = ids[s], the
+    projection alone where ids[s] is outside [0, L).
+
+    x [T, K], w [N, K], a [L, R, K], b [L, N, R], float16 or bfloat16; ids int32
+    [T]; scale float32 [L], 1 when None.  Adapters of a smaller rank are padded
+    with zeros."""
+    _half(x, "x", (None, None))
+    T, K = x.shape
+    device = x.device
+    _operand(w, "w", (x.dtype,), (None, K), device)
+    N = w.shape[0]
+    _operand(a, "a", (x.dtype,), (None, None, K), device)
+    L, R = a.shape[:2]
+    _operand(b, "b", (x.dtype,), (L, N, R), device)
+    _operand(ids, "ids", _INT, (T,), device)
+    if scale is not None:
+        _operand(scale, "scale", _FLOAT, (L,), device)
+    library = lib()
+    with _on(stream):
+        out = _out(out, "out", x.dtype, (T, N), device)
+        work = torch.empty(library.spmm_c_adapter_workspace(T, R), dtype=torch.uint8,
+                           device=device)
+        _check(library.spmm_c_adapter_mm(
+            x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
+            None if scale is None else scale.data_ptr(), _TYPES[x.dtype], T, N, K, L, R,
+            out.data_ptr(), work.data_ptr(), _stream()))
+    return out
