@@ -98,6 +98,21 @@ __device__ __forceinline__ void lds_dma_x4(u32x4 rsrc, unsigned lds, int index, 
 #pragma clang diagnostic pop
 }
 
+// The same for a raw buffer (stride 0): lane i's 16 bytes from byte `offset`;
+// an offset at or past the record count (bytes) writes zeros.
+__device__ __forceinline__ void lds_dma_raw_x4(u32x4 rsrc, unsigned lds, unsigned offset) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :
+        : "s"(lds), "v"(offset), "s"(rsrc)
+        : "m0");
+#pragma clang diagnostic pop
+}
+
 // LDS byte address of a pointer into a __shared__ array.
 __device__ __forceinline__ unsigned lds_address(const void* p) {
     return static_cast<unsigned>(reinterpret_cast<uintptr_t>(
