@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <string>
 #include <type_traits>
+#include <utility>
 
 #include "amdgcn.h"
 #include "elements.h"
@@ -38,6 +39,27 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
 }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// The same into accumulation registers.  Written out because the compiler moves
+// 256 accumulators between the register files instead of leaving them in place.
+// What the compiler would count for its own products is kept by the callers: the
+// operands come from memory reads (which it waits for), or LATE leaves the two
+// wait states that operands written by vector instructions need; sums are read
+// only after settle_sums.
+template <bool LATE = false>
+__device__ __forceinline__ void mfma_in_place(f32x4& c, f16x8 a, f16x8 b) {
+    if constexpr (LATE) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+template <bool LATE = false>
+__device__ __forceinline__ void mfma_in_place(f32x4& c, bf16x8 a, bf16x8 b) {
+    if constexpr (LATE) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void settle_sums() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 template <typename T>
 using Operand = std::conditional_t<std::is_same_v<T, _Float16>, f16x8, bf16x8>;
@@ -195,14 +217,6 @@ struct Operands {
             *reinterpret_cast<uint4*>(lds + (i * THREADS + threadIdx.x) * 8) = v[i];
         }
     }
-    // Pieces straight into LDS; ld, bound and left are multiples of the piece here, or
-    // the piece is past its bound, where the offset past the buffer's end writes zeros.
-    // lds: the wave's first place (1 KiB a wave) in LDS.
-    __device__ __forceinline__ void dma(u32x4 buffer, unsigned lds, int left, int i) const {
-        const unsigned at = index[i] < left && room[i] > 0 ? static_cast<unsigned>(base[i]) * 2u
-                                                           : 0x80000000u;
-        lds_dma_raw_x4(buffer, lds + i * THREADS * 16, at);
-    }
     // Operand of columns n0 .. n0+15, contraction steps 32 half .. +31: lane l holds
     // steps 8 (l >> 4) .. +7 of column l & 15.
     static __device__ __forceinline__ Operand<T> read(const T* lds, int n0, int half) {
@@ -223,22 +237,6 @@ struct Operands {
         }
     }
 };
-
-// Four consecutive columns of a row from lane values; `count` of them exist.
-template <typename T>
-__device__ __forceinline__ void store_four(T* p, f32x4 v, int count) {
-    T e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = static_cast<T>(v[i]);
-    if (count >= 4) {
-        __builtin_memcpy(p, e, sizeof(e));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            if (i < count) p[i] = e[i];
-        }
-    }
-}
 
 // What a workgroup works on: the first elements of its operands and its output,
 // the contraction's length, and how far a staged tile advances.
@@ -293,79 +291,148 @@ __device__ __forceinline__ bool take_tile(const TileArgs& a, Tile<T>& t) {
     return true;
 }
 
-// The adapters' extension of a wave's tile (rows r0 .. of the workgroup's, columns
-// c0 ..): the contraction goes on over the adapters of the wave's rows, for each
-// that occurs its B against h in the rows that have it.
-template <typename T, int RF, int CF>
-__device__ __forceinline__ void add_adapters(const TileArgs& a, const Tile<T>& t, int r0, int c0,
-                                             f32x4 (&acc)[CF][RF]) {
-    const int lane = threadIdx.x & 63;
-    const int s = lane & 15, q = lane >> 4;
-    const T* h = static_cast<const T*>(a.h);
-    const T* b = static_cast<const T*>(a.b);
-    int id[RF];
-#pragma unroll
-    for (int i = 0; i < RF; ++i) {
-        const int r = r0 + i * 16 + s;
-        id[i] = r < t.rows_here ? a.ids[t.row0 + r] : -1;
-        if (static_cast<unsigned>(id[i]) >= static_cast<unsigned>(a.adapters)) id[i] = -1;
-    }
-#pragma unroll
-    for (int i0 = 0; i0 < RF; ++i0) {
-        for (;;) {
-            const unsigned long long left = __ballot(id[i0] >= 0);
-            if (left == 0) break;
-            const int mine = __builtin_amdgcn_readlane(id[i0], __builtin_ctzll(left));
-            for (int k0 = 0; k0 < a.rank; k0 += 32) {
-                const int k = k0 + 8 * q;
-                Operand<T> fc[CF];
-#pragma unroll
-                for (int j = 0; j < CF; ++j) {
-                    const int c = c0 + j * 16 + s;
-                    const int n = c < a.width ? min(8, a.rank - k) : 0;
-                    const T* p = b + (static_cast<long long>(mine) * a.width + c) * a.rank + k;
-                    fc[j] = __builtin_bit_cast(Operand<T>, n == 8 ? load_piece(p)
-                                                           : n <= 0 ? uint4{0, 0, 0, 0}
-                                                                    : load_part(p, n));
-                }
-#pragma unroll
-                for (int i = i0; i < RF; ++i) {
-                    if (__ballot(id[i] == mine) == 0) continue;
-                    const int r = r0 + i * 16 + s;
-                    const uint4 v = id[i] == mine
-                        ? load_piece(h + static_cast<long long>(t.row0 + r) * a.rank32 + k)
-                        : uint4{0, 0, 0, 0};
-                    const Operand<T> fr = __builtin_bit_cast(Operand<T>, v);
-                    // A lane's sums are its own row's: other rows keep theirs,
-                    // whatever (infinities, NaN) this adapter's B holds.
-#pragma unroll
-                    for (int j = 0; j < CF; ++j) {
-                        const f32x4 next = mfma(fc[j], fr, acc[j][i]);
-                        acc[j][i] = id[i] == mine ? next : acc[j][i];
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = i0; i < RF; ++i) id[i] = id[i] == mine ? -1 : id[i];
-        }
-    }
+// f(0), f(1), ... with the index a constant, so that registers named by it stay
+// registers however much f does.
+template <int... I, typename F>
+__device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F f) {
+    (f(std::integral_constant<int, I>{}), ...);
 }
 
+// The adapters of a wave's rows (r0 .. of the workgroup's tile, columns c0 ..): the
+// contraction goes on over h against B_a.  Sixteen rows of one adapter take it in
+// place (whole_tiles); sixteen rows of several, or of some with none, get each
+// adapter's part apart, added only to its own rows (mixed_tile), so that no row
+// sees what another's adapter holds, infinities and NaN included.
 template <typename T, int RF, int CF>
-__device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, int r0, int c0,
-                                           const f32x4 (&acc)[CF][RF]) {
-    const int lane = threadIdx.x & 63;
-    const int s = lane & 15, q = lane >> 4;
+struct Adapters {
+    const T* h;
+    const T* b;
+    int      id[RF];  // of row 16 i + (lane & 15), -1 for none
+    int      width, rank, rank32, rows_left;
+    int      c0;
+
+    __device__ __forceinline__ Adapters(const TileArgs& a, const Tile<T>& t, int r0, int first_col)
+        : h(static_cast<const T*>(a.h) + static_cast<long long>(t.row0 + r0) * a.rank32),
+          b(static_cast<const T*>(a.b)), width(a.width), rank(a.rank), rank32(a.rank32),
+          rows_left(t.rows_here - r0), c0(first_col) {
+        const int s = threadIdx.x & 15;
 #pragma unroll
-    for (int i = 0; i < RF; ++i) {
-        const int r = r0 + i * 16 + s;
-        if (r >= t.rows_here) continue;
-#pragma unroll
-        for (int j = 0; j < CF; ++j) {
-            const int c = c0 + j * 16 + 4 * q;
-            store_four(t.out + static_cast<long long>(r) * a.width + c, acc[j][i], a.width - c);
+        for (int i = 0; i < RF; ++i) {
+            id[i] = i * 16 + s < rows_left ? a.ids[t.row0 + r0 + i * 16 + s] : -1;
+            if (static_cast<unsigned>(id[i]) >= static_cast<unsigned>(a.adapters)) id[i] = -1;
         }
     }
+    __device__ __forceinline__ Operand<T> read_b(int adapter, int j, int k0) const {
+        const int k = k0 + 8 * ((threadIdx.x & 63) >> 4), c = c0 + j * 16 + (threadIdx.x & 15);
+        const int n = c < width ? min(8, rank - k) : 0;
+        const T* p = b + (static_cast<long long>(adapter) * width + c) * rank + k;
+        return __builtin_bit_cast(Operand<T>, n == 8 ? load_piece(p)
+                                              : n <= 0 ? uint4{0, 0, 0, 0} : load_part(p, n));
+    }
+    // rows of other adapters read zeros
+    __device__ __forceinline__ Operand<T> read_h(int i, int mine, int adapter, int k0) const {
+        const T* p = h + static_cast<long long>(i * 16 + (threadIdx.x & 15)) * rank32 + k0 +
+                     8 * ((threadIdx.x & 63) >> 4);
+        return __builtin_bit_cast(Operand<T>, mine == adapter ? load_piece(p) : uint4{0, 0, 0, 0});
+    }
+    // The adapter that all of sixteen rows have (rows past the tile's end are never
+    // stored and may take anything); -1 where there is no such one.
+    __device__ __forceinline__ int of_all(int i) const {
+        const unsigned long long have = __ballot(id[i] >= 0);
+        if (have == 0) return -1;
+        const int first = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(have));
+        const bool here = i * 16 + static_cast<int>(threadIdx.x & 15) < rows_left;
+        return __ballot(here && id[i] != first) == 0 ? first : -1;
+    }
+    __device__ __forceinline__ bool mixed(int i) const {
+        return __ballot(id[i] >= 0) != 0 && of_all(i) < 0;
+    }
+    __device__ __forceinline__ void whole_tiles(f32x4 (&acc)[CF][RF]) const {
+        int of[RF];
+#pragma unroll
+        for (int i = 0; i < RF; ++i) of[i] = of_all(i);
+        for (;;) {
+            int adapter = -1;
+#pragma unroll
+            for (int i = RF - 1; i >= 0; --i) adapter = of[i] >= 0 ? of[i] : adapter;
+            if (adapter < 0) break;
+            for (int k0 = 0; k0 < rank; k0 += 32) {
+                Operand<T> fr[RF];
+#pragma unroll
+                for (int i = 0; i < RF; ++i) fr[i] = read_h(i, id[i], adapter, k0);
+                unrolled(std::make_integer_sequence<int, CF>{}, [&](auto j) {
+                    const Operand<T> fc = read_b(adapter, j.value, k0);
+                    unrolled(std::make_integer_sequence<int, RF>{}, [&](auto i) {
+                        if (of[i.value] == adapter) {
+                            mfma_in_place<true>(acc[j.value][i.value], fc, fr[i.value]);
+                        }
+                    });
+                });
+            }
+#pragma unroll
+            for (int i = 0; i < RF; ++i) of[i] = of[i] == adapter ? -1 : of[i];
+        }
+    }
+    // sums: the wave's sixteen rows in LDS, `pitch` floats a row.
+    __device__ __forceinline__ void mixed_tile(int i, int mine, float* sums, int pitch) const {
+        const int lane = threadIdx.x & 63;
+        float* at = sums + (lane & 15) * pitch + 4 * (lane >> 4);
+        int left_id = mine;
+        for (;;) {
+            const unsigned long long left = __ballot(left_id >= 0);
+            if (left == 0) break;
+            const int adapter = __builtin_amdgcn_readlane(left_id, __builtin_ctzll(left));
+            for (int j = 0; j < CF; ++j) {
+                f32x4 sum = f32x4(0.0f);
+                for (int k0 = 0; k0 < rank; k0 += 32) {
+                    sum = mfma(read_b(adapter, j, k0), read_h(i, mine, adapter, k0), sum);
+                }
+                f32x4* p = reinterpret_cast<f32x4*>(at + 16 * j);
+                if (mine == adapter) *p = *p + sum;
+            }
+            left_id = left_id == adapter ? -1 : left_id;
+        }
+    }
+};
+
+// Floats of LDS that a wave's stores take: sixteen rows of its columns, four more
+// a row so that rows start 16 bytes apart in the banks.
+template <int CF>
+constexpr int kStoreFloats = 16 * (CF * 16 + 4);
+
+// Stores a wave's tile, sixteen rows at a time through its own part of LDS (`sums`,
+// free in all waves), so that whole row pieces leave in 16-byte stores.
+template <typename T, int RF, int CF, typename Mixed>
+__device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, int r0, int c0,
+                                           const f32x4 (&acc)[CF][RF], float* sums, Mixed mixed) {
+    constexpr int kPitch = CF * 16 + 4, kLanes = CF * 2, kRows = 64 / kLanes;
+    const int lane = threadIdx.x & 63;
+    const int s = lane & 15, q = lane >> 4;
+    const int c = c0 + lane % kLanes * 8;
+    const int count = min(8, a.width - c);
+    unrolled(std::make_integer_sequence<int, RF>{}, [&](auto at) {
+        constexpr int i = at.value;
+        if (r0 + i * 16 < t.rows_here) {
+#pragma unroll
+            for (int j = 0; j < CF; ++j) {
+                *reinterpret_cast<f32x4*>(sums + s * kPitch + j * 16 + 4 * q) = acc[j][i];
+            }
+            mixed(at);
+#pragma unroll
+            for (int n = 0; n < 16 / kRows; ++n) {
+                const int r = n * kRows + lane / kLanes;
+                const float* from = sums + r * kPitch + lane % kLanes * 8;
+                float f[8];
+                __builtin_memcpy(f, __builtin_assume_aligned(from, 16), 32);
+                const uint4 v = piece_from_float<T>(f);
+                if (r0 + i * 16 + r < t.rows_here && count > 0) {
+                    T* p = t.out + static_cast<long long>(r0 + i * 16 + r) * a.width + c;
+                    if (count == 8) store_piece(p, v);
+                    else store_part(p, v, count);
+                }
+            }
+        }
+    });
 }
 
 // GRAD false: a product (rows operand [s][k], columns operand W as COLS_MAJOR
@@ -380,8 +447,9 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_product(TileArgs a) {
     constexpr int RF = BR / WR / 16, CF = BC / WC / 16;  // 16 x 16 tiles a wave
     using Rows = Operands<T, BR, GRAD, THREADS>;
     using Cols = Operands<T, BC, GRAD || COLS_MAJOR, THREADS>;
-    __shared__ __attribute__((aligned(16))) T s_rows[2][BR * kStep];
-    __shared__ __attribute__((aligned(16))) T s_cols[2][BC * kStep];
+    __shared__ __attribute__((aligned(16))) T s_tiles[2 * (BR + BC) * kStep];
+    auto rows_at = [&](int it) { return s_tiles + (it & 1) * BR * kStep; };
+    auto cols_at = [&](int it) { return s_tiles + (2 * BR + (it & 1) * BC) * kStep; };
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WC, wc = wave % WC;
@@ -403,8 +471,8 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_product(TileArgs a) {
     if (tiles > 0) {
         pr.load(t.rows, t.depth, vr);
         pc.load(t.cols, t.depth, vc);
-        pr.store(s_rows[0], vr);
-        pc.store(s_cols[0], vc);
+        pr.store(rows_at(0), vr);
+        pc.store(cols_at(0), vc);
     }
     for (int it = 0; it < tiles; ++it) {
         // the tile is written, and the other buffer's readers are done
@@ -415,8 +483,8 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_product(TileArgs a) {
             pr.load(t.rows + (it + 1) * t.step_rows, left, vr);
             pc.load(t.cols + (it + 1) * t.step_cols, left, vc);
         }
-        const T* lr = s_rows[it & 1];
-        const T* lc = s_cols[it & 1];
+        const T* lr = rows_at(it);
+        const T* lc = cols_at(it);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             Operand<T> fr[RF], fc[CF];
@@ -427,38 +495,96 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_product(TileArgs a) {
 #pragma unroll
             for (int j = 0; j < CF; ++j)
 #pragma unroll
-                for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc[j], fr[i], acc[j][i]);
+                for (int i = 0; i < RF; ++i) mfma_in_place(acc[j][i], fc[j], fr[i]);
         }
         if (more) {
-            pr.store(s_rows[(it + 1) & 1], vr);
-            pc.store(s_cols[(it + 1) & 1], vc);
+            pr.store(rows_at(it + 1), vr);
+            pc.store(cols_at(it + 1), vc);
         }
     }
-    if constexpr (ADAPT) add_adapters<T, RF, CF>(a, t, wr * RF * 16, t.c0 + wc * CF * 16, acc);
-    store_tile<T, RF, CF>(a, t, wr * RF * 16, t.c0 + wc * CF * 16, acc);
+    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
+    lds_barrier();  // the operands' LDS is free
+    float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
+    if constexpr (ADAPT) {
+        const Adapters<T, RF, CF> ad(a, t, r0, c0);
+        ad.whole_tiles(acc);
+        settle_sums();
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
+            constexpr int i = at.value;
+            if (ad.mixed(i)) ad.mixed_tile(i, ad.id[i], sums, CF * 16 + 4);
+        });
+    } else {
+        settle_sums();
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
+    }
 }
 
+// How 128 rows (or columns) of an operand's staged tile reach LDS in 16-byte
+// pieces by buffer loads of 256 threads: the places of Operands<T, 128, ...>.
+// Rows n = 64 p + r of the slot are the operand's rows GAP p + r.
+template <typename T, bool MAJOR, int GAP>
+struct Slot {
+    static constexpr int kPieces = 4;
+    static constexpr int kBytes  = 128 * kStep * 2;
+    unsigned at[kPieces];  // byte offset of the piece; past every buffer's end for no such row
+    int      index;        // its first contraction step, less 16 i for MAJOR
+
+    __device__ __forceinline__ void place(int ld, int first, int bound) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int p = i * 256 + threadIdx.x;
+            int k, n;  // contraction step, row of the slot
+            if constexpr (MAJOR) {
+                k = p / 16;
+                const int f = (k & 3) | ((k >> 3) & 1) << 2;
+                n = ((p % 16) ^ (f << 1)) * 8;
+            } else {
+                n = p / 8;
+                k = ((p % 8) ^ (n & 7)) * 8;
+            }
+            const int row = first + (n / 64) * GAP + n % 64;
+            const int element = MAJOR ? k * ld + row : row * ld + k;
+            at[i] = row < bound ? static_cast<unsigned>(element) * 2u : kAbsent;
+            if (i == 0) index = k;
+        }
+    }
+    // Where piece I of a tile with `left` contraction steps left lies.
+    template <int I>
+    __device__ __forceinline__ unsigned offset(int left) const {
+        return index + (MAJOR ? 16 * I : 0) < left ? at[I] : kAbsent;
+    }
+    static constexpr unsigned kAbsent = 0x80000000u;
+};
+
 // The 256 x 256 tile of large products, for operands whose rows are whole 16-byte
-// pieces: pieces go straight into LDS, and two groups of four waves (one a SIMD
-// each) take turns.  While one group reads a quarter of a staged tile's operands,
-// the other multiplies the quarter it has read; a barrier swaps them.  A quarter
-// is 16 products of 16x16x32 a wave (256 cycles), against 4 to 8 operand reads a
-// wave for four waves (128 to 256 cycles of the LDS).
-//   Buffer it & 1 is overwritten only in iteration it + 1: a group gets there
-//   after the barrier that follows the other group's last reads of it.
-//   A tile's loads are issued in the first two quarters of the tile before and
-//   waited for (each wave its own) in the last quarter before the barrier, after
-//   which either group may read it.
+// pieces.  Four waves, one a SIMD, take a quarter of 128 x 128 each; 64 steps of
+// the contraction are a tile of four slots of 16 KB in LDS: columns 0-127 (C0) and
+// 128-255 (C1), the first 64 rows of either pair of waves (L) and the last 64 (H).
+// Ten slots form a ring, filled by buffer-to-LDS loads in the order C0 C1 L H.
+//
+// A tile is multiplied in four parts: L with the first 32 steps and the last 32,
+// then H (the columns' operands stay in registers).  Behind a part's products the
+// wave issues the next part's operand reads and one slot's loads.  C0, C1 and L are
+// read by the end of part 0, H by the end of part 2; a barrier behind each of these
+// frees their slots.  So slot n is loaded seven parts before it is read, about two
+// tiles ahead: with two buffers of a tile (a quarter of that ahead) waves stood
+// still for a sixth of the time, loads that miss the L2 being waited for.
+//   Before the barriers each wave waits for its own loads: behind part 2 all but
+//   the five youngest slots (the next tile's C0, C1, L are there), behind part 0
+//   all but six (this tile's H is there), and for its operand reads.
+//   Past the contraction's end loads write zeros, so the counts always hold.
 template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT>
-__global__ __launch_bounds__(512) void tile_product_wide(TileArgs a) {
-    constexpr int BR = 256, BC = 256, THREADS = 512, RF = 8, CF = 4;
-    using Rows = Operands<T, BR, GRAD, THREADS>;
-    using Cols = Operands<T, BC, GRAD || COLS_MAJOR, THREADS>;
+__global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
+    constexpr int BR = 256, BC = 256, RF = 8, CF = 8;
+    using RowSlot = Slot<T, GRAD, 128>;
+    using ColSlot = Slot<T, GRAD || COLS_MAJOR, 64>;
+    using Rows = Operands<T, 128, GRAD, 256>;
+    using Cols = Operands<T, 128, GRAD || COLS_MAJOR, 256>;
     extern __shared__ __attribute__((aligned(16))) char s_tiles[];
-    constexpr int kTile = BR * kStep;  // elements of an operand's tile
+    constexpr int kSlot = 128 * kStep;  // elements
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wr = wave >> 2, wc = wave & 3;
+    const int wr = wave >> 1, wc = wave & 1;
     Tile<T> t;
     if (!take_tile<T, BR, BC, GRAD, COLS_MAJOR>(a, t)) return;
 
@@ -468,71 +594,125 @@ __global__ __launch_bounds__(512) void tile_product_wide(TileArgs a) {
 #pragma unroll
         for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
 
-    Rows pr;
-    Cols pc;
-    pr.place(t.ld_rows, t.rows_here);
-    pc.place(t.ld_cols, a.width - t.c0);
     const int tiles = (t.depth + kStep - 1) / kStep;
-    T* const lds = reinterpret_cast<T*>(s_tiles);
-    const unsigned lds0 = lds_address(s_tiles) + wave * 1024;
-    auto load_rows = [&](int it) {
-        const u32x4 buffer = buffer_words(t.rows + it * t.step_rows, 0, 0x7fffffff);
-#pragma unroll
-        for (int i = 0; i < Rows::kPieces; ++i) {
-            pr.dma(buffer, lds0 + (it & 1) * 4 * kTile, t.depth - it * kStep, i);
-        }
-    };
-    auto load_cols = [&](int it) {
-        const u32x4 buffer = buffer_words(t.cols + it * t.step_cols, 0, 0x7fffffff);
-#pragma unroll
-        for (int i = 0; i < Cols::kPieces; ++i) {
-            pc.dma(buffer, lds0 + (it & 1) * 4 * kTile + 2 * kTile, t.depth - it * kStep, i);
-        }
-    };
     if (tiles > 0) {
-        load_rows(0);
-        load_cols(0);
-        wait_vmcnt<0>();
+        ColSlot c0, c1;
+        RowSlot low, high;
+        c0.place(t.ld_cols, 0, a.width - t.c0);
+        c1.place(t.ld_cols, 128, a.width - t.c0);
+        low.place(t.ld_rows, 0, t.rows_here);
+        high.place(t.ld_rows, 64, t.rows_here);
+        T* const lds = reinterpret_cast<T*>(s_tiles);
+        const unsigned lds0 = lds_address(s_tiles) + wave * 1024;
+        auto place_of = [&](int slot) { return lds0 + slot * ColSlot::kBytes; };
+        // The tile that is being loaded, as buffers that begin at it, and the
+        // contraction steps left there.
+        u32x4 rows = buffer_words(t.rows, 0, 0x7fffffff);
+        u32x4 cols = buffer_words(t.cols, 0, 0x7fffffff);
+        int left = t.depth;
+        auto step = [](u32x4& buffer, long long bytes) {
+            const unsigned long long at =
+                (static_cast<unsigned long long>(buffer[1]) << 32 | buffer[0]) + bytes;
+            buffer[0] = static_cast<unsigned>(at);
+            buffer[1] = static_cast<unsigned>(at >> 32);
+        };
+        auto advance = [&] {
+            step(rows, t.step_rows * 2);
+            step(cols, t.step_cols * 2);
+            left -= kStep;
+        };
+        auto load_slot = [&](const auto& slot, const u32x4& from, unsigned to) {
+            unrolled(std::make_integer_sequence<int, 4>{}, [&](auto i) {
+                lds_dma_raw_to<i.value * 4096>(to);
+                asm volatile("s_nop 0");
+                lds_dma_raw_x4(from, slot.template offset<i.value>(left));
+            });
+        };
+
+        Operand<T> fr[2][RF / 2], fc[2][CF];
+        auto read_row = [&](int slot, int half, int i) {
+            fr[half][i] = Rows::read(lds + slot * kSlot, wr * 64 + i * 16, half);
+        };
+        auto read_col = [&](int slot, int half, int j) {
+            fc[half][j] = Cols::read(lds + slot * kSlot, j * 16, half);
+        };
+        // One part's products; behind product m, read(m) and a step of one of the four
+        // loads of `slot` into place `to`: never more than two of them, which the
+        // matrix cores' own time covers.
+        constexpr int kProducts = CF * RF / 2;
+        auto multiply = [&](int half, int second, const auto& slot, const u32x4& from, unsigned to,
+                            auto read) {
+            unsigned offset = 0;
+            __builtin_amdgcn_sched_barrier(0);
+            unrolled(std::make_integer_sequence<int, kProducts>{}, [&](auto m) {
+                constexpr int j = m.value / (RF / 2), i = m.value % (RF / 2);
+                mfma_in_place(acc[j][second * (RF / 2) + i], fc[half][j], fr[half][i]);
+                read(m);
+                if constexpr (m.value % 8 == 2) offset = slot.template offset<m.value / 8>(left);
+                if constexpr (m.value % 8 == 4) lds_dma_raw_to<m.value / 8 * 4096>(to);
+                if constexpr (m.value % 8 == 6) lds_dma_raw_x4(from, offset);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        load_slot(c0, cols, place_of(0));
+        load_slot(c1, cols, place_of(1));
+        load_slot(low, rows, place_of(2));
+        load_slot(high, rows, place_of(3));
+        advance();
+        load_slot(c0, cols, place_of(4));
+        load_slot(c1, cols, place_of(5));
+        load_slot(low, rows, place_of(6));
+        load_slot(high, rows, place_of(7));
+        advance();
+        load_slot(c0, cols, place_of(8));
+        wait_vmcnt<24>();  // slots 0, 1, 2
         lds_barrier();
-        if (wr == 1) lds_barrier();
-    }
-    for (int it = 0; it < tiles; ++it) {
-        const T* lr = lds + (it & 1) * 2 * kTile;
-        const T* lc = lr + kTile;
-        Operand<T> fc[CF], fr[RF / 2];
 #pragma unroll
-        for (int part = 0; part < 4; ++part) {
-            const int half = part >> 1, i0 = (part & 1) * (RF / 2);
-            if ((part & 1) == 0) {
+        for (int i = 0; i < RF / 2; ++i) read_row(2, 0, i);
 #pragma unroll
-                for (int j = 0; j < CF; ++j) fc[j] = Cols::read(lc, (wc * CF + j) * 16, half);
-            }
-#pragma unroll
-            for (int i = 0; i < RF / 2; ++i) {
-                fr[i] = Rows::read(lr, (wr * RF + i0 + i) * 16, half);
-            }
-            if (it + 1 < tiles) {
-                if (part == 0) load_rows(it + 1);
-                if (part == 1) load_cols(it + 1);
-            }
-            if (part == 3) wait_vmcnt<0>();
-            __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < CF; ++j) read_col(wc, 0, j);
+
+        int slot = 0;  // of this tile's C0
+        auto later = [&](int n) { return slot + n < 10 ? slot + n : slot + n - 10; };
+        for (int it = 0; it < tiles; ++it) {
+            multiply(0, 0, c1, cols, place_of(later(9)), [&](auto m) {
+                if constexpr (m.value < 8) read_col(later(wc), 1, m.value);
+                else if constexpr (m.value < 12) read_row(later(2), 1, m.value - 8);
+            });
+            wait_vmcnt<24>();
             lds_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int j = 0; j < CF; ++j)
-#pragma unroll
-                for (int i = 0; i < RF / 2; ++i) acc[j][i0 + i] = mfma(fc[j], fr[i], acc[j][i0 + i]);
-            __builtin_amdgcn_s_setprio(0);
-            __builtin_amdgcn_sched_barrier(0);
+            multiply(1, 0, low, rows, place_of(slot), [&](auto m) {
+                if constexpr (m.value < 4) read_row(later(3), 0, m.value);
+            });
+            multiply(0, 1, high, rows, place_of(later(1)), [&](auto m) {
+                if constexpr (m.value < 4) read_row(later(3), 1, m.value);
+            });
+            wait_vmcnt<20>();
             lds_barrier();
-            __builtin_amdgcn_sched_barrier(0);
+            advance();
+            multiply(1, 1, c0, cols, place_of(later(2)), [&](auto m) {
+                if constexpr (m.value < 4) read_row(later(6), 0, m.value);
+                else if constexpr (m.value < 12) read_col(later(4 + wc), 0, m.value - 4);
+            });
+            slot = later(4);
         }
+        wait_vmcnt<0>();
+        lds_barrier();  // the ring is free
     }
-    if (tiles > 0 && wr == 0) lds_barrier();  // the other group's last one
-    if constexpr (ADAPT) add_adapters<T, RF, CF>(a, t, wr * RF * 16, t.c0 + wc * CF * 16, acc);
-    store_tile<T, RF, CF>(a, t, wr * RF * 16, t.c0 + wc * CF * 16, acc);
+    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
+    float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
+    if constexpr (ADAPT) {
+        const Adapters<T, RF, CF> ad(a, t, r0, c0);
+        ad.whole_tiles(acc);
+        settle_sums();
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
+            constexpr int i = at.value;
+            if (ad.mixed(i)) ad.mixed_tile(i, ad.id[i], sums, CF * 16 + 4);
+        });
+    } else {
+        settle_sums();
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
+    }
 }
 
 // h[s, r] = scale_a sum_k X[s, k] A_a[r, k] for 16 rows s and 16 r a workgroup:
@@ -608,7 +788,7 @@ Error with_half(ElementType type, const char* name, F f) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-constexpr size_t kWideLds = 2 * 2 * 256 * kStep * 2;  // two buffers of two operands
+constexpr size_t kWideLds = 10 * 128 * kStep * 2;  // ten slots
 
 // Launches the tile kernel for a: the wide one where the operands' rows are whole
 // pieces and `wide` says that its tiles fill.
@@ -628,7 +808,7 @@ Error launch_tiles(const TileArgs& a, bool wide, hipStream_t stream, const char*
             reinterpret_cast<const void*>(tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT>),
             hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kWideLds));
         SPMM_TRY_HIP(grown, name);
-        tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT><<<blocks, 512, kWideLds, stream>>>(a);
+        tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT><<<blocks, 256, kWideLds, stream>>>(a);
     } else {
         tile_product<T, 128, 128, 2, 2, GRAD, COLS_MAJOR, ADAPT><<<blocks, 256, 0, stream>>>(a);
     }
