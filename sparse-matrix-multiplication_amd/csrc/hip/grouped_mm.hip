@@ -33,6 +33,10 @@ using namespace dev;
 
 constexpr int kStep = 64;  // contraction steps a staged tile holds
 
+// A byte offset past every buffer's 2^31 - 1 bytes, with room for the 16 that a
+// load adds: it reads zeros.
+constexpr unsigned kAbsent = 0x80000000u;
+
 // A 16-bit element type's operand of one 16x16x32 product.
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -43,22 +47,24 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 // The same into accumulation registers.  Written out because the compiler moves
 // 256 accumulators between the register files instead of leaving them in place.
 // What the compiler would count for its own products is kept by the callers: the
-// operands come from memory reads (which it waits for), or LATE leaves the two
-// wait states that operands written by vector instructions need; sums are read
-// only after settle_sums.
-template <bool LATE = false>
+// operands come from LDS reads (which it waits for), and the sums are read only
+// after settle_sums.
 __device__ __forceinline__ void mfma_in_place(f32x4& c, f16x8 a, f16x8 b) {
-    if constexpr (LATE) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-    else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-template <bool LATE = false>
 __device__ __forceinline__ void mfma_in_place(f32x4& c, bf16x8 a, bf16x8 b) {
-    if constexpr (LATE) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-    else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-__device__ __forceinline__ void settle_sums() {
+// Waits until the last products have left the pipe.  Each sum passes through an
+// (empty) statement behind the wait, so that nothing reads it earlier.
+template <int CF, int RF>
+__device__ __forceinline__ void settle_sums(f32x4 (&acc)[CF][RF]) {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < CF; ++j)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) asm volatile("" : "+a"(acc[j][i]));
     __builtin_amdgcn_sched_barrier(0);
 }
 template <typename T>
@@ -298,97 +304,81 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F f) 
     (f(std::integral_constant<int, I>{}), ...);
 }
 
-// The adapters of a wave's rows (r0 .. of the workgroup's tile, columns c0 ..): the
-// contraction goes on over h against B_a.  Sixteen rows of one adapter take it in
-// place (whole_tiles); sixteen rows of several, or of some with none, get each
-// adapter's part apart, added only to its own rows (mixed_tile), so that no row
-// sees what another's adapter holds, infinities and NaN included.
-template <typename T, int RF, int CF>
+// The adapters of a wave's rows (r0 .. of the workgroup's tile, columns c0 ..), added
+// sixteen rows at a time on their way out: for each adapter among the rows h against
+// B_a, kept only in its own rows, so that no row sees what another's adapter holds,
+// infinities and NaN included.
+//   PIECES: B's rows are whole 16-byte pieces (buffer loads, 32-bit offsets).
+template <typename T, int RF, int CF, bool PIECES>
 struct Adapters {
     const T* h;
     const T* b;
     int      id[RF];  // of row 16 i + (lane & 15), -1 for none
-    int      width, rank, rank32, rows_left;
+    int      width, rank, rank32;
     int      c0;
 
     __device__ __forceinline__ Adapters(const TileArgs& a, const Tile<T>& t, int r0, int first_col)
         : h(static_cast<const T*>(a.h) + static_cast<long long>(t.row0 + r0) * a.rank32),
           b(static_cast<const T*>(a.b)), width(a.width), rank(a.rank), rank32(a.rank32),
-          rows_left(t.rows_here - r0), c0(first_col) {
+          c0(first_col) {
         const int s = threadIdx.x & 15;
 #pragma unroll
         for (int i = 0; i < RF; ++i) {
-            id[i] = i * 16 + s < rows_left ? a.ids[t.row0 + r0 + i * 16 + s] : -1;
+            id[i] = r0 + i * 16 + s < t.rows_here ? a.ids[t.row0 + r0 + i * 16 + s] : -1;
             if (static_cast<unsigned>(id[i]) >= static_cast<unsigned>(a.adapters)) id[i] = -1;
         }
     }
-    __device__ __forceinline__ Operand<T> read_b(int adapter, int j, int k0) const {
-        const int k = k0 + 8 * ((threadIdx.x & 63) >> 4), c = c0 + j * 16 + (threadIdx.x & 15);
-        const int n = c < width ? min(8, rank - k) : 0;
-        const T* p = b + (static_cast<long long>(adapter) * width + c) * rank + k;
-        return __builtin_bit_cast(Operand<T>, n == 8 ? load_piece(p)
-                                              : n <= 0 ? uint4{0, 0, 0, 0} : load_part(p, n));
-    }
-    // rows of other adapters read zeros
-    __device__ __forceinline__ Operand<T> read_h(int i, int mine, int adapter, int k0) const {
-        const T* p = h + static_cast<long long>(i * 16 + (threadIdx.x & 15)) * rank32 + k0 +
-                     8 * ((threadIdx.x & 63) >> 4);
-        return __builtin_bit_cast(Operand<T>, mine == adapter ? load_piece(p) : uint4{0, 0, 0, 0});
-    }
-    // The adapter that all of sixteen rows have (rows past the tile's end are never
-    // stored and may take anything); -1 where there is no such one.
-    __device__ __forceinline__ int of_all(int i) const {
-        const unsigned long long have = __ballot(id[i] >= 0);
-        if (have == 0) return -1;
-        const int first = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(have));
-        const bool here = i * 16 + static_cast<int>(threadIdx.x & 15) < rows_left;
-        return __ballot(here && id[i] != first) == 0 ? first : -1;
-    }
-    __device__ __forceinline__ bool mixed(int i) const {
-        return __ballot(id[i] >= 0) != 0 && of_all(i) < 0;
-    }
-    __device__ __forceinline__ void whole_tiles(f32x4 (&acc)[CF][RF]) const {
-        int of[RF];
+    // B_a's rows c0 .. of an adapter, 32 of the rank from k0 on.
+    __device__ __forceinline__ void read_b(int adapter, int k0, Operand<T> (&fc)[CF]) const {
+        const int k = k0 + 8 * ((threadIdx.x & 63) >> 4), c = c0 + (threadIdx.x & 15);
+        const T* first = b + static_cast<long long>(adapter) * width * rank;
+        if constexpr (PIECES) {
+            const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(first), 0, 0x7fffffff, kBufWord3);
 #pragma unroll
-        for (int i = 0; i < RF; ++i) of[i] = of_all(i);
-        for (;;) {
-            int adapter = -1;
-#pragma unroll
-            for (int i = RF - 1; i >= 0; --i) adapter = of[i] >= 0 ? of[i] : adapter;
-            if (adapter < 0) break;
-            for (int k0 = 0; k0 < rank; k0 += 32) {
-                Operand<T> fr[RF];
-#pragma unroll
-                for (int i = 0; i < RF; ++i) fr[i] = read_h(i, id[i], adapter, k0);
-                unrolled(std::make_integer_sequence<int, CF>{}, [&](auto j) {
-                    const Operand<T> fc = read_b(adapter, j.value, k0);
-                    unrolled(std::make_integer_sequence<int, RF>{}, [&](auto i) {
-                        if (of[i.value] == adapter) {
-                            mfma_in_place<true>(acc[j.value][i.value], fc, fr[i.value]);
-                        }
-                    });
-                });
+            for (int j = 0; j < CF; ++j) {
+                const bool in = c + 16 * j < width && k < rank;
+                fc[j] = __builtin_bit_cast(Operand<T>, __builtin_amdgcn_raw_buffer_load_b128(
+                    buffer, in ? ((c + 16 * j) * rank + k) * 2 : static_cast<int>(kAbsent), 0, 0));
             }
+        } else {
 #pragma unroll
-            for (int i = 0; i < RF; ++i) of[i] = of[i] == adapter ? -1 : of[i];
+            for (int j = 0; j < CF; ++j) {
+                const int n = c + 16 * j < width ? min(8, rank - k) : 0;
+                const T* p = first + static_cast<long long>(c + 16 * j) * rank + k;
+                fc[j] = __builtin_bit_cast(Operand<T>, n == 8 ? load_piece(p)
+                                                       : n <= 0 ? uint4{0, 0, 0, 0}
+                                                                : load_part(p, n));
+            }
         }
     }
-    // sums: the wave's sixteen rows in LDS, `pitch` floats a row.
-    __device__ __forceinline__ void mixed_tile(int i, int mine, float* sums, int pitch) const {
+    // sums: the wave's rows 16 i .. in LDS, `pitch` floats a row; mine: id[i].
+    __device__ __forceinline__ void add(int i, int mine, float* sums, int pitch) const {
         const int lane = threadIdx.x & 63;
         float* at = sums + (lane & 15) * pitch + 4 * (lane >> 4);
+        const T* row = h + (i * 16 + (lane & 15)) * rank32 + 8 * (lane >> 4);
         int left_id = mine;
         for (;;) {
             const unsigned long long left = __ballot(left_id >= 0);
             if (left == 0) break;
             const int adapter = __builtin_amdgcn_readlane(left_id, __builtin_ctzll(left));
-            for (int j = 0; j < CF; ++j) {
-                f32x4 sum = f32x4(0.0f);
-                for (int k0 = 0; k0 < rank; k0 += 32) {
-                    sum = mfma(read_b(adapter, j, k0), read_h(i, mine, adapter, k0), sum);
+            f32x4 sum[CF];
+#pragma unroll
+            for (int j = 0; j < CF; ++j) sum[j] = f32x4(0.0f);
+            for (int k0 = 0; k0 < rank; k0 += 32) {
+                Operand<T> fc[CF];
+                read_b(adapter, k0, fc);
+                const Operand<T> fr = __builtin_bit_cast(
+                    Operand<T>, mine == adapter ? load_piece(row + k0) : uint4{0, 0, 0, 0});
+#pragma unroll
+                for (int j = 0; j < CF; ++j) sum[j] = mfma(fc[j], fr, sum[j]);
+            }
+            if (mine == adapter) {
+#pragma unroll
+                for (int j = 0; j < CF; ++j) {
+                    f32x4* p = reinterpret_cast<f32x4*>(at + 16 * j);
+                    *p = *p + sum[j];
                 }
-                f32x4* p = reinterpret_cast<f32x4*>(at + 16 * j);
-                if (mine == adapter) *p = *p + sum;
             }
             left_id = left_id == adapter ? -1 : left_id;
         }
@@ -402,9 +392,9 @@ constexpr int kStoreFloats = 16 * (CF * 16 + 4);
 
 // Stores a wave's tile, sixteen rows at a time through its own part of LDS (`sums`,
 // free in all waves), so that whole row pieces leave in 16-byte stores.
-template <typename T, int RF, int CF, typename Mixed>
+template <typename T, int RF, int CF, typename Extend>
 __device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, int r0, int c0,
-                                           const f32x4 (&acc)[CF][RF], float* sums, Mixed mixed) {
+                                           const f32x4 (&acc)[CF][RF], float* sums, Extend extend) {
     constexpr int kPitch = CF * 16 + 4, kLanes = CF * 2, kRows = 64 / kLanes;
     const int lane = threadIdx.x & 63;
     const int s = lane & 15, q = lane >> 4;
@@ -417,7 +407,7 @@ __device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, 
             for (int j = 0; j < CF; ++j) {
                 *reinterpret_cast<f32x4*>(sums + s * kPitch + j * 16 + 4 * q) = acc[j][i];
             }
-            mixed(at);
+            extend(at);
 #pragma unroll
             for (int n = 0; n < 16 / kRows; ++n) {
                 const int r = n * kRows + lane / kLanes;
@@ -462,6 +452,7 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_product(TileArgs a) {
 #pragma unroll
         for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
 
+    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
     Rows pr;
     Cols pc;
     pr.place(t.ld_rows, t.rows_here);
@@ -495,26 +486,22 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_product(TileArgs a) {
 #pragma unroll
             for (int j = 0; j < CF; ++j)
 #pragma unroll
-                for (int i = 0; i < RF; ++i) mfma_in_place(acc[j][i], fc[j], fr[i]);
+                for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc[j], fr[i], acc[j][i]);
         }
         if (more) {
             pr.store(rows_at(it + 1), vr);
             pc.store(cols_at(it + 1), vc);
         }
     }
-    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
     lds_barrier();  // the operands' LDS is free
     float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
     if constexpr (ADAPT) {
-        const Adapters<T, RF, CF> ad(a, t, r0, c0);
-        ad.whole_tiles(acc);
-        settle_sums();
+        const Adapters<T, RF, CF, false> ad(a, t, r0, c0);
         store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
             constexpr int i = at.value;
-            if (ad.mixed(i)) ad.mixed_tile(i, ad.id[i], sums, CF * 16 + 4);
+            ad.add(i, ad.id[i], sums, CF * 16 + 4);
         });
     } else {
-        settle_sums();
         store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
     }
 }
@@ -553,7 +540,6 @@ struct Slot {
     __device__ __forceinline__ unsigned offset(int left) const {
         return index + (MAJOR ? 16 * I : 0) < left ? at[I] : kAbsent;
     }
-    static constexpr unsigned kAbsent = 0x80000000u;
 };
 
 // The 256 x 256 tile of large products, for operands whose rows are whole 16-byte
@@ -594,12 +580,13 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
 #pragma unroll
         for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
 
+    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
     const int tiles = (t.depth + kStep - 1) / kStep;
     if (tiles > 0) {
-        ColSlot c0, c1;
+        ColSlot cols0, cols1;
         RowSlot low, high;
-        c0.place(t.ld_cols, 0, a.width - t.c0);
-        c1.place(t.ld_cols, 128, a.width - t.c0);
+        cols0.place(t.ld_cols, 0, a.width - t.c0);
+        cols1.place(t.ld_cols, 128, a.width - t.c0);
         low.place(t.ld_rows, 0, t.rows_here);
         high.place(t.ld_rows, 64, t.rows_here);
         T* const lds = reinterpret_cast<T*>(s_tiles);
@@ -654,17 +641,17 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
-        load_slot(c0, cols, place_of(0));
-        load_slot(c1, cols, place_of(1));
+        load_slot(cols0, cols, place_of(0));
+        load_slot(cols1, cols, place_of(1));
         load_slot(low, rows, place_of(2));
         load_slot(high, rows, place_of(3));
         advance();
-        load_slot(c0, cols, place_of(4));
-        load_slot(c1, cols, place_of(5));
+        load_slot(cols0, cols, place_of(4));
+        load_slot(cols1, cols, place_of(5));
         load_slot(low, rows, place_of(6));
         load_slot(high, rows, place_of(7));
         advance();
-        load_slot(c0, cols, place_of(8));
+        load_slot(cols0, cols, place_of(8));
         wait_vmcnt<24>();  // slots 0, 1, 2
         lds_barrier();
 #pragma unroll
@@ -675,7 +662,7 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
         int slot = 0;  // of this tile's C0
         auto later = [&](int n) { return slot + n < 10 ? slot + n : slot + n - 10; };
         for (int it = 0; it < tiles; ++it) {
-            multiply(0, 0, c1, cols, place_of(later(9)), [&](auto m) {
+            multiply(0, 0, cols1, cols, place_of(later(9)), [&](auto m) {
                 if constexpr (m.value < 8) read_col(later(wc), 1, m.value);
                 else if constexpr (m.value < 12) read_row(later(2), 1, m.value - 8);
             });
@@ -690,79 +677,316 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
             wait_vmcnt<20>();
             lds_barrier();
             advance();
-            multiply(1, 1, c0, cols, place_of(later(2)), [&](auto m) {
+            multiply(1, 1, cols0, cols, place_of(later(2)), [&](auto m) {
                 if constexpr (m.value < 4) read_row(later(6), 0, m.value);
                 else if constexpr (m.value < 12) read_col(later(4 + wc), 0, m.value - 4);
             });
             slot = later(4);
         }
+        settle_sums(acc);
         wait_vmcnt<0>();
         lds_barrier();  // the ring is free
     }
-    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
     float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
     if constexpr (ADAPT) {
-        const Adapters<T, RF, CF> ad(a, t, r0, c0);
-        ad.whole_tiles(acc);
-        settle_sums();
+        const Adapters<T, RF, CF, true> ad(a, t, r0, c0);
         store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
             constexpr int i = at.value;
-            if (ad.mixed(i)) ad.mixed_tile(i, ad.id[i], sums, CF * 16 + 4);
+            ad.add(i, ad.id[i], sums, CF * 16 + 4);
         });
     } else {
-        settle_sums();
         store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
     }
 }
 
-// h[s, r] = scale_a sum_k X[s, k] A_a[r, k] for 16 rows s and 16 r a workgroup:
-// four waves share the contraction, every adapter among the rows takes a turn.
-// h is rounded to the operands' type: it feeds matrix cores again, and its
-// rounding adds less to the result than the result's own (the adapter's part of
-// an output averages `rank` such roundings).
-template <typename T>
-__global__ __launch_bounds__(256) void adapter_shrink(TileArgs a, const T* __restrict__ down,
-                                                      const float* __restrict__ scale,
-                                                      T* __restrict__ h) {
-    __shared__ f32x4 s_part[4][64];
+// Sums of a wave's share of the contraction for CF x 16 columns (rows of `cols`,
+// `width` of them from its first) and RF x 16 rows (of `rows`, `rows_here`), all
+// with `depth` contiguous elements: wave w of WAVES takes every WAVES-th 64 steps.
+// Operands come straight from memory; U times 64 steps' loads are in flight.
+template <typename T, int RF, int CF, int WAVES, int U>
+__device__ __forceinline__ void wave_share(const T* rows, int rows_here, const T* cols, int width,
+                                           int depth, f32x4 (&acc)[CF][RF]) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int s = lane & 15, q = lane >> 4;
-    const int row = blockIdx.x * 16 + s;
-    const int r0  = blockIdx.y * 16;
-    int id = row < a.total ? a.ids[row] : -1;
-    if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.adapters)) id = -1;
-    const T* x = static_cast<const T*>(a.rows) + static_cast<long long>(row) * a.depth;
-    int left_id = id;
-    for (;;) {
-        const unsigned long long left = __ballot(left_id >= 0);
-        if (left == 0) break;
-        const int mine = __builtin_amdgcn_readlane(left_id, __builtin_ctzll(left));
-        const T* d = down + (static_cast<long long>(mine) * a.rank + r0 + s) * a.depth;
-        f32x4 acc = f32x4(0.0f);
-        for (int k = wave * 32 + 8 * q; k < (a.depth + 31) / 32 * 32 + 8 * q; k += 128) {
-            const int n = min(8, a.depth - k);
-            uint4 vx = {0, 0, 0, 0}, va = {0, 0, 0, 0};
-            if (n > 0) {
-                if (id == mine) vx = n == 8 ? load_piece(x + k) : load_part(x + k, n);
-                if (r0 + s < a.rank) va = n == 8 ? load_piece(d + k) : load_part(d + k, n);
-            }
-            acc = mfma(__builtin_bit_cast(Operand<T>, va), __builtin_bit_cast(Operand<T>, vx), acc);
-        }
-        s_part[wave][lane] = acc;
-        __syncthreads();
-        if (wave == 0 && id == mine) {
-            const float f = scale != nullptr ? scale[mine] : 1.0f;
-            T e[4];
+    // a row past the end reads the first one: its products are never stored
+    const T* pr[RF];
+    const T* pc[CF];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e[i] = static_cast<T>(f * ((s_part[0][lane][i] + s_part[1][lane][i]) +
-                                           (s_part[2][lane][i] + s_part[3][lane][i])));
+    for (int i = 0; i < RF; ++i) {
+        const int r = i * 16 + s;
+        pr[i] = rows + static_cast<long long>(r < rows_here ? r : 0) * depth + 8 * q;
+    }
+#pragma unroll
+    for (int j = 0; j < CF; ++j) {
+        const int c = j * 16 + s;
+        pc[j] = cols + static_cast<long long>(c < width ? c : 0) * depth + 8 * q;
+    }
+    int k = wave * 64;
+    for (; k + (U - 1) * WAVES * 64 + 64 <= depth; k += U * WAVES * 64) {
+        uint4 vr[2 * U][RF], vc[2 * U][CF];
+#pragma unroll
+        for (int u = 0; u < 2 * U; ++u) {
+            const int at = k + u / 2 * WAVES * 64 + u % 2 * 32;
+#pragma unroll
+            for (int j = 0; j < CF; ++j) vc[u][j] = load_piece(pc[j] + at);
+#pragma unroll
+            for (int i = 0; i < RF; ++i) vr[u][i] = load_piece(pr[i] + at);
+        }
+#pragma unroll
+        for (int u = 0; u < 2 * U; ++u)
+#pragma unroll
+            for (int j = 0; j < CF; ++j)
+#pragma unroll
+                for (int i = 0; i < RF; ++i) {
+                    acc[j][i] = mfma(__builtin_bit_cast(Operand<T>, vc[u][j]),
+                                     __builtin_bit_cast(Operand<T>, vr[u][i]), acc[j][i]);
+                }
+    }
+    for (; k < depth; k += WAVES * 64) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int at = k + 32 * half;
+            const int n = min(8, depth - at - 8 * q);
+            auto read = [&](const T* p) {
+                return __builtin_bit_cast(Operand<T>, n == 8 ? load_piece(p + at)
+                                                      : n <= 0 ? uint4{0, 0, 0, 0}
+                                                               : load_part(p + at, n));
+            };
+            Operand<T> fr[RF];
+#pragma unroll
+            for (int i = 0; i < RF; ++i) fr[i] = read(pr[i]);
+#pragma unroll
+            for (int j = 0; j < CF; ++j) {
+                const Operand<T> fc = read(pc[j]);
+#pragma unroll
+                for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc, fr[i], acc[j][i]);
             }
-            __builtin_memcpy(h + static_cast<long long>(row) * a.rank32 + r0 + 4 * q, e, 8);
+        }
+    }
+}
+
+// wave_share for operands whose rows are whole 16-byte pieces (the same sums in the
+// same order): a wave's pieces go through a ring of D stages of LDS of its own (no
+// barriers).  A load then brings eight rows' whole cache lines; operands read
+// straight from memory are 64 bytes of sixteen rows, which the cache serves at a
+// third of the rate (48 rows by 16 columns of 4096 steps: 17 us against 9).
+//   ring: WAVES x D x (RF + CF) x 2 KB.
+template <typename T, int RF, int CF, int WAVES, int D>
+__device__ __forceinline__ void ring_share(char* ring, const T* rows, int rows_here, const T* cols,
+                                           int width, int depth, f32x4 (&acc)[CF][RF]) {
+    constexpr int kLoads = 2 * (RF + CF), kStage = kLoads * 1024;
+    static_assert(kLoads * (D - 1) < 64, "vmcnt is 6 bits");
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int s = lane & 15, q = lane >> 4;
+    // load i brings rows 8 i .. 8 i + 7; piece p of a row is at place p ^ (row & 7)
+    const int piece = (lane & 7) ^ (lane >> 3);
+    unsigned at_col[2 * CF], at_row[2 * RF];
+#pragma unroll
+    for (int i = 0; i < 2 * CF; ++i) {
+        const int n = 8 * i + (lane >> 3);
+        at_col[i] = n < width ? static_cast<unsigned>(n * depth + piece * 8) * 2u : kAbsent;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * RF; ++i) {
+        const int n = 8 * i + (lane >> 3);
+        at_row[i] = n < rows_here ? static_cast<unsigned>(n * depth + piece * 8) * 2u : kAbsent;
+    }
+    const unsigned lds0 = lds_address(ring) + wave * D * kStage;
+    const char* own = ring + wave * D * kStage;
+    const int stages = ((depth + 63) / 64 - wave + WAVES - 1) / WAVES;  // may be 0
+    auto load = [&](int n, int slot) {
+        const int k = (n * WAVES + wave) * 64;
+        const bool in = piece * 8 < depth - k;  // past the end: zeros
+        const u32x4 bc = buffer_words(cols + k, 0, 0x7fffffff);
+        const u32x4 br = buffer_words(rows + k, 0, 0x7fffffff);
+        unrolled(std::make_integer_sequence<int, 2 * CF>{}, [&](auto i) {
+            lds_dma_raw_to<i.value * 1024>(lds0 + slot * kStage);
+            asm volatile("s_nop 0");
+            lds_dma_raw_x4(bc, in ? at_col[i.value] : kAbsent);
+        });
+        unrolled(std::make_integer_sequence<int, 2 * RF>{}, [&](auto i) {
+            lds_dma_raw_to<(2 * CF + i.value) * 1024>(lds0 + slot * kStage);
+            asm volatile("s_nop 0");
+            lds_dma_raw_x4(br, in ? at_row[i.value] : kAbsent);
+        });
+    };
+#pragma unroll
+    for (int n = 0; n < D - 1; ++n) load(n, n);
+    int slot = 0, to = D - 1;
+    for (int n = 0; n < stages; ++n) {
+        load(n + D - 1, to);
+        wait_vmcnt<kLoads * (D - 1)>();
+        asm volatile("" ::: "memory");  // reads below, not before
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            Operand<T> fr[RF], fc[CF];
+            auto read = [&](int tile) {
+                return *reinterpret_cast<const Operand<T>*>(
+                    own + slot * kStage + tile * 2048 + s * 128 + ((4 * half + q) ^ (s & 7)) * 16);
+            };
+#pragma unroll
+            for (int j = 0; j < CF; ++j) fc[j] = read(j);
+#pragma unroll
+            for (int i = 0; i < RF; ++i) fr[i] = read(CF + i);
+#pragma unroll
+            for (int j = 0; j < CF; ++j)
+#pragma unroll
+                for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc[j], fr[i], acc[j][i]);
+        }
+        // the slot's reads are done before the next load may overwrite it
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        slot = slot + 1 < D ? slot + 1 : 0;
+        to   = to + 1 < D ? to + 1 : 0;
+    }
+    wait_vmcnt<0>();
+}
+
+// Adds the waves' shares up in LDS in a fixed order: afterwards total(c, r) is the
+// sum for column c and row r of the workgroup's tile.
+template <int RF, int CF, int WAVES>
+struct Shares {
+    static constexpr int kBytes = WAVES * CF * RF * 1024;
+    float (*parts)[CF][RF][64][4];
+    __device__ __forceinline__ explicit Shares(char* lds)
+        : parts(reinterpret_cast<float (*)[CF][RF][64][4]>(lds)) {}
+    __device__ __forceinline__ void put(const f32x4 (&acc)[CF][RF]) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int j = 0; j < CF; ++j)
+#pragma unroll
+            for (int i = 0; i < RF; ++i) *reinterpret_cast<f32x4*>(parts[wave][j][i][lane]) = acc[j][i];
+    }
+    __device__ __forceinline__ float total(int c, int r) const {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            sum += parts[w][c / 16][r / 16][(c % 16) / 4 * 16 + r % 16][c % 4];
+        }
+        return sum;
+    }
+};
+
+// h[s, r] = scale_a sum_k X[s, k] A_a[r, k] for RF x 16 rows s and CF x 16 r a
+// workgroup, whose eight waves share the contraction.  h is rounded to the operands'
+// type: it feeds matrix cores again, and its rounding adds less to the result than
+// the result's own (the adapter's part of an output averages `rank` such roundings).
+//   LEADER: one workgroup a row; it works only if its row is the first of its
+//   sixteen with this adapter, for all of those that have it.  So few rows with an
+//   adapter each still spread over the chip.  Otherwise the workgroup takes the
+//   adapters of its rows in turn.
+//   D: stages of ring_share; 0: wave_share, for rows that are no whole pieces.
+template <typename T, int RF, int CF, int WAVES, int D, bool LEADER>
+__global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T* __restrict__ down,
+                                                             const float* __restrict__ scale,
+                                                             T* __restrict__ h) {
+    static_assert(!LEADER || RF == 1, "sixteen rows");
+    extern __shared__ __attribute__((aligned(16))) char s_ring[];  // and then the shares
+    __shared__ int s_id[RF * 16];
+    const int lane = threadIdx.x & 63;
+    const int row0 = (LEADER ? blockIdx.x / 16 : blockIdx.x) * RF * 16;
+    const int r0   = blockIdx.y * CF * 16;
+    const int rows_here = min(RF * 16, a.total - row0);
+    // every wave looks at all the rows' adapters
+    int id = lane < rows_here ? a.ids[row0 + lane] : -1;
+    if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.adapters)) id = -1;
+    if (threadIdx.x < RF * 16) s_id[threadIdx.x] = id;
+    unsigned long long left = __ballot(id >= 0);
+    if constexpr (LEADER) {
+        const int mine = __builtin_amdgcn_readlane(id, blockIdx.x % 16);
+        const unsigned long long same = __ballot(id == mine && lane < 16);
+        if (mine < 0 || __builtin_ctzll(same) != static_cast<int>(blockIdx.x % 16)) return;
+        left = 1ull << (blockIdx.x % 16);
+    }
+    while (left != 0) {
+        const int mine = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        f32x4 acc[CF][RF];
+#pragma unroll
+        for (int j = 0; j < CF; ++j)
+#pragma unroll
+            for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
+        const T* x = static_cast<const T*>(a.rows) + static_cast<long long>(row0) * a.depth;
+        const T* d = down + (static_cast<long long>(mine) * a.rank + r0) * a.depth;
+        if constexpr (D > 0) {
+            ring_share<T, RF, CF, WAVES, D>(s_ring, x, rows_here, d, a.rank - r0, a.depth, acc);
+            __syncthreads();
+        } else {
+            wave_share<T, RF, CF, WAVES, 2>(x, rows_here, d, a.rank - r0, a.depth, acc);
+        }
+        Shares<RF, CF, WAVES> shares(s_ring);
+        shares.put(acc);
+        __syncthreads();
+        const float f = scale != nullptr ? scale[mine] : 1.0f;
+        for (int e = threadIdx.x; e < RF * 16 * CF * 16; e += WAVES * 64) {
+            const int s = e / (CF * 16), r = e % (CF * 16);
+            if (s_id[s] == mine && r0 + r < a.rank32) {
+                h[static_cast<long long>(row0 + s) * a.rank32 + r0 + r] =
+                    static_cast<T>(r0 + r < a.rank ? f * shares.total(r, s) : 0.0f);
+            }
         }
         __syncthreads();
-        left_id = left_id == mine ? -1 : left_id;
+        left &= ~__ballot(id == mine);
+        if constexpr (LEADER) break;
+    }
+}
+
+// Products of few rows, bound by reading the weights (W [c][k]) once: a workgroup
+// takes CF x 16 columns and up to RF x 16 rows of a group, its eight waves share the
+// contraction, so that a projection of a few thousand columns still has a workgroup
+// a CU.  D: as for adapter_shrink.
+template <typename T, int RF, int CF, int D, bool ADAPT>
+__global__ __launch_bounds__(512) void few_rows_product(TileArgs a) {
+    constexpr int WAVES = 8;
+    extern __shared__ __attribute__((aligned(16))) char s_ring[];  // and then the shares
+    const int col_tiles = (a.width + CF * 16 - 1) / (CF * 16);
+    const RowTile t = find_tile<RF * 16>(a, blockIdx.x / col_tiles);
+    if (t.group < 0) return;
+    const int c0 = blockIdx.x % col_tiles * CF * 16;
+    const int rows_here = t.end - t.first;
+    T* out = static_cast<T*>(a.out) + static_cast<long long>(t.first) * a.width;
+    f32x4 acc[CF][RF];
+#pragma unroll
+    for (int j = 0; j < CF; ++j)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
+    if (t.group < a.groups) {  // rows in no group: zeros
+        const T* x = static_cast<const T*>(a.rows) + static_cast<long long>(t.first) * a.depth;
+        const T* w = static_cast<const T*>(a.cols) +
+                     (static_cast<long long>(t.group) * a.width + c0) * a.depth;
+        if constexpr (D > 0) {
+            ring_share<T, RF, CF, WAVES, D>(s_ring, x, rows_here, w, a.width - c0, a.depth, acc);
+            __syncthreads();
+        } else {
+            wave_share<T, RF, CF, WAVES, 2>(x, rows_here, w, a.width - c0, a.depth, acc);
+        }
+    }
+    Shares<RF, CF, WAVES> shares(s_ring);
+    shares.put(acc);
+    __syncthreads();
+    const int c = threadIdx.x % (CF * 16);
+    if (c0 + c >= a.width) return;
+    for (int s = threadIdx.x / (CF * 16); s < rows_here; s += WAVES * 4 / CF) {
+        float sum = shares.total(c, s);
+        if constexpr (ADAPT) {
+            const int id = a.ids[t.first + s];
+            if (static_cast<unsigned>(id) < static_cast<unsigned>(a.adapters)) {
+                const T* h = static_cast<const T*>(a.h) + static_cast<long long>(t.first + s) * a.rank32;
+                const T* b = static_cast<const T*>(a.b) +
+                             (static_cast<long long>(id) * a.width + c0 + c) * a.rank;
+                float part = 0.0f;
+                for (int k = 0; k < a.rank; k += 8) {
+                    const int n = min(8, a.rank - k);
+                    float x[8], y[8];
+                    piece_to_float<T>(load_piece(h + k), x);
+                    piece_to_float<T>(n == 8 ? load_piece(b + k) : load_part(b + k, n), y);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) part = fmaf(x[i], y[i], part);
+                }
+                sum += part;
+            }
+        }
+        out[static_cast<long long>(s) * a.width + c0 + c] = static_cast<T>(sum);
     }
 }
 
@@ -788,7 +1012,70 @@ Error with_half(ElementType type, const char* name, F f) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-constexpr size_t kWideLds = 10 * 128 * kStep * 2;  // ten slots
+constexpr int kWideLds = 10 * 128 * kStep * 2;  // ten slots
+
+// Launches kernel with `lds` bytes of dynamic LDS, asked for once.
+template <auto kernel, typename... Args>
+Error launch_with_lds(dim3 grid, int threads, int lds, hipStream_t stream, const char* name,
+                      Args... args) {
+    static const hipError_t grown = hipFuncSetAttribute(
+        reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    SPMM_TRY_HIP(grown, name);
+    kernel<<<grid, threads, lds, stream>>>(args...);
+    SPMM_TRY_HIP(hipGetLastError(), name);
+    return Error{};
+}
+
+// Stages of a ring of `waves` waves with a stage of `tiles` x 2 KB within `room`
+// bytes; the waves' shares fit in it too.
+constexpr int ring_depth(int waves, int tiles, int room) {
+    return std::min(8, room / (waves * tiles * 2048));
+}
+
+template <typename T, int RF, int CF, bool ADAPT>
+Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
+    const long long row_tiles = a.offsets == nullptr
+        ? (a.total + RF * 16 - 1) / (RF * 16)
+        : a.total / (RF * 16) + std::min<long long>(a.groups + 1LL, a.total);
+    const long long blocks = row_tiles * ((a.width + CF * 16 - 1) / (CF * 16));
+    if (blocks > 0x7fffffffLL) return Error{kUnsupported, std::string(name) + ": too many tiles"};
+    const dim3 grid(static_cast<unsigned>(blocks));
+    constexpr int shares = Shares<RF, CF, 8>::kBytes;
+    if (!pieces) {
+        return launch_with_lds<few_rows_product<T, RF, CF, 0, ADAPT>>(grid, 512, shares, stream, name, a);
+    }
+    constexpr int depth = ring_depth(8, RF + CF, 160 * 1024);
+    constexpr int lds = std::max(shares, 8 * depth * (RF + CF) * 2048);
+    return launch_with_lds<few_rows_product<T, RF, CF, depth, ADAPT>>(grid, 512, lds, stream, name, a);
+}
+// Launches few_rows_product for groups of up to `rows` rows or so (all are right).
+template <typename T, bool ADAPT>
+Error launch_few_rows(const TileArgs& a, long long rows, bool pieces, hipStream_t stream,
+                      const char* name) {
+    if (rows <= 16) return launch_few_rows_of<T, 1, 1, ADAPT>(a, pieces, stream, name);
+    if (rows <= 32) return launch_few_rows_of<T, 2, 1, ADAPT>(a, pieces, stream, name);
+    if (rows <= 48) return launch_few_rows_of<T, 3, 1, ADAPT>(a, pieces, stream, name);
+    return launch_few_rows_of<T, 4, 1, ADAPT>(a, pieces, stream, name);
+}
+
+template <typename T, int RF, int CF, int WAVES, bool LEADER>
+Error launch_shrink(const TileArgs& a, bool pieces, const void* down, const float* scale,
+                    hipStream_t stream) {
+    // the last columns of h, up to a whole product of 32, are written (zero) too
+    const dim3 grid((a.total + RF * 16 - 1) / (RF * 16) * (LEADER ? 16 : 1),
+                    (a.rank32 + CF * 16 - 1) / (CF * 16));
+    const T* d = static_cast<const T*>(down);
+    T* h = static_cast<T*>(const_cast<void*>(a.h));
+    constexpr int shares = Shares<RF, CF, WAVES>::kBytes;
+    if (!pieces) {
+        return launch_with_lds<adapter_shrink<T, RF, CF, WAVES, 0, LEADER>>(
+            grid, WAVES * 64, shares, stream, "adapter_shrink", a, d, scale, h);
+    }
+    constexpr int depth = ring_depth(WAVES, RF + CF, 160 * 1024 - 1024);
+    constexpr int lds = std::max(shares, WAVES * depth * (RF + CF) * 2048);
+    return launch_with_lds<adapter_shrink<T, RF, CF, WAVES, depth, LEADER>>(
+        grid, WAVES * 64, lds, stream, "adapter_shrink", a, d, scale, h);
+}
 
 // Launches the tile kernel for a: the wide one where the operands' rows are whole
 // pieces and `wide` says that its tiles fill.
@@ -804,14 +1091,10 @@ Error launch_tiles(const TileArgs& a, bool wide, hipStream_t stream, const char*
     const long long blocks = (row_tiles * ((a.width + edge - 1) / edge) + 7) / 8 * 8;
     if (blocks > 0x7fffffffLL) return Error{kUnsupported, std::string(name) + ": too many tiles"};
     if (wide) {
-        static const hipError_t grown = hipFuncSetAttribute(
-            reinterpret_cast<const void*>(tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT>),
-            hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kWideLds));
-        SPMM_TRY_HIP(grown, name);
-        tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT><<<blocks, 256, kWideLds, stream>>>(a);
-    } else {
-        tile_product<T, 128, 128, 2, 2, GRAD, COLS_MAJOR, ADAPT><<<blocks, 256, 0, stream>>>(a);
+        return launch_with_lds<tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT>>(
+            dim3(static_cast<unsigned>(blocks)), 256, kWideLds, stream, name, a);
     }
+    tile_product<T, 128, 128, 2, 2, GRAD, COLS_MAJOR, ADAPT><<<blocks, 256, 0, stream>>>(a);
     SPMM_TRY_HIP(hipGetLastError(), name);
     return Error{};
 }
@@ -837,8 +1120,13 @@ Error launch_grouped_mm(const void* x, const void* w, ElementType type, const in
     a.depth = depth;
     const bool pieces = depth % 8 == 0 && (!w_in_rows || width % 8 == 0) && aligned16(x) && aligned16(w);
     const bool wide = pieces && total >= 192LL * groups && width >= 192;
+    const long long mean = total / std::min(groups, total);
     return with_half(type, "grouped_mm", [&](auto zero) {
         using T = decltype(zero);
+        // twice the mean, so that few groups need a second tile that reads W again
+        if (!w_in_rows && mean <= 32) {
+            return launch_few_rows<T, false>(a, 2 * mean, pieces, stream, "grouped_mm");
+        }
         return w_in_rows ? launch_tiles<T, false, true, false>(a, wide, stream, "grouped_mm")
                          : launch_tiles<T, false, false, false>(a, wide, stream, "grouped_mm");
     });
@@ -899,13 +1187,16 @@ Error launch_adapter_mm(const void* x, const void* w, const void* down, const vo
     a.adapters = adapters;
     a.rank = rank;
     a.rank32 = (rank + 31) / 32 * 32;
-    const bool wide = depth % 8 == 0 && aligned16(x) && aligned16(w) && total >= 192 && width >= 192;
+    const bool pieces = depth % 8 == 0 && aligned16(x) && aligned16(w);
+    const bool wide = pieces && rank % 8 == 0 && aligned16(up) && total >= 192 && width >= 192;
     return with_half(type, "adapter_mm", [&](auto zero) {
         using T = decltype(zero);
-        // whole products of 32: the second half of h's columns is written (zero) too
-        adapter_shrink<T><<<dim3((total + 15) / 16, a.rank32 / 16), 256, 0, stream>>>(
-            a, static_cast<const T*>(down), scale, static_cast<T*>(workspace));
-        SPMM_TRY_HIP(hipGetLastError(), "adapter_shrink");
+        if (total <= 512) {
+            SPMM_TRY((launch_shrink<T, 1, 1, 8, true>(a, pieces && aligned16(down), down, scale, stream)));
+        } else {
+            SPMM_TRY((launch_shrink<T, 2, 4, 4, false>(a, pieces && aligned16(down), down, scale, stream)));
+        }
+        if (total <= 64) return launch_few_rows<T, true>(a, total, pieces, stream, "adapter_mm");
         return launch_tiles<T, false, false, true>(a, wide, stream, "adapter_mm");
     });
 }
