@@ -16,6 +16,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 #include <type_traits>
 #include <utility>
@@ -425,87 +426,6 @@ __device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, 
     });
 }
 
-// GRAD false: a product (rows operand [s][k], columns operand W as COLS_MAJOR
-// says).  GRAD true: a weight gradient (both operands lie along s).
-// ADAPT: with the adapters' extension.
-//
-// tile_product takes any sizes and alignment: pieces go through registers, those
-// at an edge element by element.
-template <typename T, int BR, int BC, int WR, int WC, bool GRAD, bool COLS_MAJOR, bool ADAPT>
-__global__ __launch_bounds__(WR * WC * 64) void tile_product(TileArgs a) {
-    constexpr int THREADS = WR * WC * 64;
-    constexpr int RF = BR / WR / 16, CF = BC / WC / 16;  // 16 x 16 tiles a wave
-    using Rows = Operands<T, BR, GRAD, THREADS>;
-    using Cols = Operands<T, BC, GRAD || COLS_MAJOR, THREADS>;
-    __shared__ __attribute__((aligned(16))) T s_tiles[2 * (BR + BC) * kStep];
-    auto rows_at = [&](int it) { return s_tiles + (it & 1) * BR * kStep; };
-    auto cols_at = [&](int it) { return s_tiles + (2 * BR + (it & 1) * BC) * kStep; };
-
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wr = wave / WC, wc = wave % WC;
-    Tile<T> t;
-    if (!take_tile<T, BR, BC, GRAD, COLS_MAJOR>(a, t)) return;
-
-    f32x4 acc[CF][RF];
-#pragma unroll
-    for (int j = 0; j < CF; ++j)
-#pragma unroll
-        for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
-
-    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
-    Rows pr;
-    Cols pc;
-    pr.place(t.ld_rows, t.rows_here);
-    pc.place(t.ld_cols, a.width - t.c0);
-    const int tiles = (t.depth + kStep - 1) / kStep;
-    uint4 vr[Rows::kPieces], vc[Cols::kPieces];
-    if (tiles > 0) {
-        pr.load(t.rows, t.depth, vr);
-        pc.load(t.cols, t.depth, vc);
-        pr.store(rows_at(0), vr);
-        pc.store(cols_at(0), vc);
-    }
-    for (int it = 0; it < tiles; ++it) {
-        // the tile is written, and the other buffer's readers are done
-        __syncthreads();
-        const bool more = it + 1 < tiles;
-        if (more) {
-            const int left = t.depth - (it + 1) * kStep;
-            pr.load(t.rows + (it + 1) * t.step_rows, left, vr);
-            pc.load(t.cols + (it + 1) * t.step_cols, left, vc);
-        }
-        const T* lr = rows_at(it);
-        const T* lc = cols_at(it);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            Operand<T> fr[RF], fc[CF];
-#pragma unroll
-            for (int i = 0; i < RF; ++i) fr[i] = Rows::read(lr, (wr * RF + i) * 16, half);
-#pragma unroll
-            for (int j = 0; j < CF; ++j) fc[j] = Cols::read(lc, (wc * CF + j) * 16, half);
-#pragma unroll
-            for (int j = 0; j < CF; ++j)
-#pragma unroll
-                for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc[j], fr[i], acc[j][i]);
-        }
-        if (more) {
-            pr.store(rows_at(it + 1), vr);
-            pc.store(cols_at(it + 1), vc);
-        }
-    }
-    lds_barrier();  // the operands' LDS is free
-    float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
-    if constexpr (ADAPT) {
-        const Adapters<T, RF, CF, false> ad(a, t, r0, c0);
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
-            constexpr int i = at.value;
-            ad.add(i, ad.id[i], sums, CF * 16 + 4);
-        });
-    } else {
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
-    }
-}
-
 // How 128 rows (or columns) of an operand's staged tile reach LDS in 16-byte
 // pieces by buffer loads of 256 threads: the places of Operands<T, 128, ...>.
 // Rows n = 64 p + r of the slot are the operand's rows GAP p + r.
@@ -541,6 +461,121 @@ struct Slot {
         return index + (MAJOR ? 16 * I : 0) < left ? at[I] : kAbsent;
     }
 };
+
+// GRAD false: a product (rows operand [s][k], columns operand W as COLS_MAJOR
+// says).  GRAD true: a weight gradient (both operands lie along s).
+// ADAPT: with the adapters' extension.
+//
+// The 128 x 128 tile of medium products, and of any sizes and alignment: four waves
+// take a quarter each, two buffers of 64 steps.  PIECES: the operands' rows are
+// whole 16-byte pieces, which go straight into LDS; otherwise through registers,
+// those at an edge element by element.
+template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT, bool PIECES>
+__global__ __launch_bounds__(256) void tile_product(TileArgs a) {
+    constexpr int BR = 128, BC = 128, WC = 2, RF = 4, CF = 4;
+    using Rows = Operands<T, BR, GRAD, 256>;
+    using Cols = Operands<T, BC, GRAD || COLS_MAJOR, 256>;
+    __shared__ __attribute__((aligned(16))) T s_tiles[2 * (BR + BC) * kStep];
+    auto rows_at = [&](int it) { return s_tiles + (it & 1) * BR * kStep; };
+    auto cols_at = [&](int it) { return s_tiles + (2 * BR + (it & 1) * BC) * kStep; };
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave / WC, wc = wave % WC;
+    Tile<T> t;
+    if (!take_tile<T, BR, BC, GRAD, COLS_MAJOR>(a, t)) return;
+
+    f32x4 acc[CF][RF];
+#pragma unroll
+    for (int j = 0; j < CF; ++j)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
+
+    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
+    const int tiles = (t.depth + kStep - 1) / kStep;
+    auto multiply = [&](int it) {
+        const T* lr = rows_at(it);
+        const T* lc = cols_at(it);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            Operand<T> fr[RF], fc[CF];
+#pragma unroll
+            for (int i = 0; i < RF; ++i) fr[i] = Rows::read(lr, (wr * RF + i) * 16, half);
+#pragma unroll
+            for (int j = 0; j < CF; ++j) fc[j] = Cols::read(lc, (wc * CF + j) * 16, half);
+#pragma unroll
+            for (int j = 0; j < CF; ++j)
+#pragma unroll
+                for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc[j], fr[i], acc[j][i]);
+        }
+    };
+    if constexpr (PIECES) {
+        Slot<T, GRAD, 64> pr;
+        Slot<T, GRAD || COLS_MAJOR, 64> pc;
+        pr.place(t.ld_rows, 0, t.rows_here);
+        pc.place(t.ld_cols, 0, a.width - t.c0);
+        auto load = [&](int it) {
+            const u32x4 br = buffer_words(t.rows + it * t.step_rows, 0, 0x7fffffff);
+            const u32x4 bc = buffer_words(t.cols + it * t.step_cols, 0, 0x7fffffff);
+            const unsigned lr = lds_address(rows_at(it)) + wave * 1024;
+            const unsigned lc = lds_address(cols_at(it)) + wave * 1024;
+            const int left = t.depth - it * kStep;
+            unrolled(std::make_integer_sequence<int, 4>{}, [&](auto i) {
+                lds_dma_raw_to<i.value * 4096>(lr);
+                asm volatile("s_nop 0");
+                lds_dma_raw_x4(br, pr.template offset<i.value>(left));
+                lds_dma_raw_to<i.value * 4096>(lc);
+                asm volatile("s_nop 0");
+                lds_dma_raw_x4(bc, pc.template offset<i.value>(left));
+            });
+        };
+        if (tiles > 0) load(0);
+        for (int it = 0; it < tiles; ++it) {
+            // every wave's pieces are there, and the other buffer's readers are done
+            wait_vmcnt<0>();
+            lds_barrier();
+            if (it + 1 < tiles) load(it + 1);
+            multiply(it);
+        }
+    } else {
+        Rows pr;
+        Cols pc;
+        pr.place(t.ld_rows, t.rows_here);
+        pc.place(t.ld_cols, a.width - t.c0);
+        uint4 vr[Rows::kPieces], vc[Cols::kPieces];
+        if (tiles > 0) {
+            pr.load(t.rows, t.depth, vr);
+            pc.load(t.cols, t.depth, vc);
+            pr.store(rows_at(0), vr);
+            pc.store(cols_at(0), vc);
+        }
+        for (int it = 0; it < tiles; ++it) {
+            // the tile is written, and the other buffer's readers are done
+            __syncthreads();
+            const bool more = it + 1 < tiles;
+            if (more) {
+                const int left = t.depth - (it + 1) * kStep;
+                pr.load(t.rows + (it + 1) * t.step_rows, left, vr);
+                pc.load(t.cols + (it + 1) * t.step_cols, left, vc);
+            }
+            multiply(it);
+            if (more) {
+                pr.store(rows_at(it + 1), vr);
+                pc.store(cols_at(it + 1), vc);
+            }
+        }
+    }
+    lds_barrier();  // the operands' LDS is free
+    float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
+    if constexpr (ADAPT) {
+        const Adapters<T, RF, CF, PIECES> ad(a, t, r0, c0);
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
+            constexpr int i = at.value;
+            ad.add(i, ad.id[i], sums, CF * 16 + 4);
+        });
+    } else {
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
+    }
+}
 
 // The 256 x 256 tile of large products, for operands whose rows are whole 16-byte
 // pieces.  Four waves, one a SIMD, take a quarter of 128 x 128 each; 64 steps of
@@ -872,20 +907,18 @@ struct Shares {
 // workgroup, whose eight waves share the contraction.  h is rounded to the operands'
 // type: it feeds matrix cores again, and its rounding adds less to the result than
 // the result's own (the adapter's part of an output averages `rank` such roundings).
-//   LEADER: one workgroup a row; it works only if its row is the first of its
-//   sixteen with this adapter, for all of those that have it.  So few rows with an
-//   adapter each still spread over the chip.  Otherwise the workgroup takes the
-//   adapters of its rows in turn.
+// The workgroups (x, y, 0 ..) take the adapters among their rows in turn: one each
+// where there are as many of them as rows, so that few rows with an adapter each
+// still spread over the chip.
 //   D: stages of ring_share; 0: wave_share, for rows that are no whole pieces.
-template <typename T, int RF, int CF, int WAVES, int D, bool LEADER>
+template <typename T, int RF, int CF, int WAVES, int D>
 __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T* __restrict__ down,
                                                              const float* __restrict__ scale,
                                                              T* __restrict__ h) {
-    static_assert(!LEADER || RF == 1, "sixteen rows");
     extern __shared__ __attribute__((aligned(16))) char s_ring[];  // and then the shares
     __shared__ int s_id[RF * 16];
     const int lane = threadIdx.x & 63;
-    const int row0 = (LEADER ? blockIdx.x / 16 : blockIdx.x) * RF * 16;
+    const int row0 = blockIdx.x * RF * 16;
     const int r0   = blockIdx.y * CF * 16;
     const int rows_here = min(RF * 16, a.total - row0);
     // every wave looks at all the rows' adapters
@@ -893,14 +926,15 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T
     if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.adapters)) id = -1;
     if (threadIdx.x < RF * 16) s_id[threadIdx.x] = id;
     unsigned long long left = __ballot(id >= 0);
-    if constexpr (LEADER) {
-        const int mine = __builtin_amdgcn_readlane(id, blockIdx.x % 16);
-        const unsigned long long same = __ballot(id == mine && lane < 16);
-        if (mine < 0 || __builtin_ctzll(same) != static_cast<int>(blockIdx.x % 16)) return;
-        left = 1ull << (blockIdx.x % 16);
-    }
+    int skip = blockIdx.z;
     while (left != 0) {
         const int mine = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        left &= ~__ballot(id == mine);
+        if (skip > 0) {
+            --skip;
+            continue;
+        }
+        skip = gridDim.z - 1;
         f32x4 acc[CF][RF];
 #pragma unroll
         for (int j = 0; j < CF; ++j)
@@ -926,18 +960,15 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T
             }
         }
         __syncthreads();
-        left &= ~__ballot(id == mine);
-        if constexpr (LEADER) break;
     }
 }
 
 // Products of few rows, bound by reading the weights (W [c][k]) once: a workgroup
-// takes CF x 16 columns and up to RF x 16 rows of a group, its eight waves share the
+// takes CF x 16 columns and up to RF x 16 rows of a group, its waves share the
 // contraction, so that a projection of a few thousand columns still has a workgroup
 // a CU.  D: as for adapter_shrink.
-template <typename T, int RF, int CF, int D, bool ADAPT>
-__global__ __launch_bounds__(512) void few_rows_product(TileArgs a) {
-    constexpr int WAVES = 8;
+template <typename T, int RF, int CF, int WAVES, int D, bool ADAPT>
+__global__ __launch_bounds__(WAVES * 64) void few_rows_product(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char s_ring[];  // and then the shares
     const int col_tiles = (a.width + CF * 16 - 1) / (CF * 16);
     const RowTile t = find_tile<RF * 16>(a, blockIdx.x / col_tiles);
@@ -1032,7 +1063,7 @@ constexpr int ring_depth(int waves, int tiles, int room) {
     return std::min(8, room / (waves * tiles * 2048));
 }
 
-template <typename T, int RF, int CF, bool ADAPT>
+template <typename T, int RF, int CF, int WAVES, int ROOM, bool ADAPT>
 Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
     const long long row_tiles = a.offsets == nullptr
         ? (a.total + RF * 16 - 1) / (RF * 16)
@@ -1040,48 +1071,104 @@ Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, con
     const long long blocks = row_tiles * ((a.width + CF * 16 - 1) / (CF * 16));
     if (blocks > 0x7fffffffLL) return Error{kUnsupported, std::string(name) + ": too many tiles"};
     const dim3 grid(static_cast<unsigned>(blocks));
-    constexpr int shares = Shares<RF, CF, 8>::kBytes;
+    constexpr int shares = Shares<RF, CF, WAVES>::kBytes;
     if (!pieces) {
-        return launch_with_lds<few_rows_product<T, RF, CF, 0, ADAPT>>(grid, 512, shares, stream, name, a);
+        return launch_with_lds<few_rows_product<T, RF, CF, WAVES, 0, ADAPT>>(
+            grid, WAVES * 64, shares, stream, name, a);
     }
-    constexpr int depth = ring_depth(8, RF + CF, 160 * 1024);
-    constexpr int lds = std::max(shares, 8 * depth * (RF + CF) * 2048);
-    return launch_with_lds<few_rows_product<T, RF, CF, depth, ADAPT>>(grid, 512, lds, stream, name, a);
+    constexpr int depth = ring_depth(WAVES, RF + CF, ROOM);
+    constexpr int lds = std::max(shares, WAVES * depth * (RF + CF) * 2048);
+    return launch_with_lds<few_rows_product<T, RF, CF, WAVES, depth, ADAPT>>(
+        grid, WAVES * 64, lds, stream, name, a);
 }
-// Launches few_rows_product for groups of up to `rows` rows or so (all are right).
+// Launches few_rows_product, its tiles for groups of `rows` rows or so (all are right).
 template <typename T, bool ADAPT>
 Error launch_few_rows(const TileArgs& a, long long rows, bool pieces, hipStream_t stream,
                       const char* name) {
-    if (rows <= 16) return launch_few_rows_of<T, 1, 1, ADAPT>(a, pieces, stream, name);
-    if (rows <= 32) return launch_few_rows_of<T, 2, 1, ADAPT>(a, pieces, stream, name);
-    if (rows <= 48) return launch_few_rows_of<T, 3, 1, ADAPT>(a, pieces, stream, name);
-    return launch_few_rows_of<T, 4, 1, ADAPT>(a, pieces, stream, name);
+    constexpr int kAll = 160 * 1024;
+    const long long row_tiles = a.offsets == nullptr ? (rows + 63) / 64 : a.groups;
+    if (rows > 32 && row_tiles * ((a.width + 63) / 64) >= 192) {
+        // the rows' own traffic counts, and 64 columns share it (2048 rows over 64 groups
+        // of 2048 x 4096: 211 us, 282 with sixteen columns)
+        return launch_few_rows_of<T, 4, 4, 4, 80 * 1024, ADAPT>(a, pieces, stream, name);
+    }
+    if (a.groups > 1 && rows <= 32) {
+        // several workgroups a CU hide each other's beginnings and ends (256 rows over 64
+        // groups of 2048 x 4096: 167 us with three, 227 with one)
+        if (rows <= 16) return launch_few_rows_of<T, 1, 1, 4, 54 * 1024, ADAPT>(a, pieces, stream, name);
+        return launch_few_rows_of<T, 2, 1, 4, 54 * 1024, ADAPT>(a, pieces, stream, name);
+    }
+    // one workgroup a CU or so: all of the LDS for its loads
+    if (rows <= 16) return launch_few_rows_of<T, 1, 1, 8, kAll, ADAPT>(a, pieces, stream, name);
+    if (rows <= 32) return launch_few_rows_of<T, 2, 1, 8, kAll, ADAPT>(a, pieces, stream, name);
+    if (rows <= 48) return launch_few_rows_of<T, 3, 1, 8, kAll, ADAPT>(a, pieces, stream, name);
+    return launch_few_rows_of<T, 4, 1, 8, kAll, ADAPT>(a, pieces, stream, name);
 }
 
-template <typename T, int RF, int CF, int WAVES, bool LEADER>
-Error launch_shrink(const TileArgs& a, bool pieces, const void* down, const float* scale,
+template <typename T, int RF, int CF, int WAVES, int ROOM>
+Error launch_shrink(const TileArgs& a, bool pieces, const void* down, const float* scale, int turns,
                     hipStream_t stream) {
     // the last columns of h, up to a whole product of 32, are written (zero) too
-    const dim3 grid((a.total + RF * 16 - 1) / (RF * 16) * (LEADER ? 16 : 1),
-                    (a.rank32 + CF * 16 - 1) / (CF * 16));
+    const dim3 grid((a.total + RF * 16 - 1) / (RF * 16), (a.rank32 + CF * 16 - 1) / (CF * 16), turns);
     const T* d = static_cast<const T*>(down);
     T* h = static_cast<T*>(const_cast<void*>(a.h));
     constexpr int shares = Shares<RF, CF, WAVES>::kBytes;
     if (!pieces) {
-        return launch_with_lds<adapter_shrink<T, RF, CF, WAVES, 0, LEADER>>(
+        return launch_with_lds<adapter_shrink<T, RF, CF, WAVES, 0>>(
             grid, WAVES * 64, shares, stream, "adapter_shrink", a, d, scale, h);
     }
-    constexpr int depth = ring_depth(WAVES, RF + CF, 160 * 1024 - 1024);
+    constexpr int depth = ring_depth(WAVES, RF + CF, ROOM);
     constexpr int lds = std::max(shares, WAVES * depth * (RF + CF) * 2048);
-    return launch_with_lds<adapter_shrink<T, RF, CF, WAVES, depth, LEADER>>(
+    return launch_with_lds<adapter_shrink<T, RF, CF, WAVES, depth>>(
         grid, WAVES * 64, lds, stream, "adapter_shrink", a, d, scale, h);
 }
 
-// Launches the tile kernel for a: the wide one where the operands' rows are whole
-// pieces and `wide` says that its tiles fill.
+// The kernels a product can take: few_rows_product, tile_product through registers
+// or with pieces straight into LDS, tile_product_wide.
+enum class Form { FewRows, Any, Pieces, Wide };
+
+// Estimated microseconds of a form for `row_tiles(edge)` x width tiles of `steps`
+// steps, from measured rates: 64 steps of a 128 x 128 tile take 0.62 us where a CU has
+// one and 0.95 us where it has two (through registers 1.15 us), of a 256 x 256 tile
+// 1.55 us, one a CU; `weights` bytes come at 5.6 TB/s.
+template <typename F>
+double tile_time(Form form, F row_tiles, int width, double steps, double weights) {
+    const int edge = form == Form::Wide ? 256 : 128;
+    const double tiles = row_tiles(edge) * std::ceil(static_cast<double>(width) / edge);
+    const double rounds = std::ceil(steps / kStep);
+    if (form == Form::Wide) {
+        return std::max(std::ceil(tiles / 256) * (6 + 1.55 * rounds), weights / 5.6e6);
+    }
+    const double two = form == Form::Any ? 1.15 : 0.95, one = form == Form::Any ? 1.15 : 0.62;
+    const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
+    const double time = whole * (3 + two * rounds) +
+                        (rest == 0 ? 0 : 3 + (rest <= 256 ? one : two) * rounds);
+    return std::max(time, weights / 5.6e6);
+}
+// The form with the least time; each is right for all sizes that its flag allows.
+Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
+    const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
+    const double mean = a.total / groups;
+    const double weights = 2.0 * groups * a.width * a.depth;
+    // groups of all lengths end, on average, in the middle of a tile
+    auto row_tiles = [&](int edge) {
+        return groups == 1 ? std::ceil(mean / edge) : groups * std::max(1.0, mean / edge + 0.5);
+    };
+    // few_rows_product: 6.3 TB/s of weights, less where the rows' own reading counts, and
+    // 430 TFLOP/s (256 rows over 64 groups of 2048 x 4096: 167 us, tiles 190; 1024 rows:
+    // 206 us, tiles 184); operands that are no whole pieces come at a third of that
+    const double few = 4 + std::max(weights / 6.3e6 * (1 + mean / 64),
+                                    2e-6 * a.total * a.width * a.depth / 430) * (pieces ? 1 : 3);
+    auto time = [&](Form f) { return tile_time(f, row_tiles, a.width, a.depth, weights); };
+    Form best = pieces ? Form::Pieces : Form::Any;
+    if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
+    return few_allowed && few <= time(best) ? Form::FewRows : best;
+}
+
+// Launches the tile kernel of a form.
 template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT>
-Error launch_tiles(const TileArgs& a, bool wide, hipStream_t stream, const char* name) {
-    const int edge = wide ? 256 : 128;
+Error launch_tiles(const TileArgs& a, Form form, hipStream_t stream, const char* name) {
+    const int edge = form == Form::Wide ? 256 : 128;
     // every group may end in a part-filled tile, and so may the rows in no group
     const long long row_tiles =
         GRAD ? static_cast<long long>(a.groups) * ((a.height + edge - 1) / edge)
@@ -1090,11 +1177,15 @@ Error launch_tiles(const TileArgs& a, bool wide, hipStream_t stream, const char*
     // a whole number of workgroups for each XCD
     const long long blocks = (row_tiles * ((a.width + edge - 1) / edge) + 7) / 8 * 8;
     if (blocks > 0x7fffffffLL) return Error{kUnsupported, std::string(name) + ": too many tiles"};
-    if (wide) {
+    if (form == Form::Wide) {
         return launch_with_lds<tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT>>(
             dim3(static_cast<unsigned>(blocks)), 256, kWideLds, stream, name, a);
     }
-    tile_product<T, 128, 128, 2, 2, GRAD, COLS_MAJOR, ADAPT><<<blocks, 256, 0, stream>>>(a);
+    if (form == Form::Pieces) {
+        tile_product<T, GRAD, COLS_MAJOR, ADAPT, true><<<blocks, 256, 0, stream>>>(a);
+    } else {
+        tile_product<T, GRAD, COLS_MAJOR, ADAPT, false><<<blocks, 256, 0, stream>>>(a);
+    }
     SPMM_TRY_HIP(hipGetLastError(), name);
     return Error{};
 }
@@ -1119,16 +1210,14 @@ Error launch_grouped_mm(const void* x, const void* w, ElementType type, const in
     a.width = width;
     a.depth = depth;
     const bool pieces = depth % 8 == 0 && (!w_in_rows || width % 8 == 0) && aligned16(x) && aligned16(w);
-    const bool wide = pieces && total >= 192LL * groups && width >= 192;
-    const long long mean = total / std::min(groups, total);
+    const Form form = choose_form(a, pieces, !w_in_rows);
+    // twice the mean, so that few groups need a second tile that reads W again
+    const long long rows = 2LL * total / std::min(groups, total);
     return with_half(type, "grouped_mm", [&](auto zero) {
         using T = decltype(zero);
-        // twice the mean, so that few groups need a second tile that reads W again
-        if (!w_in_rows && mean <= 32) {
-            return launch_few_rows<T, false>(a, 2 * mean, pieces, stream, "grouped_mm");
-        }
-        return w_in_rows ? launch_tiles<T, false, true, false>(a, wide, stream, "grouped_mm")
-                         : launch_tiles<T, false, false, false>(a, wide, stream, "grouped_mm");
+        if (form == Form::FewRows) return launch_few_rows<T, false>(a, rows, pieces, stream, "grouped_mm");
+        return w_in_rows ? launch_tiles<T, false, true, false>(a, form, stream, "grouped_mm")
+                         : launch_tiles<T, false, false, false>(a, form, stream, "grouped_mm");
     });
 }
 
@@ -1149,10 +1238,15 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
     a.height = height;
     a.width = width;
     const bool pieces = height % 8 == 0 && width % 8 == 0 && aligned16(p) && aligned16(q);
-    const bool wide = pieces && height >= 192 && width >= 192;
+    auto row_tiles = [&](int edge) { return std::ceil(static_cast<double>(height) / edge) * groups; };
+    auto time = [&](Form f) {
+        return tile_time(f, row_tiles, width, static_cast<double>(total) / groups, 0);
+    };
+    const Form form = !pieces ? Form::Any
+                      : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
     return with_half(type, "grouped_outer", [&](auto zero) {
         using T = decltype(zero);
-        return launch_tiles<T, true, true, false>(a, wide, stream, "grouped_outer");
+        return launch_tiles<T, true, true, false>(a, form, stream, "grouped_outer");
     });
 }
 
@@ -1188,16 +1282,20 @@ Error launch_adapter_mm(const void* x, const void* w, const void* down, const vo
     a.rank = rank;
     a.rank32 = (rank + 31) / 32 * 32;
     const bool pieces = depth % 8 == 0 && aligned16(x) && aligned16(w);
-    const bool wide = pieces && rank % 8 == 0 && aligned16(up) && total >= 192 && width >= 192;
+    Form form = choose_form(a, pieces, true);
+    if ((form == Form::Wide || form == Form::Pieces) && (rank % 8 != 0 || !aligned16(up))) {
+        form = Form::Any;
+    }
     return with_half(type, "adapter_mm", [&](auto zero) {
         using T = decltype(zero);
+        const bool whole = pieces && aligned16(down);
         if (total <= 512) {
-            SPMM_TRY((launch_shrink<T, 1, 1, 8, true>(a, pieces && aligned16(down), down, scale, stream)));
+            SPMM_TRY((launch_shrink<T, 1, 1, 8, 159 * 1024>(a, whole, down, scale, std::max(1, std::min(16, adapters)), stream)));
         } else {
-            SPMM_TRY((launch_shrink<T, 2, 4, 4, false>(a, pieces && aligned16(down), down, scale, stream)));
+            SPMM_TRY((launch_shrink<T, 1, 4, 2, 53 * 1024>(a, whole, down, scale, std::max(1, std::min(8, adapters)), stream)));
         }
-        if (total <= 64) return launch_few_rows<T, true>(a, total, pieces, stream, "adapter_mm");
-        return launch_tiles<T, false, false, true>(a, wide, stream, "adapter_mm");
+        if (form == Form::FewRows) return launch_few_rows<T, true>(a, total, pieces, stream, "adapter_mm");
+        return launch_tiles<T, false, false, true>(a, form, stream, "adapter_mm");
     });
 }
 
