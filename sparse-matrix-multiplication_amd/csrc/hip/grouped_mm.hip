@@ -942,7 +942,9 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T
             for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
         const T* x = static_cast<const T*>(a.rows) + static_cast<long long>(row0) * a.depth;
         const T* d = down + (static_cast<long long>(mine) * a.rank + r0) * a.depth;
-        if constexpr (D > 0) {
+        if (r0 >= a.rank) {
+            // only zeros up to rank32
+        } else if constexpr (D > 0) {
             ring_share<T, RF, CF, WAVES, D>(s_ring, x, rows_here, d, a.rank - r0, a.depth, acc);
             __syncthreads();
         } else {
@@ -1081,24 +1083,30 @@ Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, con
     return launch_with_lds<few_rows_product<T, RF, CF, WAVES, depth, ADAPT>>(
         grid, WAVES * 64, lds, stream, name, a);
 }
-// Launches few_rows_product, its tiles for groups of `rows` rows or so (all are right).
+// How few_rows_product is launched for groups of `rows` rows or so (all are right).
+//   Columns: the rows' own reading counts, and 64 columns share it (2048 rows over 64
+//     groups of 2048 x 4096: 211 us, 282 with sixteen columns).
+//   Groups: several workgroups a CU hide each other's beginnings and ends (256 rows over
+//     64 groups of 2048 x 4096: 167 us with three, 227 with one).
+//   Single: a workgroup a CU or so, which has all of the LDS for its loads.
+enum class Few { Columns, Groups, Single };
+Few few_form(const TileArgs& a, double rows) {
+    const double row_tiles = a.offsets == nullptr ? std::ceil(rows / 64) : a.groups;
+    if (rows > 32 && row_tiles * std::ceil(a.width / 64.0) >= 192) return Few::Columns;
+    return a.groups > 1 && rows <= 32 ? Few::Groups : Few::Single;
+}
 template <typename T, bool ADAPT>
 Error launch_few_rows(const TileArgs& a, long long rows, bool pieces, hipStream_t stream,
                       const char* name) {
     constexpr int kAll = 160 * 1024;
-    const long long row_tiles = a.offsets == nullptr ? (rows + 63) / 64 : a.groups;
-    if (rows > 32 && row_tiles * ((a.width + 63) / 64) >= 192) {
-        // the rows' own traffic counts, and 64 columns share it (2048 rows over 64 groups
-        // of 2048 x 4096: 211 us, 282 with sixteen columns)
-        return launch_few_rows_of<T, 4, 4, 4, 80 * 1024, ADAPT>(a, pieces, stream, name);
+    switch (few_form(a, static_cast<double>(rows))) {
+        case Few::Columns:
+            return launch_few_rows_of<T, 4, 4, 4, 80 * 1024, ADAPT>(a, pieces, stream, name);
+        case Few::Groups:
+            if (rows <= 16) return launch_few_rows_of<T, 1, 1, 4, 54 * 1024, ADAPT>(a, pieces, stream, name);
+            return launch_few_rows_of<T, 2, 1, 4, 54 * 1024, ADAPT>(a, pieces, stream, name);
+        case Few::Single: break;
     }
-    if (a.groups > 1 && rows <= 32) {
-        // several workgroups a CU hide each other's beginnings and ends (256 rows over 64
-        // groups of 2048 x 4096: 167 us with three, 227 with one)
-        if (rows <= 16) return launch_few_rows_of<T, 1, 1, 4, 54 * 1024, ADAPT>(a, pieces, stream, name);
-        return launch_few_rows_of<T, 2, 1, 4, 54 * 1024, ADAPT>(a, pieces, stream, name);
-    }
-    // one workgroup a CU or so: all of the LDS for its loads
     if (rows <= 16) return launch_few_rows_of<T, 1, 1, 8, kAll, ADAPT>(a, pieces, stream, name);
     if (rows <= 32) return launch_few_rows_of<T, 2, 1, 8, kAll, ADAPT>(a, pieces, stream, name);
     if (rows <= 48) return launch_few_rows_of<T, 3, 1, 8, kAll, ADAPT>(a, pieces, stream, name);
@@ -1130,20 +1138,20 @@ enum class Form { FewRows, Any, Pieces, Wide };
 // Estimated microseconds of a form for `row_tiles(edge)` x width tiles of `steps`
 // steps, from measured rates: 64 steps of a 128 x 128 tile take 0.62 us where a CU has
 // one and 0.95 us where it has two (through registers 1.15 us), of a 256 x 256 tile
-// 1.55 us, one a CU; `weights` bytes come at 5.6 TB/s.
+// 1.55 us, one a CU; `weights` microseconds is what reading the weights takes.
 template <typename F>
 double tile_time(Form form, F row_tiles, int width, double steps, double weights) {
     const int edge = form == Form::Wide ? 256 : 128;
     const double tiles = row_tiles(edge) * std::ceil(static_cast<double>(width) / edge);
     const double rounds = std::ceil(steps / kStep);
     if (form == Form::Wide) {
-        return std::max(std::ceil(tiles / 256) * (6 + 1.55 * rounds), weights / 5.6e6);
+        return std::max(std::ceil(tiles / 256) * (6 + 1.55 * rounds), weights);
     }
     const double two = form == Form::Any ? 1.15 : 0.95, one = form == Form::Any ? 1.15 : 0.62;
     const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
     const double time = whole * (3 + two * rounds) +
                         (rest == 0 ? 0 : 3 + (rest <= 256 ? one : two) * rounds);
-    return std::max(time, weights / 5.6e6);
+    return std::max(time, weights);
 }
 // The form with the least time; each is right for all sizes that its flag allows.
 Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
@@ -1154,12 +1162,31 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
     auto row_tiles = [&](int edge) {
         return groups == 1 ? std::ceil(mean / edge) : groups * std::max(1.0, mean / edge + 0.5);
     };
-    // few_rows_product: 6.3 TB/s of weights, less where the rows' own reading counts, and
-    // 430 TFLOP/s (256 rows over 64 groups of 2048 x 4096: 167 us, tiles 190; 1024 rows:
-    // 206 us, tiles 184); operands that are no whole pieces come at a third of that
-    const double few = 4 + std::max(weights / 6.3e6 * (1 + mean / 64),
-                                    2e-6 * a.total * a.width * a.depth / 430) * (pieces ? 1 : 3);
-    auto time = [&](Form f) { return tile_time(f, row_tiles, a.width, a.depth, weights); };
+    // few_rows_product reads weights at 6.3 TB/s, less where the rows' own reading counts;
+    // a round of its workgroups takes 2.2 us for 256 steps (64 columns, two a CU) or 1 us
+    // for 512 (sixteen, one a CU).  Operands that are no whole pieces take three times as
+    // long.  Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s,
+    // W [k][c] at 5.8.
+    // (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows 257, 285)
+    const double rows = groups == 1 ? mean : 2 * mean;
+    const double tiles64 = groups == 1 ? std::ceil(mean / 64)
+                                       : groups * std::max(1.0, mean / 64 + 0.5);
+    double few = weights / 6.3e6 * (1 + mean / 160);
+    switch (few_form(a, rows)) {
+        case Few::Columns:
+            few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 64.0) / 512) *
+                                    (2 + 2.2 * std::ceil(a.depth / 256.0)));
+            break;
+        case Few::Single:
+            few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 16.0) / 256) *
+                                    (3 + std::ceil(a.depth / 512.0)));
+            break;
+        case Few::Groups: break;
+    }
+    few = 4 + few * (pieces ? 1 : 3);
+    // adapters that change within sixteen rows hold tiles up
+    const double reading = weights / (few_allowed ? 4.1e6 : 5.8e6) + (a.ids != nullptr ? 8 : 0);
+    auto time = [&](Form f) { return tile_time(f, row_tiles, a.width, a.depth, reading); };
     Form best = pieces ? Form::Pieces : Form::Any;
     if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
     return few_allowed && few <= time(best) ? Form::FewRows : best;

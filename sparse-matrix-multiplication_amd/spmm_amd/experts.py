@@ -30,28 +30,37 @@ _FLOAT = (torch.float32,)
 
 
 def _operand(t, name: str, dtypes, shape, device=None) -> None:
-    """One contiguous operand of the given type and shape (None: any size) on
-    the current device, and on `device` where that is given."""
+    """One contiguous operand of the given types and shape (a tuple, or the number
+    of dimensions) on `device`, or on the current device where that is not given."""
+    try:
+        got = t.shape
+        if (got == shape or len(got) == shape) and t.dtype in dtypes and t.is_contiguous():
+            where = t.device
+            if where == device or (device is None and where.type == "cuda"
+                                   and where.index == torch.cuda.current_device()):
+                return
+    except (AttributeError, TypeError):
+        pass
+    _refuse(t, name, dtypes, shape, device)
+
+
+def _refuse(t, name: str, dtypes, shape, device) -> None:
+    """What is wrong with an operand, as an SpmmError."""
     if not isinstance(t, torch.Tensor):
         raise SpmmError(SPMM_INVALID, f"{name}: expected a torch tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise SpmmError(SPMM_INVALID, f"{name}: must be a cuda tensor (got {t.device})")
-    where = t.device
     if device is None:
-        if where.index != torch.cuda.current_device():
-            raise SpmmError(SPMM_INVALID, f"{name}: on {where}, the current device is "
-                                          f"cuda:{torch.cuda.current_device()}")
-    elif where != device:
-        raise SpmmError(SPMM_INVALID, f"{name}: on {where}, expected {device}")
+        device = torch.device("cuda", torch.cuda.current_device())
+    if t.device != device:
+        raise SpmmError(SPMM_INVALID, f"{name}: on {t.device}, expected {device}")
     if t.dtype not in dtypes:
         want = " or ".join(str(d) for d in dtypes)
         raise SpmmError(SPMM_INVALID, f"{name}: dtype {t.dtype}, expected {want}")
-    got = t.shape
-    if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
-        want = ", ".join("any" if w is None else str(w) for w in shape)
-        raise SpmmError(SPMM_INVALID, f"{name}: shape {tuple(got)}, expected ({want})")
     if not t.is_contiguous():
         raise SpmmError(SPMM_INVALID, f"{name}: must be contiguous (row-major)")
+    want = f"{shape} dimensions" if isinstance(shape, int) else f"shape {tuple(shape)}"
+    raise SpmmError(SPMM_INVALID, f"{name}: shape {tuple(t.shape)}, expected {want}")
 
 
 def _out(t, name: str, dtype, shape, device):
@@ -60,6 +69,11 @@ def _out(t, name: str, dtype, shape, device):
         return torch.empty(shape, dtype=dtype, device=device)
     _operand(t, name, (dtype,), shape, device)
     return t
+
+
+def _rows(t, name: str, rows: int) -> None:
+    if t.shape[0] != rows:
+        raise SpmmError(SPMM_INVALID, f"{name}: {t.shape[0]} rows, expected {rows}")
 
 
 _here = contextlib.nullcontext()
@@ -71,8 +85,9 @@ def _on(stream):
     return _here if stream is None else torch.cuda.stream(stream)
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+def _stream(device) -> int:
+    # the handle alone: torch.cuda.current_stream builds a Stream object around it
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 @dataclass
@@ -117,7 +132,7 @@ def route(logits, k: int, over: str = "chosen", stream=None) -> Routing:
     the entries' order by expert.  Ties go to the lowest expert; -inf is never
     chosen; a NaN is above all numbers and makes its token's weights NaN."""
     over_id = _over_id(over)
-    _operand(logits, "logits", _TYPES, (None, None))
+    _operand(logits, "logits", _TYPES, 2)
     T, E = logits.shape
     k = int(k)
     if not 1 <= k <= E:
@@ -135,7 +150,7 @@ def route(logits, k: int, over: str = "chosen", stream=None) -> Routing:
         _check(L.spmm_c_route(logits.data_ptr(), _TYPES[logits.dtype], T, E, k, over_id,
                               experts.data_ptr(), weights.data_ptr(), offsets.data_ptr(),
                               entries.data_ptr(), slots.data_ptr(),
-                              work.data_ptr() if room else None, _stream()))
+                              work.data_ptr() if room else None, _stream(device)))
     return Routing(experts, weights, offsets, entries, slots, over)
 
 
@@ -143,18 +158,21 @@ def route_backward(logits, routing: Routing, dweights, out=None, stream=None):
     """The gradient of ``route``'s weights with respect to the logits, of the
     logits' type: [T, E]."""
     over_id = _over_id(routing.over)
-    _operand(logits, "logits", _TYPES, (None, None))
+    _operand(logits, "logits", _TYPES, 2)
     T, E = logits.shape
     device = logits.device
-    _operand(routing.weights, "routing.weights", _FLOAT, (T, None), device)
+    _operand(routing.weights, "routing.weights", _FLOAT, 2, device)
     k = routing.weights.shape[1]
+    if routing.weights.shape[0] != T or not 1 <= k <= E:
+        raise SpmmError(SPMM_INVALID, f"routing: of {tuple(routing.weights.shape)} choices, "
+                                      f"logits are {tuple(logits.shape)}")
     _operand(routing.experts, "routing.experts", _INT, (T, k), device)
     _operand(dweights, "dweights", _FLOAT, (T, k), device)
     with _on(stream):
         out = _out(out, "out", logits.dtype, (T, E), device)
         _check(lib().spmm_c_route_backward(
             logits.data_ptr(), _TYPES[logits.dtype], T, E, k, over_id, routing.experts.data_ptr(),
-            routing.weights.data_ptr(), dweights.data_ptr(), out.data_ptr(), _stream()))
+            routing.weights.data_ptr(), dweights.data_ptr(), out.data_ptr(), _stream(device)))
     return out
 
 
@@ -178,14 +196,15 @@ def group_entries(ids, groups: int, stream=None):
         work = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         _check(L.spmm_c_group_entries(ids.data_ptr(), n, groups, offsets.data_ptr(),
                                       entries.data_ptr(), slots.data_ptr(),
-                                      work.data_ptr() if room else None, _stream()))
+                                      work.data_ptr() if room else None, _stream(device)))
     return offsets, entries, slots
 
 
 def dispatch(x, routing: Routing, out=None, stream=None):
     """Rows of x [T, D] into expert order: [T * k, D]; rows without an entry are zero."""
     T, k, E = routing._sizes()
-    _operand(x, "x", _TYPES, (T, None))
+    _operand(x, "x", _TYPES, 2)
+    _rows(x, "x", T)
     D, device = x.shape[1], x.device
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
     _operand(routing.offsets, "routing.offsets", _INT, (E + 1,), device)
@@ -193,13 +212,14 @@ def dispatch(x, routing: Routing, out=None, stream=None):
         out = _out(out, "out", x.dtype, (T * k, D), device)
         _check(lib().spmm_c_dispatch(x.data_ptr(), _TYPES[x.dtype], T, k, D,
                                      routing.slots.data_ptr(), routing.offsets.data_ptr(), E,
-                                     out.data_ptr(), _stream()))
+                                     out.data_ptr(), _stream(device)))
     return out
 
 
 def _gather(ys, name: str, routing: Routing, weighted: bool, out, stream):
     T, k, _ = routing._sizes()
-    _operand(ys, name, _TYPES, (T * k, None))
+    _operand(ys, name, _TYPES, 2)
+    _rows(ys, name, T * k)
     D, device = ys.shape[1], ys.device
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
     if weighted:
@@ -209,7 +229,7 @@ def _gather(ys, name: str, routing: Routing, weighted: bool, out, stream):
         _check(lib().spmm_c_combine(ys.data_ptr(), _TYPES[ys.dtype], T, k, D,
                                     routing.slots.data_ptr(),
                                     routing.weights.data_ptr() if weighted else None,
-                                    out.data_ptr(), _stream()))
+                                    out.data_ptr(), _stream(device)))
     return out
 
 
@@ -226,7 +246,8 @@ def combine(ys, routing: Routing, out=None, stream=None):
 def combine_backward(dy, ys, routing: Routing, stream=None):
     """The gradients of ``combine`` for dy [T, D]: (dys [T * k, D], dweights fp32 [T, k])."""
     T, k, E = routing._sizes()
-    _operand(ys, "ys", _TYPES, (T * k, None))
+    _operand(ys, "ys", _TYPES, 2)
+    _rows(ys, "ys", T * k)
     D, device = ys.shape[1], ys.device
     _operand(dy, "dy", (ys.dtype,), (T, D), device)
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
@@ -238,51 +259,60 @@ def combine_backward(dy, ys, routing: Routing, stream=None):
         _check(lib().spmm_c_combine_backward(
             dy.data_ptr(), ys.data_ptr(), _TYPES[ys.dtype], T, k, D, routing.slots.data_ptr(),
             routing.weights.data_ptr(), routing.offsets.data_ptr(), E, dys.data_ptr(),
-            dweights.data_ptr(), _stream()))
+            dweights.data_ptr(), _stream(device)))
     return dys, dweights
 
 
 _HALF = (torch.float16, torch.bfloat16)
 
 
-def _half(t, name: str, shape) -> None:
+def _half(t, name: str) -> None:
     if isinstance(t, torch.Tensor) and t.dtype == torch.float32:
         raise SpmmError(SPMM_UNSUPPORTED, f"{name}: float16 or bfloat16 (matrix cores)")
-    _operand(t, name, _HALF, shape)
+    _operand(t, name, _HALF, 2)
+
+
+def _weights(w, dtype, K: int, w_in_rows: bool, device):
+    """(G, N) of weights [G, N, K], or [G, K, N] with w_in_rows."""
+    _operand(w, "w", (dtype,), 3, device)
+    G, n, k = w.shape
+    if w_in_rows:
+        n, k = k, n
+    if k != K:
+        raise SpmmError(SPMM_INVALID, f"w: shape {tuple(w.shape)} for rows of {K} elements")
+    return G, n
 
 
 def grouped_mm(x, w, offsets, w_in_rows: bool = False, out=None, stream=None):
     """Rows of x [S, K] times their group's weights: [S, N].  Group g has rows
     offsets[g] to offsets[g + 1] (int32 [G + 1]); w is [G, N, K], or [G, K, N] with
     w_in_rows.  Rows in no group are zero."""
-    _half(x, "x", (None, None))
+    _half(x, "x")
     S, K = x.shape
     device = x.device
-    _operand(w, "w", (x.dtype,), (None, K, None) if w_in_rows else (None, None, K), device)
-    G, N = w.shape[0], w.shape[2 if w_in_rows else 1]
+    G, N = _weights(w, x.dtype, K, w_in_rows, device)
     _operand(offsets, "offsets", _INT, (G + 1,), device)
     with _on(stream):
         out = _out(out, "out", x.dtype, (S, N), device)
         _check(lib().spmm_c_grouped_mm(x.data_ptr(), w.data_ptr(), _TYPES[x.dtype],
                                        offsets.data_ptr(), G, S, N, K, int(bool(w_in_rows)),
-                                       out.data_ptr(), _stream()))
+                                       out.data_ptr(), _stream(device)))
     return out
 
 
 def grouped_mm_backward(dy, x, w, offsets, w_in_rows: bool = False, stream=None):
     """The gradients of ``grouped_mm`` for dy [S, N]: (dx [S, K], dw like w)."""
-    _half(x, "x", (None, None))
+    _half(x, "x")
     S, K = x.shape
     device = x.device
-    _operand(w, "w", (x.dtype,), (None, K, None) if w_in_rows else (None, None, K), device)
-    G, N = w.shape[0], w.shape[2 if w_in_rows else 1]
+    G, N = _weights(w, x.dtype, K, w_in_rows, device)
     _operand(dy, "dy", (x.dtype,), (S, N), device)
     _operand(offsets, "offsets", _INT, (G + 1,), device)
     p, q, height, width = (x, dy, K, N) if w_in_rows else (dy, x, N, K)
     with _on(stream):
         dw = torch.empty_like(w)
         dx = torch.empty_like(x)
-        L, s = lib(), _stream()
+        L, s = lib(), _stream(device)
         _check(L.spmm_c_grouped_mm(dy.data_ptr(), w.data_ptr(), _TYPES[x.dtype],
                                    offsets.data_ptr(), G, S, K, N, int(not w_in_rows),
                                    dx.data_ptr(), s))
@@ -299,13 +329,15 @@ def adapter_mm(x, w, a, b, ids, scale=None, out=None, stream=None):
     x [T, K], w [N, K], a [L, R, K], b [L, N, R], float16 or bfloat16; ids int32
     [T]; scale float32 [L], 1 when None.  Adapters of a smaller rank are padded
     with zeros."""
-    _half(x, "x", (None, None))
+    _half(x, "x")
     T, K = x.shape
     device = x.device
-    _operand(w, "w", (x.dtype,), (None, K), device)
+    _operand(w, "w", (x.dtype,), 2, device)
     N = w.shape[0]
-    _operand(a, "a", (x.dtype,), (None, None, K), device)
+    _operand(w, "w", (x.dtype,), (N, K), device)
+    _operand(a, "a", (x.dtype,), 3, device)
     L, R = a.shape[:2]
+    _operand(a, "a", (x.dtype,), (L, R, K), device)
     _operand(b, "b", (x.dtype,), (L, N, R), device)
     _operand(ids, "ids", _INT, (T,), device)
     if scale is not None:
@@ -318,5 +350,5 @@ def adapter_mm(x, w, a, b, ids, scale=None, out=None, stream=None):
         _check(library.spmm_c_adapter_mm(
             x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
             None if scale is None else scale.data_ptr(), _TYPES[x.dtype], T, N, K, L, R,
-            out.data_ptr(), work.data_ptr(), _stream()))
+            out.data_ptr(), work.data_ptr(), _stream(device)))
     return out
