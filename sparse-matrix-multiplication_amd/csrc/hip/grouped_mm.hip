@@ -98,8 +98,8 @@ __device__ __forceinline__ int row_bound(const TileArgs& a, int i) {
 }
 
 // The row tiles of all groups, counted group by group; past the last group come
-// the tiles of the rows in no group (group = groups).  Lane i looks at group i of
-// each 64.
+// the tiles of the rows in no group, those behind the last (group = groups) and
+// those before the first (group = groups + 1).  Lane i looks at group i of each 64.
 struct RowTile {
     int group, first, end;  // rows [first, end), end <= first + BR; group < 0: no such tile
 };
@@ -108,13 +108,15 @@ __device__ __forceinline__ void group_rows(const TileArgs& a, int g, int& lo, in
     if (g <= a.groups) {
         lo = row_bound(a, g);
         hi = g < a.groups ? max(row_bound(a, g + 1), lo) : a.total;
+    } else if (g == a.groups + 1) {
+        hi = row_bound(a, 0);
     }
 }
 template <int BR>
 __device__ __forceinline__ int count_tiles(const TileArgs& a) {
     if (a.offsets == nullptr) return (a.total + BR - 1) / BR;
     int tiles = 0;
-    for (int g0 = 0; g0 <= a.groups; g0 += 64) {
+    for (int g0 = 0; g0 <= a.groups + 1; g0 += 64) {
         int lo, hi;
         group_rows(a, g0 + (threadIdx.x & 63), lo, hi);
         tiles += __shfl(wave_prefix((hi - lo + BR - 1) / BR), 63);
@@ -129,7 +131,7 @@ __device__ __forceinline__ RowTile find_tile(const TileArgs& a, int tile) {
         return first < a.total ? RowTile{0, first, min(first + BR, a.total)} : RowTile{-1, 0, 0};
     }
     int before = 0;
-    for (int g0 = 0; g0 <= a.groups; g0 += 64) {
+    for (int g0 = 0; g0 <= a.groups + 1; g0 += 64) {
         int lo, hi;
         group_rows(a, g0 + (threadIdx.x & 63), lo, hi);
         const int tiles = (hi - lo + BR - 1) / BR;
@@ -1069,14 +1071,16 @@ template <typename T, int RF, int CF, int WAVES, int ROOM, bool ADAPT>
 Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
     const long long row_tiles = a.offsets == nullptr
         ? (a.total + RF * 16 - 1) / (RF * 16)
-        : a.total / (RF * 16) + std::min<long long>(a.groups + 1LL, a.total);
+        : a.total / (RF * 16) + std::min<long long>(a.groups + 2LL, a.total);
     const long long blocks = row_tiles * ((a.width + CF * 16 - 1) / (CF * 16));
     if (blocks > 0x7fffffffLL) return Error{kUnsupported, std::string(name) + ": too many tiles"};
     const dim3 grid(static_cast<unsigned>(blocks));
     constexpr int shares = Shares<RF, CF, WAVES>::kBytes;
-    if (!pieces) {
-        return launch_with_lds<few_rows_product<T, RF, CF, WAVES, 0, ADAPT>>(
-            grid, WAVES * 64, shares, stream, name, a);
+    if constexpr (CF == 1) {
+        if (!pieces) {
+            return launch_with_lds<few_rows_product<T, RF, CF, WAVES, 0, ADAPT>>(
+                grid, WAVES * 64, shares, stream, name, a);
+        }
     }
     constexpr int depth = ring_depth(WAVES, RF + CF, ROOM);
     constexpr int lds = std::max(shares, WAVES * depth * (RF + CF) * 2048);
@@ -1174,6 +1178,7 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
     double few = weights / 6.3e6 * (1 + mean / 160);
     switch (few_form(a, rows)) {
         case Few::Columns:
+            if (!pieces) return Form::Any;  // never behind it: three times its time is more
             few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 64.0) / 512) *
                                     (2 + 2.2 * std::ceil(a.depth / 256.0)));
             break;
@@ -1196,11 +1201,11 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
 template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT>
 Error launch_tiles(const TileArgs& a, Form form, hipStream_t stream, const char* name) {
     const int edge = form == Form::Wide ? 256 : 128;
-    // every group may end in a part-filled tile, and so may the rows in no group
+    // every group may end in a part-filled tile, and so may the rows before and behind them
     const long long row_tiles =
         GRAD ? static_cast<long long>(a.groups) * ((a.height + edge - 1) / edge)
         : a.offsets == nullptr ? (a.total + edge - 1) / edge
-                               : a.total / edge + std::min<long long>(a.groups + 1LL, a.total);
+                               : a.total / edge + std::min<long long>(a.groups + 2LL, a.total);
     // a whole number of workgroups for each XCD
     const long long blocks = (row_tiles * ((a.width + edge - 1) / edge) + 7) / 8 * 8;
     if (blocks > 0x7fffffffLL) return Error{kUnsupported, std::string(name) + ": too many tiles"};

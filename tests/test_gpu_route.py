@@ -47,6 +47,39 @@ def test_route(S, T, E, k, over):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k", [(1, 16, 16), (3, 129, 1), (66, 200, 9), (130, 255, 16),
+                                   (4, 256, 16), (5, 256, 17), (1025, 65, 5), (7, 257, 3)])
+@pytest.mark.parametrize("over", ["chosen", "all"])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_route_16_bit(S, T, E, k, over, name):
+    """Around the widths and choices where 16-bit logits are taken four tokens a wave."""
+    for n, (masked, ties) in enumerate([(0.0, False), (0.5, False), (0.02, True)]):
+        logits = _logits(T, E, R.TYPES[name], T * E + n, masked, ties)
+        r = S.route(logits.cuda(), k, over=over)
+        want = R.route(logits.double().numpy(), k, over)
+        _check_order(r, want)
+        assert np.abs(r.weights.cpu().numpy() - want[1]).max() <= WEIGHT
+
+
+@pytest.mark.gpu
+def test_route_masks_ties_and_nan_16_bit(S):
+    inf, nan = float("inf"), float("nan")
+    rows = [[-inf] * 5, [1, 1, 1, 1, 1], [-0.0, 0.0, -0.0, 0.0, -1.0], [nan, 1, 2, nan, 3],
+            [1, nan, -inf, inf, 0], [-inf, -inf, -inf, -inf, 5], [0.0, -0.0, -inf, -0.0, 0.0]]
+    for dtype in (torch.float16, torch.bfloat16):
+        low = torch.finfo(dtype).min
+        logits = torch.tensor(rows + [[low] * 5, [low, -inf, low, -inf, -inf]]).to(dtype)
+        for over in ("chosen", "all"):
+            r = S.route(logits.cuda(), 3, over=over)
+            want = R.route(logits.double().numpy(), 3, over)
+            _check_order(r, want)
+            got = r.weights.cpu().numpy()
+            assert np.array_equal(np.isnan(got), np.isnan(want[1]))
+            fine = ~np.isnan(got)
+            assert np.abs(got[fine] - want[1][fine]).max() <= WEIGHT
+
+
+@pytest.mark.gpu
 def test_route_masks_ties_and_nan(S):
     inf, nan = float("inf"), float("nan")
     low = torch.finfo(torch.float32).min
