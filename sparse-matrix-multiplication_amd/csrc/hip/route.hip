@@ -11,6 +11,10 @@
 // expert while they choose (or from given ids), then every block places its own
 // entries from all blocks' counts.  Places follow from counts alone, never from
 // the order of atomics, so equal experts keep their entries' order.
+//
+// Up to 512 entries or so are one block's, which chooses and places in one launch: a
+// call for one token of 64 experts, k = 6, is then bound by its host side (15.8 us;
+// 18.5 with two launches).
 
 #include <hip/hip_runtime.h>
 
@@ -131,132 +135,26 @@ struct Order {
     int*       slots;    // n
 };
 
-template <typename T, int PER>
-__global__ __launch_bounds__(kChooseWaves * 64) void route_choose(
-    const T* __restrict__ logits, int tokens, int experts, int k, int all, int per_block,
-    int* __restrict__ out_experts, float* __restrict__ out_weights, int* __restrict__ counts) {
-    extern __shared__ int s_count[];
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) s_count[e] = 0;
-    __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t1 = min((static_cast<int>(blockIdx.x) + 1) * per_block, tokens);
-    for (int t = blockIdx.x * per_block + wave; t < t1; t += kChooseWaves) {
-        float v[PER];
-        load_logits<T, PER>(logits + static_cast<long long>(t) * experts, experts, v);
-        int   expert;
-        float weight;
-        choose<PER>(v, k, all != 0, expert, weight);
-        if (lane < k) {
-            out_experts[static_cast<long long>(t) * k + lane] = expert;
-            out_weights[static_cast<long long>(t) * k + lane] = weight;
-            if (expert >= 0) atomicAdd(&s_count[expert], 1);
-        }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-        counts[static_cast<long long>(blockIdx.x) * experts + e] = s_count[e];
-    }
-}
-
-// route_choose for 16-bit logits and k <= 16: the token's lane j < k holds choice j.
-// 16384 tokens, 128 experts, k = 8: 7.0 us, one token a wave 14.5.
-template <typename T, int PER>
-__global__ __launch_bounds__(kChooseWaves * 64) void route_choose_quads(
-    const T* __restrict__ logits, int tokens, int experts, int k, int all, int per_block,
-    int* __restrict__ out_experts, float* __restrict__ out_weights, int* __restrict__ counts) {
-    extern __shared__ int s_count[];
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) s_count[e] = 0;
-    __syncthreads();
-    const int lane = threadIdx.x & 15;
-    const int t1 = min((static_cast<int>(blockIdx.x) + 1) * per_block, tokens);
-    // whole waves stay together: the rotations need all lanes of a row
-    for (int t0 = blockIdx.x * per_block; t0 < t1; t0 += kChooseWaves * 4) {
-        const int t = t0 + static_cast<int>(threadIdx.x >> 4);
-        unsigned key[PER];
-        float v[PER];
-        const T* row = logits + static_cast<long long>(t < t1 ? t : t1 - 1) * experts;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = i * 16 + lane;
-            const T x = e < experts ? row[e] : static_cast<T>(0.0f);
-            v[i] = e < experts ? static_cast<float>(x) : -__builtin_inff();
-            const bool none = v[i] == -__builtin_inff();
-            key[i] = none ? 0u : order16(__builtin_bit_cast(unsigned short, x), v[i] != v[i]) << 16 |
-                                     (0xffffu - e);
-        }
-        int expert = -1;
-        unsigned mine = 0u, first = 0u;
-        for (int j = 0; j < k; ++j) {
-            unsigned m = key[0];
-#pragma unroll
-            for (int i = 1; i < PER; ++i) m = m > key[i] ? m : key[i];
-            m = row_max(m);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) key[i] = key[i] == m ? 0u : key[i];
-            first = j == 0 ? m : first;
-            mine = lane == j ? m : mine;
-        }
-        auto value = [](unsigned m) {
-            const unsigned u = m >> 16;
-            const unsigned short bits = static_cast<unsigned short>(u & 0x8000u ? u & 0x7fffu : ~u);
-            return static_cast<float>(__builtin_bit_cast(T, bits));
-        };
-        const float largest = first != 0u ? value(first) : 0.0f;
-        expert = mine != 0u ? static_cast<int>(0xffffu - (mine & 0xffffu)) : -1;
-        const float e = mine != 0u ? expf(value(mine) - largest) : 0.0f;
-        float part = e;
-        if (all) {
-            part = 0.0f;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) part += expf(v[i] - largest);
-        }
-        const float total = row_sum(part);
-        if (lane < k && t < t1) {
-            out_experts[static_cast<long long>(t) * k + lane] = expert;
-            out_weights[static_cast<long long>(t) * k + lane] = expert >= 0 ? e / total : 0.0f;
-            if (expert >= 0) atomicAdd(&s_count[expert], 1);
-        }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-        counts[static_cast<long long>(blockIdx.x) * experts + e] = s_count[e];
-    }
-}
-
-__global__ __launch_bounds__(256) void group_count(Order o) {
-    extern __shared__ int s_count[];
-    for (int g = threadIdx.x; g < o.groups; g += 256) s_count[g] = 0;
-    __syncthreads();
-    const int i1 = min((static_cast<int>(blockIdx.x) + 1) * o.chunk, o.n);
-    for (int i = blockIdx.x * o.chunk + threadIdx.x; i < i1; i += 256) {
-        const int id = o.ids[i];
-        if (static_cast<unsigned>(id) < static_cast<unsigned>(o.groups)) atomicAdd(&s_count[id], 1);
-    }
-    __syncthreads();
-    for (int g = threadIdx.x; g < o.groups; g += 256) {
-        o.counts[static_cast<long long>(blockIdx.x) * o.groups + g] = s_count[g];
-    }
-}
-
 // Places chunk b: entry i of expert e goes to offsets[e] + (entries of e in
 // earlier chunks) + (in earlier waves' parts) + (in earlier rounds and lanes).
 // Every block sums the other blocks' counts itself: blocks x groups ints from
 // L2 a block, less than a third launch between the two would cost.
-__global__ __launch_bounds__(kPlaceWaves * 64) void group_place(Order o) {
-    extern __shared__ int s[];
+// A block that is alone counts its own entries and reads nobody's.
+template <int WAVES>
+__device__ __forceinline__ void place_chunk(const Order& o, int* s) {
     int* s_start = s;                     // kPlaceWaves x groups: next place, by wave
     int* s_total = s + kPlaceWaves * o.groups;
     int* s_before = s_total + o.groups;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    constexpr int threads = kPlaceWaves * 64;
+    constexpr int threads = WAVES * 64;  // those past kPlaceWaves have no entries
     for (int i = threadIdx.x; i < (kPlaceWaves + 2) * o.groups; i += threads) s[i] = 0;
     __syncthreads();
 
     // counts of all blocks and of the earlier ones: `parts` threads share a column
     const int parts = max(1, threads / o.groups);
     const int blocks = gridDim.x;
-    for (int i = threadIdx.x; i < parts * o.groups; i += threads) {
+    for (int i = threadIdx.x; blocks > 1 && i < parts * o.groups; i += threads) {
         const int g = i % o.groups;
         int total = 0, before = 0;
 #pragma unroll 16
@@ -280,6 +178,14 @@ __global__ __launch_bounds__(kPlaceWaves * 64) void group_place(Order o) {
         }
     }
     __syncthreads();
+    if (blocks == 1) {
+        for (int g = threadIdx.x; g < o.groups; g += threads) {
+            int c = 0;
+            for (int w = 0; w < kPlaceWaves; ++w) c += s_start[w * o.groups + g];
+            s_total[g] = c;
+        }
+        __syncthreads();
+    }
     // s_total becomes each group's first place
     if (wave == 0) {
         int run = 0;
@@ -334,6 +240,130 @@ __global__ __launch_bounds__(kPlaceWaves * 64) void group_place(Order o) {
     for (int i = placed + blockIdx.x * threads + threadIdx.x; i < o.n; i += gridDim.x * threads) {
         o.entries[i] = -1;
     }
+}
+
+template <typename T, int PER, bool ALONE>
+__global__ __launch_bounds__(kChooseWaves * 64) void route_choose(
+    const T* __restrict__ logits, int tokens, int experts, int k, int all, int per_block,
+    float* __restrict__ out_weights, int* out_experts, Order order) {
+    extern __shared__ int s_count[];
+    if constexpr (!ALONE) {
+        for (int e = threadIdx.x; e < experts; e += blockDim.x) s_count[e] = 0;
+        __syncthreads();
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t1 = min((static_cast<int>(blockIdx.x) + 1) * per_block, tokens);
+    for (int t = blockIdx.x * per_block + wave; t < t1; t += kChooseWaves) {
+        float v[PER];
+        load_logits<T, PER>(logits + static_cast<long long>(t) * experts, experts, v);
+        int   expert;
+        float weight;
+        choose<PER>(v, k, all != 0, expert, weight);
+        if (lane < k) {
+            out_experts[static_cast<long long>(t) * k + lane] = expert;
+            out_weights[static_cast<long long>(t) * k + lane] = weight;
+            if (!ALONE && expert >= 0) atomicAdd(&s_count[expert], 1);
+        }
+    }
+    __syncthreads();
+    if constexpr (ALONE) {
+        place_chunk<kChooseWaves>(order, s_count);
+    } else {
+        for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+            order.counts[static_cast<long long>(blockIdx.x) * experts + e] = s_count[e];
+        }
+    }
+}
+
+// route_choose for 16-bit logits and k <= 16: the token's lane j < k holds choice j.
+// 16384 tokens, 128 experts, k = 8: 7.0 us, one token a wave 14.5.
+template <typename T, int PER, bool ALONE>
+__global__ __launch_bounds__(kChooseWaves * 64) void route_choose_quads(
+    const T* __restrict__ logits, int tokens, int experts, int k, int all, int per_block,
+    float* __restrict__ out_weights, int* out_experts, Order order) {
+    extern __shared__ int s_count[];
+    if constexpr (!ALONE) {
+        for (int e = threadIdx.x; e < experts; e += blockDim.x) s_count[e] = 0;
+        __syncthreads();
+    }
+    const int lane = threadIdx.x & 15;
+    const int t1 = min((static_cast<int>(blockIdx.x) + 1) * per_block, tokens);
+    // whole waves stay together: the rotations need all lanes of a row
+    for (int t0 = blockIdx.x * per_block; t0 < t1; t0 += kChooseWaves * 4) {
+        const int t = t0 + static_cast<int>(threadIdx.x >> 4);
+        unsigned key[PER];
+        float v[PER];
+        const T* row = logits + static_cast<long long>(t < t1 ? t : t1 - 1) * experts;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = i * 16 + lane;
+            const T x = e < experts ? row[e] : static_cast<T>(0.0f);
+            v[i] = e < experts ? static_cast<float>(x) : -__builtin_inff();
+            const bool none = v[i] == -__builtin_inff();
+            key[i] = none ? 0u : order16(__builtin_bit_cast(unsigned short, x), v[i] != v[i]) << 16 |
+                                     (0xffffu - e);
+        }
+        int expert = -1;
+        unsigned mine = 0u, first = 0u;
+        for (int j = 0; j < k; ++j) {
+            unsigned m = key[0];
+#pragma unroll
+            for (int i = 1; i < PER; ++i) m = m > key[i] ? m : key[i];
+            m = row_max(m);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) key[i] = key[i] == m ? 0u : key[i];
+            first = j == 0 ? m : first;
+            mine = lane == j ? m : mine;
+        }
+        auto value = [](unsigned m) {
+            const unsigned u = m >> 16;
+            const unsigned short bits = static_cast<unsigned short>(u & 0x8000u ? u & 0x7fffu : ~u);
+            return static_cast<float>(__builtin_bit_cast(T, bits));
+        };
+        const float largest = first != 0u ? value(first) : 0.0f;
+        expert = mine != 0u ? static_cast<int>(0xffffu - (mine & 0xffffu)) : -1;
+        const float e = mine != 0u ? expf(value(mine) - largest) : 0.0f;
+        float part = e;
+        if (all) {
+            part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) part += expf(v[i] - largest);
+        }
+        const float total = row_sum(part);
+        if (lane < k && t < t1) {
+            out_experts[static_cast<long long>(t) * k + lane] = expert;
+            out_weights[static_cast<long long>(t) * k + lane] = expert >= 0 ? e / total : 0.0f;
+            if (!ALONE && expert >= 0) atomicAdd(&s_count[expert], 1);
+        }
+    }
+    __syncthreads();
+    if constexpr (ALONE) {
+        place_chunk<kChooseWaves>(order, s_count);
+    } else {
+        for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+            order.counts[static_cast<long long>(blockIdx.x) * experts + e] = s_count[e];
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void group_count(Order o) {
+    extern __shared__ int s_count[];
+    for (int g = threadIdx.x; g < o.groups; g += 256) s_count[g] = 0;
+    __syncthreads();
+    const int i1 = min((static_cast<int>(blockIdx.x) + 1) * o.chunk, o.n);
+    for (int i = blockIdx.x * o.chunk + threadIdx.x; i < i1; i += 256) {
+        const int id = o.ids[i];
+        if (static_cast<unsigned>(id) < static_cast<unsigned>(o.groups)) atomicAdd(&s_count[id], 1);
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < o.groups; g += 256) {
+        o.counts[static_cast<long long>(blockIdx.x) * o.groups + g] = s_count[g];
+    }
+}
+
+__global__ __launch_bounds__(kPlaceWaves * 64) void group_place(Order o) {
+    extern __shared__ int s[];
+    place_chunk<kPlaceWaves>(o, s);
 }
 
 template <typename T, int PER>
@@ -415,9 +445,9 @@ Error check_sizes(int tokens, int experts, int k) {
     return Error{};
 }
 
+size_t place_lds(int groups) { return sizeof(int) * ((kPlaceWaves + 2) * groups + 1); }
 Error place(Order o, int blocks, hipStream_t stream) {
-    const size_t lds = sizeof(int) * ((kPlaceWaves + 2) * o.groups + 1);
-    group_place<<<blocks, kPlaceWaves * 64, lds, stream>>>(o);
+    group_place<<<blocks, kPlaceWaves * 64, place_lds(o.groups), stream>>>(o);
     SPMM_TRY_HIP(hipGetLastError(), "group_place");
     return Error{};
 }
@@ -479,11 +509,12 @@ Error launch_group_entries(const int* ids, int n, int groups, int* offsets, int*
     if (n > 0x3fffffff) return Error{kUnsupported, "group_entries: over 2^30 entries"};
     if (offsets == nullptr) return Error{kInvalid, "group_entries: null offsets"};
     if (n == 0) return no_entries(groups, offsets, stream);
+    const Order o{ids, n, groups, chunk_of(n), static_cast<int*>(workspace), offsets, entries, slots};
+    const int blocks = blocks_of(n, o.chunk);
     if (ids == nullptr || entries == nullptr || slots == nullptr || workspace == nullptr) {
         return Error{kInvalid, "group_entries: null pointer"};
     }
-    const Order o{ids, n, groups, chunk_of(n), static_cast<int*>(workspace), offsets, entries, slots};
-    const int blocks = blocks_of(n, o.chunk);
+    if (blocks == 1) return place(o, 1, stream);
     group_count<<<blocks, 256, sizeof(int) * groups, stream>>>(o);
     SPMM_TRY_HIP(hipGetLastError(), "group_count");
     return place(o, blocks, stream);
@@ -495,35 +526,42 @@ Error launch_route(const void* logits, ElementType type, int tokens, int experts
     SPMM_TRY(check_sizes(tokens, experts, k));
     if (offsets == nullptr) return Error{kInvalid, "route: null offsets"};
     if (tokens == 0) return no_entries(experts, offsets, stream);
+    const int per = tokens_per_block(tokens, k);
+    const int blocks = blocks_of(tokens, per);
     if (logits == nullptr || out_experts == nullptr || out_weights == nullptr ||
         entries == nullptr || slots == nullptr || workspace == nullptr) {
         return Error{kInvalid, "route: null pointer"};
     }
-    const int per = tokens_per_block(tokens, k);
-    const int blocks = blocks_of(tokens, per);
-    int* counts = static_cast<int*>(workspace);
+    const Order order{out_experts, tokens * k, experts, per * k, static_cast<int*>(workspace),
+                      offsets, entries, slots};
+    const bool alone = blocks == 1;
     SPMM_TRY(with_type(type, [&](auto zero) {
         using T = decltype(zero);
         auto launch = [&](auto kernel) {
-            kernel<<<blocks, kChooseWaves * 64, sizeof(int) * experts, stream>>>(
-                static_cast<const T*>(logits), tokens, experts, k, all ? 1 : 0, per, out_experts,
-                out_weights, counts);
+            kernel<<<blocks, kChooseWaves * 64, alone ? place_lds(experts) : sizeof(int) * experts,
+                     stream>>>(static_cast<const T*>(logits), tokens, experts, k, all ? 1 : 0, per,
+                               out_weights, out_experts, order);
         };
         if constexpr (sizeof(T) == 2) {
             if (k <= 16 && experts <= 256) {
-                if (experts <= 64) launch(route_choose_quads<T, 4>);
-                else if (experts <= 128) launch(route_choose_quads<T, 8>);
-                else launch(route_choose_quads<T, 16>);
+                auto quads = [&](auto n) {
+                    launch(alone ? route_choose_quads<T, n.value, true>
+                                 : route_choose_quads<T, n.value, false>);
+                };
+                if (experts <= 64) quads(std::integral_constant<int, 4>{});
+                else if (experts <= 128) quads(std::integral_constant<int, 8>{});
+                else quads(std::integral_constant<int, 16>{});
                 SPMM_TRY_HIP(hipGetLastError(), "route_choose");
                 return Error{};
             }
         }
-        with_per(experts, [&](auto n) { launch(route_choose<T, n.value>); });
+        with_per(experts, [&](auto n) {
+            launch(alone ? route_choose<T, n.value, true> : route_choose<T, n.value, false>);
+        });
         SPMM_TRY_HIP(hipGetLastError(), "route_choose");
         return Error{};
     }));
-    return place(Order{out_experts, tokens * k, experts, per * k, counts, offsets, entries, slots},
-                 blocks, stream);
+    return alone ? Error{} : place(order, blocks, stream);
 }
 
 Error launch_route_backward(const void* logits, ElementType type, int tokens, int experts, int k,
