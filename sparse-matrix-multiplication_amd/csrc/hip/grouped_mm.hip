@@ -112,14 +112,35 @@ __device__ __forceinline__ void group_rows(const TileArgs& a, int g, int& lo, in
         hi = row_bound(a, 0);
     }
 }
+// Tiles of group g, the first row of the first of them, and the group's end.
+template <int BR>
+__device__ __forceinline__ int group_tiles(const TileArgs& a, int g, int& lo, int& hi) {
+    group_rows(a, g, lo, hi);
+    return (hi - lo + BR - 1) / BR;
+}
+// The tile whose number lies in [upto - tiles, upto) of some lane's group.
+template <int BR>
+__device__ __forceinline__ bool tile_among(int tile, int g0, int lo, int hi, int tiles, int upto,
+                                           RowTile& r) {
+    const unsigned long long at = __ballot(tile >= upto - tiles && tile < upto);
+    if (at == 0) return false;
+    const int l = __builtin_ctzll(at);
+    const int first = __shfl(lo + (tile - (upto - tiles)) * BR, l);
+    r = RowTile{g0 + l, first, min(first + BR, __shfl(hi, l))};
+    return true;
+}
+// The same for the whole wave, which the compiler does not see.
+__device__ __forceinline__ RowTile uniform(RowTile r) {
+    return RowTile{__builtin_amdgcn_readfirstlane(r.group), __builtin_amdgcn_readfirstlane(r.first),
+                   __builtin_amdgcn_readfirstlane(r.end)};
+}
 template <int BR>
 __device__ __forceinline__ int count_tiles(const TileArgs& a) {
-    if (a.offsets == nullptr) return (a.total + BR - 1) / BR;
     int tiles = 0;
     for (int g0 = 0; g0 <= a.groups + 1; g0 += 64) {
         int lo, hi;
-        group_rows(a, g0 + (threadIdx.x & 63), lo, hi);
-        tiles += __shfl(wave_prefix((hi - lo + BR - 1) / BR), 63);
+        const int n = group_tiles<BR>(a, g0 + (threadIdx.x & 63), lo, hi);
+        tiles += __shfl(wave_prefix(n), 63);
     }
     return __builtin_amdgcn_readfirstlane(tiles);
 }
@@ -130,23 +151,16 @@ __device__ __forceinline__ RowTile find_tile(const TileArgs& a, int tile) {
         const int first = tile * BR;
         return first < a.total ? RowTile{0, first, min(first + BR, a.total)} : RowTile{-1, 0, 0};
     }
+    RowTile r{-1, 0, 0};
     int before = 0;
     for (int g0 = 0; g0 <= a.groups + 1; g0 += 64) {
         int lo, hi;
-        group_rows(a, g0 + (threadIdx.x & 63), lo, hi);
-        const int tiles = (hi - lo + BR - 1) / BR;
+        const int tiles = group_tiles<BR>(a, g0 + (threadIdx.x & 63), lo, hi);
         const int upto = before + wave_prefix(tiles);
-        const unsigned long long at = __ballot(tile >= upto - tiles && tile < upto);
-        if (at != 0) {
-            const int l = __builtin_ctzll(at);
-            const int first = __shfl(lo + (tile - (upto - tiles)) * BR, l);
-            return RowTile{__builtin_amdgcn_readfirstlane(g0 + l),
-                           __builtin_amdgcn_readfirstlane(first),
-                           __builtin_amdgcn_readfirstlane(min(first + BR, __shfl(hi, l)))};
-        }
+        if (tile_among<BR>(tile, g0, lo, hi, tiles, upto, r)) break;
         before = __shfl(upto, 63);
     }
-    return RowTile{-1, 0, 0};
+    return uniform(r);
 }
 
 // The tile of a workgroup: work item w of row_tiles x col_tiles.  Workgroup b
@@ -165,6 +179,29 @@ __device__ __forceinline__ bool tile_of_block(int row_tiles, int col_tiles, int&
     rt = 8 * band + rest % high;
     ct = rest / high;
     return true;
+}
+
+// The row tile and column tile of a workgroup of a product.  Up to 62 groups are
+// looked at once, for their number of tiles and for the tile itself.
+template <int BR>
+__device__ __forceinline__ bool row_tile_of_block(const TileArgs& a, int col_tiles, RowTile& r,
+                                                  int& ct) {
+    int rt;
+    if (a.offsets == nullptr) {
+        if (!tile_of_block((a.total + BR - 1) / BR, col_tiles, rt, ct)) return false;
+        r = find_tile<BR>(a, rt);
+        return true;
+    }
+    if (a.groups + 2 <= 64) {
+        int lo, hi;
+        const int tiles = group_tiles<BR>(a, threadIdx.x & 63, lo, hi);
+        const int upto = wave_prefix(tiles);
+        const int all = __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+        return tile_of_block(all, col_tiles, rt, ct) && tile_among<BR>(rt, 0, lo, hi, tiles, upto, r);
+    }
+    if (!tile_of_block(count_tiles<BR>(a), col_tiles, rt, ct)) return false;
+    r = find_tile<BR>(a, rt);
+    return r.group >= 0;
 }
 
 // How one operand lies in memory and in LDS.
@@ -263,8 +300,9 @@ __device__ __forceinline__ bool take_tile(const TileArgs& a, Tile<T>& t) {
     t.rows = static_cast<const T*>(a.rows);
     t.cols = static_cast<const T*>(a.cols);
     t.out  = static_cast<T*>(a.out);
-    int rt, ct;
+    int ct;
     if constexpr (GRAD) {
+        int rt;
         const int row_tiles = (a.height + BR - 1) / BR;
         if (!tile_of_block(a.groups * row_tiles, col_tiles, rt, ct)) return false;
         const int g = rt / row_tiles;
@@ -281,9 +319,9 @@ __device__ __forceinline__ bool take_tile(const TileArgs& a, Tile<T>& t) {
         t.step_rows = static_cast<long long>(kStep) * t.ld_rows;
         t.step_cols = static_cast<long long>(kStep) * t.ld_cols;
     } else {
-        if (!tile_of_block(count_tiles<BR>(a), col_tiles, rt, ct)) return false;
-        const RowTile r = find_tile<BR>(a, rt);
-        if (r.group < 0) return false;
+        RowTile r;
+        if (!row_tile_of_block<BR>(a, col_tiles, r, ct)) return false;
+        r = uniform(r);
         t.row0 = r.first;
         t.rows_here = r.end - r.first;
         t.c0 = ct * BC;
@@ -464,6 +502,19 @@ struct Slot {
     }
 };
 
+// Zeros where nothing is summed: rows in no group, the gradient of an empty one.
+template <int BC, typename T>
+__device__ __forceinline__ void zero_tile(const TileArgs& a, const Tile<T>& t) {
+    const int c = t.c0 + threadIdx.x % (BC / 8) * 8;
+    const int count = min(8, a.width - c);
+    if (count <= 0) return;
+    for (int r = threadIdx.x / (BC / 8); r < t.rows_here; r += blockDim.x / (BC / 8)) {
+        T* p = t.out + static_cast<long long>(r) * a.width + c;
+        if (count == 8) store_piece(p, uint4{});
+        else store_part(p, uint4{}, count);
+    }
+}
+
 // GRAD false: a product (rows operand [s][k], columns operand W as COLS_MAJOR
 // says).  GRAD true: a weight gradient (both operands lie along s).
 // ADAPT: with the adapters' extension.
@@ -612,14 +663,10 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
     if (!take_tile<T, BR, BC, GRAD, COLS_MAJOR>(a, t)) return;
 
     f32x4 acc[CF][RF];
-#pragma unroll
-    for (int j = 0; j < CF; ++j)
-#pragma unroll
-        for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
-
     const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
     const int tiles = (t.depth + kStep - 1) / kStep;
-    if (tiles > 0) {
+    if (tiles == 0) return zero_tile<BC>(a, t);
+    {
         ColSlot cols0, cols1;
         RowSlot low, high;
         cols0.place(t.ld_cols, 0, a.width - t.c0);
@@ -689,6 +736,15 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
         load_slot(high, rows, place_of(7));
         advance();
         load_slot(cols0, cols, place_of(8));
+        // the sums begin at 0 while the loads are under way
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < CF; ++j)
+#pragma unroll
+            for (int i = 0; i < RF; ++i) {
+                acc[j][i] = f32x4(0.0f);
+                asm volatile("" : "+a"(acc[j][i]));
+            }
         wait_vmcnt<24>();  // slots 0, 1, 2
         lds_barrier();
 #pragma unroll
