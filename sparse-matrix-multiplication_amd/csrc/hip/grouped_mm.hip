@@ -88,6 +88,7 @@ struct TileArgs {
     int         adapters;
     int         rank;
     int         rank32;   // rank rounded up to whole products of 32
+    bool        b_pieces; // B's rows are whole 16-byte pieces
 };
 
 // The group's rows as the kernels use them: in range and in order whatever the
@@ -502,6 +503,21 @@ struct Slot {
     }
 };
 
+// Stores a wave's tile with its rows' adapters added.
+template <typename T, int RF, int CF>
+__device__ __forceinline__ void store_adapted(const TileArgs& a, const Tile<T>& t, int r0, int c0,
+                                              const f32x4 (&acc)[CF][RF], float* sums) {
+    auto store = [&](auto pieces) {
+        const Adapters<T, RF, CF, pieces.value> ad(a, t, r0, c0);
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
+            constexpr int i = at.value;
+            ad.add(i, ad.id[i], sums, CF * 16 + 4);
+        });
+    };
+    if (a.b_pieces) store(std::true_type{});
+    else store(std::false_type{});
+}
+
 // Zeros where nothing is summed: rows in no group, the gradient of an empty one.
 template <int BC, typename T>
 __device__ __forceinline__ void zero_tile(const TileArgs& a, const Tile<T>& t) {
@@ -620,11 +636,7 @@ __global__ __launch_bounds__(256) void tile_product(TileArgs a) {
     lds_barrier();  // the operands' LDS is free
     float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
     if constexpr (ADAPT) {
-        const Adapters<T, RF, CF, PIECES> ad(a, t, r0, c0);
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
-            constexpr int i = at.value;
-            ad.add(i, ad.id[i], sums, CF * 16 + 4);
-        });
+        store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
     } else {
         store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
     }
@@ -782,11 +794,7 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
     }
     float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
     if constexpr (ADAPT) {
-        const Adapters<T, RF, CF, true> ad(a, t, r0, c0);
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
-            constexpr int i = at.value;
-            ad.add(i, ad.id[i], sums, CF * 16 + 4);
-        });
+        store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
     } else {
         store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
     }
@@ -1370,14 +1378,12 @@ Error launch_adapter_mm(const void* x, const void* w, const void* down, const vo
     a.rank = rank;
     a.rank32 = (rank + 31) / 32 * 32;
     const bool pieces = depth % 8 == 0 && aligned16(x) && aligned16(w);
-    Form form = choose_form(a, pieces, true);
-    if ((form == Form::Wide || form == Form::Pieces) && (rank % 8 != 0 || !aligned16(up))) {
-        form = Form::Any;
-    }
+    a.b_pieces = rank % 8 == 0 && aligned16(up);
+    const Form form = choose_form(a, pieces, true);
     return with_half(type, "adapter_mm", [&](auto zero) {
         using T = decltype(zero);
         const bool whole = pieces && aligned16(down);
-        if (total <= 512) {
+        if (total <= 512 || (!whole && total <= 2048)) {
             SPMM_TRY((launch_shrink<T, 1, 1, 8, 159 * 1024>(a, whole, down, scale, std::max(1, std::min(16, adapters)), stream)));
         } else {
             SPMM_TRY((launch_shrink<T, 1, 4, 2, 53 * 1024>(a, whole, down, scale, std::max(1, std::min(8, adapters)), stream)));
