@@ -25,6 +25,11 @@ __device__ __forceinline__ uint4 load_piece(const void* p) {
     return v;
 }
 __device__ __forceinline__ void store_piece(void* p, uint4 v) { __builtin_memcpy(p, &v, 16); }
+// The same for data that the caches are not to keep.
+__device__ __forceinline__ void stream_piece(void* p, uint4 v) {
+    typedef unsigned words __attribute__((ext_vector_type(4), aligned(2)));
+    __builtin_nontemporal_store(words{v.x, v.y, v.z, v.w}, static_cast<words*>(p));
+}
 
 // The first `count` elements of a piece (count < kPiece), zeros behind them.
 template <typename T>

@@ -34,9 +34,24 @@ __device__ __forceinline__ int slot_of(const int* slots, long long i) {
     return __builtin_amdgcn_readfirstlane(slots[i]);
 }
 
+// Zeros in the rows that no entry has, a row a workgroup at a time.
+template <typename T>
+__device__ __forceinline__ void zero_rows(T* rows, int placed, const Rows& r) {
+    constexpr int P = kPiece<T>;
+    const int total = r.tokens * r.k;
+    for (long long s = static_cast<long long>(min(max(placed, 0), total)) + blockIdx.x; s < total;
+         s += gridDim.x) {
+        T* row = rows + s * r.features;
+        for (int c = threadIdx.x * P; c < r.features; c += 256 * P) {
+            if (r.features - c >= P) store_piece(row + c, uint4{});
+            else store_part(row + c, uint4{}, r.features - c);
+        }
+    }
+}
+
 // Copies rows of `features` T; WAVES waves of a workgroup share a token's row
-// (WAVES = 1: the workgroup's four waves take a token each).
-template <typename T, int WAVES>
+// (WAVES = 1: the workgroup's four waves take a token each).  STREAM: past the caches.
+template <typename T, int WAVES, bool STREAM>
 __global__ __launch_bounds__(256) void tokens_dispatch(const T* __restrict__ x,
                                                        const int* __restrict__ slots,
                                                        const int* __restrict__ placed, Rows r,
@@ -62,7 +77,10 @@ __global__ __launch_bounds__(256) void tokens_dispatch(const T* __restrict__ x,
                 T* dst = xs + static_cast<long long>(s) * r.features;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if (c + u * step < whole) store_piece(dst + c + u * step, v[u]);
+                    if (c + u * step < whole) {
+                        if constexpr (STREAM) stream_piece(dst + c + u * step, v[u]);
+                        else store_piece(dst + c + u * step, v[u]);
+                    }
                 }
             }
         }
@@ -76,13 +94,7 @@ __global__ __launch_bounds__(256) void tokens_dispatch(const T* __restrict__ x,
             }
         }
     }
-    // rows that no entry has
-    const long long end = static_cast<long long>(total) * r.features;
-    const int first = min(max(*placed, 0), total);
-    for (long long i = (static_cast<long long>(first) + blockIdx.x) * r.features; i < end;
-         i += static_cast<long long>(gridDim.x) * r.features) {
-        for (int c = threadIdx.x; c < r.features; c += 256) xs[i + c] = static_cast<T>(0.0f);
-    }
+    zero_rows(xs, *placed, r);
 }
 
 // Sum over a token's slots, weighted where weights are given.  B slots' pieces
@@ -209,12 +221,7 @@ __global__ __launch_bounds__(256) void tokens_combine_grad(
             }
         }
     }
-    const long long end = static_cast<long long>(total) * r.features;
-    const int first = min(max(*placed, 0), total);
-    for (long long i = (static_cast<long long>(first) + blockIdx.x) * r.features; i < end;
-         i += static_cast<long long>(gridDim.x) * r.features) {
-        for (int c = threadIdx.x; c < r.features; c += 256) dys[i + c] = static_cast<T>(0.0f);
-    }
+    zero_rows(dys, *placed, r);
 }
 
 Error check_rows(const Rows& r, const char* name) {
@@ -230,6 +237,11 @@ Error check_rows(const Rows& r, const char* name) {
 // One wave a token fills the chip's 1024 SIMDs from about this many tokens on;
 // below, four waves share a token.
 constexpr int kWaveTokens = 4096;
+
+// Rows that the 256 MB cache in front of memory cannot hold are stored past it: 8192
+// tokens x 8 x 4096 bf16 (512 MB) take 106 us, 120 with plain stores; 5003 x 4 x 2050
+// (80 MB), which the cache holds for the next reader, 17 us with plain stores, 22 so.
+constexpr long long kStreamBytes = 256LL << 20;
 
 template <typename F>
 Error with_shape(ElementType type, int tokens, F f) {
@@ -259,8 +271,11 @@ Error launch_dispatch(const void* x, ElementType type, int tokens, int k, int fe
     }
     return with_shape(type, tokens, [&](auto zero, auto waves, int blocks) {
         using T = decltype(zero);
-        tokens_dispatch<T, waves.value><<<blocks, 256, 0, stream>>>(
-            static_cast<const T*>(x), slots, offsets + experts, r, static_cast<T*>(xs));
+        const bool past = static_cast<long long>(tokens) * k * features * sizeof(T) >= kStreamBytes;
+        auto kernel = past ? tokens_dispatch<T, waves.value, true>
+                           : tokens_dispatch<T, waves.value, false>;
+        kernel<<<blocks, 256, 0, stream>>>(static_cast<const T*>(x), slots, offsets + experts, r,
+                                           static_cast<T*>(xs));
         SPMM_TRY_HIP(hipGetLastError(), "dispatch");
         return Error{};
     });

@@ -144,3 +144,24 @@ def test_adapter_forms(S, T, N, K, L, rank, name, order):
     allowed = u * want.abs() + (1 + u) * ((K + rank) * 2.0 ** -24 * size + low * (1 + u)) \
         + R.TINY[dtype]
     assert (off <= allowed).all(), float((off / allowed).max())
+
+
+@pytest.mark.gpu
+def test_more_than_32_bits_of_elements(S):
+    """Weights and their gradient of more than 2^31 elements, each way round."""
+    G, N, K, each = 64, 8192, 4224, 3
+    o, offsets = _bounds([each] * G)
+    x, dy = _values((o[-1], K), torch.bfloat16, 1), _values((o[-1], N), torch.bfloat16, 2)
+    w = torch.zeros((G, N, K), dtype=torch.bfloat16, device="cuda")
+    for g in (0, G - 2, G - 1):
+        w[g] = _values((N, K), torch.bfloat16, 3 + g, K ** -0.5)
+    y = S.grouped_mm(x, w, offsets)
+    dx, dw = S.grouped_mm_backward(dy, x, w, offsets)
+    z = S.grouped_mm(dy, w, offsets, w_in_rows=True)
+    assert torch.equal(z, dx)
+    for g in (0, 5, G - 2, G - 1):
+        s = slice(o[g], o[g + 1])
+        X, DY, W = x[s].double(), dy[s].double(), w[g].double()
+        _check(y[s], X @ W.t(), X.abs() @ W.abs().t(), K)
+        _check(dx[s], DY @ W, DY.abs() @ W.abs(), N)
+        _check(dw[g], DY.t() @ X, DY.abs().t() @ X.abs(), each)

@@ -125,3 +125,27 @@ def test_refusals(S):
         with pytest.raises(S.SpmmError) as e:
             bad()
         assert e.value.code == S.SPMM_INVALID
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k,D,name", [(8200, 32, 8, 2050, "f32"), (2000, 40, 16, 2100, "f32"),
+                                          (4100, 20, 8, 4099, "bf16"), (70000, 64, 8, 4000, "f16")])
+def test_rows_beyond_the_caches(S, T, E, k, D, name):
+    """256 MB and more in expert order; the last size has more than 2^31 elements there."""
+    torch.manual_seed(T)
+    r = S.route(torch.randn(T, E, device="cuda"), k)
+    x = torch.randn(T, D, device="cuda").to(R.TYPES[name])
+    xs = S.dispatch(x, r)
+    assert torch.equal(xs, x[(r.entries // k).long()])  # copies: exact
+    # a token's rows are all itself: k equal terms with weights that add up to one; the
+    # weights carry 64 fp32 roundings, the sum k more
+    y, back = S.combine(xs, r), S.dispatch_backward(xs, r)
+    u = R.ROUNDOFF[x.dtype]
+    off = (y.float() - x.float()).abs()
+    assert (off <= (u + (64 + k) * 2.0 ** -24) * x.float().abs() + R.TINY[x.dtype]).all()
+    off = (back.float() - k * x.float()).abs()
+    assert (off <= (u + k * 2.0 ** -24) * k * x.float().abs() * (1 + u) + R.TINY[x.dtype]).all()
+    dys, dw = S.combine_backward(x, xs, r)
+    assert torch.equal(dys[-1], (x[r.entries[-1] // k].float() * r.weights.view(-1)[r.entries[-1]]).to(x.dtype))
+    want = (x.double() ** 2).sum(1, keepdim=True)
+    assert ((dw.double() - want).abs() <= (D // 64 + 16) * 2.0 ** -24 * want).all()
