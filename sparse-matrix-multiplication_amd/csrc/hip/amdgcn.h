@@ -98,22 +98,6 @@ __device__ __forceinline__ void lds_dma_x4(u32x4 rsrc, unsigned lds, int index, 
 #pragma clang diagnostic pop
 }
 
-// The same for a raw buffer (stride 0), in two steps that other instructions may
-// come between (none that reads or writes M0): where the load goes, then the load
-// of lane i's 16 bytes from byte `offset` to LDS address lds + ADD + 16 i.  An
-// offset at or past the record count (bytes) writes zeros.  M0 has to be written
-// at least one instruction before the load.
-template <int ADD>
-__device__ __forceinline__ void lds_dma_raw_to(unsigned lds) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-    asm volatile("s_add_u32 m0, %0, %1" : : "s"(lds), "n"(ADD) : "m0", "scc");
-#pragma clang diagnostic pop
-}
-__device__ __forceinline__ void lds_dma_raw_x4(u32x4 rsrc, unsigned offset) {
-    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(offset), "s"(rsrc));
-}
-
 // LDS byte address of a pointer into a __shared__ array.
 __device__ __forceinline__ unsigned lds_address(const void* p) {
     return static_cast<unsigned>(reinterpret_cast<uintptr_t>(

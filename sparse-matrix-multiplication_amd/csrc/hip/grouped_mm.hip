@@ -32,6 +32,22 @@ namespace {
 
 using namespace dev;
 
+// A buffer-to-LDS load from a raw buffer (stride 0), in two steps that other
+// instructions may come between (none that reads or writes M0): where the load goes,
+// then the load of lane i's 16 bytes from byte `offset` to LDS address lds + ADD + 16 i.
+// An offset at or past the record count (bytes) writes zeros.  M0 has to be written at
+// least one instruction before the load.
+template <int ADD>
+__device__ __forceinline__ void lds_dma_raw_to(unsigned lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_add_u32 m0, %0, %1" : : "s"(lds), "n"(ADD) : "m0", "scc");
+#pragma clang diagnostic pop
+}
+__device__ __forceinline__ void lds_dma_raw_x4(u32x4 rsrc, unsigned offset) {
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(offset), "s"(rsrc));
+}
+
 constexpr int kStep = 64;  // contraction steps a staged tile holds
 
 // A byte offset past every buffer's 2^31 - 1 bytes, with room for the 16 that a
