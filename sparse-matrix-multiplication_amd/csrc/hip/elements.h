@@ -24,6 +24,29 @@ __device__ __forceinline__ uint4 load_piece(const void* p) {
     __builtin_memcpy(&v, p, 16);
     return v;
 }
+// The same in whole words around an address that may lie between two of them, where
+// one access would take twice the time.  No word is read that has no element of the
+// piece (so the access stays within the pages of the operand).  The piece itself comes
+// out of the words later, so that nothing waits for the load.
+struct WordPiece {
+    uint4    words;
+    unsigned next;
+};
+__device__ __forceinline__ WordPiece load_words(const void* p) {
+    const unsigned odd = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) & 2u;
+    const char* first = static_cast<const char*>(p) - odd;
+    WordPiece v;
+    __builtin_memcpy(&v.words, __builtin_assume_aligned(first, 4), 16);
+    __builtin_memcpy(&v.next, __builtin_assume_aligned(first + (odd ? 16 : 12), 4), 4);
+    return v;
+}
+__device__ __forceinline__ uint4 piece_of(WordPiece v, const void* p) {
+    const unsigned shift = (static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) & 2u) * 8u;
+    return uint4{__builtin_amdgcn_alignbit(v.words.y, v.words.x, shift),
+                 __builtin_amdgcn_alignbit(v.words.z, v.words.y, shift),
+                 __builtin_amdgcn_alignbit(v.words.w, v.words.z, shift),
+                 __builtin_amdgcn_alignbit(v.next, v.words.w, shift)};
+}
 __device__ __forceinline__ void store_piece(void* p, uint4 v) { __builtin_memcpy(p, &v, 16); }
 // The same for data that the caches are not to keep.
 __device__ __forceinline__ void stream_piece(void* p, uint4 v) {

@@ -840,25 +840,39 @@ __device__ __forceinline__ void wave_share(const T* rows, int rows_here, const T
         pc[j] = cols + static_cast<long long>(c < width ? c : 0) * depth + 8 * q;
     }
     int k = wave * 64;
-    for (; k + (U - 1) * WAVES * 64 + 64 <= depth; k += U * WAVES * 64) {
-        uint4 vr[2 * U][RF], vc[2 * U][CF];
+    auto whole = [&](auto load, auto piece) {
+        for (; k + (U - 1) * WAVES * 64 + 64 <= depth; k += U * WAVES * 64) {
+            decltype(load(pr[0])) vr[2 * U][RF], vc[2 * U][CF];
 #pragma unroll
-        for (int u = 0; u < 2 * U; ++u) {
-            const int at = k + u / 2 * WAVES * 64 + u % 2 * 32;
+            for (int u = 0; u < 2 * U; ++u) {
+                const int at = k + u / 2 * WAVES * 64 + u % 2 * 32;
 #pragma unroll
-            for (int j = 0; j < CF; ++j) vc[u][j] = load_piece(pc[j] + at);
+                for (int j = 0; j < CF; ++j) vc[u][j] = load(pc[j] + at);
 #pragma unroll
-            for (int i = 0; i < RF; ++i) vr[u][i] = load_piece(pr[i] + at);
-        }
+                for (int i = 0; i < RF; ++i) vr[u][i] = load(pr[i] + at);
+            }
 #pragma unroll
-        for (int u = 0; u < 2 * U; ++u)
+            for (int u = 0; u < 2 * U; ++u) {
+                Operand<T> fr[RF];
 #pragma unroll
-            for (int j = 0; j < CF; ++j)
+                for (int i = 0; i < RF; ++i) fr[i] = __builtin_bit_cast(Operand<T>, piece(vr[u][i], pr[i]));
 #pragma unroll
-                for (int i = 0; i < RF; ++i) {
-                    acc[j][i] = mfma(__builtin_bit_cast(Operand<T>, vc[u][j]),
-                                     __builtin_bit_cast(Operand<T>, vr[u][i]), acc[j][i]);
+                for (int j = 0; j < CF; ++j) {
+                    const Operand<T> fc = __builtin_bit_cast(Operand<T>, piece(vc[u][j], pc[j]));
+#pragma unroll
+                    for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc, fr[i], acc[j][i]);
                 }
+            }
+        }
+    };
+    // rows that begin between two words
+    const bool between = ((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(cols)) & 2) != 0 ||
+                         (depth & 1) != 0;
+    if (between) {
+        whole([](const T* p) { return load_words(p); },
+              [](const WordPiece& v, const T* p) { return piece_of(v, p); });
+    } else {
+        whole([](const T* p) { return load_piece(p); }, [](uint4 v, const T*) { return v; });
     }
     for (; k < depth; k += WAVES * 64) {
 #pragma unroll
@@ -1169,21 +1183,22 @@ Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, con
 }
 // How few_rows_product is launched for groups of `rows` rows or so (all are right).
 //   Columns: the rows' own reading counts, and 64 columns share it (2048 rows over 64
-//     groups of 2048 x 4096: 211 us, 282 with sixteen columns).
+//     groups of 2048 x 4096: 211 us, 282 with sixteen columns).  For whole pieces only:
+//     others, which take longer, are tiles' from there on.
 //   Groups: several workgroups a CU hide each other's beginnings and ends (256 rows over
 //     64 groups of 2048 x 4096: 167 us with three, 227 with one).
 //   Single: a workgroup a CU or so, which has all of the LDS for its loads.
 enum class Few { Columns, Groups, Single };
-Few few_form(const TileArgs& a, double rows) {
+Few few_form(const TileArgs& a, double rows, bool pieces) {
     const double row_tiles = a.offsets == nullptr ? std::ceil(rows / 64) : a.groups;
-    if (rows > 32 && row_tiles * std::ceil(a.width / 64.0) >= 192) return Few::Columns;
+    if (pieces && rows > 32 && row_tiles * std::ceil(a.width / 64.0) >= 192) return Few::Columns;
     return a.groups > 1 && rows <= 32 ? Few::Groups : Few::Single;
 }
 template <typename T, bool ADAPT>
 Error launch_few_rows(const TileArgs& a, long long rows, bool pieces, hipStream_t stream,
                       const char* name) {
     constexpr int kAll = 160 * 1024;
-    switch (few_form(a, static_cast<double>(rows))) {
+    switch (few_form(a, static_cast<double>(rows), pieces)) {
         case Few::Columns:
             return launch_few_rows_of<T, 4, 4, 4, 80 * 1024, ADAPT>(a, pieces, stream, name);
         case Few::Groups:
@@ -1221,7 +1236,7 @@ enum class Form { FewRows, Any, Pieces, Wide };
 
 // Estimated microseconds of a form for `row_tiles(edge)` x width tiles of `steps`
 // steps, from measured rates: 64 steps of a 128 x 128 tile take 0.62 us where a CU has
-// one and 0.95 us where it has two (through registers 1.15 us), of a 256 x 256 tile
+// one and 0.95 us where it has two (through registers 1.45 and 2 us), of a 256 x 256 tile
 // 1.55 us, one a CU; `weights` microseconds is what reading the weights takes.
 template <typename F>
 double tile_time(Form form, F row_tiles, int width, double steps, double weights) {
@@ -1231,13 +1246,24 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
     if (form == Form::Wide) {
         return std::max(std::ceil(tiles / 256) * (6 + 1.55 * rounds), weights);
     }
-    const double two = form == Form::Any ? 1.15 : 0.95, one = form == Form::Any ? 1.15 : 0.62;
+    const double two = form == Form::Any ? 2.0 : 0.95, one = form == Form::Any ? 1.45 : 0.62;
     const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
     const double time = whole * (3 + two * rounds) +
                         (rest == 0 ? 0 : 3 + (rest <= 256 ? one : two) * rounds);
     return std::max(time, weights);
 }
 // The form with the least time; each is right for all sizes that its flag allows.
+//   few_rows_product reads weights at 6.3 TB/s, less where the rows' own reading counts;
+//     a round of its workgroups takes 2.2 us for 256 steps (64 columns, two a CU) or 1 us
+//     for 512 (sixteen, one a CU).
+//   Rows that are no whole pieces: 1.1 times as long to read (8 groups of 4000 x 4098,
+//     32 rows: 50 us; tiles 90), twice where they begin between two words (64 groups of
+//     2048 x 4097, 256 rows: 344 us; tiles 258), and 1 us a round for 340 steps, 1.3 or
+//     1.65 times (200 rows x 4000 x 4098: 70 us, tiles 91; x 4097: 90, tiles 92; 192 x
+//     6942 x 1010: 42, tiles 32).
+//   Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s, W [k][c]
+//     at 5.8 (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows
+//     257, 285).  Adapters that change within sixteen rows hold them up.
 Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
     const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     const double mean = a.total / groups;
@@ -1246,32 +1272,31 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
     auto row_tiles = [&](int edge) {
         return groups == 1 ? std::ceil(mean / edge) : groups * std::max(1.0, mean / edge + 0.5);
     };
-    // few_rows_product reads weights at 6.3 TB/s, less where the rows' own reading counts;
-    // a round of its workgroups takes 2.2 us for 256 steps (64 columns, two a CU) or 1 us
-    // for 512 (sixteen, one a CU).  Operands that are no whole pieces take three times as
-    // long.  Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s,
-    // W [k][c] at 5.8.
-    // (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows 257, 285)
+    const bool words = a.depth % 2 == 0 && ((reinterpret_cast<uintptr_t>(a.rows) |
+                                             reinterpret_cast<uintptr_t>(a.cols)) & 2) == 0;
     const double rows = groups == 1 ? mean : 2 * mean;
     const double tiles64 = groups == 1 ? std::ceil(mean / 64)
                                        : groups * std::max(1.0, mean / 64 + 0.5);
-    double few = weights / 6.3e6 * (1 + mean / 160);
-    switch (few_form(a, rows)) {
+    double few = weights / 6.3e6 * (1 + mean / 160) * (pieces ? 1 : words ? 1.1 : 2);
+    switch (few_form(a, rows, pieces)) {
         case Few::Columns:
-            if (!pieces) return Form::Any;  // never behind it: three times its time is more
             few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 64.0) / 512) *
                                     (2 + 2.2 * std::ceil(a.depth / 256.0)));
             break;
-        case Few::Single:
-            few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 16.0) / 256) *
-                                    (3 + std::ceil(a.depth / 512.0)));
+        case Few::Single: {
+            const double round = pieces ? 3 + std::ceil(a.depth / 512.0)
+                                        : (1 + a.depth / 340.0) * (words ? 1.3 : 1.65);
+            few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 16.0) / 256) * round);
             break;
+        }
         case Few::Groups: break;
     }
-    few = 4 + few * (pieces ? 1 : 3);
-    // adapters that change within sixteen rows hold tiles up
+    few += 4;
     const double reading = weights / (few_allowed ? 4.1e6 : 5.8e6) + (a.ids != nullptr ? 8 : 0);
-    auto time = [&](Form f) { return tile_time(f, row_tiles, a.width, a.depth, reading); };
+    auto time = [&](Form f) {
+        return tile_time(f, row_tiles, a.width, a.depth, reading) +
+               (f == Form::Any && a.ids != nullptr ? 6 : 0);
+    };
     Form best = pieces ? Form::Pieces : Form::Any;
     if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
     return few_allowed && few <= time(best) ? Form::FewRows : best;
