@@ -375,7 +375,8 @@ int spmm_c_hybrid_run(const spmm_hybrid_plan_t* plan, const spmm_csr_t* h_A,
  * route: d_logits [tokens, experts].  The k largest, ties to the lowest expert;
  *   -inf is never chosen (a token of only -inf has no expert), NaN is above all
  *   numbers and makes the token's weights NaN.  over: the softmax over the
- *   chosen experts, or over all.  d_workspace: spmm_c_route_workspace bytes.
+ *   chosen experts, or over all.  d_workspace: spmm_c_route_workspace bytes;
+ *   calls that share one must not overlap.
  *   experts <= 1024, k <= 64, k <= experts (SPMM_UNSUPPORTED, SPMM_INVALID).
  * route_backward: d_dlogits of the logits' type; d_logits is read for
  *   SPMM_OVER_ALL only.
@@ -415,8 +416,10 @@ int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int to
  * grouped_mm: the block-diagonal product of rows in group order with their
  *   group's weights.  Group g has rows [d_offsets[g], d_offsets[g+1]) of d_x
  *   [rows, depth]; d_w is [groups, width, depth], or [groups, depth, width]
- *   with w_in_rows; d_out [rows, width], rows in no group zero.  The gradient
- *   for x is the same call on dout with w_in_rows the other way round.
+ *   with w_in_rows; d_out [rows, width], rows in no group (before the first and
+ *   behind the last) zero.  d_offsets ascends from any row on; values outside
+ *   [0, rows] are taken as its ends.  The gradient for x is the same call on dout
+ *   with w_in_rows the other way round.
  * grouped_outer: d_out[g] [height, width] = the sum over the group's rows of
  *   p[s]^T q[s], zero for an empty group: the gradient of the weights (p = dout,
  *   q = x, or the other way round for w_in_rows).
