@@ -40,8 +40,8 @@ __device__ __forceinline__ WordPiece load_words(const void* p) {
     __builtin_memcpy(&v.next, __builtin_assume_aligned(first + (odd ? 16 : 12), 4), 4);
     return v;
 }
-__device__ __forceinline__ uint4 piece_of(WordPiece v, const void* p) {
-    const unsigned shift = (static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) & 2u) * 8u;
+__device__ __forceinline__ uint4 piece_of(WordPiece v, unsigned byte) {
+    const unsigned shift = (byte & 2u) * 8u;  // byte: where the piece begins
     return uint4{__builtin_amdgcn_alignbit(v.words.y, v.words.x, shift),
                  __builtin_amdgcn_alignbit(v.words.z, v.words.y, shift),
                  __builtin_amdgcn_alignbit(v.words.w, v.words.z, shift),

@@ -236,48 +236,70 @@ struct Operands {
     static_assert(N * kStep / 8 % THREADS == 0, "whole pieces a thread");
     static_assert(!MAJOR || N >= 128, "the places of a row are 32 bytes x 8");
 
-    int base[kPieces];   // element offset of the piece from the tile's first element
-    int index[kPieces];  // its first contraction step inside the tile
-    int room[kPieces];   // valid elements of the piece in the other direction's bound (0 - 8)
+    unsigned at[kPieces];     // byte offset of the piece from the tile's first word
+    int      index[kPieces];  // its first contraction step inside the tile
+    int      ld, bound;
 
-    // ld: elements between memory rows; bound: valid rows (columns for MAJOR).
-    __device__ __forceinline__ void place(int ld, int bound) {
+    // The tile's first element lies at `first`; ld: elements between memory rows;
+    // bound: valid rows (columns for MAJOR), of which there may be more than N.
+    __device__ __forceinline__ void place(const T* first, int row_elements, int valid) {
+        ld    = row_elements;
+        bound = valid;
+        const unsigned odd = static_cast<unsigned>(reinterpret_cast<uintptr_t>(first)) & 2u;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int p = i * THREADS + threadIdx.x;
+            int n, element;
             if constexpr (MAJOR) {
                 const int k = p / (N / 8);
                 const int f = (k & 3) | ((k >> 3) & 1) << 2;
-                const int c = (p % (N / 8)) ^ (f << 1);
-                base[i]  = k * ld + c * 8;
+                n        = ((p % (N / 8)) ^ (f << 1)) * 8;
+                element  = k * ld + n;
                 index[i] = k;
-                room[i]  = max(0, min(8, bound - c * 8));
             } else {
-                const int n = p / 8;
-                const int c = (p % 8) ^ (n & 7);
-                base[i]  = n * ld + c * 8;
-                index[i] = c * 8;
-                room[i]  = n < bound ? 8 : 0;
+                n        = p / 8;
+                index[i] = ((p % 8) ^ (n & 7)) * 8;
+                element  = n * ld + index[i];
             }
+            at[i] = n < bound ? static_cast<unsigned>(element) * 2u + odd : kAbsent;
         }
     }
-    // Elements of piece i that exist when `left` contraction steps are left.
-    __device__ __forceinline__ int count(int i, int left) const {
-        if constexpr (MAJOR) return index[i] < left ? room[i] : 0;
-        return room[i] == 0 ? 0 : max(0, min(8, left - index[i]));
-    }
-    __device__ __forceinline__ void load(const T* tile, int left, uint4 (&v)[kPieces]) const {
+    // Loads the tile at `tile` with `left` contraction steps left, in whole words.  The
+    // buffer ends with the tile's last valid row, so that no word without an element is
+    // read; what a piece holds behind its row's end is cut off by store (MAJOR: it belongs
+    // to columns past the bound, which are never stored).  ODD: pieces may begin between
+    // two words.
+    template <bool ODD>
+    __device__ __forceinline__ void load(const T* tile, int left, WordPiece (&v)[kPieces]) const {
+        const long long rows = MAJOR ? min(left, kStep) : min(bound, N);
+        const long long end  = ((rows - 1) * ld + (MAJOR ? bound : left)) * 2;
+        const uintptr_t first = reinterpret_cast<uintptr_t>(tile);
+        const long long bytes = (end + static_cast<long long>(first & 2) + 3) / 4 * 4;
+        const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(
+            reinterpret_cast<void*>(first & ~uintptr_t{2}), 0,
+            static_cast<int>(min(bytes, 0x7ffffffcLL)), kBufWord3);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int n = count(i, left);
-            v[i] = n == 8 ? load_piece(tile + base[i]) : n == 0 ? uint4{0, 0, 0, 0}
-                                                                : load_part(tile + base[i], n);
+            const unsigned o = index[i] < left ? at[i] & ~3u : kAbsent;
+            v[i].words = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buffer, o, 0, 0));
+            if constexpr (ODD) v[i].next = __builtin_amdgcn_raw_buffer_load_b32(buffer, o, 16, 0);
         }
     }
-    __device__ __forceinline__ void store(T* lds, const uint4 (&v)[kPieces]) const {
+    template <bool ODD>
+    __device__ __forceinline__ void store(T* lds, int left, const WordPiece (&v)[kPieces]) const {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            *reinterpret_cast<uint4*>(lds + (i * THREADS + threadIdx.x) * 8) = v[i];
+            uint4 x = ODD ? piece_of(v[i], at[i]) : v[i].words;
+            if constexpr (!MAJOR) {
+                if (left < kStep) {
+                    const int n = left - index[i];  // elements of the piece that exist
+                    auto cut = [&](unsigned w, int e) {
+                        return n >= e + 2 ? w : n == e + 1 ? w & 0xffffu : 0u;
+                    };
+                    x = uint4{cut(x.x, 0), cut(x.y, 2), cut(x.z, 4), cut(x.w, 6)};
+                }
+            }
+            *reinterpret_cast<uint4*>(lds + (i * THREADS + threadIdx.x) * 8) = x;
         }
     }
     // Operand of columns n0 .. n0+15, contraction steps 32 half .. +31: lane l holds
@@ -553,10 +575,14 @@ __device__ __forceinline__ void zero_tile(const TileArgs& a, const Tile<T>& t) {
 //
 // The 128 x 128 tile of medium products, and of any sizes and alignment: four waves
 // take a quarter each, two buffers of 64 steps.  PIECES: the operands' rows are
-// whole 16-byte pieces, which go straight into LDS; otherwise through registers,
-// those at an edge element by element.
+// whole 16-byte pieces, which go straight into LDS.  Otherwise they go through
+// registers, as the words around each piece, from buffers that end with the operand:
+// straight code with eight or sixteen loads under way.  (With a branch a piece for those
+// at an edge the compiler waited for each load: 8 groups of 4000 x 4098 over 16384 rows
+// 930 us, 810 so; their weights' gradient 1280, 790.  Two workgroups a CU need the
+// registers bounded: 1390 with one.)
 template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT, bool PIECES>
-__global__ __launch_bounds__(256) void tile_product(TileArgs a) {
+__global__ __launch_bounds__(256, PIECES ? 1 : 2) void tile_product(TileArgs a) {
     constexpr int BR = 128, BC = 128, WC = 2, RF = 4, CF = 4;
     using Rows = Operands<T, BR, GRAD, 256>;
     using Cols = Operands<T, BC, GRAD || COLS_MAJOR, 256>;
@@ -624,29 +650,37 @@ __global__ __launch_bounds__(256) void tile_product(TileArgs a) {
     } else {
         Rows pr;
         Cols pc;
-        pr.place(t.ld_rows, t.rows_here);
-        pc.place(t.ld_cols, a.width - t.c0);
-        uint4 vr[Rows::kPieces], vc[Cols::kPieces];
-        if (tiles > 0) {
-            pr.load(t.rows, t.depth, vr);
-            pc.load(t.cols, t.depth, vc);
-            pr.store(rows_at(0), vr);
-            pc.store(cols_at(0), vc);
-        }
-        for (int it = 0; it < tiles; ++it) {
-            // the tile is written, and the other buffer's readers are done
-            __syncthreads();
-            const bool more = it + 1 < tiles;
-            if (more) {
-                const int left = t.depth - (it + 1) * kStep;
-                pr.load(t.rows + (it + 1) * t.step_rows, left, vr);
-                pc.load(t.cols + (it + 1) * t.step_cols, left, vc);
+        pr.place(t.rows, t.ld_rows, t.rows_here);
+        pc.place(t.cols, t.ld_cols, a.width - t.c0);
+        WordPiece vr[Rows::kPieces], vc[Cols::kPieces];
+        auto run = [&](auto odd) {
+            auto load = [&](int it) {
+                const int left = t.depth - it * kStep;
+                pr.template load<odd.value>(t.rows + it * t.step_rows, left, vr);
+                pc.template load<odd.value>(t.cols + it * t.step_cols, left, vc);
+            };
+            auto store = [&](int it) {
+                const int left = t.depth - it * kStep;
+                pr.template store<odd.value>(rows_at(it), left, vr);
+                pc.template store<odd.value>(cols_at(it), left, vc);
+            };
+            load(0);
+            store(0);
+            for (int it = 0; it < tiles; ++it) {
+                // the tile is written, and the other buffer's readers are done
+                __syncthreads();
+                if (it + 1 < tiles) load(it + 1);
+                multiply(it);
+                if (it + 1 < tiles) store(it + 1);
             }
-            multiply(it);
-            if (more) {
-                pr.store(rows_at(it + 1), vr);
-                pc.store(cols_at(it + 1), vc);
-            }
+        };
+        const uintptr_t ends = reinterpret_cast<uintptr_t>(t.rows) | reinterpret_cast<uintptr_t>(t.cols) |
+                               static_cast<uintptr_t>(t.ld_rows | t.ld_cols) * 2;
+        if (tiles == 0) {
+        } else if ((ends & 2) != 0) {
+            run(std::true_type{});
+        } else {
+            run(std::false_type{});
         }
     }
     lds_barrier();  // the operands' LDS is free
@@ -870,7 +904,9 @@ __device__ __forceinline__ void wave_share(const T* rows, int rows_here, const T
                          (depth & 1) != 0;
     if (between) {
         whole([](const T* p) { return load_words(p); },
-              [](const WordPiece& v, const T* p) { return piece_of(v, p); });
+              [](const WordPiece& v, const T* p) {
+                  return piece_of(v, static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)));
+              });
     } else {
         whole([](const T* p) { return load_piece(p); }, [](uint4 v, const T*) { return v; });
     }
@@ -1236,7 +1272,7 @@ enum class Form { FewRows, Any, Pieces, Wide };
 
 // Estimated microseconds of a form for `row_tiles(edge)` x width tiles of `steps`
 // steps, from measured rates: 64 steps of a 128 x 128 tile take 0.62 us where a CU has
-// one and 0.95 us where it has two (through registers 1.45 and 2 us), of a 256 x 256 tile
+// one and 0.95 us where it has two (through registers 1 and 1.5 us), of a 256 x 256 tile
 // 1.55 us, one a CU; `weights` microseconds is what reading the weights takes.
 template <typename F>
 double tile_time(Form form, F row_tiles, int width, double steps, double weights) {
@@ -1246,7 +1282,7 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
     if (form == Form::Wide) {
         return std::max(std::ceil(tiles / 256) * (6 + 1.55 * rounds), weights);
     }
-    const double two = form == Form::Any ? 2.0 : 0.95, one = form == Form::Any ? 1.45 : 0.62;
+    const double two = form == Form::Any ? 1.5 : 0.95, one = form == Form::Any ? 1 : 0.62;
     const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
     const double time = whole * (3 + two * rounds) +
                         (rest == 0 ? 0 : 3 + (rest <= 256 ? one : two) * rounds);
@@ -1257,10 +1293,10 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
 //     a round of its workgroups takes 2.2 us for 256 steps (64 columns, two a CU) or 1 us
 //     for 512 (sixteen, one a CU).
 //   Rows that are no whole pieces: 1.1 times as long to read (8 groups of 4000 x 4098,
-//     32 rows: 50 us; tiles 90), twice where they begin between two words (64 groups of
-//     2048 x 4097, 256 rows: 344 us; tiles 258), and 1 us a round for 340 steps, 1.3 or
-//     1.65 times (200 rows x 4000 x 4098: 70 us, tiles 91; x 4097: 90, tiles 92; 192 x
-//     6942 x 1010: 42, tiles 32).
+//     32 rows: 50 us; tiles 60), twice where they begin between two words (64 groups of
+//     2048 x 4097, 256 rows: 344 us; tiles 222), and 1 us a round for 340 steps, 1.3 or
+//     1.65 times (100 rows x 4000 x 4098: 40 us, tiles 65; 192 x 6942 x 1010: 42, tiles
+//     27).
 //   Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s, W [k][c]
 //     at 5.8 (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows
 //     257, 285).  Adapters that change within sixteen rows hold them up.
