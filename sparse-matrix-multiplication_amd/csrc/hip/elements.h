@@ -6,6 +6,8 @@
 
 #include <cstdint>
 
+#include "amdgcn.h"
+
 namespace spmm {
 namespace engine {
 namespace dev {
@@ -24,28 +26,43 @@ __device__ __forceinline__ uint4 load_piece(const void* p) {
     __builtin_memcpy(&v, p, 16);
     return v;
 }
-// The same in whole words around an address that may lie between two of them, where
-// one access would take twice the time.  No word is read that has no element of the
-// piece (so the access stays within the pages of the operand).  The piece itself comes
-// out of the words later, so that nothing waits for the load.
+// Pieces of 16-bit elements in whole words, from a buffer that begins at the word of an
+// operand's first element and ends with the word of its last, so that no other word is
+// read; past it are zeros (each word is looked at by itself; no elements: all zeros).
+// Sixteen bytes from between two words would take twice the time: those come as the
+// words around them and a shift.  Pieces come out of the words later, so that nothing
+// waits for a load.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t words_buffer(const void* first, long long elements) {
+    const uintptr_t at    = reinterpret_cast<uintptr_t>(first);
+    const long long bytes =
+        elements > 0 ? (2 * elements + static_cast<long long>(at & 2) + 3) / 4 * 4 : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(at & ~uintptr_t{2}), 0,
+                                             static_cast<int>(bytes < 0x7ffffffc ? bytes : 0x7ffffffc),
+                                             kBufWord3);
+}
 struct WordPiece {
     uint4    words;
-    unsigned next;
+    unsigned next;  // ODD only
 };
-__device__ __forceinline__ WordPiece load_words(const void* p) {
-    const unsigned odd = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) & 2u;
-    const char* first = static_cast<const char*>(p) - odd;
+// byte: from the buffer's begin; at or past 2^31 there are zeros.
+template <bool ODD>
+__device__ __forceinline__ WordPiece load_words(__amdgpu_buffer_rsrc_t buffer, unsigned byte) {
     WordPiece v;
-    __builtin_memcpy(&v.words, __builtin_assume_aligned(first, 4), 16);
-    __builtin_memcpy(&v.next, __builtin_assume_aligned(first + (odd ? 16 : 12), 4), 4);
+    v.words = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buffer, byte & ~3u, 0, 0));
+    v.next  = ODD ? __builtin_amdgcn_raw_buffer_load_b32(buffer, byte & ~3u, 16, 0) : 0u;
     return v;
 }
 __device__ __forceinline__ uint4 piece_of(WordPiece v, unsigned byte) {
-    const unsigned shift = (byte & 2u) * 8u;  // byte: where the piece begins
+    const unsigned shift = (byte & 2u) * 8u;
     return uint4{__builtin_amdgcn_alignbit(v.words.y, v.words.x, shift),
                  __builtin_amdgcn_alignbit(v.words.z, v.words.y, shift),
                  __builtin_amdgcn_alignbit(v.words.w, v.words.z, shift),
                  __builtin_amdgcn_alignbit(v.next, v.words.w, shift)};
+}
+// The first n elements of a piece (any n), zeros behind them.
+__device__ __forceinline__ uint4 first_of(uint4 v, int n) {
+    auto cut = [&](unsigned w, int e) { return n >= e + 2 ? w : n == e + 1 ? w & 0xffffu : 0u; };
+    return uint4{cut(v.x, 0), cut(v.y, 2), cut(v.z, 4), cut(v.w, 6)};
 }
 __device__ __forceinline__ void store_piece(void* p, uint4 v) { __builtin_memcpy(p, &v, 16); }
 // The same for data that the caches are not to keep.

@@ -272,17 +272,11 @@ struct Operands {
     template <bool ODD>
     __device__ __forceinline__ void load(const T* tile, int left, WordPiece (&v)[kPieces]) const {
         const long long rows = MAJOR ? min(left, kStep) : min(bound, N);
-        const long long end  = ((rows - 1) * ld + (MAJOR ? bound : left)) * 2;
-        const uintptr_t first = reinterpret_cast<uintptr_t>(tile);
-        const long long bytes = (end + static_cast<long long>(first & 2) + 3) / 4 * 4;
-        const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(
-            reinterpret_cast<void*>(first & ~uintptr_t{2}), 0,
-            static_cast<int>(min(bytes, 0x7ffffffcLL)), kBufWord3);
+        const __amdgpu_buffer_rsrc_t buffer =
+            words_buffer(tile, (rows - 1) * ld + (MAJOR ? bound : left));
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const unsigned o = index[i] < left ? at[i] & ~3u : kAbsent;
-            v[i].words = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buffer, o, 0, 0));
-            if constexpr (ODD) v[i].next = __builtin_amdgcn_raw_buffer_load_b32(buffer, o, 16, 0);
+            v[i] = load_words<ODD>(buffer, index[i] < left ? at[i] : kAbsent);
         }
     }
     template <bool ODD>
@@ -291,13 +285,7 @@ struct Operands {
         for (int i = 0; i < kPieces; ++i) {
             uint4 x = ODD ? piece_of(v[i], at[i]) : v[i].words;
             if constexpr (!MAJOR) {
-                if (left < kStep) {
-                    const int n = left - index[i];  // elements of the piece that exist
-                    auto cut = [&](unsigned w, int e) {
-                        return n >= e + 2 ? w : n == e + 1 ? w & 0xffffu : 0u;
-                    };
-                    x = uint4{cut(x.x, 0), cut(x.y, 2), cut(x.z, 4), cut(x.w, 6)};
-                }
+                if (left < kStep) x = first_of(x, left - index[i]);
             }
             *reinterpret_cast<uint4*>(lds + (i * THREADS + threadIdx.x) * 8) = x;
         }
@@ -410,26 +398,18 @@ struct Adapters {
     }
     // B_a's rows c0 .. of an adapter, 32 of the rank from k0 on.
     __device__ __forceinline__ void read_b(int adapter, int k0, Operand<T> (&fc)[CF]) const {
-        const int k = k0 + 8 * ((threadIdx.x & 63) >> 4), c = c0 + (threadIdx.x & 15);
-        const T* first = b + static_cast<long long>(adapter) * width * rank;
-        if constexpr (PIECES) {
-            const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<T*>(first), 0, 0x7fffffff, kBufWord3);
+        const int k = k0 + 8 * ((threadIdx.x & 63) >> 4);
+        const int here = min(width - c0, CF * 16);  // may be below 1
+        const T* first = b + (static_cast<long long>(adapter) * width + c0) * rank;
+        const unsigned odd = PIECES ? 0u : static_cast<unsigned>(reinterpret_cast<uintptr_t>(first)) & 2u;
+        const __amdgpu_buffer_rsrc_t buffer = words_buffer(first, static_cast<long long>(max(here, 0)) * rank);
 #pragma unroll
-            for (int j = 0; j < CF; ++j) {
-                const bool in = c + 16 * j < width && k < rank;
-                fc[j] = __builtin_bit_cast(Operand<T>, __builtin_amdgcn_raw_buffer_load_b128(
-                    buffer, in ? ((c + 16 * j) * rank + k) * 2 : static_cast<int>(kAbsent), 0, 0));
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < CF; ++j) {
-                const int n = c + 16 * j < width ? min(8, rank - k) : 0;
-                const T* p = first + static_cast<long long>(c + 16 * j) * rank + k;
-                fc[j] = __builtin_bit_cast(Operand<T>, n == 8 ? load_piece(p)
-                                                       : n <= 0 ? uint4{0, 0, 0, 0}
-                                                                : load_part(p, n));
-            }
+        for (int j = 0; j < CF; ++j) {
+            const int c = j * 16 + (threadIdx.x & 15);
+            const unsigned at = c < here && k < rank ? static_cast<unsigned>(c * rank + k) * 2u + odd
+                                                     : kAbsent;
+            const WordPiece v = load_words<!PIECES>(buffer, at);
+            fc[j] = __builtin_bit_cast(Operand<T>, PIECES ? v.words : first_of(piece_of(v, at), rank - k));
         }
     }
     // sums: the wave's rows 16 i .. in LDS, `pitch` floats a row; mine: id[i].
@@ -853,84 +833,68 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
 // Sums of a wave's share of the contraction for CF x 16 columns (rows of `cols`,
 // `width` of them from its first) and RF x 16 rows (of `rows`, `rows_here`), all
 // with `depth` contiguous elements: wave w of WAVES takes every WAVES-th 64 steps.
-// Operands come straight from memory; U times 64 steps' loads are in flight.
-template <typename T, int RF, int CF, int WAVES, int U>
+// Operands come straight from memory, as the words around each piece; 64 steps' loads
+// are under way (with 128, fewer workgroups a CU: 50 rows x 8000 x 1002 15 us, 10 so).
+template <typename T, int RF, int CF, int WAVES>
 __device__ __forceinline__ void wave_share(const T* rows, int rows_here, const T* cols, int width,
                                            int depth, f32x4 (&acc)[CF][RF]) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int s = lane & 15, q = lane >> 4;
-    // a row past the end reads the first one: its products are never stored
-    const T* pr[RF];
-    const T* pc[CF];
+    const unsigned odd_r = static_cast<unsigned>(reinterpret_cast<uintptr_t>(rows)) & 2u;
+    const unsigned odd_c = static_cast<unsigned>(reinterpret_cast<uintptr_t>(cols)) & 2u;
+    const __amdgpu_buffer_rsrc_t br = words_buffer(rows, static_cast<long long>(rows_here) * depth);
+    const __amdgpu_buffer_rsrc_t bc = words_buffer(cols, static_cast<long long>(min(width, CF * 16)) * depth);
+    unsigned ar[RF], ac[CF];  // byte offsets of the first piece; rows past the end are zeros
 #pragma unroll
     for (int i = 0; i < RF; ++i) {
         const int r = i * 16 + s;
-        pr[i] = rows + static_cast<long long>(r < rows_here ? r : 0) * depth + 8 * q;
+        ar[i] = r < rows_here ? static_cast<unsigned>(r * depth + 8 * q) * 2u + odd_r : kAbsent;
     }
 #pragma unroll
     for (int j = 0; j < CF; ++j) {
         const int c = j * 16 + s;
-        pc[j] = cols + static_cast<long long>(c < width ? c : 0) * depth + 8 * q;
+        ac[j] = c < width ? static_cast<unsigned>(c * depth + 8 * q) * 2u + odd_c : kAbsent;
     }
-    int k = wave * 64;
-    auto whole = [&](auto load, auto piece) {
-        for (; k + (U - 1) * WAVES * 64 + 64 <= depth; k += U * WAVES * 64) {
-            decltype(load(pr[0])) vr[2 * U][RF], vc[2 * U][CF];
+    auto run = [&](auto odd) {
+        for (int k = wave * 64; k < depth; k += WAVES * 64) {
+            WordPiece vr[2][RF], vc[2][CF];
 #pragma unroll
-            for (int u = 0; u < 2 * U; ++u) {
-                const int at = k + u / 2 * WAVES * 64 + u % 2 * 32;
-#pragma unroll
-                for (int j = 0; j < CF; ++j) vc[u][j] = load(pc[j] + at);
-#pragma unroll
-                for (int i = 0; i < RF; ++i) vr[u][i] = load(pr[i] + at);
-            }
-#pragma unroll
-            for (int u = 0; u < 2 * U; ++u) {
-                Operand<T> fr[RF];
-#pragma unroll
-                for (int i = 0; i < RF; ++i) fr[i] = __builtin_bit_cast(Operand<T>, piece(vr[u][i], pr[i]));
+            for (int half = 0; half < 2; ++half) {
+                const int at = k + 32 * half;
+                const bool in = at + 8 * q < depth;
 #pragma unroll
                 for (int j = 0; j < CF; ++j) {
-                    const Operand<T> fc = __builtin_bit_cast(Operand<T>, piece(vc[u][j], pc[j]));
+                    vc[half][j] = load_words<odd.value>(bc, in ? ac[j] + 2u * at : kAbsent);
+                }
+#pragma unroll
+                for (int i = 0; i < RF; ++i) {
+                    vr[half][i] = load_words<odd.value>(br, in ? ar[i] + 2u * at : kAbsent);
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int left = depth - k - 32 * half;
+                auto operand = [&](const WordPiece& v, unsigned byte) {
+                    uint4 x = odd.value ? piece_of(v, byte) : v.words;
+                    if (left < 32) x = first_of(x, left - 8 * q);
+                    return __builtin_bit_cast(Operand<T>, x);
+                };
+                Operand<T> fr[RF];
+#pragma unroll
+                for (int i = 0; i < RF; ++i) fr[i] = operand(vr[half][i], ar[i]);
+#pragma unroll
+                for (int j = 0; j < CF; ++j) {
+                    const Operand<T> fc = operand(vc[half][j], ac[j]);
 #pragma unroll
                     for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc, fr[i], acc[j][i]);
                 }
             }
         }
     };
-    // rows that begin between two words
-    const bool between = ((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(cols)) & 2) != 0 ||
-                         (depth & 1) != 0;
-    if (between) {
-        whole([](const T* p) { return load_words(p); },
-              [](const WordPiece& v, const T* p) {
-                  return piece_of(v, static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)));
-              });
-    } else {
-        whole([](const T* p) { return load_piece(p); }, [](uint4 v, const T*) { return v; });
-    }
-    for (; k < depth; k += WAVES * 64) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int at = k + 32 * half;
-            const int n = min(8, depth - at - 8 * q);
-            auto read = [&](const T* p) {
-                return __builtin_bit_cast(Operand<T>, n == 8 ? load_piece(p + at)
-                                                      : n <= 0 ? uint4{0, 0, 0, 0}
-                                                               : load_part(p + at, n));
-            };
-            Operand<T> fr[RF];
-#pragma unroll
-            for (int i = 0; i < RF; ++i) fr[i] = read(pr[i]);
-#pragma unroll
-            for (int j = 0; j < CF; ++j) {
-                const Operand<T> fc = read(pc[j]);
-#pragma unroll
-                for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc, fr[i], acc[j][i]);
-            }
-        }
-    }
+    // rows that begin between two words, or not
+    if (((odd_r | odd_c) & 2u) != 0 || (depth & 1) != 0) run(std::true_type{});
+    else run(std::false_type{});
 }
 
 // wave_share for operands whose rows are whole 16-byte pieces (the same sums in the
@@ -1080,7 +1044,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T
             ring_share<T, RF, CF, WAVES, D>(s_ring, x, rows_here, d, a.rank - r0, a.depth, acc);
             __syncthreads();
         } else {
-            wave_share<T, RF, CF, WAVES, 2>(x, rows_here, d, a.rank - r0, a.depth, acc);
+            wave_share<T, RF, CF, WAVES>(x, rows_here, d, a.rank - r0, a.depth, acc);
         }
         Shares<RF, CF, WAVES> shares(s_ring);
         shares.put(acc);
@@ -1123,7 +1087,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_product(TileArgs a) {
             ring_share<T, RF, CF, WAVES, D>(s_ring, x, rows_here, w, a.width - c0, a.depth, acc);
             __syncthreads();
         } else {
-            wave_share<T, RF, CF, WAVES, 2>(x, rows_here, w, a.width - c0, a.depth, acc);
+            wave_share<T, RF, CF, WAVES>(x, rows_here, w, a.width - c0, a.depth, acc);
         }
     }
     Shares<RF, CF, WAVES> shares(s_ring);
@@ -1293,9 +1257,9 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
 //     a round of its workgroups takes 2.2 us for 256 steps (64 columns, two a CU) or 1 us
 //     for 512 (sixteen, one a CU).
 //   Rows that are no whole pieces: 1.1 times as long to read (8 groups of 4000 x 4098,
-//     32 rows: 50 us; tiles 60), twice where they begin between two words (64 groups of
+//     32 rows: 47 us; tiles 60), twice where they begin between two words (64 groups of
 //     2048 x 4097, 256 rows: 344 us; tiles 222), and 1 us a round for 340 steps, 1.3 or
-//     1.65 times (100 rows x 4000 x 4098: 40 us, tiles 65; 192 x 6942 x 1010: 42, tiles
+//     1.65 times (100 rows x 4000 x 4098: 35 us, tiles 65; 192 x 6942 x 1010: 42, tiles
 //     27).
 //   Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s, W [k][c]
 //     at 5.8 (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows

@@ -165,3 +165,26 @@ def test_more_than_32_bits_of_elements(S):
         _check(y[s], X @ W.t(), X.abs() @ W.abs().t(), K)
         _check(dx[s], DY @ W, DY.abs() @ W.abs(), N)
         _check(dw[g], DY.t() @ X, DY.abs().t() @ X.abs(), each)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 200])
+def test_adapters_of_many_columns(S, T):
+    """An adapter's second matrix of more than 2^31 bytes."""
+    N, K, rank = 2100000, 8, 520
+    dtype, u = torch.bfloat16, R.ROUNDOFF[torch.bfloat16]
+    x, w = _values((T, K), dtype, 1), _values((N, K), dtype, 2, K ** -0.5)
+    a = _values((1, rank, K), dtype, 3, K ** -0.5)
+    b = torch.zeros((1, N, rank), dtype=dtype, device="cuda")
+    b[:, -300:] = _values((1, 300, rank), dtype, 4, rank ** -0.5)
+    ids = torch.zeros(T, dtype=torch.int32, device="cuda")
+    y = S.adapter_mm(x, w, a, b, ids)
+    X, W, A, B = (v.double() for v in (x, w[-400:], a[0], b[0, -400:]))
+    h = X @ A.t()
+    want = X @ W.t() + h @ B.t()
+    size = X.abs() @ W.abs().t() + h.abs() @ B.abs().t()
+    low = (u * h.abs() + (K + 1) * 2.0 ** -24 * (X.abs() @ A.abs().t())) @ B.abs().t()
+    off = (y[:, -400:].double() - want).abs()
+    allowed = u * want.abs() + (1 + u) * ((K + rank) * 2.0 ** -24 * size + low * (1 + u)) \
+        + R.TINY[dtype]
+    assert (off <= allowed).all(), float((off / allowed).max())
