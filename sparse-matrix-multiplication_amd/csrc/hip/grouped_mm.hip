@@ -8,10 +8,10 @@
 //
 // The first is the product of a block-diagonal matrix (each group's rows a block)
 // with dense weights, and the adapters extend the contraction by a block-sparse
-// operand: one block of h a row against the stacked B.  One tile kernel does all
-// three.  A workgroup computes BR rows x BC columns on matrix cores
-// (v_mfma_f32_16x16x32, fp32 sums), staging 64 steps of the contraction at a time
-// through two LDS buffers.
+// operand: one block of h a row against the stacked B.  Tile kernels (256 x 256, 128 x
+// 128) and a kernel for few rows do all three on matrix cores (v_mfma_f32_16x16x32,
+// fp32 sums), 64 steps of the contraction at a time through LDS.  Many rows are bound by
+// the matrix cores and the clock they leave, few by reading W.
 
 #include <hip/hip_runtime.h>
 
@@ -689,6 +689,11 @@ __global__ __launch_bounds__(256, PIECES ? 1 : 2) void tile_product(TileArgs a) 
 //   the five youngest slots (the next tile's C0, C1, L are there), behind part 0
 //   all but six (this tile's H is there), and for its operand reads.
 //   Past the contraction's end loads write zeros, so the counts always hold.
+//
+// 8 groups of 8192 x 4096 over 16384 rows: 864 us, 1270 TFLOP/s; in one group 776 us,
+// 1420.  The matrix cores are busy for 72% of the time, and at that the clock falls to
+// 1.4 - 1.65 GHz (data of zeros takes a sixth less time).  A tile costs 6 us beside its
+// 1.55 us for 64 steps: beginning, first loads and stores.
 template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT>
 __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
     constexpr int BR = 256, BC = 256, RF = 8, CF = 8;
@@ -900,8 +905,8 @@ __device__ __forceinline__ void wave_share(const T* rows, int rows_here, const T
 // wave_share for operands whose rows are whole 16-byte pieces (the same sums in the
 // same order): a wave's pieces go through a ring of D stages of LDS of its own (no
 // barriers).  A load then brings eight rows' whole cache lines; operands read
-// straight from memory are 64 bytes of sixteen rows, which the cache serves at a
-// third of the rate (48 rows by 16 columns of 4096 steps: 17 us against 9).
+// straight from memory are 64 bytes of sixteen rows, which the cache serves more
+// slowly (8 groups of 4000 columns, 32 rows: 4096 steps 42 us, 4098 47).
 //   ring: WAVES x D x (RF + CF) x 2 KB.
 template <typename T, int RF, int CF, int WAVES, int D>
 __device__ __forceinline__ void ring_share(char* ring, const T* rows, int rows_here, const T* cols,
@@ -1000,12 +1005,14 @@ struct Shares {
 };
 
 // h[s, r] = scale_a sum_k X[s, k] A_a[r, k] for RF x 16 rows s and CF x 16 r a
-// workgroup, whose eight waves share the contraction.  h is rounded to the operands'
+// workgroup, whose waves share the contraction.  h is rounded to the operands'
 // type: it feeds matrix cores again, and its rounding adds less to the result than
 // the result's own (the adapter's part of an output averages `rank` such roundings).
 // The workgroups (x, y, 0 ..) take the adapters among their rows in turn: one each
 // where there are as many of them as rows, so that few rows with an adapter each
-// still spread over the chip.
+// still spread over the chip.  Few rows are bound by one workgroup's chain of loads (48
+// rows of 4096 with an adapter of rank 16 each: 6.4 us), many by reading the adapters for
+// every sixteen rows (8192 rows of 4096, rank 64: 28 us).
 //   D: stages of ring_share; 0: wave_share, for rows that are no whole pieces.
 template <typename T, int RF, int CF, int WAVES, int D>
 __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T* __restrict__ down,
@@ -1064,7 +1071,8 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T
 // Products of few rows, bound by reading the weights (W [c][k]) once: a workgroup
 // takes CF x 16 columns and up to RF x 16 rows of a group, its waves share the
 // contraction, so that a projection of a few thousand columns still has a workgroup
-// a CU.  D: as for adapter_shrink.
+// a CU.  D: as for adapter_shrink.  64 groups of 2048 x 4096, 256 rows: 168 us, 6.4 TB/s,
+// what reads alone reach; 48 rows x 4096 x 4096 with adapters 10.3 us.
 template <typename T, int RF, int CF, int WAVES, int D, bool ADAPT>
 __global__ __launch_bounds__(WAVES * 64) void few_rows_product(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char s_ring[];  // and then the shares

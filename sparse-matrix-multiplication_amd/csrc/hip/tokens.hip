@@ -8,7 +8,10 @@
 // All of it is memory traffic.  A token's row is read once and written to its k
 // slots (or the other way round), in 16-byte pieces, by one wave, or by a
 // workgroup where there are too few tokens to fill the chip with waves.  Sums
-// run over j in order, in fp32, and are rounded once.
+// run over j in order, in fp32, and are rounded once.  8192 tokens x 8 x 4096 bf16:
+// dispatch 105 us (5.7 TB/s; a copy reaches 5.2), combine_backward 252 (4.5).  5003 x 4 x
+// 2050 fp32, whose rows start inside lines: combine_backward 77 us, dispatch's gradient 56
+// (4.9 and 3.6 TB/s).
 
 #include <hip/hip_runtime.h>
 
