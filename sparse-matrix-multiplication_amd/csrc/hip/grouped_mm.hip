@@ -228,13 +228,19 @@ __device__ __forceinline__ bool row_tile_of_block(const TileArgs& a, int col_til
 //   MAJOR true: the contraction's steps are the rows, N elements each (W [k][c],
 //     and both operands of a gradient).  LDS rows of N elements, pieces at place
 //     p ^ 2 f(k), f(k) = (k & 3) | ((k >> 3) & 1) << 2: the transposing read of
-//     32 lanes takes 32 bytes of rows {0-3, 8-11}, f spreads them over all banks.
+//     32 lanes takes 32 bytes of rows {0-3, 8-11}, f spreads them over all banks (rows
+//     of 64 elements: f(k) = bit 1 | bit 3 << 1, bit 0 being in the address).
 template <typename T, int N, bool MAJOR, int THREADS>
 struct Operands {
     static constexpr int kPieces = N * kStep / 8 / THREADS;
     static constexpr int kRow    = MAJOR ? N : kStep;  // elements of an LDS row
     static_assert(N * kStep / 8 % THREADS == 0, "whole pieces a thread");
-    static_assert(!MAJOR || N >= 128, "the places of a row are 32 bytes x 8");
+    static_assert(!MAJOR || N == 64 || N == 128, "the places of a row are 32 bytes x 4 or 8");
+
+    // f(k), from step k's bits 0, 1 and 3
+    static __device__ __forceinline__ int spread(int low, int bit3) {
+        return N == 64 ? low >> 1 | bit3 << 1 : low | bit3 << 2;
+    }
 
     unsigned at[kPieces];     // byte offset of the piece from the tile's first word
     int      index[kPieces];  // its first contraction step inside the tile
@@ -248,11 +254,11 @@ struct Operands {
         const unsigned odd = static_cast<unsigned>(reinterpret_cast<uintptr_t>(first)) & 2u;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int p = i * THREADS + threadIdx.x;
+            const int p = i * THREADS + threadIdx.x % THREADS;
             int n, element;
             if constexpr (MAJOR) {
                 const int k = p / (N / 8);
-                const int f = (k & 3) | ((k >> 3) & 1) << 2;
+                const int f = spread(k & 3, (k >> 3) & 1);
                 n        = ((p % (N / 8)) ^ (f << 1)) * 8;
                 element  = k * ld + n;
                 index[i] = k;
@@ -287,7 +293,7 @@ struct Operands {
             if constexpr (!MAJOR) {
                 if (left < kStep) x = first_of(x, left - index[i]);
             }
-            *reinterpret_cast<uint4*>(lds + (i * THREADS + threadIdx.x) * 8) = x;
+            *reinterpret_cast<uint4*>(lds + (i * THREADS + threadIdx.x % THREADS) * 8) = x;
         }
     }
     // Operand of columns n0 .. n0+15, contraction steps 32 half .. +31: lane l holds
@@ -297,7 +303,7 @@ struct Operands {
         const int q = lane >> 4, s = lane & 15;
         if constexpr (MAJOR) {
             const int k = 32 * half + 8 * q + (s >> 2);
-            const int f = (s >> 2) | (q & 1) << 2;
+            const int f = spread(s >> 2, q & 1);
             const int c = ((n0 / 16) ^ f) * 16 + (s & 3) * 4;
             const _Float16* p = reinterpret_cast<const _Float16*>(lds) + k * kRow + c;
             const s16x4 x = lds_read_tr16(p);
@@ -665,6 +671,102 @@ __global__ __launch_bounds__(256, PIECES ? 1 : 2) void tile_product(TileArgs a) 
     }
     lds_barrier();  // the operands' LDS is free
     float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
+    if constexpr (ADAPT) {
+        store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
+    } else {
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
+    }
+}
+
+// The 64 x 64 tile of products with few tiles and a long contraction: sixteen waves in
+// four groups share the contraction, each with its own two buffers, and add up in a fixed
+// order.  Any sizes and alignment, as the words around each piece.  Bound by a load's way
+// through registers into LDS, about 1 us a turn of 256 steps.  128 rows x 64 x 5120, W
+// [k][c], two such tiles or one of 128 x 128: 25 us, 46 with the latter; 1024 x 1024 x
+// 4096 24, 43; 823 x 768 x 6787 with adapters 70, 145; a gradient of 256 x 256 from 32768
+// rows 136, 287.
+template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT>
+__global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
+    constexpr int BR = 64, BC = 64, WC = 2, RF = 2, CF = 2, GROUPS = 4;
+    using Rows = Operands<T, BR, GRAD, 256>;
+    using Cols = Operands<T, BC, GRAD || COLS_MAJOR, 256>;
+    extern __shared__ __attribute__((aligned(16))) char s_tiles[];
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int wave  = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    T* const own = reinterpret_cast<T*>(s_tiles) + group * 2 * (BR + BC) * kStep;
+    auto rows_at = [&](int it) { return own + (it & 1) * (BR + BC) * kStep; };
+    auto cols_at = [&](int it) { return rows_at(it) + BR * kStep; };
+    const int wr = wave / WC, wc = wave % WC;
+    Tile<T> t;
+    if (!take_tile<T, BR, BC, GRAD, COLS_MAJOR>(a, t)) return;
+
+    f32x4 acc[CF][RF];
+#pragma unroll
+    for (int j = 0; j < CF; ++j)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) acc[j][i] = f32x4(0.0f);
+    const int r0 = wr * RF * 16, c0 = t.c0 + wc * CF * 16;
+    // all groups go through as many turns: past the end there are zeros
+    const int turns = (t.depth + GROUPS * kStep - 1) / (GROUPS * kStep);
+    Rows pr;
+    Cols pc;
+    pr.place(t.rows, t.ld_rows, t.rows_here);
+    pc.place(t.cols, t.ld_cols, a.width - t.c0);
+    WordPiece vr[Rows::kPieces], vc[Cols::kPieces];
+    auto run = [&](auto odd) {
+        auto load = [&](int it) {
+            const int n = it * GROUPS + group, left = t.depth - n * kStep;
+            pr.template load<odd.value>(t.rows + n * t.step_rows, left, vr);
+            pc.template load<odd.value>(t.cols + n * t.step_cols, left, vc);
+        };
+        auto store = [&](int it) {
+            const int left = t.depth - (it * GROUPS + group) * kStep;
+            pr.template store<odd.value>(rows_at(it), left, vr);
+            pc.template store<odd.value>(cols_at(it), left, vc);
+        };
+        load(0);
+        store(0);
+        for (int it = 0; it < turns; ++it) {
+            __syncthreads();
+            if (it + 1 < turns) load(it + 1);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                Operand<T> fr[RF], fc[CF];
+#pragma unroll
+                for (int i = 0; i < RF; ++i) fr[i] = Rows::read(rows_at(it), (wr * RF + i) * 16, half);
+#pragma unroll
+                for (int j = 0; j < CF; ++j) fc[j] = Cols::read(cols_at(it), (wc * CF + j) * 16, half);
+#pragma unroll
+                for (int j = 0; j < CF; ++j)
+#pragma unroll
+                    for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc[j], fr[i], acc[j][i]);
+            }
+            if (it + 1 < turns) store(it + 1);
+        }
+    };
+    const uintptr_t ends = reinterpret_cast<uintptr_t>(t.rows) | reinterpret_cast<uintptr_t>(t.cols) |
+                           static_cast<uintptr_t>(t.ld_rows | t.ld_cols) * 2;
+    if (turns > 0) {
+        if ((ends & 2) != 0) run(std::true_type{});
+        else run(std::false_type{});
+    }
+    __syncthreads();  // the operands' LDS is free
+    f32x4(*parts)[4][CF][RF][64] = reinterpret_cast<f32x4(*)[4][CF][RF][64]>(s_tiles);
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < CF; ++j)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) parts[group][wave][j][i][lane] = acc[j][i];
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int j = 0; j < CF; ++j)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) {
+            for (int g = 1; g < GROUPS; ++g) acc[j][i] = acc[j][i] + parts[g][wave][j][i][lane];
+        }
+    // behind the shares: the other waves may still read theirs
+    float* sums = reinterpret_cast<float*>(s_tiles + sizeof(*parts) * GROUPS) + wave * kStoreFloats<CF>;
     if constexpr (ADAPT) {
         store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
     } else {
@@ -1149,7 +1251,8 @@ Error with_half(ElementType type, const char* name, F f) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-constexpr int kWideLds = 10 * 128 * kStep * 2;  // ten slots
+constexpr int kWideLds   = 10 * 128 * kStep * 2;      // ten slots
+constexpr int kSharedLds = 4 * 2 * 128 * kStep * 2;  // four groups' two buffers
 
 // Launches kernel with `lds` bytes of dynamic LDS, asked for once.
 template <auto kernel, typename... Args>
@@ -1239,18 +1342,22 @@ Error launch_shrink(const TileArgs& a, bool pieces, const void* down, const floa
 }
 
 // The kernels a product can take: few_rows_product, tile_product through registers
-// or with pieces straight into LDS, tile_product_wide.
-enum class Form { FewRows, Any, Pieces, Wide };
+// or with pieces straight into LDS, tile_product_wide, tile_product_shared.
+enum class Form { FewRows, Any, Pieces, Wide, Shared };
+constexpr int edge_of(Form form) { return form == Form::Wide ? 256 : form == Form::Shared ? 64 : 128; }
 
 // Estimated microseconds of a form for `row_tiles(edge)` x width tiles of `steps`
 // steps, from measured rates: 64 steps of a 128 x 128 tile take 0.62 us where a CU has
 // one and 0.95 us where it has two (through registers 1 and 1.5 us), of a 256 x 256 tile
-// 1.55 us, one a CU; `weights` microseconds is what reading the weights takes.
+// 1.55 us, one a CU, and 256 steps of a 64 x 64 tile 1.1 us, one a CU; `weights` microseconds is what reading the weights takes.
 template <typename F>
 double tile_time(Form form, F row_tiles, int width, double steps, double weights) {
-    const int edge = form == Form::Wide ? 256 : 128;
+    const int edge = edge_of(form);
     const double tiles = row_tiles(edge) * std::ceil(static_cast<double>(width) / edge);
     const double rounds = std::ceil(steps / kStep);
+    if (form == Form::Shared) {
+        return std::max(std::ceil(tiles / 256) * (4 + 1.1 * std::ceil(rounds / 4)), weights);
+    }
     if (form == Form::Wide) {
         return std::max(std::ceil(tiles / 256) * (6 + 1.55 * rounds), weights);
     }
@@ -1303,17 +1410,18 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
     const double reading = weights / (few_allowed ? 4.1e6 : 5.8e6) + (a.ids != nullptr ? 8 : 0);
     auto time = [&](Form f) {
         return tile_time(f, row_tiles, a.width, a.depth, reading) +
-               (f == Form::Any && a.ids != nullptr ? 6 : 0);
+               ((f == Form::Any || f == Form::Shared) && a.ids != nullptr ? 6 : 0);
     };
     Form best = pieces ? Form::Pieces : Form::Any;
     if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
+    if (time(Form::Shared) < time(best)) best = Form::Shared;
     return few_allowed && few <= time(best) ? Form::FewRows : best;
 }
 
 // Launches the tile kernel of a form.
 template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT>
 Error launch_tiles(const TileArgs& a, Form form, hipStream_t stream, const char* name) {
-    const int edge = form == Form::Wide ? 256 : 128;
+    const int edge = edge_of(form);
     // every group may end in a part-filled tile, and so may the rows before and behind them
     const long long row_tiles =
         GRAD ? static_cast<long long>(a.groups) * ((a.height + edge - 1) / edge)
@@ -1325,6 +1433,10 @@ Error launch_tiles(const TileArgs& a, Form form, hipStream_t stream, const char*
     if (form == Form::Wide) {
         return launch_with_lds<tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT>>(
             dim3(static_cast<unsigned>(blocks)), 256, kWideLds, stream, name, a);
+    }
+    if (form == Form::Shared) {
+        return launch_with_lds<tile_product_shared<T, GRAD, COLS_MAJOR, ADAPT>>(
+            dim3(static_cast<unsigned>(blocks)), 1024, kSharedLds, stream, name, a);
     }
     if (form == Form::Pieces) {
         tile_product<T, GRAD, COLS_MAJOR, ADAPT, true><<<blocks, 256, 0, stream>>>(a);
@@ -1387,8 +1499,9 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
     auto time = [&](Form f) {
         return tile_time(f, row_tiles, width, static_cast<double>(total) / groups, 0);
     };
-    const Form form = !pieces ? Form::Any
-                      : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
+    Form form = !pieces ? Form::Any
+                : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
+    if (time(Form::Shared) < time(form)) form = Form::Shared;
     return with_half(type, "grouped_outer", [&](auto zero) {
         using T = decltype(zero);
         return launch_tiles<T, true, true, false>(a, form, stream, "grouped_outer");

@@ -1,5 +1,5 @@
 """Grouped products and adapters at sizes that take each of their kernels: tiles of 256
-x 256 and 128 x 128, few rows with sixteen and with 64 columns, operands that are no whole
+x 256, 128 x 128 and 64 x 64, few rows with sixteen and with 64 columns, operands that are no whole
 pieces; and groups that do not begin at row zero.  Compared in 64 bits on the GPU."""
 import pytest
 
@@ -37,6 +37,8 @@ FORMS = [
     ([70, 90], 160, 700, 2056),        # few rows, one workgroup a CU
     ([2500, 1400], 4000, 1001, 519),   # no whole pieces
     ([3] * 20, 64, 301, 1027),
+    ([600], 600, 1024, 4096),      # 64 x 64 tiles whose waves share the contraction
+    ([300, 1, 0, 20], 333, 200, 5121), ([3999], 4000, 130, 190), ([3000, 900], 3907, 129, 65),
     ([12], 12, 1500, 2057), ([20], 20, 1500, 2057), ([40], 40, 1500, 2057), ([60], 60, 1500, 2057),
 ]
 
@@ -110,6 +112,8 @@ ADAPTERS = [
     (513, 264, 776, 20, 33),     # more adapters than workgroups share a row tile
     (512, 264, 776, 20, 33),
     (40, 520, 2056, 30, 8),
+    (823, 200, 6787, 7, 12),     # 64 x 64 tiles
+    (300, 256, 4096, 3, 48),
     (12, 1500, 2057, 3, 24), (20, 1500, 2057, 3, 9), (40, 1500, 2057, 3, 24), (60, 1500, 2057, 3, 24),
 ]
 
