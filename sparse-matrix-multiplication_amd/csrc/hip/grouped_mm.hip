@@ -1372,13 +1372,15 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
 //     a round of its workgroups takes 2.2 us for 256 steps (64 columns, two a CU) or 1 us
 //     for 512 (sixteen, one a CU).
 //   Rows that are no whole pieces: 1.1 times as long to read (8 groups of 4000 x 4098,
-//     32 rows: 47 us; tiles 60), twice where they begin between two words (64 groups of
-//     2048 x 4097, 256 rows: 344 us; tiles 222), and 1 us a round for 340 steps, 1.3 or
-//     1.65 times (100 rows x 4000 x 4098: 35 us, tiles 65; 192 x 6942 x 1010: 42, tiles
-//     27).
+//     32 rows: 47 us; 64 x 64 tiles 40, 128 x 128 60), twice where they begin between two
+//     words (64 groups of 2048 x 4097, 256 rows: 344 us; tiles 222), and 1 us a round for
+//     340 steps, 1.3 or 1.65 times, less with fewer rows (20 rows x 4000 x 4097: 17 us,
+//     tiles 27).
 //   Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s, W [k][c]
 //     at 5.8 (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows
-//     257, 285).  Adapters that change within sixteen rows hold them up.
+//     257, 285).  Adapters hold tiles up by 6 us, those of 64 x 64 by 5.
+//   64 x 64 tiles: 300 rows x 1024 x 1024 with adapters 14 us, 128 x 128 21; 100 rows x
+//     4000 x 4097 30, few_rows_product 43; 12 rows x 1504 x 2057 15, few_rows_product 8.
 Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
     const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     const double mean = a.total / groups;
@@ -1399,18 +1401,19 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
                                     (2 + 2.2 * std::ceil(a.depth / 256.0)));
             break;
         case Few::Single: {
+            const double high  = std::ceil(std::min(rows, 64.0) / 16);  // its rows' share of the loads
             const double round = pieces ? 3 + std::ceil(a.depth / 512.0)
-                                        : (1 + a.depth / 340.0) * (words ? 1.3 : 1.65);
+                                        : (1 + a.depth / 340.0) * (words ? 1.3 : 1.65) * (high + 2) / 6;
             few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 16.0) / 256) * round);
             break;
         }
         case Few::Groups: break;
     }
     few += 4;
-    const double reading = weights / (few_allowed ? 4.1e6 : 5.8e6) + (a.ids != nullptr ? 8 : 0);
+    const double reading = weights / (few_allowed ? 4.1e6 : 5.8e6);
     auto time = [&](Form f) {
         return tile_time(f, row_tiles, a.width, a.depth, reading) +
-               ((f == Form::Any || f == Form::Shared) && a.ids != nullptr ? 6 : 0);
+               (a.ids == nullptr ? 0 : f == Form::Shared ? 5 : 6);
     };
     Form best = pieces ? Form::Pieces : Form::Any;
     if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
