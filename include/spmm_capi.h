@@ -426,9 +426,9 @@ int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int to
  * adapter_mm: d_out[s] = x[s] w^T + scale[a] (x[s] A_a^T) B_a^T with a =
  *   d_ids[s], d_w [width, depth], d_a [adapters, rank, depth], d_b [adapters,
  *   width, rank], d_scale [adapters] fp32 or null; rows whose id is outside
- *   [0, adapters) take the projection alone.  x A_a^T is rounded to the
- *   operands' type.  d_workspace: spmm_c_adapter_workspace bytes; calls that
- *   share one must not overlap.  rank <= 1024. */
+ *   [0, adapters) take the projection alone.  scale[a] (x A_a^T) stays in fp32
+ *   in d_workspace (spmm_c_adapter_workspace bytes, aligned for fp32; calls that
+ *   share one must not overlap).  rank <= 1024. */
 int spmm_c_grouped_mm(const void* d_x, const void* d_w, int type, const int* d_offsets,
                       int groups, int rows, int width, int depth, int w_in_rows, void* d_out,
                       void* stream);

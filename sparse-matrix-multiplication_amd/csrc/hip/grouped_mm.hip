@@ -99,11 +99,11 @@ struct TileArgs {
     int         depth;    // product: contraction
     // adapters (ids null: none)
     const int*  ids;      // total
-    const void* h;        // [total, rank32]
+    const float* h;       // [total, rank16]
     const void* b;        // [adapters, width, rank]
     int         adapters;
     int         rank;
-    int         rank32;   // rank rounded up to whole products of 32
+    int         rank16;   // rank rounded up to whole tiles of adapter_shrink
     bool        b_pieces; // B's rows are whole 16-byte pieces
 };
 
@@ -378,6 +378,27 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F f) 
     (f(std::integral_constant<int, I>{}), ...);
 }
 
+// Eight values of h as two operands: high + low is h * 2^-shift but for 2^-16 of it
+// (bf16) or 2^-22 (fp16), a sixteenth and less of what the result's own rounding takes.
+//   shift: brings a row's largest value below 2^14 in fp16, whose range is short of fp32's
+//     (bf16 needs none).
+//   low is no number where high is not finite.
+template <typename T>
+struct Parts {
+    Operand<T> high, low;
+};
+template <typename T>
+__device__ __forceinline__ Parts<T> parts_of(const float (&v)[8], int shift) {
+    T high[8], low[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = std::is_same_v<T, _Float16> ? ldexpf(v[i], -shift) : v[i];
+        high[i] = static_cast<T>(x);
+        low[i]  = static_cast<T>(x - static_cast<float>(high[i]));
+    }
+    return Parts<T>{__builtin_bit_cast(Operand<T>, high), __builtin_bit_cast(Operand<T>, low)};
+}
+
 // The adapters of a wave's rows (r0 .. of the workgroup's tile, columns c0 ..), added
 // sixteen rows at a time on their way out: for each adapter among the rows h against
 // B_a, kept only in its own rows, so that no row sees what another's adapter holds,
@@ -385,15 +406,17 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F f) 
 //   PIECES: B's rows are whole 16-byte pieces (buffer loads, 32-bit offsets).
 template <typename T, int RF, int CF, bool PIECES>
 struct Adapters {
-    const T* h;
-    const T* b;
-    int      id[RF];  // of row 16 i + (lane & 15), -1 for none
-    int      width, rank, rank32;
-    int      c0;
+    static constexpr bool kShift = std::is_same_v<T, _Float16>;
+    const float* h;
+    const T*     b;
+    int          id[RF];     // of row 16 i + (lane & 15), -1 for none
+    int          shift[RF];  // of that row's h (kShift only)
+    int          width, rank, rank16;
+    int          c0;
 
     __device__ __forceinline__ Adapters(const TileArgs& a, const Tile<T>& t, int r0, int first_col)
-        : h(static_cast<const T*>(a.h) + static_cast<long long>(t.row0 + r0) * a.rank32),
-          b(static_cast<const T*>(a.b)), width(a.width), rank(a.rank), rank32(a.rank32),
+        : h(a.h + static_cast<long long>(t.row0 + r0) * a.rank16),
+          b(static_cast<const T*>(a.b)), width(a.width), rank(a.rank), rank16(a.rank16),
           c0(first_col) {
         const int s = threadIdx.x & 15;
 #pragma unroll
@@ -401,6 +424,43 @@ struct Adapters {
             id[i] = r0 + i * 16 + s < t.rows_here ? a.ids[t.row0 + r0 + i * 16 + s] : -1;
             if (static_cast<unsigned>(id[i]) >= static_cast<unsigned>(a.adapters)) id[i] = -1;
         }
+        if constexpr (kShift) {
+            float most[RF];
+#pragma unroll
+            for (int i = 0; i < RF; ++i) most[i] = 0.0f;
+            for (int k0 = 0; k0 < rank; k0 += 32) {
+#pragma unroll
+                for (int i = 0; i < RF; ++i) {
+                    float v[8];
+                    read_h(i, k0, id[i] >= 0, v);
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const float m = fabsf(v[n]);
+                        most[i] = m < __builtin_inff() ? fmaxf(most[i], m) : most[i];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < RF; ++i) {
+                most[i]  = fmaxf(most[i], __shfl_xor(most[i], 16));
+                most[i]  = fmaxf(most[i], __shfl_xor(most[i], 32));
+                shift[i] = __builtin_amdgcn_frexp_expf(most[i]) - 14;
+            }
+        }
+    }
+    // Eight values of h, from k0 + 8 (lane >> 4) on, of row 16 i + (lane & 15); zeros where
+    // the row is not `wanted`, and past the rank.
+    __device__ __forceinline__ void read_h(int i, int k0, bool wanted, float (&v)[8]) const {
+        const int lane = threadIdx.x & 63;
+        const int k = k0 + 8 * (lane >> 4);
+        const float* at = h + (i * 16 + (lane & 15)) * rank16 + k;
+        uint4 x{}, y{};
+        if (wanted && k < rank16) {
+            x = load_piece(at);
+            y = load_piece(at + 4);
+        }
+        __builtin_memcpy(v, &x, 16);
+        __builtin_memcpy(v + 4, &y, 16);
     }
     // B_a's rows c0 .. of an adapter, 32 of the rank from k0 on.
     __device__ __forceinline__ void read_b(int adapter, int k0, Operand<T> (&fc)[CF]) const {
@@ -418,35 +478,68 @@ struct Adapters {
             fc[j] = __builtin_bit_cast(Operand<T>, PIECES ? v.words : first_of(piece_of(v, at), rank - k));
         }
     }
-    // sums: the wave's rows 16 i .. in LDS, `pitch` floats a row; mine: id[i].
-    __device__ __forceinline__ void add(int i, int mine, float* sums, int pitch) const {
+    // Sums for the rows 16 i .. that `adapter` has (`own`), of both parts of h or the high
+    // one alone.
+    template <bool LOW>
+    __device__ __forceinline__ void multiply(int i, int adapter, bool own, int up,
+                                             f32x4 (&sum)[CF]) const {
+#pragma unroll
+        for (int j = 0; j < CF; ++j) sum[j] = f32x4(0.0f);
+        for (int k0 = 0; k0 < rank; k0 += 32) {
+            Operand<T> fc[CF];
+            read_b(adapter, k0, fc);
+            float v[8];
+            read_h(i, k0, own, v);
+            const Parts<T> fr = parts_of<T>(v, up);
+            if constexpr (LOW) {
+#pragma unroll
+                for (int j = 0; j < CF; ++j) sum[j] = mfma(fc[j], fr.low, sum[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < CF; ++j) sum[j] = mfma(fc[j], fr.high, sum[j]);
+        }
+    }
+    // sums: the wave's rows 16 i .. in LDS, `pitch` floats a row; mine, up: id[i], shift[i].
+    // An infinity in h or B can make the two parts inf - inf or 0 inf where their sum is an
+    // infinity: those elements take the high part's sum.
+    __device__ __forceinline__ void add(int i, int mine, int up, float* sums, int pitch) const {
         const int lane = threadIdx.x & 63;
         float* at = sums + (lane & 15) * pitch + 4 * (lane >> 4);
-        const T* row = h + (i * 16 + (lane & 15)) * rank32 + 8 * (lane >> 4);
         int left_id = mine;
         for (;;) {
             const unsigned long long left = __ballot(left_id >= 0);
             if (left == 0) break;
             const int adapter = __builtin_amdgcn_readlane(left_id, __builtin_ctzll(left));
+            const bool own = mine == adapter;
             f32x4 sum[CF];
+            multiply<true>(i, adapter, own, up, sum);
+            f32x4 none(0.0f);  // stays 0 while all are finite
 #pragma unroll
-            for (int j = 0; j < CF; ++j) sum[j] = f32x4(0.0f);
-            for (int k0 = 0; k0 < rank; k0 += 32) {
-                Operand<T> fc[CF];
-                read_b(adapter, k0, fc);
-                const Operand<T> fr = __builtin_bit_cast(
-                    Operand<T>, mine == adapter ? load_piece(row + k0) : uint4{0, 0, 0, 0});
+            for (int j = 0; j < CF; ++j) none = sum[j] * 0.0f + none;
+            const bool finite = (none[0] + none[1]) + (none[2] + none[3]) == 0.0f;
+            if (__ballot(own && !finite) != 0) {
+                f32x4 high[CF];
+                multiply<false>(i, adapter, own, up, high);
 #pragma unroll
-                for (int j = 0; j < CF; ++j) sum[j] = mfma(fc[j], fr, sum[j]);
+                for (int j = 0; j < CF; ++j)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        sum[j][n] = fabsf(sum[j][n]) < __builtin_inff() ? sum[j][n] : high[j][n];
+                    }
             }
-            if (mine == adapter) {
+            if (own) {
 #pragma unroll
                 for (int j = 0; j < CF; ++j) {
                     f32x4* p = reinterpret_cast<f32x4*>(at + 16 * j);
-                    *p = *p + sum[j];
+                    f32x4 more = sum[j];
+                    if constexpr (kShift) {
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) more[n] = ldexpf(more[n], up);
+                    }
+                    *p = *p + more;
                 }
             }
-            left_id = left_id == adapter ? -1 : left_id;
+            left_id = own ? -1 : left_id;
         }
     }
 };
@@ -535,7 +628,7 @@ __device__ __forceinline__ void store_adapted(const TileArgs& a, const Tile<T>& 
         const Adapters<T, RF, CF, pieces.value> ad(a, t, r0, c0);
         store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
             constexpr int i = at.value;
-            ad.add(i, ad.id[i], sums, CF * 16 + 4);
+            ad.add(i, ad.id[i], ad.kShift ? ad.shift[i] : 0, sums, CF * 16 + 4);
         });
     };
     if (a.b_pieces) store(std::true_type{});
@@ -1107,9 +1200,8 @@ struct Shares {
 };
 
 // h[s, r] = scale_a sum_k X[s, k] A_a[r, k] for RF x 16 rows s and CF x 16 r a
-// workgroup, whose waves share the contraction.  h is rounded to the operands'
-// type: it feeds matrix cores again, and its rounding adds less to the result than
-// the result's own (the adapter's part of an output averages `rank` such roundings).
+// workgroup, whose waves share the contraction.  h stays in fp32, up to the next whole
+// 16 of the rank (zeros behind it).
 // The workgroups (x, y, 0 ..) take the adapters among their rows in turn: one each
 // where there are as many of them as rows, so that few rows with an adapter each
 // still spread over the chip.  Few rows are bound by one workgroup's chain of loads (48
@@ -1119,7 +1211,7 @@ struct Shares {
 template <typename T, int RF, int CF, int WAVES, int D>
 __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T* __restrict__ down,
                                                              const float* __restrict__ scale,
-                                                             T* __restrict__ h) {
+                                                             float* __restrict__ h) {
     extern __shared__ __attribute__((aligned(16))) char s_ring[];  // and then the shares
     __shared__ int s_id[RF * 16];
     const int lane = threadIdx.x & 63;
@@ -1148,7 +1240,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T
         const T* x = static_cast<const T*>(a.rows) + static_cast<long long>(row0) * a.depth;
         const T* d = down + (static_cast<long long>(mine) * a.rank + r0) * a.depth;
         if (r0 >= a.rank) {
-            // only zeros up to rank32
+            // only zeros up to rank16
         } else if constexpr (D > 0) {
             ring_share<T, RF, CF, WAVES, D>(s_ring, x, rows_here, d, a.rank - r0, a.depth, acc);
             __syncthreads();
@@ -1161,9 +1253,9 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T
         const float f = scale != nullptr ? scale[mine] : 1.0f;
         for (int e = threadIdx.x; e < RF * 16 * CF * 16; e += WAVES * 64) {
             const int s = e / (CF * 16), r = e % (CF * 16);
-            if (s_id[s] == mine && r0 + r < a.rank32) {
-                h[static_cast<long long>(row0 + s) * a.rank32 + r0 + r] =
-                    static_cast<T>(r0 + r < a.rank ? f * shares.total(r, s) : 0.0f);
+            if (s_id[s] == mine && r0 + r < a.rank16) {
+                h[static_cast<long long>(row0 + s) * a.rank16 + r0 + r] =
+                    r0 + r < a.rank ? f * shares.total(r, s) : 0.0f;
             }
         }
         __syncthreads();
@@ -1210,14 +1302,14 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_product(TileArgs a) {
         if constexpr (ADAPT) {
             const int id = a.ids[t.first + s];
             if (static_cast<unsigned>(id) < static_cast<unsigned>(a.adapters)) {
-                const T* h = static_cast<const T*>(a.h) + static_cast<long long>(t.first + s) * a.rank32;
+                const float* h = a.h + static_cast<long long>(t.first + s) * a.rank16;
                 const T* b = static_cast<const T*>(a.b) +
                              (static_cast<long long>(id) * a.width + c0 + c) * a.rank;
                 float part = 0.0f;
                 for (int k = 0; k < a.rank; k += 8) {
                     const int n = min(8, a.rank - k);
                     float x[8], y[8];
-                    piece_to_float<T>(load_piece(h + k), x);
+                    __builtin_memcpy(x, h + k, 32);
                     piece_to_float<T>(n == 8 ? load_piece(b + k) : load_part(b + k, n), y);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) part = fmaf(x[i], y[i], part);
@@ -1326,10 +1418,10 @@ Error launch_few_rows(const TileArgs& a, long long rows, bool pieces, hipStream_
 template <typename T, int RF, int CF, int WAVES, int ROOM>
 Error launch_shrink(const TileArgs& a, bool pieces, const void* down, const float* scale, int turns,
                     hipStream_t stream) {
-    // the last columns of h, up to a whole product of 32, are written (zero) too
-    const dim3 grid((a.total + RF * 16 - 1) / (RF * 16), (a.rank32 + CF * 16 - 1) / (CF * 16), turns);
+    // the last columns of h, up to a whole 16, are written (zero) too
+    const dim3 grid((a.total + RF * 16 - 1) / (RF * 16), (a.rank16 + CF * 16 - 1) / (CF * 16), turns);
     const T* d = static_cast<const T*>(down);
-    T* h = static_cast<T*>(const_cast<void*>(a.h));
+    float* h = const_cast<float*>(a.h);
     constexpr int shares = Shares<RF, CF, WAVES>::kBytes;
     if (!pieces) {
         return launch_with_lds<adapter_shrink<T, RF, CF, WAVES, 0>>(
@@ -1513,7 +1605,7 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
 
 long long adapter_workspace(long long total, int rank) {
     if (total <= 0 || rank < 1) return 0;
-    return total * ((rank + 31LL) / 32 * 32) * 2;
+    return total * ((rank + 15LL) / 16 * 16) * static_cast<long long>(sizeof(float));
 }
 
 Error launch_adapter_mm(const void* x, const void* w, const void* down, const void* up,
@@ -1537,11 +1629,11 @@ Error launch_adapter_mm(const void* x, const void* w, const void* down, const vo
     a.width = width;
     a.depth = depth;
     a.ids = ids;
-    a.h = workspace;
+    a.h = static_cast<const float*>(workspace);
     a.b = up;
     a.adapters = adapters;
     a.rank = rank;
-    a.rank32 = (rank + 31) / 32 * 32;
+    a.rank16 = (rank + 15) / 16 * 16;
     const bool pieces = depth % 8 == 0 && aligned16(x) && aligned16(w);
     a.b_pieces = rank % 8 == 0 && aligned16(up);
     const Form form = choose_form(a, pieces, true);
