@@ -44,12 +44,13 @@ struct WordPiece {
     uint4    words;
     unsigned next;  // ODD only
 };
-// byte: from the buffer's begin; at or past 2^31 there are zeros.
+// byte: from the buffer's begin; at or past 2^31 there are zeros.  The next word's 16 is part
+// of the offset that the buffer's bounds are checked with; the scalar offset is not.
 template <bool ODD>
 __device__ __forceinline__ WordPiece load_words(__amdgpu_buffer_rsrc_t buffer, unsigned byte) {
     WordPiece v;
     v.words = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buffer, byte & ~3u, 0, 0));
-    v.next  = ODD ? __builtin_amdgcn_raw_buffer_load_b32(buffer, byte & ~3u, 16, 0) : 0u;
+    v.next  = ODD ? __builtin_amdgcn_raw_buffer_load_b32(buffer, (byte & ~3u) + 16u, 0, 0) : 0u;
     return v;
 }
 __device__ __forceinline__ uint4 piece_of(WordPiece v, unsigned byte) {

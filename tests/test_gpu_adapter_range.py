@@ -16,6 +16,8 @@ SHAPES = [
     (300, 256, 4096, 3, 48),                     # 64 x 64 tiles
     (1500, 1000, 520, 4, 8),                     # 128 x 128 tiles
     (4090, 4088, 1032, 3, 24),                   # 256 x 256 tiles
+    # rows that begin between two words, in few rows and tiles
+    (33, 130, 129, 5, 12), (823, 200, 6787, 7, 12), (1500, 1000, 521, 4, 9),
 ]
 
 
