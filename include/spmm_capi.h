@@ -377,7 +377,8 @@ int spmm_c_hybrid_run(const spmm_hybrid_plan_t* plan, const spmm_csr_t* h_A,
  *   numbers and makes the token's weights NaN.  over: the softmax over the
  *   chosen experts, or over all.  d_workspace: spmm_c_route_workspace bytes;
  *   calls that share one must not overlap.
- *   experts <= 1024, k <= 64, k <= experts (SPMM_UNSUPPORTED, SPMM_INVALID).
+ *   experts <= 1024, k <= 64, k <= experts, tokens * k <= 2^30 - 1, here and
+ *   below (SPMM_UNSUPPORTED; SPMM_INVALID for k > experts).
  * route_backward: d_dlogits of the logits' type; d_logits is read for
  *   SPMM_OVER_ALL only.
  * group_entries: the order alone, for ids of the caller's own (any id outside
@@ -412,7 +413,9 @@ int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int to
 
 /* ---- grouped products and low-rank adapters (no reference counterpart) --
  * Matrix-core products of SPMM_F16 or SPMM_BF16 operands (SPMM_UNSUPPORTED for
- * SPMM_F32), fp32 sums rounded once; contiguous device arrays, any sizes.
+ * SPMM_F32), fp32 sums rounded once; contiguous device arrays, rows of up to
+ * 2^22 elements, any number of them (SPMM_UNSUPPORTED where a launch would need
+ * 2^32 threads: some 2^24 groups or 2^29 rows with adapters).
  * grouped_mm: the block-diagonal product of rows in group order with their
  *   group's weights.  Group g has rows [d_offsets[g], d_offsets[g+1]) of d_x
  *   [rows, depth]; d_w is [groups, width, depth], or [groups, depth, width]

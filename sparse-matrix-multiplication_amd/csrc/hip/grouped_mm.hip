@@ -1343,6 +1343,12 @@ Error with_half(ElementType type, const char* name, F f) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// Refuses a launch that HIP would drop.
+Error check_threads(long long blocks, int threads, const char* name) {
+    if (blocks * threads <= kLaunchThreads) return Error{};
+    return Error{kUnsupported, std::string(name) + ": the launch would need 2^32 threads or more"};
+}
+
 constexpr int kWideLds   = 10 * 128 * kStep * 2;      // ten slots
 constexpr int kSharedLds = 4 * 2 * 128 * kStep * 2;  // four groups' two buffers
 
@@ -1370,7 +1376,7 @@ Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, con
         ? (a.total + RF * 16 - 1) / (RF * 16)
         : a.total / (RF * 16) + std::min<long long>(a.groups + 2LL, a.total);
     const long long blocks = row_tiles * ((a.width + CF * 16 - 1) / (CF * 16));
-    if (blocks > 0x7fffffffLL) return Error{kUnsupported, std::string(name) + ": too many tiles"};
+    SPMM_TRY(check_threads(blocks, WAVES * 64, name));
     const dim3 grid(static_cast<unsigned>(blocks));
     constexpr int shares = Shares<RF, CF, WAVES>::kBytes;
     if constexpr (CF == 1) {
@@ -1419,7 +1425,9 @@ template <typename T, int RF, int CF, int WAVES, int ROOM>
 Error launch_shrink(const TileArgs& a, bool pieces, const void* down, const float* scale, int turns,
                     hipStream_t stream) {
     // the last columns of h, up to a whole 16, are written (zero) too
-    const dim3 grid((a.total + RF * 16 - 1) / (RF * 16), (a.rank16 + CF * 16 - 1) / (CF * 16), turns);
+    const long long rows = (static_cast<long long>(a.total) + RF * 16 - 1) / (RF * 16);
+    SPMM_TRY(check_threads(rows, WAVES * 64, "adapter_shrink"));
+    const dim3 grid(static_cast<unsigned>(rows), (a.rank16 + CF * 16 - 1) / (CF * 16), turns);
     const T* d = static_cast<const T*>(down);
     float* h = const_cast<float*>(a.h);
     constexpr int shares = Shares<RF, CF, WAVES>::kBytes;
@@ -1436,6 +1444,7 @@ Error launch_shrink(const TileArgs& a, bool pieces, const void* down, const floa
 // The kernels a product can take: few_rows_product, tile_product through registers
 // or with pieces straight into LDS, tile_product_wide, tile_product_shared.
 enum class Form { FewRows, Any, Pieces, Wide, Shared };
+constexpr int threads_of(Form form) { return form == Form::Shared ? 1024 : 256; }
 constexpr int edge_of(Form form) { return form == Form::Wide ? 256 : form == Form::Shared ? 64 : 128; }
 
 // Estimated microseconds of a form for `row_tiles(edge)` x width tiles of `steps`
@@ -1446,6 +1455,7 @@ template <typename F>
 double tile_time(Form form, F row_tiles, int width, double steps, double weights) {
     const int edge = edge_of(form);
     const double tiles = row_tiles(edge) * std::ceil(static_cast<double>(width) / edge);
+    if (tiles * threads_of(form) > kLaunchThreads) return HUGE_VAL;
     const double rounds = std::ceil(steps / kStep);
     if (form == Form::Shared) {
         return std::max(std::ceil(tiles / 256) * (4 + 1.1 * std::ceil(rounds / 4)), weights);
@@ -1524,14 +1534,14 @@ Error launch_tiles(const TileArgs& a, Form form, hipStream_t stream, const char*
                                : a.total / edge + std::min<long long>(a.groups + 2LL, a.total);
     // a whole number of workgroups for each XCD
     const long long blocks = (row_tiles * ((a.width + edge - 1) / edge) + 7) / 8 * 8;
-    if (blocks > 0x7fffffffLL) return Error{kUnsupported, std::string(name) + ": too many tiles"};
+    SPMM_TRY(check_threads(blocks, threads_of(form), name));
     if (form == Form::Wide) {
         return launch_with_lds<tile_product_wide<T, GRAD, COLS_MAJOR, ADAPT>>(
-            dim3(static_cast<unsigned>(blocks)), 256, kWideLds, stream, name, a);
+            dim3(static_cast<unsigned>(blocks)), threads_of(Form::Wide), kWideLds, stream, name, a);
     }
     if (form == Form::Shared) {
         return launch_with_lds<tile_product_shared<T, GRAD, COLS_MAJOR, ADAPT>>(
-            dim3(static_cast<unsigned>(blocks)), 1024, kSharedLds, stream, name, a);
+            dim3(static_cast<unsigned>(blocks)), threads_of(Form::Shared), kSharedLds, stream, name, a);
     }
     if (form == Form::Pieces) {
         tile_product<T, GRAD, COLS_MAJOR, ADAPT, true><<<blocks, 256, 0, stream>>>(a);

@@ -31,6 +31,10 @@ inline Error hip_error(hipError_t e, const char* what) {
         if (spmm_err_.status != kOk) return spmm_err_;             \
     } while (0)
 
+// The most threads of a launch (along x).  HIP 7.0 takes one of 2^32 and more without an
+// error and runs none or a part of it.
+constexpr long long kLaunchThreads = 0xffffffffLL;
+
 // hipMalloc'd or hipMallocManaged memory released on scope exit.
 struct DeviceBuffer {
     void* p = nullptr;

@@ -578,12 +578,18 @@ Error launch_route_backward(const void* logits, ElementType type, int tokens, in
     }
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        with_per(experts, [&](auto n) {
-            route_grad<T, n.value><<<(tokens + 3) / 4, 256, 0, stream>>>(
-                static_cast<const T*>(logits), tokens, experts, k, all ? 1 : 0, chosen, weights,
-                dweights, static_cast<T*>(dlogits));
-        });
-        SPMM_TRY_HIP(hipGetLastError(), "route_grad");
+        // 67 M tokens of a wave each are as many as one launch has threads for
+        constexpr long long most = kLaunchThreads / 256 * 4;
+        for (long long first = 0; first < tokens; first += most) {
+            const int here = static_cast<int>(std::min(most, tokens - first));
+            with_per(experts, [&](auto n) {
+                route_grad<T, n.value><<<(here + 3) / 4, 256, 0, stream>>>(
+                    all ? static_cast<const T*>(logits) + first * experts : nullptr, here, experts, k,
+                    all ? 1 : 0, chosen + first * k, weights + first * k, dweights + first * k,
+                    static_cast<T*>(dlogits) + first * experts);
+            });
+            SPMM_TRY_HIP(hipGetLastError(), "route_grad");
+        }
         return Error{};
     });
 }

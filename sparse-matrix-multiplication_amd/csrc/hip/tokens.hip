@@ -29,7 +29,9 @@ namespace {
 using namespace dev;
 
 struct Rows {
-    int tokens, k, features;
+    int  tokens, k, features;
+    int  total;  // slots, of all launches' tokens
+    bool clear;  // this launch writes the rows without an entry
 };
 
 // A slot as a scalar: the same for a whole wave.
@@ -41,7 +43,7 @@ __device__ __forceinline__ int slot_of(const int* slots, long long i) {
 template <typename T>
 __device__ __forceinline__ void zero_rows(T* rows, int placed, const Rows& r) {
     constexpr int P = kPiece<T>;
-    const int total = r.tokens * r.k;
+    const int total = r.total;
     for (long long s = static_cast<long long>(min(max(placed, 0), total)) + blockIdx.x; s < total;
          s += gridDim.x) {
         T* row = rows + s * r.features;
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(256) void tokens_dispatch(const T* __restrict__ x,
     const int wave  = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane  = (WAVES == 1 ? threadIdx.x & 63 : threadIdx.x) * P;
     const int step  = WAVES * 64 * P;
-    const int total = r.tokens * r.k;
+    const int total = r.total;
     const int t = blockIdx.x * (4 / WAVES) + (WAVES == 1 ? wave : 0);
     if (t < r.tokens) {
         const T* src = x + static_cast<long long>(t) * r.features;
@@ -97,7 +99,7 @@ __global__ __launch_bounds__(256) void tokens_dispatch(const T* __restrict__ x,
             }
         }
     }
-    zero_rows(xs, *placed, r);
+    if (r.clear) zero_rows(xs, *placed, r);
 }
 
 // Sum over a token's slots, weighted where weights are given.  B slots' pieces
@@ -111,7 +113,7 @@ __global__ __launch_bounds__(256) void tokens_gather(const T* __restrict__ ys,
     constexpr int P = kPiece<T>, B = 4;
     const int wave  = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane  = (WAVES == 1 ? threadIdx.x & 63 : threadIdx.x) * P;
-    const int total = r.tokens * r.k;
+    const int total = r.total;
     const int t = blockIdx.x * (4 / WAVES) + (WAVES == 1 ? wave : 0);
     if (t >= r.tokens) return;
     const long long e0 = static_cast<long long>(t) * r.k;
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(256) void tokens_combine_grad(
     __shared__ float s_part[4][B];
     const int wave  = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane  = (WAVES == 1 ? threadIdx.x & 63 : threadIdx.x) * P;
-    const int total = r.tokens * r.k;
+    const int total = r.total;
     const int t = blockIdx.x * (4 / WAVES) + (WAVES == 1 ? wave : 0);
     const long long e0 = static_cast<long long>(t) * r.k;
     const T* src = dy + static_cast<long long>(t) * r.features;
@@ -224,14 +226,14 @@ __global__ __launch_bounds__(256) void tokens_combine_grad(
             }
         }
     }
-    zero_rows(dys, *placed, r);
+    if (r.clear) zero_rows(dys, *placed, r);
 }
 
-Error check_rows(const Rows& r, const char* name) {
-    if (r.tokens < 0 || r.k < 1 || r.features < 0) {
+Error check_rows(int tokens, int k, int features, const char* name) {
+    if (tokens < 0 || k < 1 || features < 0) {
         return Error{kInvalid, std::string(name) + ": sizes must be positive"};
     }
-    if (static_cast<long long>(r.tokens) * r.k > 0x3fffffffLL) {
+    if (static_cast<long long>(tokens) * k > 0x3fffffffLL) {
         return Error{kUnsupported, std::string(name) + ": over 2^30 entries"};
     }
     return Error{};
@@ -246,11 +248,23 @@ constexpr int kWaveTokens = 4096;
 // (80 MB), which the cache holds for the next reader, 17 us with plain stores, 22 so.
 constexpr long long kStreamBytes = 256LL << 20;
 
+// Calls f(element, waves a token, first token, rows, workgroups) for each launch: 67 M
+// tokens of a wave each are as many as one has threads for.
 template <typename F>
-Error with_shape(ElementType type, int tokens, F f) {
+Error with_shape(ElementType type, int tokens, int k, int features, F f) {
     auto waves = [&](auto zero) {
-        if (tokens >= kWaveTokens) return f(zero, std::integral_constant<int, 1>{}, (tokens + 3) / 4);
-        return f(zero, std::integral_constant<int, 4>{}, tokens);
+        const int total = tokens * k;
+        if (tokens < kWaveTokens) {
+            return f(zero, std::integral_constant<int, 4>{}, 0LL, Rows{tokens, k, features, total, true},
+                     tokens);
+        }
+        constexpr long long most = kLaunchThreads / 256 * 4;
+        for (long long first = 0; first < tokens; first += most) {
+            const int here = static_cast<int>(std::min(most, tokens - first));
+            SPMM_TRY(f(zero, std::integral_constant<int, 1>{}, first,
+                       Rows{here, k, features, total, first == 0}, (here + 3) / 4));
+        }
+        return Error{};
     };
     switch (type) {
         case ElementType::F32: return waves(float{});
@@ -265,19 +279,20 @@ Error with_shape(ElementType type, int tokens, F f) {
 Error launch_dispatch(const void* x, ElementType type, int tokens, int k, int features,
                       const int* slots, const int* offsets, int experts, void* xs,
                       hipStream_t stream) {
-    const Rows r{tokens, k, features};
-    SPMM_TRY(check_rows(r, "dispatch"));
+    SPMM_TRY(check_rows(tokens, k, features, "dispatch"));
     if (experts < 1) return Error{kInvalid, "dispatch: sizes must be positive"};
     if (tokens == 0 || features == 0) return Error{};
     if (x == nullptr || slots == nullptr || offsets == nullptr || xs == nullptr) {
         return Error{kInvalid, "dispatch: null pointer"};
     }
-    return with_shape(type, tokens, [&](auto zero, auto waves, int blocks) {
+    return with_shape(type, tokens, k, features, [&](auto zero, auto waves, long long first, Rows r,
+                                                     int blocks) {
         using T = decltype(zero);
         const bool past = static_cast<long long>(tokens) * k * features * sizeof(T) >= kStreamBytes;
         auto kernel = past ? tokens_dispatch<T, waves.value, true>
                            : tokens_dispatch<T, waves.value, false>;
-        kernel<<<blocks, 256, 0, stream>>>(static_cast<const T*>(x), slots, offsets + experts, r,
+        kernel<<<blocks, 256, 0, stream>>>(static_cast<const T*>(x) + first * features,
+                                           slots + first * k, offsets + experts, r,
                                            static_cast<T*>(xs));
         SPMM_TRY_HIP(hipGetLastError(), "dispatch");
         return Error{};
@@ -286,16 +301,18 @@ Error launch_dispatch(const void* x, ElementType type, int tokens, int k, int fe
 
 Error launch_combine(const void* ys, ElementType type, int tokens, int k, int features,
                      const int* slots, const float* weights, void* y, hipStream_t stream) {
-    const Rows r{tokens, k, features};
-    SPMM_TRY(check_rows(r, "combine"));
+    SPMM_TRY(check_rows(tokens, k, features, "combine"));
     if (tokens == 0 || features == 0) return Error{};
     if (ys == nullptr || slots == nullptr || y == nullptr) {
         return Error{kInvalid, "combine: null pointer"};
     }
-    return with_shape(type, tokens, [&](auto zero, auto waves, int blocks) {
+    return with_shape(type, tokens, k, features, [&](auto zero, auto waves, long long first, Rows r,
+                                                     int blocks) {
         using T = decltype(zero);
         tokens_gather<T, waves.value><<<blocks, 256, 0, stream>>>(
-            static_cast<const T*>(ys), slots, weights, r, static_cast<T*>(y));
+            static_cast<const T*>(ys), slots + first * k,
+            weights != nullptr ? weights + first * k : nullptr, r,
+            static_cast<T*>(y) + first * features);
         SPMM_TRY_HIP(hipGetLastError(), "combine");
         return Error{};
     });
@@ -305,19 +322,20 @@ Error launch_combine_backward(const void* dy, const void* ys, ElementType type, 
                               int features, const int* slots, const float* weights,
                               const int* offsets, int experts, void* dys, float* dweights,
                               hipStream_t stream) {
-    const Rows r{tokens, k, features};
-    SPMM_TRY(check_rows(r, "combine_backward"));
+    SPMM_TRY(check_rows(tokens, k, features, "combine_backward"));
     if (experts < 1) return Error{kInvalid, "combine_backward: sizes must be positive"};
     if (tokens == 0) return Error{};
     if (slots == nullptr || weights == nullptr || offsets == nullptr || dweights == nullptr ||
         (features > 0 && (dy == nullptr || ys == nullptr || dys == nullptr))) {
         return Error{kInvalid, "combine_backward: null pointer"};
     }
-    return with_shape(type, tokens, [&](auto zero, auto waves, int blocks) {
+    return with_shape(type, tokens, k, features, [&](auto zero, auto waves, long long first, Rows r,
+                                                     int blocks) {
         using T = decltype(zero);
         tokens_combine_grad<T, waves.value><<<blocks, 256, 0, stream>>>(
-            static_cast<const T*>(dy), static_cast<const T*>(ys), slots, offsets + experts,
-            weights, r, static_cast<T*>(dys), dweights);
+            static_cast<const T*>(dy) + first * features, static_cast<const T*>(ys),
+            slots + first * k, offsets + experts, weights + first * k, r, static_cast<T*>(dys),
+            dweights + first * k);
         SPMM_TRY_HIP(hipGetLastError(), "combine_backward");
         return Error{};
     });

@@ -233,3 +233,52 @@ def test_more_threads_than_a_launch_holds(S, torch, form, M, K, per, N):
     torch.cuda.synchronize()
     for i in range(0, M, 1 << 20):
         assert (C[i:i + (1 << 20)] == want).all(), i
+
+
+def test_more_tokens_than_a_launch_has_waves(S, torch):
+    """67 108 869 tokens, a wave each: 2^32 threads and more go into several launches."""
+    T, D = (1 << 26) + 5, 3
+    say(f"token moves of {T} x {D}")
+    slots = torch.arange(T - 1, -1, -1, dtype=torch.int32, device="cuda").view(T, 1)
+    slots[7] = -1  # has slot T - 8; the last slot is without an entry then
+    slots[:7] -= 1
+    offsets = torch.tensor([0, T - 1], dtype=torch.int32, device="cuda")
+    weights = torch.full((T, 1), 0.5, device="cuda")
+    r = S.Routing(None, weights, offsets, None, slots)
+    x = torch.arange(T * D, device="cuda", dtype=torch.int32).view(T, D).remainder_(509).bfloat16()
+    there = slots[:, 0] >= 0
+    at = slots[there, 0].long()
+    want = torch.zeros_like(x)
+    want[at] = x[there]
+    xs = torch.full_like(x, 7.0)
+    assert torch.equal(S.dispatch(x, r, out=xs), want)
+    back = torch.where(there[:, None], x, torch.zeros_like(x))
+    out = torch.full_like(x, 7.0)
+    assert torch.equal(S.dispatch_backward(xs, r, out=out), back)
+    assert torch.equal(S.combine(xs, r, out=out), back * 0.5)  # halves are exact
+    dys, dweights = S.combine_backward(x, xs, r)
+    assert torch.equal(dys, want * 0.5)
+    # sums of three products below 2^18, all exact in fp32
+    assert torch.equal(dweights, (back.float() ** 2).sum(1, keepdim=True))
+
+
+def test_more_tokens_than_a_launch_has_waves_in_the_router_gradient(S, torch):
+    T = (1 << 26) + 5
+    say(f"route_backward of {T} x 2")
+    logits = torch.zeros((T, 2), device="cuda")
+    logits[:, 1] = torch.arange(T, device="cuda").remainder(3).float() - 1.0
+    chosen = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda").expand(T, 2).contiguous()
+    weights = torch.full((T, 2), 0.5, device="cuda")
+    dweights = torch.stack((torch.arange(T, device="cuda").remainder(5).float(),
+                            torch.ones(T, device="cuda")), 1)
+    r = S.Routing(chosen, weights, None, None, None)
+    out = torch.full((T, 2), 7.0, device="cuda")
+    # w (dw - sum w dw) with weights of a half: exact
+    want = 0.5 * (dweights - dweights.mean(1, keepdim=True))
+    assert torch.equal(S.route_backward(logits, r, dweights, out=out), want)
+    r.over = "all"
+    p = torch.softmax(logits, 1)
+    want = p * (dweights - dweights.mean(1, keepdim=True))
+    off = (S.route_backward(logits, r, dweights, out=out) - want).abs()
+    # p: exp, a sum of two and a quotient on both sides; |dw - mean| <= 2
+    assert off.max().item() <= 2 * 16 * 2.0 ** -24
