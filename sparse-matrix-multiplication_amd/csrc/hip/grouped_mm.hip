@@ -1352,13 +1352,16 @@ Error check_threads(long long blocks, int threads, const char* name) {
 constexpr int kWideLds   = 10 * 128 * kStep * 2;      // ten slots
 constexpr int kSharedLds = 4 * 2 * 128 * kStep * 2;  // four groups' two buffers
 
-// Launches kernel with `lds` bytes of dynamic LDS, asked for once.
+// Launches kernel with `lds` bytes of dynamic LDS, asked for once a GPU.
 template <auto kernel, typename... Args>
 Error launch_with_lds(dim3 grid, int threads, int lds, hipStream_t stream, const char* name,
                       Args... args) {
-    static const hipError_t grown = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    SPMM_TRY_HIP(grown, name);
+    static OncePerDevice grown;
+    const auto ask = [&] {
+        return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    };
+    SPMM_TRY_HIP(grown(ask), name);
     kernel<<<grid, threads, lds, stream>>>(args...);
     SPMM_TRY_HIP(hipGetLastError(), name);
     return Error{};

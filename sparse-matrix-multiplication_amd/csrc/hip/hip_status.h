@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -34,6 +35,31 @@ inline Error hip_error(hipError_t e, const char* what) {
 // The most threads of a launch (along x).  HIP 7.0 takes one of 2^32 and more without an
 // error and runs none or a part of it.
 constexpr long long kLaunchThreads = 0xffffffffLL;
+
+// What each GPU of the process has to be asked once before a launch there (a kernel's
+// attributes belong to a GPU).  A failure is not kept: the next launch asks again.
+class OncePerDevice {
+public:
+    // ask() -> hipError_t, for the current GPU.
+    template <typename Ask>
+    hipError_t operator()(Ask ask) {
+        int device = 0;
+        const hipError_t e = hipGetDevice(&device);
+        return e == hipSuccess ? on(device, ask) : e;
+    }
+    template <typename Ask>
+    hipError_t on(int device, Ask ask) {
+        const bool kept = device >= 0 && device < kDevices;
+        if (kept && done_[device].load(std::memory_order_acquire)) return hipSuccess;
+        const hipError_t e = ask();
+        if (kept && e == hipSuccess) done_[device].store(true, std::memory_order_release);
+        return e;
+    }
+
+private:
+    static constexpr int kDevices = 64;  // GPUs past these are asked every time
+    std::atomic<bool> done_[kDevices] = {};
+};
 
 // hipMalloc'd or hipMallocManaged memory released on scope exit.
 struct DeviceBuffer {
