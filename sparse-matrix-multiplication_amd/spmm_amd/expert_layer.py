@@ -20,6 +20,7 @@ import argparse
 
 import torch
 
+from . import SPMM_UNSUPPORTED, SpmmError
 from .experts import (adapter_mm, combine, combine_backward, dispatch, dispatch_backward,
                       grouped_mm, grouped_mm_backward, route, route_backward)
 
@@ -35,6 +36,19 @@ def _forward(x, logits, w_in, w_out, k, over):
     return combine(ys, r), (r, xs, h, a, ys)
 
 
+class _Once(torch.autograd.Function):
+    """Hands gradients on (the first n) that kernels computed without a graph from the rest:
+    going back through them is refused, where it would count as zero otherwise."""
+
+    @staticmethod
+    def forward(ctx, n, *grads):
+        return tuple(g if g is None else g.view_as(g) for g in grads[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise SpmmError(SPMM_UNSUPPORTED, "expert layer: differentiable once, no second derivative")
+
+
 class _Experts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, logits, w_in, w_out, k, over):
@@ -45,6 +59,16 @@ class _Experts(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        with torch.no_grad():
+            grads = _Experts._gradients(ctx, dy)
+        if not torch.is_grad_enabled():
+            return grads
+        # under create_graph: what the gradients hang on besides dy (which is all that
+        # torch's once_differentiable looks at) goes along
+        return _Once.apply(len(grads), *grads, dy, *ctx.saved_tensors[:3])
+
+    @staticmethod
+    def _gradients(ctx, dy):
         logits, w_in, w_out, xs, h, a, ys = ctx.saved_tensors
         r = ctx.routing
         dys, dweights = combine_backward(dy.contiguous(), ys, r)
@@ -57,7 +81,8 @@ class _Experts(torch.autograd.Function):
 
 class ExpertLayer(torch.nn.Module):
     """`experts` two-layer networks of `width` and `hidden` units, `k` of them a token.
-    The router's logits are held in float32; `over` is what its softmax runs over."""
+    The router's logits are held in float32; `over` is what its softmax runs over.
+    Differentiable once; a second derivative raises."""
 
     def __init__(self, width: int, hidden: int, experts: int, k: int, over: str = "chosen",
                  dtype=torch.bfloat16, device="cuda"):
