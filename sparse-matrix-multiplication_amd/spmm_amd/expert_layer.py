@@ -71,12 +71,20 @@ class _Experts(torch.autograd.Function):
     def _gradients(ctx, dy):
         logits, w_in, w_out, xs, h, a, ys = ctx.saved_tensors
         r = ctx.routing
+        of_x, of_logits, of_in, of_out = ctx.needs_input_grad[:4]
+        dx = dlogits = dw_in = dw_out = None
         dys, dweights = combine_backward(dy.contiguous(), ys, r)
-        da, dw_out = grouped_mm_backward(dys, a, w_out, r.offsets)
-        dh = torch.ops.aten.silu_backward(da, h)
-        dxs, dw_in = grouped_mm_backward(dh, xs, w_in, r.offsets)
-        return (dispatch_backward(dxs, r), route_backward(logits, r, dweights), dw_in, dw_out,
-                None, None)
+        if of_logits:
+            dlogits = route_backward(logits, r, dweights)
+        hidden = of_x or of_in
+        if hidden or of_out:
+            da, dw_out = grouped_mm_backward(dys, a, w_out, r.offsets, rows=hidden, weights=of_out)
+        if hidden:
+            dh = torch.ops.aten.silu_backward(da, h)
+            dxs, dw_in = grouped_mm_backward(dh, xs, w_in, r.offsets, rows=of_x, weights=of_in)
+        if of_x:
+            dx = dispatch_backward(dxs, r)
+        return dx, dlogits, dw_in, dw_out, None, None
 
 
 class ExpertLayer(torch.nn.Module):

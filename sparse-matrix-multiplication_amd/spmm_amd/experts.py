@@ -300,8 +300,10 @@ def grouped_mm(x, w, offsets, w_in_rows: bool = False, out=None, stream=None):
     return out
 
 
-def grouped_mm_backward(dy, x, w, offsets, w_in_rows: bool = False, stream=None):
-    """The gradients of ``grouped_mm`` for dy [S, N]: (dx [S, K], dw like w)."""
+def grouped_mm_backward(dy, x, w, offsets, w_in_rows: bool = False, stream=None, rows: bool = True,
+                        weights: bool = True):
+    """The gradients of ``grouped_mm`` for dy [S, N]: (dx [S, K], dw like w).  One that is
+    not asked for (rows=False, weights=False) is not computed and None."""
     _half(x, "x")
     S, K = x.shape
     device = x.device
@@ -310,14 +312,16 @@ def grouped_mm_backward(dy, x, w, offsets, w_in_rows: bool = False, stream=None)
     _operand(offsets, "offsets", _INT, (G + 1,), device)
     p, q, height, width = (x, dy, K, N) if w_in_rows else (dy, x, N, K)
     with _on(stream):
-        dw = torch.empty_like(w)
-        dx = torch.empty_like(x)
+        dw = torch.empty_like(w) if weights else None
+        dx = torch.empty_like(x) if rows else None
         L, s = lib(), _stream(device)
-        _check(L.spmm_c_grouped_mm(dy.data_ptr(), w.data_ptr(), _TYPES[x.dtype],
-                                   offsets.data_ptr(), G, S, K, N, int(not w_in_rows),
-                                   dx.data_ptr(), s))
-        _check(L.spmm_c_grouped_outer(p.data_ptr(), q.data_ptr(), _TYPES[x.dtype],
-                                      offsets.data_ptr(), G, S, height, width, dw.data_ptr(), s))
+        if rows:
+            _check(L.spmm_c_grouped_mm(dy.data_ptr(), w.data_ptr(), _TYPES[x.dtype],
+                                       offsets.data_ptr(), G, S, K, N, int(not w_in_rows),
+                                       dx.data_ptr(), s))
+        if weights:
+            _check(L.spmm_c_grouped_outer(p.data_ptr(), q.data_ptr(), _TYPES[x.dtype],
+                                          offsets.data_ptr(), G, S, height, width, dw.data_ptr(), s))
     return dx, dw
 
 

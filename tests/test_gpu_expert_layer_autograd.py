@@ -29,3 +29,51 @@ def test_second_derivative_is_refused(S):
     g, = torch.autograd.grad(loss, layer.w_in, create_graph=True)
     with pytest.raises(S.SpmmError):
         torch.autograd.grad(g.float().sum(), x)
+
+
+def _launches(monkeypatch):
+    """Names of the products' gradients that are computed."""
+    import spmm_amd.experts as X
+    real, seen = X.lib(), []
+
+    class Watched:
+        def __getattr__(self, name):
+            if name in ("spmm_c_grouped_mm", "spmm_c_grouped_outer"):
+                seen.append(name)
+            return getattr(real, name)
+
+    monkeypatch.setattr(X, "lib", lambda: Watched())
+    return seen
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("frozen,products,outers", [
+    ((), 2, 2), (("w_in", "w_out"), 2, 0), (("w_in",), 2, 1), (("w_out",), 2, 1), (("x",), 1, 2),
+    (("x", "router", "w_in"), 0, 1), (("x", "w_in", "w_out"), 0, 0)])
+def test_frozen_parts_cost_nothing(S, monkeypatch, frozen, products, outers):
+    """What is not trained gets no gradient and no product for one; the rest is unchanged."""
+    layer, x, dy = _layer()
+    names = {"x": x, "router": layer.router, "w_in": layer.w_in, "w_out": layer.w_out}
+    want = dict(zip(names, torch.autograd.grad(layer(x), list(names.values()), dy)))
+    for n in frozen:
+        names[n].requires_grad_(False)
+    y = layer(x)
+    seen = _launches(monkeypatch)
+    y.backward(dy)
+    assert (seen.count("spmm_c_grouped_mm"), seen.count("spmm_c_grouped_outer")) == (products, outers)
+    for n, v in names.items():
+        assert v.grad is None if n in frozen else torch.equal(v.grad, want[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("w_in_rows", [False, True])
+def test_one_gradient_of_a_product(S, w_in_rows):
+    torch.manual_seed(0)
+    x, dy = torch.randn(50, 24, device="cuda").half(), torch.randn(50, 40, device="cuda").half()
+    w = torch.randn(3, *((24, 40) if w_in_rows else (40, 24)), device="cuda").half()
+    offsets = torch.tensor([0, 20, 20, 45], dtype=torch.int32, device="cuda")
+    dx, dw = S.grouped_mm_backward(dy, x, w, offsets, w_in_rows)
+    only, none = S.grouped_mm_backward(dy, x, w, offsets, w_in_rows, weights=False)
+    assert none is None and torch.equal(only, dx)
+    none, only = S.grouped_mm_backward(dy, x, w, offsets, w_in_rows, rows=False)
+    assert none is None and torch.equal(only, dw)
