@@ -103,7 +103,8 @@ class ExpertLayer(torch.nn.Module):
         self.k, self.over = k, over
 
     def forward(self, x):
-        """x [T, width] -> [T, width]"""
+        """x [T, width], of any strides -> [T, width]"""
+        x = x.contiguous()
         return _Experts.apply(x, x.float() @ self.router.t(), self.w_in, self.w_out, self.k,
                               self.over)
 
@@ -111,6 +112,7 @@ class ExpertLayer(torch.nn.Module):
     def serve(self, x, w, a, b, ids, scale=None):
         """The layer and its residual for tokens x [T, width] of requests whose adapters
         are ids [T], then the projection w with each row's adapter: [T, N]."""
+        x = x.contiguous()
         y, _ = _forward(x, x.float() @ self.router.t(), self.w_in, self.w_out, self.k, self.over)
         return adapter_mm(x + y, w, a, b, ids, scale)
 

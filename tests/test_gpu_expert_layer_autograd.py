@@ -77,3 +77,23 @@ def test_one_gradient_of_a_product(S, w_in_rows):
     assert none is None and torch.equal(only, dx)
     none, only = S.grouped_mm_backward(dy, x, w, offsets, w_in_rows, rows=False)
     assert none is None and torch.equal(only, dw)
+
+
+@pytest.mark.gpu
+def test_rows_of_any_strides(S):
+    """A transposed or sliced x gives what its copy gives, gradients included."""
+    layer, x, dy = _layer(T=40, D=64)
+    want = layer(x)
+    want.backward(dy)
+    wide = torch.zeros(40, 80, device="cuda", dtype=x.dtype)
+    wide[:, 8:72] = x.detach()
+    w, a, b = (torch.randn(s, device="cuda").bfloat16() for s in ((64, 64), (2, 8, 64), (2, 64, 8)))
+    ids = (torch.arange(40, device="cuda", dtype=torch.int32) % 3) - 1
+    served = layer.serve(x.detach(), w, a, b, ids)
+    for base, view in ((wide, lambda t: t[:, 8:72]), (x.detach().t().contiguous(), lambda t: t.t())):
+        base = base.clone().requires_grad_()
+        assert not view(base).is_contiguous()
+        y = layer(view(base))
+        y.backward(dy)
+        assert torch.equal(y, want) and torch.equal(view(base.grad), x.grad)
+        assert torch.equal(layer.serve(view(base.detach()), w, a, b, ids), served)
