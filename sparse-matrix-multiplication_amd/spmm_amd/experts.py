@@ -76,6 +76,12 @@ def _rows(t, name: str, rows: int) -> None:
         raise SpmmError(SPMM_INVALID, f"{name}: {t.shape[0]} rows, expected {rows}")
 
 
+def _counts(*sizes) -> None:
+    """Sizes go to the library as 32-bit integers, which would cut larger ones off."""
+    if max(sizes) > 0x7fffffff:
+        raise SpmmError(SPMM_UNSUPPORTED, f"sizes {sizes}: over 2^31 - 1")
+
+
 _here = contextlib.nullcontext()
 
 
@@ -137,6 +143,7 @@ def route(logits, k: int, over: str = "chosen", stream=None) -> Routing:
     k = int(k)
     if not 1 <= k <= E:
         raise SpmmError(SPMM_INVALID, f"k: {k}, expected 1 to {E} experts")
+    _counts(T, E)
     L = lib()
     device = logits.device
     with _on(stream):
@@ -166,6 +173,7 @@ def route_backward(logits, routing: Routing, dweights, out=None, stream=None):
     if routing.weights.shape[0] != T or not 1 <= k <= E:
         raise SpmmError(SPMM_INVALID, f"routing: of {tuple(routing.weights.shape)} choices, "
                                       f"logits are {tuple(logits.shape)}")
+    _counts(T, E)
     _operand(routing.experts, "routing.experts", _INT, (T, k), device)
     _operand(dweights, "dweights", _FLOAT, (T, k), device)
     with _on(stream):
@@ -187,6 +195,7 @@ def group_entries(ids, groups: int, stream=None):
     groups = int(groups)
     if groups < 1:
         raise SpmmError(SPMM_INVALID, f"groups: {groups}, expected at least 1")
+    _counts(n, groups)
     L = lib()
     with _on(stream):
         offsets = torch.empty(groups + 1, dtype=torch.int32, device=device)
@@ -206,6 +215,7 @@ def dispatch(x, routing: Routing, out=None, stream=None):
     _operand(x, "x", _TYPES, 2)
     _rows(x, "x", T)
     D, device = x.shape[1], x.device
+    _counts(T, k, D, E)
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
     _operand(routing.offsets, "routing.offsets", _INT, (E + 1,), device)
     with _on(stream):
@@ -221,6 +231,7 @@ def _gather(ys, name: str, routing: Routing, weighted: bool, out, stream):
     _operand(ys, name, _TYPES, 2)
     _rows(ys, name, T * k)
     D, device = ys.shape[1], ys.device
+    _counts(T, k, D)
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
     if weighted:
         _operand(routing.weights, "routing.weights", _FLOAT, (T, k), device)
@@ -249,6 +260,7 @@ def combine_backward(dy, ys, routing: Routing, stream=None):
     _operand(ys, "ys", _TYPES, 2)
     _rows(ys, "ys", T * k)
     D, device = ys.shape[1], ys.device
+    _counts(T, k, D, E)
     _operand(dy, "dy", (ys.dtype,), (T, D), device)
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
     _operand(routing.weights, "routing.weights", _FLOAT, (T, k), device)
@@ -280,6 +292,7 @@ def _weights(w, dtype, K: int, w_in_rows: bool, device):
         n, k = k, n
     if k != K:
         raise SpmmError(SPMM_INVALID, f"w: shape {tuple(w.shape)} for rows of {K} elements")
+    _counts(G, n, k)
     return G, n
 
 
@@ -292,6 +305,7 @@ def grouped_mm(x, w, offsets, w_in_rows: bool = False, out=None, stream=None):
     device = x.device
     G, N = _weights(w, x.dtype, K, w_in_rows, device)
     _operand(offsets, "offsets", _INT, (G + 1,), device)
+    _counts(S, N)
     with _on(stream):
         out = _out(out, "out", x.dtype, (S, N), device)
         _check(lib().spmm_c_grouped_mm(x.data_ptr(), w.data_ptr(), _TYPES[x.dtype],
@@ -310,6 +324,7 @@ def grouped_mm_backward(dy, x, w, offsets, w_in_rows: bool = False, stream=None,
     G, N = _weights(w, x.dtype, K, w_in_rows, device)
     _operand(dy, "dy", (x.dtype,), (S, N), device)
     _operand(offsets, "offsets", _INT, (G + 1,), device)
+    _counts(S, N)
     p, q, height, width = (x, dy, K, N) if w_in_rows else (dy, x, N, K)
     with _on(stream):
         dw = torch.empty_like(w) if weights else None
@@ -344,6 +359,7 @@ def adapter_mm(x, w, a, b, ids, scale=None, out=None, stream=None):
     _operand(a, "a", (x.dtype,), (L, R, K), device)
     _operand(b, "b", (x.dtype,), (L, N, R), device)
     _operand(ids, "ids", _INT, (T,), device)
+    _counts(T, N, K, L, R)
     if scale is not None:
         _operand(scale, "scale", _FLOAT, (L,), device)
     library = lib()

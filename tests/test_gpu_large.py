@@ -282,3 +282,25 @@ def test_more_tokens_than_a_launch_has_waves_in_the_router_gradient(S, torch):
     off = (S.route_backward(logits, r, dweights, out=out) - want).abs()
     # p: exp, a sum of two and a quotient on both sides; |dw - mean| <= 2
     assert off.max().item() <= 2 * 16 * 2.0 ** -24
+
+
+def test_sizes_past_32_bits_are_refused(S, torch):
+    """4 294 967 300 rows are not four."""
+    n = (1 << 32) + 4
+    say(f"refusals of {n} rows")
+    x = torch.empty((n, 1), dtype=torch.float16, device="cuda")
+    row, col = x.view(1, n), torch.zeros((1, 8, 1), dtype=torch.float16, device="cuda")
+    one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    r = S.route(torch.zeros((1, 1), device="cuda"), 1)
+    ids = row.view(torch.int32)
+    for call in (lambda: S.route(x, 1), lambda: S.route(row, 1), lambda: S.group_entries(ids, 2),
+                 lambda: S.dispatch(row, r), lambda: S.combine(row, r),
+                 lambda: S.dispatch_backward(row, r), lambda: S.combine_backward(row, row, r),
+                 lambda: S.grouped_mm(x, col, one),
+                 lambda: S.grouped_mm(col[0, :1], x.view(1, n, 1), one),
+                 lambda: S.grouped_mm_backward(x, x, col[:, :1], one),
+                 lambda: S.adapter_mm(col[0, :1], x, col[:, :1], x.view(1, n, 1), one[:1])):
+        with pytest.raises(S.SpmmError) as e:
+            call()
+        assert e.value.code == S.SPMM_UNSUPPORTED
+    assert S.group_entries(one, 2)[0].tolist() == [0, 1, 2]
