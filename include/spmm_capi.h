@@ -414,8 +414,8 @@ int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int to
 /* ---- grouped products and low-rank adapters (no reference counterpart) --
  * Matrix-core products of SPMM_F16 or SPMM_BF16 operands (SPMM_UNSUPPORTED for
  * SPMM_F32), fp32 sums rounded once; contiguous device arrays, rows of up to
- * 2^22 elements, any number of them (SPMM_UNSUPPORTED where a launch would need
- * 2^32 threads: some 2^24 groups or 2^29 rows with adapters).
+ * 2^22 elements, 2^31 - 2^16 of them (SPMM_UNSUPPORTED beyond, and where a launch
+ * would need 2^32 threads: some 2^24 groups or 2^29 rows with adapters).
  * grouped_mm: the block-diagonal product of rows in group order with their
  *   group's weights.  Group g has rows [d_offsets[g], d_offsets[g+1]) of d_x
  *   [rows, depth]; d_w is [groups, width, depth], or [groups, depth, width]

@@ -1331,6 +1331,10 @@ Error check_product(int total, int groups, int width, int depth, const char* nam
     if (256LL * std::max(width, depth) > kMostElements) {
         return Error{kUnsupported, std::string(name) + ": rows over 2^22 elements"};
     }
+    // a tile past the last row has to stay an int
+    if (total > 0x7fff0000) {
+        return Error{kUnsupported, std::string(name) + ": over 2^31 - 2^16 rows"};
+    }
     return Error{};
 }
 

@@ -236,6 +236,10 @@ Error check_rows(int tokens, int k, int features, const char* name) {
     if (static_cast<long long>(tokens) * k > 0x3fffffffLL) {
         return Error{kUnsupported, std::string(name) + ": over 2^30 entries"};
     }
+    // a step past a row's last column has to stay an int
+    if (features > 0x7fff0000) {
+        return Error{kUnsupported, std::string(name) + ": rows over 2^31 - 2^16 elements"};
+    }
     return Error{};
 }
 
