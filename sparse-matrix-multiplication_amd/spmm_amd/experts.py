@@ -85,10 +85,14 @@ def _counts(*sizes) -> None:
 _here = contextlib.nullcontext()
 
 
-def _on(stream):
+def _on(stream, device):
     """Allocations inside belong to the stream that the launch goes to, so that
     freeing them needs no wait of another stream's."""
-    return _here if stream is None else torch.cuda.stream(stream)
+    if stream is None:
+        return _here
+    if getattr(stream, "device", None) != device:
+        raise SpmmError(SPMM_INVALID, f"stream: {stream!r}, expected a torch stream on {device}")
+    return torch.cuda.stream(stream)
 
 
 def _stream(device) -> int:
@@ -146,7 +150,7 @@ def route(logits, k: int, over: str = "chosen", stream=None) -> Routing:
     _counts(T, E)
     L = lib()
     device = logits.device
-    with _on(stream):
+    with _on(stream, device):
         experts = torch.empty((T, k), dtype=torch.int32, device=device)
         slots = torch.empty((T, k), dtype=torch.int32, device=device)
         entries = torch.empty(T * k, dtype=torch.int32, device=device)
@@ -176,7 +180,7 @@ def route_backward(logits, routing: Routing, dweights, out=None, stream=None):
     _counts(T, E)
     _operand(routing.experts, "routing.experts", _INT, (T, k), device)
     _operand(dweights, "dweights", _FLOAT, (T, k), device)
-    with _on(stream):
+    with _on(stream, device):
         out = _out(out, "out", logits.dtype, (T, E), device)
         _check(lib().spmm_c_route_backward(
             logits.data_ptr(), _TYPES[logits.dtype], T, E, k, over_id, routing.experts.data_ptr(),
@@ -197,7 +201,7 @@ def group_entries(ids, groups: int, stream=None):
         raise SpmmError(SPMM_INVALID, f"groups: {groups}, expected at least 1")
     _counts(n, groups)
     L = lib()
-    with _on(stream):
+    with _on(stream, device):
         offsets = torch.empty(groups + 1, dtype=torch.int32, device=device)
         entries = torch.empty(n, dtype=torch.int32, device=device)
         slots = torch.empty_like(ids)
@@ -218,7 +222,7 @@ def dispatch(x, routing: Routing, out=None, stream=None):
     _counts(T, k, D, E)
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
     _operand(routing.offsets, "routing.offsets", _INT, (E + 1,), device)
-    with _on(stream):
+    with _on(stream, device):
         out = _out(out, "out", x.dtype, (T * k, D), device)
         _check(lib().spmm_c_dispatch(x.data_ptr(), _TYPES[x.dtype], T, k, D,
                                      routing.slots.data_ptr(), routing.offsets.data_ptr(), E,
@@ -235,7 +239,7 @@ def _gather(ys, name: str, routing: Routing, weighted: bool, out, stream):
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
     if weighted:
         _operand(routing.weights, "routing.weights", _FLOAT, (T, k), device)
-    with _on(stream):
+    with _on(stream, device):
         out = _out(out, "out", ys.dtype, (T, D), device)
         _check(lib().spmm_c_combine(ys.data_ptr(), _TYPES[ys.dtype], T, k, D,
                                     routing.slots.data_ptr(),
@@ -265,7 +269,7 @@ def combine_backward(dy, ys, routing: Routing, stream=None):
     _operand(routing.slots, "routing.slots", _INT, (T, k), device)
     _operand(routing.weights, "routing.weights", _FLOAT, (T, k), device)
     _operand(routing.offsets, "routing.offsets", _INT, (E + 1,), device)
-    with _on(stream):
+    with _on(stream, device):
         dys = torch.empty_like(ys)
         dweights = torch.empty((T, k), dtype=torch.float32, device=device)
         _check(lib().spmm_c_combine_backward(
@@ -306,7 +310,7 @@ def grouped_mm(x, w, offsets, w_in_rows: bool = False, out=None, stream=None):
     G, N = _weights(w, x.dtype, K, w_in_rows, device)
     _operand(offsets, "offsets", _INT, (G + 1,), device)
     _counts(S, N)
-    with _on(stream):
+    with _on(stream, device):
         out = _out(out, "out", x.dtype, (S, N), device)
         _check(lib().spmm_c_grouped_mm(x.data_ptr(), w.data_ptr(), _TYPES[x.dtype],
                                        offsets.data_ptr(), G, S, N, K, int(bool(w_in_rows)),
@@ -326,7 +330,7 @@ def grouped_mm_backward(dy, x, w, offsets, w_in_rows: bool = False, stream=None,
     _operand(offsets, "offsets", _INT, (G + 1,), device)
     _counts(S, N)
     p, q, height, width = (x, dy, K, N) if w_in_rows else (dy, x, N, K)
-    with _on(stream):
+    with _on(stream, device):
         dw = torch.empty_like(w) if weights else None
         dx = torch.empty_like(x) if rows else None
         L, s = lib(), _stream(device)
@@ -363,7 +367,7 @@ def adapter_mm(x, w, a, b, ids, scale=None, out=None, stream=None):
     if scale is not None:
         _operand(scale, "scale", _FLOAT, (L,), device)
     library = lib()
-    with _on(stream):
+    with _on(stream, device):
         out = _out(out, "out", x.dtype, (T, N), device)
         work = torch.empty(library.spmm_c_adapter_workspace(T, R), dtype=torch.uint8,
                            device=device)
