@@ -1397,6 +1397,12 @@ Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, con
     return launch_with_lds<few_rows_product<T, RF, CF, WAVES, depth, ADAPT>>(
         grid, WAVES * 64, lds, stream, name, a);
 }
+// Rows of a group that few_rows_product is launched for: all of one group's, and twice the
+// mean of more, so that few of them need a second tile that reads W again.
+long long few_rows(const TileArgs& a) {
+    const long long groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
+    return groups == 1 ? a.total : 2LL * a.total / groups;
+}
 // How few_rows_product is launched for groups of `rows` rows or so (all are right).
 //   Columns: the rows' own reading counts, and 64 columns share it (2048 rows over 64
 //     groups of 2048 x 4096: 211 us, 282 with sixteen columns).  For whole pieces only:
@@ -1405,16 +1411,16 @@ Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, con
 //     64 groups of 2048 x 4096: 167 us with three, 227 with one).
 //   Single: a workgroup a CU or so, which has all of the LDS for its loads.
 enum class Few { Columns, Groups, Single };
-Few few_form(const TileArgs& a, double rows, bool pieces) {
-    const double row_tiles = a.offsets == nullptr ? std::ceil(rows / 64) : a.groups;
+Few few_form(const TileArgs& a, long long rows, bool pieces) {
+    const double row_tiles = a.offsets == nullptr ? std::ceil(rows / 64.0) : a.groups;
     if (pieces && rows > 32 && row_tiles * std::ceil(a.width / 64.0) >= 192) return Few::Columns;
     return a.groups > 1 && rows <= 32 ? Few::Groups : Few::Single;
 }
 template <typename T, bool ADAPT>
-Error launch_few_rows(const TileArgs& a, long long rows, bool pieces, hipStream_t stream,
-                      const char* name) {
+Error launch_few_rows(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
     constexpr int kAll = 160 * 1024;
-    switch (few_form(a, static_cast<double>(rows), pieces)) {
+    const long long rows = few_rows(a);
+    switch (few_form(a, rows, pieces)) {
         case Few::Columns:
             return launch_few_rows_of<T, 4, 4, 4, 80 * 1024, ADAPT>(a, pieces, stream, name);
         case Few::Groups:
@@ -1500,7 +1506,7 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
     };
     const bool words = a.depth % 2 == 0 && ((reinterpret_cast<uintptr_t>(a.rows) |
                                              reinterpret_cast<uintptr_t>(a.cols)) & 2) == 0;
-    const double rows = groups == 1 ? mean : 2 * mean;
+    const long long rows = few_rows(a);
     const double tiles64 = groups == 1 ? std::ceil(mean / 64)
                                        : groups * std::max(1.0, mean / 64 + 0.5);
     double few = weights / 6.3e6 * (1 + mean / 160) * (pieces ? 1 : words ? 1.1 : 2);
@@ -1510,7 +1516,7 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {
                                     (2 + 2.2 * std::ceil(a.depth / 256.0)));
             break;
         case Few::Single: {
-            const double high  = std::ceil(std::min(rows, 64.0) / 16);  // its rows' share of the loads
+            const double high  = std::ceil(std::min(rows, 64LL) / 16.0);  // its rows' share of the loads
             const double round = pieces ? 3 + std::ceil(a.depth / 512.0)
                                         : (1 + a.depth / 340.0) * (words ? 1.3 : 1.65) * (high + 2) / 6;
             few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 16.0) / 256) * round);
@@ -1580,11 +1586,9 @@ Error launch_grouped_mm(const void* x, const void* w, ElementType type, const in
     a.depth = depth;
     const bool pieces = depth % 8 == 0 && (!w_in_rows || width % 8 == 0) && aligned16(x) && aligned16(w);
     const Form form = choose_form(a, pieces, !w_in_rows);
-    // twice the mean, so that few groups need a second tile that reads W again
-    const long long rows = 2LL * total / std::min(groups, total);
     return with_half(type, "grouped_mm", [&](auto zero) {
         using T = decltype(zero);
-        if (form == Form::FewRows) return launch_few_rows<T, false>(a, rows, pieces, stream, "grouped_mm");
+        if (form == Form::FewRows) return launch_few_rows<T, false>(a, pieces, stream, "grouped_mm");
         return w_in_rows ? launch_tiles<T, false, true, false>(a, form, stream, "grouped_mm")
                          : launch_tiles<T, false, false, false>(a, form, stream, "grouped_mm");
     });
@@ -1662,7 +1666,7 @@ Error launch_adapter_mm(const void* x, const void* w, const void* down, const vo
         } else {
             SPMM_TRY((launch_shrink<T, 1, 4, 2, 53 * 1024>(a, whole, down, scale, std::max(1, std::min(8, adapters)), stream)));
         }
-        if (form == Form::FewRows) return launch_few_rows<T, true>(a, total, pieces, stream, "adapter_mm");
+        if (form == Form::FewRows) return launch_few_rows<T, true>(a, pieces, stream, "adapter_mm");
         return launch_tiles<T, false, false, true>(a, form, stream, "adapter_mm");
     });
 }
