@@ -12,9 +12,9 @@
 // entries from all blocks' counts.  Places follow from counts alone, never from
 // the order of atomics, so equal experts keep their entries' order.
 //
-// Up to 512 entries or so are one block's, which chooses and places in one launch: a
-// call for one token of 64 experts, k = 6, is then bound by its host side (15.8 us;
-// 18.5 with two launches).
+// Few tokens are one block's, which chooses and places in one launch: a call for one
+// token of 64 experts, k = 6, is then bound by its host side (15.8 us; 18.5 with two
+// launches).
 
 #include <hip/hip_runtime.h>
 
@@ -485,10 +485,22 @@ void with_per(int experts, F f) {
     else f(std::integral_constant<int, 16>{});
 }
 
-// Tokens a block of route_choose takes: whole rounds of its waves, and about a
-// chunk of the sort's entries.
-int tokens_per_block(long long tokens, int k) {
-    const long long t = (chunk_of(tokens * k) + k - 1) / k;
+// 16-bit logits of few experts and choices go four tokens a wave.
+bool four_a_wave(ElementType type, int experts, int k) {
+    return type != ElementType::F32 && k <= 16 && experts <= 256;
+}
+
+// Tokens a block that chooses takes: at most about a chunk of the sort's entries, and so
+// few rounds of its waves (two, or one of four tokens a wave) that a block a CU shares them
+// before a block takes more.  16384 tokens of 64 experts, fp32, k = 1: 9.6 us, 28.4 with
+// chunks of entries alone; 512 tokens 7.3, 24.5 in one block; of 1024 experts 17.1, 83.
+// What one block does in less time than a second launch takes is left to it: 64 tokens of 64
+// experts, fp32, k = 1 5.7 us, 7.0 in two blocks; of 1024 experts, k = 8 43, 29 so.
+int tokens_per_block(long long tokens, int experts, int k, bool four) {
+    long long t = (chunk_of(tokens * k) + k - 1) / k;
+    if (tokens > (four ? 128 : k <= 4 && experts <= 256 ? 64 : 48)) {
+        t = std::min(t, std::max<long long>(four ? 64 : 32, (tokens + 255) / 256));
+    }
     return static_cast<int>((t + kChooseWaves - 1) / kChooseWaves * kChooseWaves);
 }
 
@@ -501,8 +513,9 @@ long long group_workspace(long long entries, int groups) {
 
 long long route_workspace(long long tokens, int experts, int k) {
     if (tokens <= 0 || experts < 1 || k < 1) return 0;
+    // the counts of any element type: one token a wave has the more blocks
     return static_cast<long long>(sizeof(int)) * experts *
-           blocks_of(tokens, tokens_per_block(tokens, k));
+           blocks_of(tokens, tokens_per_block(tokens, experts, k, false));
 }
 
 Error launch_group_entries(const int* ids, int n, int groups, int* offsets, int* entries,
@@ -529,7 +542,8 @@ Error launch_route(const void* logits, ElementType type, int tokens, int experts
     SPMM_TRY(check_sizes(tokens, experts, k));
     if (offsets == nullptr) return Error{kInvalid, "route: null offsets"};
     if (tokens == 0) return no_entries(experts, offsets, stream);
-    const int per = tokens_per_block(tokens, k);
+    const bool four = four_a_wave(type, experts, k);
+    const int per = tokens_per_block(tokens, experts, k, four);
     const int blocks = blocks_of(tokens, per);
     if (logits == nullptr || out_experts == nullptr || out_weights == nullptr ||
         entries == nullptr || slots == nullptr || workspace == nullptr) {
@@ -546,7 +560,7 @@ Error launch_route(const void* logits, ElementType type, int tokens, int experts
                                out_weights, out_experts, order);
         };
         if constexpr (sizeof(T) == 2) {
-            if (k <= 16 && experts <= 256) {
+            if (four) {
                 auto quads = [&](auto n) {
                     launch(alone ? route_choose_quads<T, n.value, true>
                                  : route_choose_quads<T, n.value, false>);
