@@ -407,6 +407,10 @@ __device__ __forceinline__ Parts<T> parts_of(const float (&v)[8], int shift) {
 template <typename T, int RF, int CF, bool PIECES>
 struct Adapters {
     static constexpr bool kShift = std::is_same_v<T, _Float16>;
+    // 32s of the rank whose parts stay for all adapters among sixteen rows (8192 rows x 4096 x
+    // 4096, rank 64, an adapter a row: 640 us with two, 685 with one; 701 x 2003 x 1001, rank
+    // 12, in 64 x 64 tiles: 32.0 with one, 33.5 with two)
+    static constexpr int kKept = CF > 2 ? 2 : 1;
     const float* h;
     const T*     b;
     int          id[RF];     // of row 16 i + (lane & 15), -1 for none
@@ -479,18 +483,25 @@ struct Adapters {
         }
     }
     // Sums for the rows 16 i .. that `adapter` has (`own`), of both parts of h or the high
-    // one alone.
+    // one alone.  kept: the parts of the rank's first kKept x 32, of every row.
     template <bool LOW>
     __device__ __forceinline__ void multiply(int i, int adapter, bool own, int up,
-                                             f32x4 (&sum)[CF]) const {
+                                             const Parts<T> (&kept)[kKept], f32x4 (&sum)[CF]) const {
 #pragma unroll
         for (int j = 0; j < CF; ++j) sum[j] = f32x4(0.0f);
         for (int k0 = 0; k0 < rank; k0 += 32) {
             Operand<T> fc[CF];
             read_b(adapter, k0, fc);
-            float v[8];
-            read_h(i, k0, own, v);
-            const Parts<T> fr = parts_of<T>(v, up);
+            Parts<T> fr;
+            if (k0 < 32 * kKept) {
+                const Parts<T> all = kKept == 1 || k0 == 0 ? kept[0] : kept[kKept - 1];
+                const Operand<T> none = __builtin_bit_cast(Operand<T>, uint4{});
+                fr = Parts<T>{own ? all.high : none, own ? all.low : none};
+            } else {
+                float v[8];
+                read_h(i, k0, own, v);
+                fr = parts_of<T>(v, up);
+            }
             if constexpr (LOW) {
 #pragma unroll
                 for (int j = 0; j < CF; ++j) sum[j] = mfma(fc[j], fr.low, sum[j]);
@@ -506,20 +517,27 @@ struct Adapters {
         const int lane = threadIdx.x & 63;
         float* at = sums + (lane & 15) * pitch + 4 * (lane >> 4);
         int left_id = mine;
-        for (;;) {
-            const unsigned long long left = __ballot(left_id >= 0);
-            if (left == 0) break;
+        unsigned long long left = __ballot(left_id >= 0);
+        if (left == 0) return;
+        Parts<T> kept[kKept];
+#pragma unroll
+        for (int n = 0; n < kKept; ++n) {
+            float v[8];
+            read_h(i, 32 * n, mine >= 0, v);
+            kept[n] = parts_of<T>(v, up);
+        }
+        for (; left != 0; left = __ballot(left_id >= 0)) {
             const int adapter = __builtin_amdgcn_readlane(left_id, __builtin_ctzll(left));
             const bool own = mine == adapter;
             f32x4 sum[CF];
-            multiply<true>(i, adapter, own, up, sum);
+            multiply<true>(i, adapter, own, up, kept, sum);
             f32x4 none(0.0f);  // stays 0 while all are finite
 #pragma unroll
             for (int j = 0; j < CF; ++j) none = sum[j] * 0.0f + none;
             const bool finite = (none[0] + none[1]) + (none[2] + none[3]) == 0.0f;
             if (__ballot(own && !finite) != 0) {
                 f32x4 high[CF];
-                multiply<false>(i, adapter, own, up, high);
+                multiply<false>(i, adapter, own, up, kept, high);
 #pragma unroll
                 for (int j = 0; j < CF; ++j)
 #pragma unroll
@@ -551,35 +569,49 @@ constexpr int kStoreFloats = 16 * (CF * 16 + 4);
 
 // Stores a wave's tile, sixteen rows at a time through its own part of LDS (`sums`,
 // free in all waves), so that whole row pieces leave in 16-byte stores.
-template <typename T, int RF, int CF, typename Extend>
+template <typename T, int RF, int CF>
+struct StoreTile {
+    static constexpr int kPitch = CF * 16 + 4, kLanes = CF * 2, kRows = 64 / kLanes;
+    const TileArgs& a;
+    const Tile<T>&  t;
+    int    r0, c0;
+    float* sums;
+
+    template <int I>
+    __device__ __forceinline__ void put(const f32x4 (&acc)[CF][RF]) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < CF; ++j) {
+            *reinterpret_cast<f32x4*>(sums + (lane & 15) * kPitch + j * 16 + 4 * (lane >> 4)) = acc[j][I];
+        }
+    }
+    __device__ __forceinline__ void store(int i) const {
+        const int lane = threadIdx.x & 63;
+        const int c = c0 + lane % kLanes * 8;
+        const int count = min(8, a.width - c);
+#pragma unroll
+        for (int n = 0; n < 16 / kRows; ++n) {
+            const int r = n * kRows + lane / kLanes;
+            const float* from = sums + r * kPitch + lane % kLanes * 8;
+            float f[8];
+            __builtin_memcpy(f, __builtin_assume_aligned(from, 16), 32);
+            const uint4 v = piece_from_float<T>(f);
+            if (r0 + i * 16 + r < t.rows_here && count > 0) {
+                T* p = t.out + static_cast<long long>(r0 + i * 16 + r) * a.width + c;
+                if (count == 8) store_piece(p, v);
+                else store_part(p, v, count);
+            }
+        }
+    }
+};
+template <typename T, int RF, int CF>
 __device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, int r0, int c0,
-                                           const f32x4 (&acc)[CF][RF], float* sums, Extend extend) {
-    constexpr int kPitch = CF * 16 + 4, kLanes = CF * 2, kRows = 64 / kLanes;
-    const int lane = threadIdx.x & 63;
-    const int s = lane & 15, q = lane >> 4;
-    const int c = c0 + lane % kLanes * 8;
-    const int count = min(8, a.width - c);
+                                           const f32x4 (&acc)[CF][RF], float* sums) {
+    const StoreTile<T, RF, CF> tile{a, t, r0, c0, sums};
     unrolled(std::make_integer_sequence<int, RF>{}, [&](auto at) {
-        constexpr int i = at.value;
-        if (r0 + i * 16 < t.rows_here) {
-#pragma unroll
-            for (int j = 0; j < CF; ++j) {
-                *reinterpret_cast<f32x4*>(sums + s * kPitch + j * 16 + 4 * q) = acc[j][i];
-            }
-            extend(at);
-#pragma unroll
-            for (int n = 0; n < 16 / kRows; ++n) {
-                const int r = n * kRows + lane / kLanes;
-                const float* from = sums + r * kPitch + lane % kLanes * 8;
-                float f[8];
-                __builtin_memcpy(f, __builtin_assume_aligned(from, 16), 32);
-                const uint4 v = piece_from_float<T>(f);
-                if (r0 + i * 16 + r < t.rows_here && count > 0) {
-                    T* p = t.out + static_cast<long long>(r0 + i * 16 + r) * a.width + c;
-                    if (count == 8) store_piece(p, v);
-                    else store_part(p, v, count);
-                }
-            }
+        if (r0 + at.value * 16 < t.rows_here) {
+            tile.template put<at.value>(acc);
+            tile.store(at.value);
         }
     });
 }
@@ -626,10 +658,24 @@ __device__ __forceinline__ void store_adapted(const TileArgs& a, const Tile<T>& 
                                               const f32x4 (&acc)[CF][RF], float* sums) {
     auto store = [&](auto pieces) {
         const Adapters<T, RF, CF, pieces.value> ad(a, t, r0, c0);
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [&](auto at) {
-            constexpr int i = at.value;
-            ad.add(i, ad.id[i], ad.kShift ? ad.shift[i] : 0, sums, CF * 16 + 4);
-        });
+        const StoreTile<T, RF, CF> tile{a, t, r0, c0, sums};
+        // one body for all sixteens of rows: they are gone through once, and as many bodies
+        // would come from memory first (8192 rows x 4096 x 4096, rank 64, an adapter a run of
+        // rows: fp16 254 us, 262 so; a different one a row 668 both, 748 with the parts made
+        // again for each)
+#pragma unroll 1
+        for (int i = 0; i < RF && r0 + i * 16 < t.rows_here; ++i) {
+            int mine = -1, up = 0;
+            unrolled(std::make_integer_sequence<int, RF>{}, [&](auto at) {
+                if (at.value == i) {
+                    tile.template put<at.value>(acc);
+                    mine = ad.id[at.value];
+                    if constexpr (ad.kShift) up = ad.shift[at.value];
+                }
+            });
+            ad.add(i, mine, up, sums, tile.kPitch);
+            tile.store(i);
+        }
     };
     if (a.b_pieces) store(std::true_type{});
     else store(std::false_type{});
@@ -767,7 +813,7 @@ __global__ __launch_bounds__(256, PIECES ? 1 : 2) void tile_product(TileArgs a) 
     if constexpr (ADAPT) {
         store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
     } else {
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums);
     }
 }
 
@@ -863,7 +909,7 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
     if constexpr (ADAPT) {
         store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
     } else {
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums);
     }
 }
 
@@ -1026,7 +1072,7 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
     if constexpr (ADAPT) {
         store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
     } else {
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums, [](auto) {});
+        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums);
     }
 }
 
