@@ -14,8 +14,9 @@ SPLIT = {torch.float16: 2.0 ** -22, torch.bfloat16: 2.0 ** -16}
 SHAPES = [
     (5, 64, 64, 3, 16), (48, 256, 512, 20, 16),  # few rows
     (300, 256, 4096, 3, 48),                     # 64 x 64 tiles
-    (1500, 1000, 520, 4, 8),                     # 128 x 128 tiles
-    (4090, 4088, 1032, 3, 24),                   # 256 x 256 tiles
+    (1500, 1000, 520, 4, 8),                     # few rows, 64 columns a workgroup
+    (4000, 1024, 1024, 4, 16), (4000, 1024, 1024, 3, 76),  # 128 x 128 tiles
+    (4090, 4088, 1032, 3, 24), (4090, 4088, 1032, 3, 100),  # 256 x 256 tiles
     # rows that begin between two words, in few rows and tiles
     (33, 130, 129, 5, 12), (823, 200, 6787, 7, 12), (1500, 1000, 521, 4, 9),
 ]
