@@ -9,9 +9,10 @@
 // The first is the product of a block-diagonal matrix (each group's rows a block)
 // with dense weights, and the adapters extend the contraction by a block-sparse
 // operand: one block of h a row against the stacked B.  Tile kernels (256 x 256, 128 x
-// 128) and a kernel for few rows do all three on matrix cores (v_mfma_f32_16x16x32,
-// fp32 sums), 64 steps of the contraction at a time through LDS.  Many rows are bound by
-// the matrix cores and the clock they leave, few by reading W.
+// 128, and 64 x 64 for few tiles with a long contraction) and a kernel for few rows do all
+// three on matrix cores (v_mfma_f32_16x16x32, fp32 sums), 64 steps of the contraction at a
+// time through LDS.  Many rows are bound by how well the matrix cores are fed and by the
+// clock that they leave, few by reading W.
 
 #include <hip/hip_runtime.h>
 
@@ -931,10 +932,13 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
 //   all but six (this tile's H is there), and for its operand reads.
 //   Past the contraction's end loads write zeros, so the counts always hold.
 //
-// 8 groups of 8192 x 4096 over 16384 rows: 864 us, 1270 TFLOP/s; in one group 776 us,
-// 1420.  The matrix cores are busy for 72% of the time, and at that the clock falls to
-// 1.4 - 1.65 GHz (data of zeros takes a sixth less time).  A tile costs 6 us beside its
-// 1.55 us for 64 steps: beginning, first loads and stores.
+// 8 groups of 8192 x 4096 over 16384 rows: 887 us a call, 1240 TFLOP/s (the kernel alone
+// 869 at best); in one group 783 us at best, 1400, and 808 on average.  The matrix cores
+// are busy for 73% of the time, and at that the clock falls to 1.4 - 1.65 GHz (data of
+// zeros takes a sixth less time).  That is no limit of the card: a library product of the
+// one group keeps them at 89% and takes 740 at best, 789 on average.  What is left lies in
+// the two barriers a tile, with their waits for loads, and in the 6 us that a tile costs
+// beside its 1.55 us for 64 steps: beginning, first loads and stores.
 template <typename T, bool GRAD, bool COLS_MAJOR, bool ADAPT>
 __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
     constexpr int BR = 256, BC = 256, RF = 8, CF = 8;
@@ -1251,7 +1255,7 @@ struct Shares {
 // The workgroups (x, y, 0 ..) take the adapters among their rows in turn: one each
 // where there are as many of them as rows, so that few rows with an adapter each
 // still spread over the chip.  Few rows are bound by one workgroup's chain of loads (48
-// rows of 4096 with an adapter of rank 16 each: 6.4 us), many by reading the adapters for
+// rows of 4096 with an adapter of rank 16 each: 6.3 us), many by reading the adapters for
 // every sixteen rows (8192 rows of 4096, rank 64: 28 us).
 //   D: stages of ring_share; 0: wave_share, for rows that are no whole pieces.
 template <typename T, int RF, int CF, int WAVES, int D>
@@ -1312,7 +1316,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_shrink(TileArgs a, const T
 // takes CF x 16 columns and up to RF x 16 rows of a group, its waves share the
 // contraction, so that a projection of a few thousand columns still has a workgroup
 // a CU.  D: as for adapter_shrink.  64 groups of 2048 x 4096, 256 rows: 168 us, 6.4 TB/s,
-// what reads alone reach; 48 rows x 4096 x 4096 with adapters 10.3 us.
+// what reads alone reach; 48 rows x 4096 x 4096 with adapters 10.5 us.
 template <typename T, int RF, int CF, int WAVES, int D, bool ADAPT>
 __global__ __launch_bounds__(WAVES * 64) void few_rows_product(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char s_ring[];  // and then the shares
@@ -1539,7 +1543,9 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
 //     tiles 27).
 //   Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s, W [k][c]
 //     at 5.8 (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows
-//     257, 285).  Adapters hold tiles up by 6 us, those of 64 x 64 by 5.
+//     257, 285).  Adapters hold tiles up by 6 us, those of 64 x 64 by 5: about what a run of
+//     rows with one adapter costs (4000 x 1024 x 1024, rank 16: 5; 701 x 2003 x 1001, rank
+//     12: 5; two rounds of 256 x 256, rank 64: 25), less than an adapter a row does (11).
 //   64 x 64 tiles: 300 rows x 1024 x 1024 with adapters 14 us, 128 x 128 21; 100 rows x
 //     4000 x 4097 30, few_rows_product 43; 12 rows x 1504 x 2057 15, few_rows_product 8.
 Form choose_form(const TileArgs& a, bool pieces, bool few_allowed) {

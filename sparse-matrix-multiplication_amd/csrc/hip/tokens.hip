@@ -9,9 +9,10 @@
 // slots (or the other way round), in 16-byte pieces, by one wave, or by a
 // workgroup where there are too few tokens to fill the chip with waves.  Sums
 // run over j in order, in fp32, and are rounded once.  8192 tokens x 8 x 4096 bf16:
-// dispatch 105 us (5.7 TB/s; a copy reaches 5.2), combine_backward 252 (4.5).  5003 x 4 x
-// 2050 fp32, whose rows start inside lines: combine_backward 77 us, dispatch's gradient 56
-// (4.9 and 3.6 TB/s).
+// dispatch 105 us (5.7 TB/s; a copy reaches 5.2), combine 130 (4.6), combine_backward 249
+// (4.6).  5003 x 4 x 2050 fp32, whose rows start inside lines: combine_backward 77 us,
+// dispatch's gradient 57 (4.9 and 3.6 TB/s; four 16-byte loads a lane are under way, and
+// the next columns' begin when they are used).
 
 #include <hip/hip_runtime.h>
 
@@ -243,8 +244,11 @@ Error check_rows(int tokens, int k, int features, const char* name) {
     return Error{};
 }
 
-// One wave a token fills the chip's 1024 SIMDs from about this many tokens on;
-// below, four waves share a token.
+// One wave a token fills the chip's 1024 SIMDs from about this many tokens on; below, four
+// waves share a token.  Measured both ways over 126 sizes: 8192 tokens x 8 x 128 bf16 5.9,
+// 7.2 and 11.6 us (dispatch, combine, combine_backward) with one wave, 7.5, 9.0 and 25.1
+// with four; 1024 x 1 x 7168 4.9, 14.5 and 14.2, 4.7, 8.6 and 8.1.  Rows of 8 KB and more
+// are up to 15% faster with four waves past it too.
 constexpr int kWaveTokens = 4096;
 
 // Rows that the 256 MB cache in front of memory cannot hold are stored past it: 8192

@@ -11,7 +11,10 @@ low-rank adapter.
 
 Operands are contiguous cuda tensors on the current device; outputs are
 allocated where none is given, on the stream that the launch goes to (`stream`
-or the current one).  Nothing synchronises.
+or the current one).  An output given must not share memory with an operand.
+Nothing synchronises.  Results carry no autograd graph, whatever the operands
+require: a training step calls the gradients, or takes ``ExpertLayer``
+(expert_layer.py), which does so under autograd.
 """
 from __future__ import annotations
 
