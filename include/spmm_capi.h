@@ -421,8 +421,8 @@ int spmm_c_combine_backward(const void* d_dy, const void* d_ys, int type, int to
  *   [rows, depth]; d_w is [groups, width, depth], or [groups, depth, width]
  *   with w_in_rows; d_out [rows, width], rows in no group (before the first and
  *   behind the last) zero.  d_offsets ascends from any row on; values outside
- *   [0, rows] are taken as its ends.  The gradient for x is the same call on dout
- *   with w_in_rows the other way round.
+ *   [0, rows] are taken as its ends; null with one group: it has all rows.  The gradient
+ *   for x is the same call on dout with w_in_rows the other way round.
  * grouped_outer: d_out[g] [height, width] = the sum over the group's rows of
  *   p[s]^T q[s], zero for an empty group: the gradient of the weights (p = dout,
  *   q = x, or the other way round for w_in_rows).
@@ -442,6 +442,52 @@ int spmm_c_adapter_mm(const void* d_x, const void* d_w, const void* d_a, const v
                       const int* d_ids, const float* d_scale, int type, int rows, int width,
                       int depth, int adapters, int rank, void* d_out, void* d_workspace,
                       void* stream);
+
+/* ---- gated feed-forward blocks, activations kept in 8 bits, products in 8-bit
+ * integers (no reference counterpart) ------------------------------------
+ * Groups as for grouped_mm (d_offsets null: one group of all rows).
+ * gated_mm: h = act(g) * u with g, u = d_x times both halves of the group's weights
+ *   d_w [groups, 2, width, depth], the gates' rows first; fp16 or bf16, fp32 sums.  act
+ *   0: silu, 1: gelu, 2: gelu by tanh.  d_out [rows, width], rows in no group zero.
+ *   d_kept: null, or g and u [rows, 2, width] for the gradients, of the operands' type or,
+ *   with d_kept_scales, packed as by pack8 from their fp32 sums.
+ * gated_grad: from d_dh [rows, width] and what was kept, d_dkept [rows, 2, width], the
+ *   gradients of g and u, and h again in d_h where that is not null.  The gradients of x
+ *   and of the weights are grouped_mm (w_in_rows) and grouped_outer of d_dkept as rows of
+ *   2 width.
+ * pack8: blocks of 32 values along a row (the last may be shorter) as int8 d_values
+ *   [rows, width] and a scale byte each, d_scales [rows, width / 32 rounded up]: the value
+ *   is q 2^(scale - 133), scale the exponent byte of the block's largest magnitude in fp32
+ *   (at least 7), q the nearest integer to even, at most 127 in magnitude; scale 255, and
+ *   NaN all its values, for a block with an infinity or NaN.  fp32, fp16 or bf16.
+ * unpack8: the values, rounded to the output's type (exact in bf16).
+ * quantize_rows: d_values int8 [rows, width rounded up to 16], zero past width, and fp32
+ *   d_scales [rows]: scale = max / 127 and q = x (127 / max) rounded to the nearest integer,
+ *   max a row's largest magnitude, at least 2^-100; scale 0 for a row of zeros, NaN for
+ *   one with an infinity or NaN.
+ * int8_mm: d_out[s, c] = x_scales[s] w_scales[c] sum_k x[s, k] w[c, k] for quantised rows
+ *   d_x [rows, depth], d_w [groups, width, depth], d_w_scales [groups, width]; depth as
+ *   padded, a multiple of 16 up to 131056, values 16-byte aligned.  The sum is exact,
+ *   d_out fp32, fp16 or bf16 (out_type).
+ * gated_int8_mm: gated_mm of quantised rows, d_w [groups, 2, width, depth], d_w_scales
+ *   [groups, 2, width]. */
+int spmm_c_gated_mm(const void* d_x, const void* d_w, int type, const int* d_offsets, int groups,
+                    int rows, int width, int depth, int act, void* d_out, void* d_kept,
+                    void* d_kept_scales, void* stream);
+int spmm_c_gated_grad(const void* d_dh, int type, const void* d_kept, const void* d_kept_scales,
+                      int rows, int width, int act, void* d_dkept, void* d_h, void* stream);
+int spmm_c_pack8(const void* d_x, int type, long long rows, int width, void* d_values,
+                 void* d_scales, void* stream);
+int spmm_c_unpack8(const void* d_values, const void* d_scales, int type, long long rows, int width,
+                   void* d_out, void* stream);
+int spmm_c_quantize_rows(const void* d_x, int type, long long rows, int width, void* d_values,
+                         float* d_scales, void* stream);
+int spmm_c_int8_mm(const void* d_x, const float* d_x_scales, const void* d_w,
+                   const float* d_w_scales, const int* d_offsets, int groups, int rows, int width,
+                   int depth, int out_type, void* d_out, void* stream);
+int spmm_c_gated_int8_mm(const void* d_x, const float* d_x_scales, const void* d_w,
+                         const float* d_w_scales, const int* d_offsets, int groups, int rows,
+                         int width, int depth, int act, int out_type, void* d_out, void* stream);
 
 /* ---- measurement helpers (no reference counterpart) -------------------
  * Launch one entry point `reps` times back to back on `stream` without

@@ -1111,4 +1111,81 @@ int spmm_c_adapter_mm(const void* d_x, const void* d_w, const void* d_a, const v
     });
 }
 
+int spmm_c_gated_mm(const void* d_x, const void* d_w, int type, const int* d_offsets, int groups,
+                    int rows, int width, int depth, int act, void* d_out, void* d_kept,
+                    void* d_kept_scales, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_gated_mm(
+            d_x, d_w, t, d_offsets, groups, rows, width, depth, static_cast<spmm::engine::Act>(act),
+            d_out, d_kept, d_kept_scales, as_stream(stream)));
+    });
+}
+
+int spmm_c_gated_grad(const void* d_dh, int type, const void* d_kept, const void* d_kept_scales,
+                      int rows, int width, int act, void* d_dkept, void* d_h, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_gated_grad(
+            d_dh, t, d_kept, d_kept_scales, rows, width, static_cast<spmm::engine::Act>(act), d_dkept,
+            d_h, as_stream(stream)));
+    });
+}
+
+int spmm_c_pack8(const void* d_x, int type, long long rows, int width, void* d_values, void* d_scales,
+                 void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_pack8(d_x, t, rows, width, d_values, d_scales,
+                                                      as_stream(stream)));
+    });
+}
+
+int spmm_c_unpack8(const void* d_values, const void* d_scales, int type, long long rows, int width,
+                   void* d_out, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_unpack8(d_values, d_scales, t, rows, width, d_out,
+                                                        as_stream(stream)));
+    });
+}
+
+int spmm_c_quantize_rows(const void* d_x, int type, long long rows, int width, void* d_values,
+                         float* d_scales, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_quantize_rows(d_x, t, rows, width, d_values, d_scales,
+                                                              as_stream(stream)));
+    });
+}
+
+int spmm_c_int8_mm(const void* d_x, const float* d_x_scales, const void* d_w, const float* d_w_scales,
+                   const int* d_offsets, int groups, int rows, int width, int depth, int out_type,
+                   void* d_out, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(out_type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_int8_mm(d_x, d_x_scales, d_w, d_w_scales, d_offsets,
+                                                        groups, rows, width, depth, t, d_out,
+                                                        as_stream(stream)));
+    });
+}
+
+int spmm_c_gated_int8_mm(const void* d_x, const float* d_x_scales, const void* d_w,
+                         const float* d_w_scales, const int* d_offsets, int groups, int rows,
+                         int width, int depth, int act, int out_type, void* d_out, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(out_type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_gated_int8_mm(
+            d_x, d_x_scales, d_w, d_w_scales, d_offsets, groups, rows, width, depth,
+            static_cast<spmm::engine::Act>(act), t, d_out, as_stream(stream)));
+    });
+}
+
 }  // extern "C"

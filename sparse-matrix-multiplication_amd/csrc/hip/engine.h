@@ -312,10 +312,43 @@ Error launch_combine_backward(const void* dy, const void* ys, ElementType type, 
                               const int* offsets, int experts, void* dys, float* dweights,
                               hipStream_t stream);
 
+// ---- gated products (gated_mm.hip) ---------------------------------------
+enum class Act : int { Silu = 0, Gelu = 1, GeluTanh = 2 };
+// h = act(g) * u, [g | u] = x W^T for the rows of each group (offsets null: one group of all
+// rows), fp16 or bf16.  W is [groups, 2, width, depth], the gates' rows first; rows in no
+// group are zeroed.  kept: g and u [total, 2, width] of the operands' type, or with
+// kept_scales packed (launch_pack8); null: not kept.
+Error launch_gated_mm(const void* x, const void* w, ElementType type, const int* offsets, int groups,
+                      int total, int width, int depth, Act act, void* out, void* kept,
+                      void* kept_scales, hipStream_t stream);
+// From dh and kept (packed: kept_scales): the gradients of g and u [total, 2, width], and h
+// again where that is not null.
+Error launch_gated_grad(const void* dh, ElementType type, const void* kept, const void* kept_scales,
+                        int total, int width, Act act, void* dkept, void* h, hipStream_t stream);
+
+// ---- values in eight bits (eight_bits.hip, int8_mm.hip) -----------------
+// Blocks of 32 along rows with a power-of-two scale (eight_bits.h): values int8 [rows, width]
+// and scales uint8 [rows, width / 32 rounded up].
+Error launch_pack8(const void* x, ElementType type, long long rows, int width, void* values,
+                   void* scales, hipStream_t stream);
+Error launch_unpack8(const void* values, const void* scales, ElementType type, long long rows,
+                     int width, void* out, hipStream_t stream);
+// Rows with an fp32 scale each: values int8 [rows, width rounded up to 16], zero past width.
+Error launch_quantize_rows(const void* x, ElementType type, long long rows, int width, void* values,
+                           float* scales, hipStream_t stream);
+// out[s, c] = x_scales[s] w_scales[c] sum_k x[s, k] w[c, k] of quantised rows, the sum exact;
+// groups as for launch_grouped_mm, W [groups, width, depth], or gated as for launch_gated_mm.
+Error launch_int8_mm(const void* x, const float* x_scales, const void* w, const float* w_scales,
+                     const int* offsets, int groups, int total, int width, int depth,
+                     ElementType out_type, void* out, hipStream_t stream);
+Error launch_gated_int8_mm(const void* x, const float* x_scales, const void* w, const float* w_scales,
+                           const int* offsets, int groups, int total, int width, int depth, Act act,
+                           ElementType out_type, void* out, hipStream_t stream);
+
 // ---- grouped products and adapters (grouped_mm.hip), fp16 and bf16 ------
 // out[s] = x[s] W_g^T for the rows offsets[g] <= s < offsets[g + 1] of group g;
 // rows in no group are zeroed.  W is [groups, width, depth], or with w_in_rows
-// [groups, depth, width].
+// [groups, depth, width].  offsets null: one group of all rows.
 Error launch_grouped_mm(const void* x, const void* w, ElementType type, const int* offsets,
                         int groups, int total, int width, int depth, bool w_in_rows, void* out,
                         hipStream_t stream);

@@ -167,6 +167,13 @@ _SIGNATURES = {
     "spmm_c_grouped_outer": (_int, [_vp, _vp, _int, _vp] + [_int] * 4 + [_vp, _vp]),
     "spmm_c_adapter_workspace": (ctypes.c_longlong, [_int] * 2),
     "spmm_c_adapter_mm": (_int, [_vp] * 6 + [_int] * 6 + [_vp] * 3),
+    "spmm_c_gated_mm": (_int, [_vp, _vp, _int, _vp] + [_int] * 5 + [_vp] * 4),
+    "spmm_c_gated_grad": (_int, [_vp, _int, _vp, _vp] + [_int] * 3 + [_vp] * 3),
+    "spmm_c_pack8": (_int, [_vp, _int, ctypes.c_longlong, _int] + [_vp] * 3),
+    "spmm_c_unpack8": (_int, [_vp, _vp, _int, ctypes.c_longlong, _int] + [_vp] * 2),
+    "spmm_c_quantize_rows": (_int, [_vp, _int, ctypes.c_longlong, _int] + [_vp] * 3),
+    "spmm_c_int8_mm": (_int, [_vp] * 5 + [_int] * 5 + [_vp] * 2),
+    "spmm_c_gated_int8_mm": (_int, [_vp] * 5 + [_int] * 6 + [_vp] * 2),
     "spmm_c_route_workspace": (ctypes.c_longlong, [_int] * 3),
     "spmm_c_group_workspace": (ctypes.c_longlong, [_int] * 2),
     "spmm_c_route": (_int, [_vp] + [_int] * 5 + [_vp] * 7),
@@ -1049,16 +1056,24 @@ def time_repeat(kernel: str, A, B, C, reps: int, stream=None) -> float:
     return ms.value
 
 
-# Mixture-of-experts routing and products, low-rank adapters (experts.py needs
-# torch, which host-only users of this module never import).
-_EXPERTS = ("Routing", "route", "route_backward", "group_entries", "dispatch", "dispatch_backward",
-            "combine", "combine_backward", "grouped_mm", "grouped_mm_backward", "adapter_mm")
+# Mixture-of-experts routing and products, low-rank adapters (experts.py), gated
+# feed-forward blocks and values in 8 bits (gated.py), which need torch; host-only users of
+# this module never import it.
+_TORCH_PARTS = {
+    "experts": ("Routing", "route", "route_backward", "group_entries", "dispatch",
+                "dispatch_backward", "combine", "combine_backward", "grouped_mm",
+                "grouped_mm_backward", "adapter_mm"),
+    "gated": ("Packed8", "Rows8", "gated_mm", "gated_mm_backward", "pack8", "unpack8",
+              "quantize_rows", "int8_mm"),
+}
 
 
 def __getattr__(name: str):
-    if name in _EXPERTS:
-        from . import experts
-        for n in _EXPERTS:
-            globals()[n] = getattr(experts, n)
-        return globals()[name]
+    for part, names in _TORCH_PARTS.items():
+        if name in names:
+            from importlib import import_module
+            module = import_module(f".{part}", __name__)
+            for n in names:
+                globals()[n] = getattr(module, n)
+            return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
