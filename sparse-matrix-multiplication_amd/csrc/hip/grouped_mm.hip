@@ -107,6 +107,99 @@ Error launch_shrink(const TileArgs& a, bool pieces, const void* down, const floa
         grid, WAVES * 64, lds, stream, "adapter_shrink", a, d, scale, h);
 }
 
+// How few_rows_product is launched for groups of `rows` rows or so (all are right).
+//   Columns: the rows' own reading counts, and 64 columns share it (2048 rows over 64
+//     groups of 2048 x 4096: 211 us, 282 with sixteen columns).  For whole pieces only:
+//     others, which take longer, are tiles' from there on.
+//   Groups: several workgroups a CU hide each other's beginnings and ends (256 rows over
+//     64 groups of 2048 x 4096: 167 us with three, 227 with one).
+//   Single: a workgroup a CU or so, which has all of the LDS for its loads.
+enum class Few { Columns, Groups, Single };
+Few few_form(const TileArgs& a, long long rows, bool pieces) {
+    const double row_tiles = a.offsets == nullptr ? std::ceil(rows / 64.0) : a.groups;
+    if (pieces && rows > 32 && row_tiles * std::ceil(a.width / 64.0) >= 192) return Few::Columns;
+    return a.groups > 1 && rows <= 32 ? Few::Groups : Few::Single;
+}
+template <typename T, Ends E>
+Error launch_few_rows(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
+    constexpr int kAll = 160 * 1024;
+    const long long rows = few_rows(a);
+    switch (few_form(a, rows, pieces)) {
+        case Few::Columns:
+            return launch_few_rows_of<T, 4, 4, 4, 80 * 1024, E>(a, pieces, stream, name);
+        case Few::Groups:
+            if (rows <= 16) return launch_few_rows_of<T, 1, 1, 4, 54 * 1024, E>(a, pieces, stream, name);
+            return launch_few_rows_of<T, 2, 1, 4, 54 * 1024, E>(a, pieces, stream, name);
+        case Few::Single: break;
+    }
+    if (rows <= 16) return launch_few_rows_of<T, 1, 1, 8, kAll, E>(a, pieces, stream, name);
+    if (rows <= 32) return launch_few_rows_of<T, 2, 1, 8, kAll, E>(a, pieces, stream, name);
+    if (rows <= 48) return launch_few_rows_of<T, 3, 1, 8, kAll, E>(a, pieces, stream, name);
+    return launch_few_rows_of<T, 4, 1, 8, kAll, E>(a, pieces, stream, name);
+}
+
+// The form with the least time; each is right for all sizes that its flag allows.
+//   few_rows_product reads weights at 6.3 TB/s, less where the rows' own reading counts;
+//     a round of its workgroups takes 2.2 us for 256 steps (64 columns, two a CU) or 1 us
+//     for 512 (sixteen, one a CU).
+//   Rows that are no whole pieces: 1.1 times as long to read (8 groups of 4000 x 4098,
+//     32 rows: 47 us; 64 x 64 tiles 40, 128 x 128 60), twice where they begin between two
+//     words (64 groups of 2048 x 4097, 256 rows: 344 us; tiles 222), and 1 us a round for
+//     340 steps, 1.3 or 1.65 times, less with fewer rows (20 rows x 4000 x 4097: 17 us,
+//     tiles 27).
+//   Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s, W [k][c]
+//     at 5.8 (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows
+//     257, 285).  Adapters hold tiles up by 6 us, those of 64 x 64 by 5: about what a run of
+//     rows with one adapter costs (4000 x 1024 x 1024, rank 16: 5; 701 x 2003 x 1001, rank
+//     12: 5; two rounds of 256 x 256, rank 64: 25), less than an adapter a row does (11).
+//   64 x 64 tiles: 300 rows x 1024 x 1024 with adapters 14 us, 128 x 128 21; 100 rows x
+//     4000 x 4097 30, few_rows_product 43; 12 rows x 1504 x 2057 15, few_rows_product 8.
+//   Rows of whole words that are no pieces: in tiles as those of pieces, one of 128 x 128 a CU
+//     in a ring (the same sums in the same order as through registers).
+Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie) {
+    const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
+    const double mean = a.total / groups;
+    const double weights = 2.0 * groups * a.width * a.depth;
+    // groups of all lengths end, on average, in the middle of a tile
+    auto row_tiles = [&](int edge) {
+        return groups == 1 ? std::ceil(mean / edge) : groups * std::max(1.0, mean / edge + 0.5);
+    };
+    const bool words = a.depth % 2 == 0 && ((reinterpret_cast<uintptr_t>(a.rows) |
+                                             reinterpret_cast<uintptr_t>(a.cols)) & 2) == 0;
+    const long long rows = few_rows(a);
+    const double tiles64 = groups == 1 ? std::ceil(mean / 64)
+                                       : groups * std::max(1.0, mean / 64 + 0.5);
+    double few = weights / 6.3e6 * (1 + mean / 160) * (pieces ? 1 : words ? 1.1 : 2);
+    switch (few_form(a, rows, pieces)) {
+        case Few::Columns:
+            few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 64.0) / 512) *
+                                    (2 + 2.2 * std::ceil(a.depth / 256.0)));
+            break;
+        case Few::Single: {
+            const double high  = std::ceil(std::min(rows, 64LL) / 16.0);  // its rows' share of the loads
+            const double round = pieces ? 3 + std::ceil(a.depth / 512.0)
+                                        : (1 + a.depth / 340.0) * (words ? 1.3 : 1.65) * (high + 2) / 6;
+            few = std::max(few, std::ceil(tiles64 * std::ceil(a.width / 16.0) / 256) * round);
+            break;
+        }
+        case Few::Groups: break;
+    }
+    few += 4;
+    const double reading = weights / (few_allowed ? 4.1e6 : 5.8e6);
+    auto time = [&](Form f) {
+        return tile_time(f, row_tiles, a.width, a.depth, reading) +
+               (a.ids == nullptr ? 0 : f == Form::Shared ? 5 : 6);
+    };
+    Form best = pieces ? Form::Pieces : Form::Any;
+    if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
+    if (a.ids == nullptr && lie == Lie::Words) {
+        if (time(Form::Ring128) < time(best)) best = Form::Ring128;
+        if (time(Form::Wide) < time(best)) best = Form::Wide;
+    }
+    if (time(Form::Shared) < time(best)) best = Form::Shared;
+    return few_allowed && few <= time(best) ? Form::FewRows : best;
+}
+
 }  // namespace
 
 Error launch_grouped_mm(const void* x, const void* w, ElementType type, const int* offsets,
@@ -127,12 +220,15 @@ Error launch_grouped_mm(const void* x, const void* w, ElementType type, const in
     a.width = width;
     a.depth = depth;
     const bool pieces = depth % 8 == 0 && (!w_in_rows || width % 8 == 0) && aligned16(x) && aligned16(w);
-    const Form form = choose_form(a, width, pieces, !w_in_rows);
+    a.rows_end = static_cast<const char*>(x) + 2LL * total * depth;
+    a.cols_end = static_cast<const char*>(w) + 2LL * groups * width * depth;
+    const Lie lie = lie_of(a, depth, w_in_rows ? width : depth);
+    const Form form = choose_form(a, pieces, !w_in_rows, lie);
     return with_half(type, "grouped_mm", [&](auto zero) {
         using T = decltype(zero);
         if (form == Form::FewRows) return launch_few_rows<T, Ends::Plain>(a, pieces, stream, "grouped_mm");
-        return w_in_rows ? launch_tiles<T, false, true, Ends::Plain>(a, form, stream, "grouped_mm")
-                         : launch_tiles<T, false, false, Ends::Plain>(a, form, stream, "grouped_mm");
+        return w_in_rows ? launch_tiles<T, false, true, Ends::Plain>(a, form, lie, stream, "grouped_mm")
+                         : launch_tiles<T, false, false, Ends::Plain>(a, form, lie, stream, "grouped_mm");
     });
 }
 
@@ -157,12 +253,19 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
     auto time = [&](Form f) {
         return tile_time(f, row_tiles, width, static_cast<double>(total) / groups, 0);
     };
+    a.rows_end = static_cast<const char*>(p) + 2LL * total * height;
+    a.cols_end = static_cast<const char*>(q) + 2LL * total * width;
+    const Lie lie = lie_of(a, height, width);
     Form form = !pieces ? Form::Any
                 : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
+    if (lie == Lie::Words) {
+        if (time(Form::Ring128) < time(form)) form = Form::Ring128;
+        if (time(Form::Wide) < time(form)) form = Form::Wide;
+    }
     if (time(Form::Shared) < time(form)) form = Form::Shared;
     return with_half(type, "grouped_outer", [&](auto zero) {
         using T = decltype(zero);
-        return launch_tiles<T, true, true, Ends::Plain>(a, form, stream, "grouped_outer");
+        return launch_tiles<T, true, true, Ends::Plain>(a, form, lie, stream, "grouped_outer");
     });
 }
 
@@ -199,7 +302,7 @@ Error launch_adapter_mm(const void* x, const void* w, const void* down, const vo
     a.rank16 = (rank + 15) / 16 * 16;
     const bool pieces = depth % 8 == 0 && aligned16(x) && aligned16(w);
     a.b_pieces = rank % 8 == 0 && aligned16(up);
-    const Form form = choose_form(a, width, pieces, true);
+    const Form form = choose_form(a, pieces, true, Lie::Pieces);
     return with_half(type, "adapter_mm", [&](auto zero) {
         using T = decltype(zero);
         const bool whole = pieces && aligned16(down);
@@ -209,7 +312,7 @@ Error launch_adapter_mm(const void* x, const void* w, const void* down, const vo
             SPMM_TRY((launch_shrink<T, 1, 4, 2, 53 * 1024>(a, whole, down, scale, std::max(1, std::min(8, adapters)), stream)));
         }
         if (form == Form::FewRows) return launch_few_rows<T, Ends::Adapters>(a, pieces, stream, "adapter_mm");
-        return launch_tiles<T, false, false, Ends::Adapters>(a, form, stream, "adapter_mm");
+        return launch_tiles<T, false, false, Ends::Adapters>(a, form, Lie::Pieces, stream, "adapter_mm");
     });
 }
 

@@ -43,6 +43,7 @@ __device__ __forceinline__ void lds_dma_raw_x4(u32x4 rsrc, unsigned offset) {
 }
 
 constexpr int kStep = 64;  // contraction steps a staged tile holds
+constexpr int kRingLds = 160 * 1024;
 
 // A byte offset past every buffer's 2^31 - 1 bytes, with room for the 16 that a
 // load adds: it reads zeros.
@@ -128,6 +129,9 @@ struct TileArgs {
     const float* row_scales;  // total
     const float* col_scales;  // [groups, width], gated [groups, 2, width]
     ElementType out_type;
+    // where the operands end, for rows that are no whole pieces
+    const void* rows_end;
+    const void* cols_end;
 };
 
 // The group's rows as the kernels use them: in range and in order whatever the
@@ -864,6 +868,25 @@ __device__ __forceinline__ void zero_tile(const TileArgs& a, const Tile<T>& t) {
     }
 }
 
+// How operands lie in memory for buffer-to-LDS loads: rows of whole 16-byte pieces, of whole
+// words, or of 16-bit elements that may begin between two words.
+enum class Lie { Pieces, Words, Odd };
+
+// A buffer from `at` (down to its word) on; past `end` (up to its word) there are zeros.
+// Pieces need no end: each is there as a whole or absent.
+template <Lie L>
+__device__ __forceinline__ u32x4 operand_words(const void* at, const void* end) {
+    if constexpr (L == Lie::Pieces) return buffer_words(at, 0, 0x7fffffff);
+    const uintptr_t from = reinterpret_cast<uintptr_t>(at) & ~uintptr_t{3};
+    const long long left = static_cast<long long>((reinterpret_cast<uintptr_t>(end) + 3) & ~uintptr_t{3}) -
+                           static_cast<long long>(from);
+    // compared by halves: the scalar unit compares no 64 bits
+    const int high = static_cast<int>(left >> 32);
+    const unsigned low = static_cast<unsigned>(left), most = 0x7ffffffcu;
+    const unsigned records = high < 0 ? 0u : high > 0 || low > most ? most : low;
+    return buffer_words(reinterpret_cast<const void*>(from), 0, static_cast<int>(records));
+}
+
 // Whether a tile's sums leave as they are, through store_tile (or with adapters).
 template <typename T, Ends E>
 constexpr bool kPlainEnds = E != Ends::Gated && !std::is_same_v<T, Int8Pair>;
@@ -1111,7 +1134,7 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
 }
 
 // The 256 x 256 tile of large products, for operands whose rows are whole 16-byte
-// pieces.  Four waves, one a SIMD, take a quarter of 128 x 128 each; 64 steps of
+// pieces or words.  Four waves, one a SIMD, take a quarter of 128 x 128 each; 64 steps of
 // the contraction are a tile of four slots of 16 KB in LDS: columns 0-127 (C0) and
 // 128-255 (C1), the first 64 rows of either pair of waves (L) and the last 64 (H).
 // Ten slots form a ring, filled by buffer-to-LDS loads in the order C0 C1 L H.
@@ -1127,6 +1150,9 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
 //   the five youngest slots (the next tile's C0, C1, L are there), behind part 0
 //   all but six (this tile's H is there), and for its operand reads.
 //   Past the contraction's end loads write zeros, so the counts always hold.
+//   Words: the last piece of a row may hold the next row's first elements, which are cut off
+//     in LDS before its slot is read (contraction along rows; other operands only have them
+//     in columns past the tile's).
 //
 // 8 groups of 8192 x 4096 over 16384 rows: 887 us a call, 1240 TFLOP/s (the kernel alone
 // 869 at best); in one group 783 us at best, 1400, and 808 on average.  The matrix cores
@@ -1135,8 +1161,9 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
 // one group keeps them at 89% and takes 740 at best, 789 on average.  What is left lies in
 // the two barriers a tile, with their waits for loads, and in the 6 us that a tile costs
 // beside its 1.55 us for 64 steps: beginning, first loads and stores.
-template <typename T, bool GRAD, bool COLS_MAJOR, Ends E>
+template <typename T, bool GRAD, bool COLS_MAJOR, Ends E, Lie L = Lie::Pieces>
 __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
+    static_assert(L != Lie::Odd, "rows of whole words");
     constexpr bool GATED = E == Ends::Gated;
     constexpr int BR = 256, BC = 256, RF = 8, CF = 8, OUT = GATED ? BC / 2 : BC;
     using RowSlot = Slot<T, GRAD, 128>;
@@ -1170,10 +1197,11 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
         auto place_of = [&](int slot) { return lds0 + slot * ColSlot::kBytes; };
         // The tile that is being loaded, as buffers that begin at it, and the
         // contraction steps left there.
-        u32x4 rows = buffer_words(t.rows, 0, 0x7fffffff);
-        u32x4 cols = buffer_words(t.cols, 0, 0x7fffffff);
-        u32x4 second = GATED ? buffer_words(t.second, 0, 0x7fffffff) : cols;
+        u32x4 rows = operand_words<L>(t.rows, a.rows_end);
+        u32x4 cols = operand_words<L>(t.cols, a.cols_end);
+        u32x4 second = GATED ? operand_words<L>(t.second, a.cols_end) : cols;
         int left = t.depth;
+        long long steps = 0;
         auto step = [](u32x4& buffer, long long bytes) {
             const unsigned long long at =
                 (static_cast<unsigned long long>(buffer[1]) << 32 | buffer[0]) + bytes;
@@ -1181,10 +1209,32 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
             buffer[1] = static_cast<unsigned>(at >> 32);
         };
         auto advance = [&] {
+            left -= kStep;
+            if constexpr (L == Lie::Words) {
+                ++steps;
+                rows = operand_words<L>(t.rows + steps * t.step_rows, a.rows_end);
+                cols = operand_words<L>(t.cols + steps * t.step_cols, a.cols_end);
+                if constexpr (GATED) second = operand_words<L>(t.second + steps * t.step_cols, a.cols_end);
+                return;
+            }
             step(rows, t.step_rows * 2);
             step(cols, t.step_cols * 2);
             if constexpr (GATED) step(second, t.step_cols * 2);
-            left -= kStep;
+        };
+        // Cuts the rows of a tile's slots off at their end: the columns' (two threads a pair of
+        // slots) or one of rows.
+        const int last = t.depth - (tiles - 1) * kStep;
+        const bool partial = L == Lie::Words && !GRAD && last % 8 != 0;
+        auto cut = [&](int slot) {
+            const int n = threadIdx.x & 127;
+            uint4* piece = reinterpret_cast<uint4*>(s_tiles + slot * ColSlot::kBytes + n * kStep * 2 +
+                                                    ((last / 8) ^ (n & 7)) * 16);
+            *piece = first_of(*piece, last % 8);
+        };
+        auto cut_cols = [&](int slot0, int slot1, int low_slot) {
+            if constexpr (!COLS_MAJOR) cut(threadIdx.x < 128 ? slot0 : slot1);
+            if (threadIdx.x < 128) cut(low_slot);
+            lds_barrier();
         };
         // what load i of a slot of columns is from
         auto half_of = [&](auto i, const u32x4& from) -> const u32x4& {
@@ -1247,6 +1297,7 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
             }
         wait_vmcnt<24>();  // slots 0, 1, 2
         lds_barrier();
+        if (partial && tiles == 1) cut_cols(0, 1, 2);
 #pragma unroll
         for (int i = 0; i < RF / 2; ++i) read_row(2, 0, i);
 #pragma unroll
@@ -1261,6 +1312,10 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
             });
             wait_vmcnt<24>();
             lds_barrier();
+            if (partial && it + 1 == tiles) {
+                if (threadIdx.x < 128) cut(later(3));
+                lds_barrier();
+            }
             multiply(1, 0, low, rows, place_of(slot), [&](auto m) {
                 if constexpr (m.value < 4) read_row(later(3), 0, m.value);
             });
@@ -1269,12 +1324,240 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
             });
             wait_vmcnt<20>();
             lds_barrier();
+            if (partial && it + 2 == tiles) cut_cols(later(4), later(5), later(6));
             advance();
             multiply(1, 1, cols0, cols, place_of(later(2)), [&](auto m) {
                 if constexpr (m.value < 4) read_row(later(6), 0, m.value);
                 else if constexpr (m.value < 12) read_col(later(4 + wc), 0, m.value - 4);
             });
             slot = later(4);
+        }
+        settle_sums(acc);
+        wait_vmcnt<0>();
+        lds_barrier();  // the ring is free
+    }
+    float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
+    leave<T, RF, CF, E>(a, t, r0, c0, acc, sums);
+}
+
+// The tile of 32 RF x 128 of products that the 256 x 256 tiles are too few of, and of rows
+// that are no whole pieces: four waves of 16 RF x 64 over a ring of S stages of 64 steps,
+// filled by buffer-to-LDS loads S stages ahead, so that reading weights from memory keeps
+// up where a CU has one tile.  A stage is multiplied in two halves; a wave reads the next
+// half's operands from LDS before it multiplies one.  One barrier a stage, in its middle:
+// behind it the stage's slot is free, as all waves hold its second half in registers.
+//   Past the contraction's end loads write zeros, so the counts of loads always hold.
+//   Words: the last piece of a row may hold the next row's first elements, which are cut
+//     off in LDS before its stage is read (contraction along rows; other operands only have
+//     them in columns past the tile's).
+//   Odd: rows are staged from the word of their first element on, and shifted by one
+//     element as they are read, with the word behind a piece, which for a row's last piece
+//     of a stage lies in the next stage.
+template <typename T, bool GRAD, bool COLS_MAJOR, Ends E, Lie L, int RF>
+__global__ __launch_bounds__(256, 1) void tile_product_ring(TileArgs a) {
+    constexpr bool GATED = E == Ends::Gated, ODD = L == Lie::Odd;
+    constexpr int BR = 32 * RF, BC = 128, WC = 2, CF = 4, OUT = GATED ? BC / 2 : BC;
+    constexpr int kRowLoads = BR / 32, kLoads = kRowLoads + 4, kRowBytes = BR * kStep * 2;
+    constexpr int kStage = kRowBytes + BC * kStep * 2, S = kRingLds / kStage;
+    constexpr int kAhead = ODD ? 3 : 2;  // stages that have to be there before one is read, and one
+    static_assert(!ODD || (!GRAD && !COLS_MAJOR), "rows along the contraction are shifted");
+    static_assert(!GRAD || RF == 4, "slots of 128 rows");
+    using Rows = Operands<T, 128, GRAD, 256>;
+    using Cols = Operands<T, 128, GRAD || COLS_MAJOR, 256>;
+    extern __shared__ __attribute__((aligned(16))) char s_tiles[];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave / WC, wc = wave % WC;
+    const int lane = threadIdx.x & 63, q = lane >> 4, s = lane & 15;
+    Tile<T> t;
+    if (!take_tile<T, BR, OUT, GRAD, COLS_MAJOR, GATED>(a, t)) return;
+
+    Sums<T> acc[CF][RF];
+#pragma unroll
+    for (int j = 0; j < CF; ++j)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) {
+            acc[j][i] = Sums<T>(0);
+            asm volatile("" : "+a"(acc[j][i]));
+        }
+    const int r0 = wr * RF * 16, c0 = t.c0 + wc * (OUT / WC);
+    const int stages = (t.depth + kStep - 1) / kStep;
+    if constexpr (!kPlainEnds<T, E>) {
+        if (stages == 0) return finish_zeros<OUT, T, GATED>(a, t);
+    }
+    auto column = [&](int j) {
+        return GATED ? j / (CF / 2) * (BC / 2) + (wc * (CF / 2) + j % (CF / 2)) * 16 : (wc * CF + j) * 16;
+    };
+    if (stages > 0) {
+        Slot<T, GRAD, 64> pr;
+        Slot<T, GRAD || COLS_MAJOR, GATED ? 0 : 64> pc;
+        pr.place(t.ld_rows, 0, t.rows_here);
+        pc.place(t.ld_cols, 0, a.width - t.c0);
+        // Odd: whether an operand begins between two words, and the shift of a lane's row
+        unsigned odd_rows = 0, odd_cols = 0, odd_second = 0;
+        if constexpr (ODD) {
+            auto odd = [](const T* p) { return static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) & 2u; };
+            odd_rows = odd(t.rows);
+            odd_cols = odd(t.cols);
+            odd_second = GATED ? odd(t.second) : odd_cols;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (pr.at[i] != kAbsent) pr.at[i] = (pr.at[i] + odd_rows) & ~3u;
+                if (pc.at[i] != kAbsent) pc.at[i] = (pc.at[i] + (i < 2 ? odd_cols : odd_second)) & ~3u;
+            }
+        }
+        const unsigned odd_ld_rows = ODD ? t.ld_rows & 1 : 0, odd_ld_cols = ODD ? t.ld_cols & 1 : 0;
+        const unsigned shift_rows = ((odd_rows / 2 + (s & odd_ld_rows)) & 1u) * 16u;
+        const unsigned shift_cols = ((odd_cols / 2 + (s & odd_ld_cols)) & 1u) * 16u;
+        const unsigned shift_second = ((odd_second / 2 + (s & odd_ld_cols)) & 1u) * 16u;
+
+        const unsigned lds0 = lds_address(s_tiles) + wave * 1024;
+        // The stage that is being loaded: what it is from, where it goes, and its steps.
+        struct Source {
+            u32x4 rows, cols, second;
+            unsigned to;
+            int left;
+        };
+        auto source = [&](int n, int slot) {
+            Source from;
+            from.rows = operand_words<L>(t.rows + n * t.step_rows, a.rows_end);
+            from.cols = operand_words<L>(t.cols + n * t.step_cols, a.cols_end);
+            from.second = GATED ? operand_words<L>(t.second + n * t.step_cols, a.cols_end) : from.cols;
+            from.to = lds0 + slot * kStage;
+            from.left = t.depth - n * kStep + ODD;  // may be below 1
+            return from;
+        };
+        // Load i of a stage, the rows' first, in three steps that products come between.
+        auto load_offset = [&](auto i, const Source& from) {
+            if constexpr (i.value < kRowLoads) return pr.template offset<i.value>(from.left);
+            else return pc.template offset<i.value - kRowLoads>(from.left);
+        };
+        auto load_to = [&](auto i, const Source& from) {
+            constexpr int at = i.value < kRowLoads ? i.value * 4096 : kRowBytes + (i.value - kRowLoads) * 4096;
+            lds_dma_raw_to<at>(from.to);
+        };
+        auto load_from = [&](auto i, const Source& from, unsigned offset) {
+            lds_dma_raw_x4(i.value < kRowLoads ? from.rows : i.value < kRowLoads + 2 ? from.cols : from.second,
+                           offset);
+        };
+        Operand<T> fr[2][RF], fc[2][CF];
+        WordPiece raw[2][ODD ? RF + CF : 1];  // Odd: what the operands are shifted from
+        // Sixteen rows from n0 on of an operand in `slot`.
+        auto read = [&](auto m, int slot, int next, int half) {
+            constexpr bool COLS = m.value >= RF;
+            using Op = std::conditional_t<COLS, Cols, Rows>;
+            const int n0 = COLS ? column(m.value - RF) : (wr * RF + m.value) * 16;
+            const char* at = s_tiles + slot * kStage + (COLS ? kRowBytes : 0);
+            if constexpr (!ODD) {
+                const Operand<T> x = Op::read(reinterpret_cast<const T*>(at), n0, half);
+                if constexpr (COLS) fc[half][m.value - RF] = x;
+                else fr[half][m.value] = x;
+            } else {
+                const int c = 4 * half + q, row = (n0 + s) * kStep * 2;
+                const char* behind = c == 7 ? s_tiles + next * kStage + (COLS ? kRowBytes : 0) : at;
+                raw[half][m.value].words = *reinterpret_cast<const uint4*>(at + row + (c ^ (s & 7)) * 16);
+                raw[half][m.value].next =
+                    *reinterpret_cast<const unsigned*>(behind + row + (((c + 1) & 7) ^ (s & 7)) * 16);
+            }
+        };
+        // Read m of a half: the rows' operands, then the columns'.
+        auto read_one = [&](auto m, int slot, int next, int half) {
+            if constexpr (m.value < RF + CF) read(m, slot, next, half);
+        };
+        // Odd: operand m from its words.
+        auto shift_one = [&](auto m, int half) {
+            constexpr bool COLS = m.value >= RF;
+            const unsigned shift = !COLS ? shift_rows
+                                   : GATED && m.value - RF >= CF / 2 ? shift_second : shift_cols;
+            Operand<T> x = __builtin_bit_cast(Operand<T>, piece_of(raw[half][m.value], shift / 8));
+            asm volatile("" : "+v"(x));
+            if constexpr (COLS) fc[half][m.value - RF] = x;
+            else fr[half][m.value] = x;
+        };
+        // The stage whose rows end inside a piece, -1 for none, and what cuts them there: a
+        // thread a row.  Odd: a row that begins between two words goes one element further,
+        // for which the last stage may have one behind it.
+        const int last = t.depth - (stages - 1) * kStep;
+        const int partial = L == Lie::Pieces || (GRAD && L == Lie::Words) ? -1
+                            : ODD && last == kStep ? stages
+                            : ODD || last % 8 != 0 ? stages - 1 : -1;
+        auto cut = [&](int slot) {
+            const int left = partial == stages ? 0 : last, n = threadIdx.x & 127;
+            const bool of_cols = threadIdx.x >= 128;
+            if (of_cols ? !COLS_MAJOR : n < BR) {
+                char* row = s_tiles + slot * kStage + (of_cols ? kRowBytes : 0) + n * kStep * 2;
+                // values, not places: a choice between members would put t into memory
+                const int row_further = (odd_rows / 2 + (n & odd_ld_rows)) & 1;
+                const int col_further = ((GATED && n >= 64 ? odd_second : odd_cols) / 2 + (n & odd_ld_cols)) & 1;
+                const int further = of_cols ? col_further : row_further;
+                uint4* piece = reinterpret_cast<uint4*>(row + ((left / 8) ^ (n & 7)) * 16);
+                *piece = first_of(*piece, left % 8 + further);
+            }
+            __syncthreads();
+        };
+        // A half's products; behind product m, f(m).
+        constexpr int kProducts = CF * RF;
+        auto multiply = [&](int half, auto f) {
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (ODD) {
+                unrolled(std::make_integer_sequence<int, RF + 1>{}, [&](auto m) { shift_one(m, half); });
+                // what the vector unit wrote can be read two cycles later, which the compiler
+                // would see to for its own products
+                asm volatile("s_nop 3");
+            }
+            unrolled(std::make_integer_sequence<int, kProducts>{}, [&](auto m) {
+                mfma_in_place(acc[m.value / RF][m.value % RF], fc[half][m.value / RF], fr[half][m.value % RF]);
+                f(m);
+                if constexpr (ODD && m.value % RF == 0 && m.value / RF + 1 < CF) {
+                    shift_one(std::integral_constant<int, RF + m.value / RF + 1>{}, half);
+                    if constexpr (RF < 4) asm volatile("s_nop 1");
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+#pragma unroll
+        for (int n = 0; n < S; ++n) {
+            const Source from = source(n, n);
+            unrolled(std::make_integer_sequence<int, kLoads>{}, [&](auto i) {
+                load_to(i, from);
+                asm volatile("s_nop 0");
+                load_from(i, from, load_offset(i, from));
+            });
+        }
+        wait_vmcnt<kLoads * (S - kAhead + 1)>();
+        lds_barrier();
+        int slot = 0, next = 1;
+        // stages 0 (Odd: and 1) are there
+        if (L != Lie::Pieces && partial >= 0 && partial <= kAhead - 2) cut(partial);
+        unrolled(std::make_integer_sequence<int, RF + CF>{}, [&](auto m) { read_one(m, 0, 1, 0); });
+        for (int n = 0; n < stages; ++n) {
+            const int after = next + 1 < S ? next + 1 : 0;
+            multiply(0, [&](auto m) { read_one(m, slot, next, 1); });
+            wait_vmcnt<kLoads * (S - kAhead)>();
+            lds_barrier();
+            if (L != Lie::Pieces && partial == n + kAhead - 1) cut(ODD ? after : next);
+            const Source from = source(n + S, slot);
+            unsigned offset[2];
+            multiply(1, [&](auto m) {
+                // past the last stage there are zeros to read
+                read_one(m, next, after, 0);
+                constexpr int kEach = kProducts / kLoads;  // products a load: 2, or 1 and all steps at once
+                if constexpr (kEach >= 2) {
+                    if constexpr (m.value % 2 == 0) {
+                        offset[0] = load_offset(std::integral_constant<int, m.value / 2>{}, from);
+                        load_to(std::integral_constant<int, m.value / 2>{}, from);
+                    } else {
+                        load_from(std::integral_constant<int, m.value / 2>{}, from, offset[0]);
+                    }
+                } else if constexpr (m.value < kLoads) {
+                    load_to(m, from);
+                    offset[1] = load_offset(m, from);
+                    asm volatile("s_nop 0");
+                    load_from(m, from, offset[1]);
+                }
+            });
+            slot = next;
+            next = after;
         }
         settle_sums(acc);
         wait_vmcnt<0>();
@@ -1627,11 +1910,10 @@ constexpr int ring_depth(int waves, int tiles, int room) {
     return std::min(8, room / (waves * tiles * 2048));
 }
 
-template <typename T, int RF, int COLS, int WAVES, int ROOM, Ends E>
+template <typename T, int RF, int CF, int WAVES, int ROOM, Ends E>
 Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
     constexpr bool gated = E == Ends::Gated, adapt = E == Ends::Adapters;
-    // gated: as many columns of the weights, at least sixteen of both
-    constexpr int CF = gated ? std::max(COLS, 2) : COLS, OUT = gated ? CF * 8 : CF * 16;
+    constexpr int OUT = gated ? CF * 8 : CF * 16;
     const long long row_tiles = a.offsets == nullptr
         ? (a.total + RF * 16 - 1) / (RF * 16)
         : a.total / (RF * 16) + std::min<long long>(a.groups + 2LL, a.total);
@@ -1639,7 +1921,7 @@ Error launch_few_rows_of(const TileArgs& a, bool pieces, hipStream_t stream, con
     SPMM_TRY(check_threads(blocks, WAVES * 64, name));
     const dim3 grid(static_cast<unsigned>(blocks));
     constexpr int shares = Shares<RF, CF, WAVES>::kBytes;
-    if constexpr (COLS == 1 && !std::is_same_v<T, Int8Pair>) {
+    if constexpr (CF == (gated ? 2 : 1) && !std::is_same_v<T, Int8Pair>) {
         if (!pieces) {
             return launch_with_lds<few_rows_product<T, RF, CF, WAVES, 0, gated, adapt>>(
                 grid, WAVES * 64, shares, stream, name, a);
@@ -1656,42 +1938,41 @@ long long few_rows(const TileArgs& a) {
     const long long groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     return groups == 1 ? a.total : 2LL * a.total / groups;
 }
-// How few_rows_product is launched for groups of `rows` rows or so (all are right).
-//   Columns: the rows' own reading counts, and 64 columns share it (2048 rows over 64
-//     groups of 2048 x 4096: 211 us, 282 with sixteen columns).  For whole pieces only:
-//     others, which take longer, are tiles' from there on.
-//   Groups: several workgroups a CU hide each other's beginnings and ends (256 rows over
-//     64 groups of 2048 x 4096: 167 us with three, 227 with one).
-//   Single: a workgroup a CU or so, which has all of the LDS for its loads.
-enum class Few { Columns, Groups, Single };
-Few few_form(const TileArgs& a, int width, long long rows, bool pieces) {
-    const double row_tiles = a.offsets == nullptr ? std::ceil(rows / 64.0) : a.groups;
-    if (pieces && rows > 32 && row_tiles * std::ceil(width / 64.0) >= 192) return Few::Columns;
-    return a.groups > 1 && rows <= 32 ? Few::Groups : Few::Single;
-}
+// How few_rows_product is launched for gated products and for those in 8-bit integers: four waves and two workgroups a
+// CU with sixteen columns of either projection, or 32 (rows of integers are half as long, and
+// the rows' own reading counts twice as much: 64 groups of 2048 x 4096, 256 rows 93 us, 107
+// with sixteen columns; a single group has the workgroups to hide that: 8192 x 8192, 16 rows
+// 15.4, 19.9 with 32).  All of the LDS where a gated product has one workgroup a CU and its
+// rows leave no stages else (2 x 1024 x 4096, 64 rows: 15 us, 20).
 template <typename T, Ends E>
-Error launch_few_rows(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
-    constexpr int kAll = 160 * 1024;
+Error launch_few_finished(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
+    constexpr int kTwo = 80 * 1024, kAll = 160 * 1024;
     const long long rows = few_rows(a);
-    switch (few_form(a, E == Ends::Gated ? 2 * a.width : a.width, rows, pieces)) {
-        case Few::Columns:
-            return launch_few_rows_of<T, 4, 4, 4, 80 * 1024, E>(a, pieces, stream, name);
-        case Few::Groups:
-            if (rows <= 16) return launch_few_rows_of<T, 1, 1, 4, 54 * 1024, E>(a, pieces, stream, name);
-            return launch_few_rows_of<T, 2, 1, 4, 54 * 1024, E>(a, pieces, stream, name);
-        case Few::Single: break;
+    if constexpr (E == Ends::Gated) {
+        const long long row_tiles = a.offsets == nullptr ? (a.total + 63) / 64 : a.groups;
+        if (rows <= 16) return launch_few_rows_of<T, 1, 2, 4, kTwo, E>(a, pieces, stream, name);
+        if (rows <= 32) return launch_few_rows_of<T, 2, 2, 4, kTwo, E>(a, pieces, stream, name);
+        if (pieces && row_tiles * ((a.width + 15) / 16) <= 256) {
+            return launch_few_rows_of<T, 4, 2, 4, kAll, E>(a, pieces, stream, name);
+        }
+        return launch_few_rows_of<T, 4, 2, 4, kTwo, E>(a, pieces, stream, name);
+    } else if (a.offsets == nullptr || a.groups == 1) {
+        if (rows <= 16) return launch_few_rows_of<T, 1, 1, 4, kTwo, E>(a, pieces, stream, name);
+        if (rows <= 32) return launch_few_rows_of<T, 2, 1, 4, kTwo, E>(a, pieces, stream, name);
+        return launch_few_rows_of<T, 4, 1, 4, kTwo, E>(a, pieces, stream, name);
+    } else {
+        if (rows <= 16) return launch_few_rows_of<T, 1, 2, 4, kTwo, E>(a, pieces, stream, name);
+        if (rows <= 32) return launch_few_rows_of<T, 2, 2, 4, kTwo, E>(a, pieces, stream, name);
+        return launch_few_rows_of<T, 4, 2, 4, kTwo, E>(a, pieces, stream, name);
     }
-    if (rows <= 16) return launch_few_rows_of<T, 1, 1, 8, kAll, E>(a, pieces, stream, name);
-    if (rows <= 32) return launch_few_rows_of<T, 2, 1, 8, kAll, E>(a, pieces, stream, name);
-    if (rows <= 48) return launch_few_rows_of<T, 3, 1, 8, kAll, E>(a, pieces, stream, name);
-    return launch_few_rows_of<T, 4, 1, 8, kAll, E>(a, pieces, stream, name);
 }
-
 // The kernels a product can take: few_rows_product, tile_product through registers
-// or with pieces straight into LDS, tile_product_wide, tile_product_shared.
-enum class Form { FewRows, Any, Pieces, Wide, Shared };
+// or with pieces straight into LDS, tile_product_wide, tile_product_shared, tile_product_ring
+// of 64 or 128 rows.
+enum class Form { FewRows, Any, Pieces, Wide, Shared, Ring64, Ring128 };
 constexpr int threads_of(Form form) { return form == Form::Shared ? 1024 : 256; }
 constexpr int edge_of(Form form) { return form == Form::Wide ? 256 : form == Form::Shared ? 64 : 128; }
+constexpr int rows_of(Form form) { return form == Form::Ring64 ? 64 : edge_of(form); }
 
 // Estimated microseconds of a form for `row_tiles(edge)` x width tiles of `steps`
 // steps, from measured rates: 64 steps of a 128 x 128 tile take 0.62 us where a CU has
@@ -1709,95 +1990,140 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
     if (form == Form::Wide) {
         return std::max(std::ceil(tiles / 256) * (6 + 1.55 * rounds), weights);
     }
+    if (form == Form::Ring128) {
+        return std::max(std::ceil(tiles / 256) * (3 + 0.62 * rounds), weights);
+    }
     const double two = form == Form::Any ? 1.5 : 0.95, one = form == Form::Any ? 1 : 0.62;
     const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
     const double time = whole * (3 + two * rounds) +
                         (rest == 0 ? 0 : 3 + (rest <= 256 ? one : two) * rounds);
     return std::max(time, weights);
 }
-// The form with the least time; each is right for all sizes that its flag allows.
-//   few_rows_product reads weights at 6.3 TB/s, less where the rows' own reading counts;
-//     a round of its workgroups takes 2.2 us for 256 steps (64 columns, two a CU) or 1 us
-//     for 512 (sixteen, one a CU).
-//   Rows that are no whole pieces: 1.1 times as long to read (8 groups of 4000 x 4098,
-//     32 rows: 47 us; 64 x 64 tiles 40, 128 x 128 60), twice where they begin between two
-//     words (64 groups of 2048 x 4097, 256 rows: 344 us; tiles 222), and 1 us a round for
-//     340 steps, 1.3 or 1.65 times, less with fewer rows (20 rows x 4000 x 4097: 17 us,
-//     tiles 27).
-//   Tiles read W [c][k], a line of each of 128 columns at a time, at 4.1 TB/s, W [k][c]
-//     at 5.8 (64 groups of 2048 x 4096, W [c][k]: 256 rows 167 us, tiles 262; 4096 rows
-//     257, 285).  Adapters hold tiles up by 6 us, those of 64 x 64 by 5: about what a run of
-//     rows with one adapter costs (4000 x 1024 x 1024, rank 16: 5; 701 x 2003 x 1001, rank
-//     12: 5; two rounds of 256 x 256, rank 64: 25), less than an adapter a row does (11).
-//   64 x 64 tiles: 300 rows x 1024 x 1024 with adapters 14 us, 128 x 128 21; 100 rows x
-//     4000 x 4097 30, few_rows_product 43; 12 rows x 1504 x 2057 15, few_rows_product 8.
-//   width: rows of a group's weights; of both projections of a gated product.
-//   packs: the sums leave packed by blocks of 32 columns, which a wave of the 64 x 64 tile
-//     and a workgroup of few_rows_product may not have.
-Form choose_form(const TileArgs& a, int width, bool pieces, bool few_allowed, bool packs = false) {
+// How a product's operands lie (x and w: all rows of both).
+inline Lie lie_of(const TileArgs& a, long long ld_rows, long long ld_cols) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(a.cols);
+    const long long ld = ld_rows | ld_cols;
+    return ld % 8 == 0 && at % 16 == 0 ? Lie::Pieces : ld % 2 == 0 && at % 4 == 0 ? Lie::Words : Lie::Odd;
+}
+
+// The form of a gated product or one in 8-bit integers (whose depth is in pairs), by its
+// estimated time; width: rows of a group's weights, of both projections of a gated one.
+//   few_rows_product: weights at 6.3 TB/s, more slowly as the rows' own reading counts and
+//     where a second tile of rows reads them again; 512 workgroups at a time go through a
+//     contraction of 1000 steps in 1.4 us with 16 rows, in 2.6 with 64 (2 x 8192 x 4096: 16
+//     rows 27 us, 64 36, 128 59; 2 x 1024 x 2048: 16 rows 5.0, 256 8.6).  1.1 times as long
+//     for rows that are no whole pieces, twice where they begin between two words.
+//   tile_product_ring: 64 steps of a 64 x 128 tile take 0.42 us, of 128 x 128 0.57, more where
+//     rows are cut or shifted, one tile a CU; weights at 3.5 TB/s (2 x 8192 x 4096: 128 rows
+//     39 and 49 us, 256 68 and 49; tile_product 62, 68).
+//   tile_product: 0.85 us with one tile a CU, 1.15 with two, through registers 1.2 and 1.5;
+//     tile_product_wide 1.55 (2 x 8192 x 4096: 512 rows 79 us in tile_product, 88 in the ring,
+//     1024 rows 113 wide, 154 and 167).
+inline Form choose_finished(const TileArgs& a, int width, Lie lie, bool packs) {
     const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
-    const double mean = a.total / groups;
-    const double weights = 2.0 * groups * width * a.depth;
+    const double mean = a.total / groups, weights = 2.0 * groups * width * a.depth;
     // groups of all lengths end, on average, in the middle of a tile
     auto row_tiles = [&](int edge) {
         return groups == 1 ? std::ceil(mean / edge) : groups * std::max(1.0, mean / edge + 0.5);
     };
-    const bool words = a.depth % 2 == 0 && ((reinterpret_cast<uintptr_t>(a.rows) |
-                                             reinterpret_cast<uintptr_t>(a.cols)) & 2) == 0;
-    const long long rows = few_rows(a);
-    const double tiles64 = groups == 1 ? std::ceil(mean / 64)
-                                       : groups * std::max(1.0, mean / 64 + 0.5);
-    double few = weights / 6.3e6 * (1 + mean / 160) * (pieces ? 1 : words ? 1.1 : 2);
-    switch (few_form(a, width, rows, pieces)) {
-        case Few::Columns:
-            few = std::max(few, std::ceil(tiles64 * std::ceil(width / 64.0) / 512) *
-                                    (2 + 2.2 * std::ceil(a.depth / 256.0)));
-            break;
-        case Few::Single: {
-            const double high  = std::ceil(std::min(rows, 64LL) / 16.0);  // its rows' share of the loads
-            const double round = pieces ? 3 + std::ceil(a.depth / 512.0)
-                                        : (1 + a.depth / 340.0) * (words ? 1.3 : 1.65) * (high + 2) / 6;
-            few = std::max(few, std::ceil(tiles64 * std::ceil(width / 16.0) / 256) * round);
-            break;
-        }
-        case Few::Groups: break;
-    }
-    few += 4;
-    const double reading = weights / (few_allowed ? 4.1e6 : 5.8e6);
-    auto time = [&](Form f) {
-        return tile_time(f, row_tiles, width, a.depth, reading) +
-               (a.ids == nullptr ? 0 : f == Form::Shared ? 5 : 6);
+    const int l = static_cast<int>(lie);
+    const double rounds = std::ceil(static_cast<double>(a.depth) / kStep);
+    auto ring = [&](Form f, double stage) {
+        const double tiles = row_tiles(rows_of(f)) * std::ceil(width / 128.0);
+        if (tiles * 256 > kLaunchThreads) return HUGE_VAL;
+        return std::max(std::ceil(tiles / 256) * (3 + stage * rounds), weights / 3.5e6);
     };
-    Form best = pieces ? Form::Pieces : Form::Any;
-    if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
-    if (!packs && time(Form::Shared) < time(best)) best = Form::Shared;
-    return few_allowed && !packs && few <= time(best) ? Form::FewRows : best;
+    constexpr double stage64[] = {0.42, 0.48, 0.75}, stage128[] = {0.57, 0.62, 0.9};
+    double best = ring(Form::Ring64, stage64[l]);
+    Form form = Form::Ring64;
+    auto take = [&](Form f, double time) {
+        if (time < best) {
+            best = time;
+            form = f;
+        }
+    };
+    take(Form::Ring128, ring(Form::Ring128, stage128[l]));
+    const double tiles = row_tiles(128) * std::ceil(width / 128.0);
+    if (tiles * 256 <= kLaunchThreads && lie != Lie::Words) {
+        const double one = lie == Lie::Pieces ? 0.85 : 1.2, two = lie == Lie::Pieces ? 1.15 : 1.5;
+        const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
+        take(lie == Lie::Pieces ? Form::Pieces : Form::Any,
+             std::max(whole * (3 + two * rounds) + (rest == 0 ? 0 : 3 + (rest <= 256 ? one : two) * rounds),
+                      weights / 3.5e6));
+    }
+    if (lie != Lie::Odd) take(Form::Wide, tile_time(Form::Wide, row_tiles, width, a.depth, weights / 3.5e6));
+    if (!packs) {
+        const double again = row_tiles(64) / groups;
+        const double reading = weights / 6.3e6 * std::max(1 + mean / 160, again > 1 ? 1.15 * again : 0.0);
+        const double workgroups = row_tiles(64) * std::ceil(width / 32.0);
+        const double chain = a.depth / 1000.0 * (1 + std::min(mean, 64.0) / 40);
+        take(Form::FewRows, (4 + std::max(reading, std::ceil(workgroups / 512) * chain)) *
+                                (lie == Lie::Pieces ? 1 : lie == Lie::Words ? 1.1 : 2));
+    }
+    return form;
+}
+
+template <typename T, bool GRAD, bool COLS_MAJOR, Ends E, Lie L, int RF>
+Error launch_ring(const TileArgs& a, long long blocks, hipStream_t stream, const char* name) {
+    return launch_with_lds<tile_product_ring<T, GRAD, COLS_MAJOR, E, L, RF>>(
+        dim3(static_cast<unsigned>(blocks)), 256, kRingLds, stream, name, a);
 }
 
 // Launches the tile kernel of a form.
 template <typename T, bool GRAD, bool COLS_MAJOR, Ends E>
-Error launch_tiles(const TileArgs& a, Form form, hipStream_t stream, const char* name) {
-    const int edge = edge_of(form), out = E == Ends::Gated ? edge / 2 : edge;
+Error launch_tiles(const TileArgs& a, Form form, Lie lie, hipStream_t stream, const char* name) {
+    const int edge = edge_of(form), out = E == Ends::Gated ? edge / 2 : edge, rows = rows_of(form);
     // every group may end in a part-filled tile, and so may the rows before and behind them
     const long long row_tiles =
-        GRAD ? static_cast<long long>(a.groups) * ((a.height + edge - 1) / edge)
-        : a.offsets == nullptr ? (a.total + edge - 1) / edge
-                               : a.total / edge + std::min<long long>(a.groups + 2LL, a.total);
+        GRAD ? static_cast<long long>(a.groups) * ((a.height + rows - 1) / rows)
+        : a.offsets == nullptr ? (a.total + rows - 1) / rows
+                               : a.total / rows + std::min<long long>(a.groups + 2LL, a.total);
     // a whole number of workgroups for each XCD
     const long long blocks = (row_tiles * ((a.width + out - 1) / out) + 7) / 8 * 8;
     SPMM_TRY(check_threads(blocks, threads_of(form), name));
+    const dim3 grid(static_cast<unsigned>(blocks));
+    constexpr bool kNew = !kPlainEnds<T, E>, kInt = std::is_same_v<T, Int8Pair>;
     if (form == Form::Wide) {
+        if constexpr (!kInt && E != Ends::Adapters) {
+            if (lie == Lie::Words) {
+                return launch_with_lds<tile_product_wide<T, GRAD, COLS_MAJOR, E, Lie::Words>>(
+                    grid, threads_of(Form::Wide), kWideLds, stream, name, a);
+            }
+        }
         return launch_with_lds<tile_product_wide<T, GRAD, COLS_MAJOR, E>>(
-            dim3(static_cast<unsigned>(blocks)), threads_of(Form::Wide), kWideLds, stream, name, a);
+            grid, threads_of(Form::Wide), kWideLds, stream, name, a);
     }
-    if (form == Form::Shared) {
-        return launch_with_lds<tile_product_shared<T, GRAD, COLS_MAJOR, E>>(
-            dim3(static_cast<unsigned>(blocks)), threads_of(Form::Shared), kSharedLds, stream, name, a);
+    if constexpr (kNew) {
+        const bool low = form == Form::Ring64;
+        if (low || form == Form::Ring128) {
+            if constexpr (!kInt) {
+                if (lie == Lie::Words) {
+                    return low ? launch_ring<T, false, false, E, Lie::Words, 2>(a, blocks, stream, name)
+                               : launch_ring<T, false, false, E, Lie::Words, 4>(a, blocks, stream, name);
+                }
+                if (lie == Lie::Odd) {
+                    return low ? launch_ring<T, false, false, E, Lie::Odd, 2>(a, blocks, stream, name)
+                               : launch_ring<T, false, false, E, Lie::Odd, 4>(a, blocks, stream, name);
+                }
+            }
+            return low ? launch_ring<T, false, false, E, Lie::Pieces, 2>(a, blocks, stream, name)
+                       : launch_ring<T, false, false, E, Lie::Pieces, 4>(a, blocks, stream, name);
+        }
+    } else {
+        if constexpr (E == Ends::Plain) {
+            if (form == Form::Ring128) {
+                return launch_ring<T, GRAD, COLS_MAJOR, E, Lie::Words, 4>(a, blocks, stream, name);
+            }
+        }
+        if (form == Form::Shared) {
+            return launch_with_lds<tile_product_shared<T, GRAD, COLS_MAJOR, E>>(
+                grid, threads_of(Form::Shared), kSharedLds, stream, name, a);
+        }
     }
     if (form == Form::Pieces) {
-        tile_product<T, GRAD, COLS_MAJOR, E, true><<<blocks, 256, 0, stream>>>(a);
-    } else if constexpr (!std::is_same_v<T, Int8Pair>) {  // whose rows are whole pieces
-        tile_product<T, GRAD, COLS_MAJOR, E, false><<<blocks, 256, 0, stream>>>(a);
+        tile_product<T, GRAD, COLS_MAJOR, E, true><<<grid, 256, 0, stream>>>(a);
+    } else if constexpr (!kInt) {  // whose rows are whole pieces
+        tile_product<T, GRAD, COLS_MAJOR, E, false><<<grid, 256, 0, stream>>>(a);
     }
     SPMM_TRY_HIP(hipGetLastError(), name);
     return Error{};
