@@ -154,8 +154,9 @@ Error launch_few_rows(const TileArgs& a, bool pieces, hipStream_t stream, const 
 //     12: 5; two rounds of 256 x 256, rank 64: 25), less than an adapter a row does (11).
 //   64 x 64 tiles: 300 rows x 1024 x 1024 with adapters 14 us, 128 x 128 21; 100 rows x
 //     4000 x 4097 30, few_rows_product 43; 12 rows x 1504 x 2057 15, few_rows_product 8.
-//   Rows of whole words that are no pieces: in tiles as those of pieces, one of 128 x 128 a CU
-//     in a ring (the same sums in the same order as through registers).
+//   Rows of whole words that are no pieces: in tiles as those of pieces, or one of 128 x 128 a
+//     CU in a ring (3001 rows in seven groups, 2002 x 1030, W [k][c]: 29 us, 36 in
+//     tile_product).  All have the same sums in the same order as through registers.
 Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie) {
     const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     const double mean = a.total / groups;
@@ -193,7 +194,7 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie) {
     Form best = pieces ? Form::Pieces : Form::Any;
     if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
     if (a.ids == nullptr && lie == Lie::Words) {
-        if (time(Form::Ring128) < time(best)) best = Form::Ring128;
+        best = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
         if (time(Form::Wide) < time(best)) best = Form::Wide;
     }
     if (time(Form::Shared) < time(best)) best = Form::Shared;
@@ -259,7 +260,7 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
     Form form = !pieces ? Form::Any
                 : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
     if (lie == Lie::Words) {
-        if (time(Form::Ring128) < time(form)) form = Form::Ring128;
+        form = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
         if (time(Form::Wide) < time(form)) form = Form::Wide;
     }
     if (time(Form::Shared) < time(form)) form = Form::Shared;

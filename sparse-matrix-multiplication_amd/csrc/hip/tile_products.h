@@ -909,15 +909,15 @@ __device__ __forceinline__ void leave(const TileArgs& a, const Tile<T>& t, int r
 // sums and the others' next to each other in a wave, which needs both.
 //
 // The 128 x 128 tile of medium products, and of any sizes and alignment: four waves
-// take a quarter each, two buffers of 64 steps.  PIECES: the operands' rows are
-// whole 16-byte pieces, which go straight into LDS.  Otherwise they go through
-// registers, as the words around each piece, from buffers that end with the operand:
+// take a quarter each, two buffers of 64 steps.  The operands' rows of whole 16-byte
+// pieces or words go straight into LDS (words cut there as in tile_product_wide).  Odd:
+// others go through registers, as the words around each piece, from buffers that end with the operand:
 // straight code with eight or sixteen loads under way.  (With a branch a piece for those
 // at an edge the compiler waited for each load: 8 groups of 4000 x 4098 over 16384 rows
 // 930 us, 810 so; their weights' gradient 1280, 790.  Two workgroups a CU need the
 // registers bounded: 1390 with one.)
-template <typename T, bool GRAD, bool COLS_MAJOR, Ends E, bool PIECES>
-__global__ __launch_bounds__(256, PIECES ? 1 : 2) void tile_product(TileArgs a) {
+template <typename T, bool GRAD, bool COLS_MAJOR, Ends E, Lie L>
+__global__ __launch_bounds__(256, L == Lie::Odd ? 2 : 1) void tile_product(TileArgs a) {
     constexpr bool GATED = E == Ends::Gated;
     constexpr int BR = 128, BC = 128, WC = 2, RF = 4, CF = 4, OUT = GATED ? BC / 2 : BC;
     using Rows = Operands<T, BR, GRAD, 256>;
@@ -962,15 +962,15 @@ __global__ __launch_bounds__(256, PIECES ? 1 : 2) void tile_product(TileArgs a) 
                 for (int i = 0; i < RF; ++i) acc[j][i] = mfma(fc[j], fr[i], acc[j][i]);
         }
     };
-    if constexpr (PIECES) {
+    if constexpr (L != Lie::Odd) {
         Slot<T, GRAD, 64> pr;
         Slot<T, GRAD || COLS_MAJOR, GATED ? 0 : 64> pc;
         pr.place(t.ld_rows, 0, t.rows_here);
         pc.place(t.ld_cols, 0, a.width - t.c0);
         auto load = [&](int it) {
-            const u32x4 br = buffer_words(t.rows + it * t.step_rows, 0, 0x7fffffff);
-            const u32x4 bc = buffer_words(t.cols + it * t.step_cols, 0, 0x7fffffff);
-            const u32x4 bs = GATED ? buffer_words(t.second + it * t.step_cols, 0, 0x7fffffff) : bc;
+            const u32x4 br = operand_words<L>(t.rows + it * t.step_rows, a.rows_end);
+            const u32x4 bc = operand_words<L>(t.cols + it * t.step_cols, a.cols_end);
+            const u32x4 bs = GATED ? operand_words<L>(t.second + it * t.step_cols, a.cols_end) : bc;
             const unsigned lr = lds_address(rows_at(it)) + wave * 1024;
             const unsigned lc = lds_address(cols_at(it)) + wave * 1024;
             const int left = t.depth - it * kStep;
@@ -988,6 +988,15 @@ __global__ __launch_bounds__(256, PIECES ? 1 : 2) void tile_product(TileArgs a) 
             // every wave's pieces are there, and the other buffer's readers are done
             wait_vmcnt<0>();
             lds_barrier();
+            if (L == Lie::Words && !GRAD && it + 1 == tiles && t.depth % 8 != 0) {
+                const int last = t.depth - it * kStep, n = threadIdx.x & 127;
+                if (threadIdx.x < 128 || !COLS_MAJOR) {
+                    T* row = (threadIdx.x < 128 ? rows_at(it) : cols_at(it)) + n * kStep;
+                    uint4* piece = reinterpret_cast<uint4*>(row) + ((last / 8) ^ (n & 7));
+                    *piece = first_of(*piece, last % 8);
+                }
+                lds_barrier();
+            }
             if (it + 1 < tiles) load(it + 1);
             multiply(it);
         }
@@ -2044,10 +2053,10 @@ inline Form choose_finished(const TileArgs& a, int width, Lie lie, bool packs) {
     };
     take(Form::Ring128, ring(Form::Ring128, stage128[l]));
     const double tiles = row_tiles(128) * std::ceil(width / 128.0);
-    if (tiles * 256 <= kLaunchThreads && lie != Lie::Words) {
-        const double one = lie == Lie::Pieces ? 0.85 : 1.2, two = lie == Lie::Pieces ? 1.15 : 1.5;
+    if (tiles * 256 <= kLaunchThreads) {
+        const double one = lie != Lie::Odd ? 0.85 : 1.2, two = lie != Lie::Odd ? 1.15 : 1.5;
         const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
-        take(lie == Lie::Pieces ? Form::Pieces : Form::Any,
+        take(lie != Lie::Odd ? Form::Pieces : Form::Any,
              std::max(whole * (3 + two * rounds) + (rest == 0 ? 0 : 3 + (rest <= 256 ? one : two) * rounds),
                       weights / 3.5e6));
     }
@@ -2120,10 +2129,14 @@ Error launch_tiles(const TileArgs& a, Form form, Lie lie, hipStream_t stream, co
                 grid, threads_of(Form::Shared), kSharedLds, stream, name, a);
         }
     }
-    if (form == Form::Pieces) {
-        tile_product<T, GRAD, COLS_MAJOR, E, true><<<grid, 256, 0, stream>>>(a);
-    } else if constexpr (!kInt) {  // whose rows are whole pieces
-        tile_product<T, GRAD, COLS_MAJOR, E, false><<<grid, 256, 0, stream>>>(a);
+    if constexpr (kInt) {  // whose rows are whole pieces
+        tile_product<T, GRAD, COLS_MAJOR, E, Lie::Pieces><<<grid, 256, 0, stream>>>(a);
+    } else if (form == Form::Any) {
+        tile_product<T, GRAD, COLS_MAJOR, E, Lie::Odd><<<grid, 256, 0, stream>>>(a);
+    } else if (lie == Lie::Pieces) {
+        tile_product<T, GRAD, COLS_MAJOR, E, Lie::Pieces><<<grid, 256, 0, stream>>>(a);
+    } else if constexpr (E != Ends::Adapters) {
+        tile_product<T, GRAD, COLS_MAJOR, E, Lie::Words><<<grid, 256, 0, stream>>>(a);
     }
     SPMM_TRY_HIP(hipGetLastError(), name);
     return Error{};

@@ -207,24 +207,26 @@ def int8_mm(x, w: Rows8, offsets=None, dtype=None, out=None, stream=None):
     return _int8(x, w, offsets, False, 0, dtype, out, stream)
 
 
-def gated_mm(x, w, offsets=None, act: str = "silu", keep=None, out=None, stream=None):
+def gated_mm(x, w, offsets=None, act: str = "silu", keep=None, dtype=None, out=None, stream=None):
     """act(g) * u with g = x w[0]^T and u = x w[1]^T: [S, N].
 
     x [S, K], w [2, N, K], or [G, 2, N, K] with offsets (``grouped_mm``'s; rows in no group
     are zero), float16 or bfloat16.  act: "silu", "gelu" or "gelu_tanh".  keep: "full" returns
     g and u [S, 2, N] of x's type too, for ``gated_mm_backward``, "8bit" the same as Packed8.
-    x and w may be quantised rows (``int8_mm``'s operands: x a tensor or Rows8, w Rows8);
-    nothing can be kept then."""
+    x and w may be quantised rows (``int8_mm``'s operands: x a tensor or Rows8, w Rows8), with
+    ``int8_mm``'s dtype; nothing can be kept then."""
     act_id = _act_id(act)
     if keep not in (None, "full", "8bit"):
         raise SpmmError(SPMM_INVALID, f"keep: {keep!r}, expected None, 'full' or '8bit'")
     if isinstance(w, Rows8):
         if keep is not None:
             raise SpmmError(SPMM_UNSUPPORTED, "keep: products in 8-bit integers have no gradients")
-        return _int8(x, w, offsets, True, act_id, None, out, stream)
+        return _int8(x, w, offsets, True, act_id, dtype, out, stream)
     if isinstance(x, Rows8):
         raise SpmmError(SPMM_INVALID, "w: expected Rows8 next to x of Rows8")
     _half(x, "x")
+    if dtype not in (None, x.dtype):
+        raise SpmmError(SPMM_INVALID, f"dtype: {dtype}, expected {x.dtype}, x's")
     S, K = x.shape
     device = x.device
     G, N, at = _pairs(w, x.dtype, K, offsets, device)
