@@ -20,7 +20,7 @@ from typing import Any
 import torch
 
 from . import SPMM_INVALID, SPMM_UNSUPPORTED, SpmmError, _check, lib
-from .experts import (_FLOAT, _INT, _TYPES, _counts, _half, _on, _operand, _out, _refuse, _rows,
+from .experts import (_FLOAT, _INT, _TYPES, _counts, _half, _on, _operand, _out, _refuse,
                       _stream, grouped_mm)
 
 _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
@@ -140,7 +140,7 @@ def quantize_rows(x, stream=None) -> Rows8:
     return Rows8(values, scales, width)
 
 
-def _groups(offsets, w_shape, lead: int, device):
+def _groups(offsets, w_shape, device):
     """(groups, pointer) of offsets, None for one group of all rows, whose weights then have
     no dimension for groups."""
     if offsets is None:
@@ -152,50 +152,39 @@ def _groups(offsets, w_shape, lead: int, device):
     return G, offsets.data_ptr()
 
 
-def _quantised(x, dtype, stream):
-    """x as Rows8 and the type of a product with it."""
-    if isinstance(x, Rows8):
-        x._checked("x", 2)
-        return x, torch.bfloat16 if dtype is None else dtype
-    if isinstance(x, torch.Tensor):
-        _operand(x, "x", _TYPES, 2)
-    else:
-        _refuse(x, "x", _TYPES, 2, None)
-    return quantize_rows(x, stream), x.dtype if dtype is None else dtype
-
-
-def _int8(x, w, offsets, pair: bool, act, dtype, out, stream):
+def _int8(x, w, offsets, pair: bool, act: int, dtype, out, stream):
     if not isinstance(w, Rows8):
         raise SpmmError(SPMM_INVALID, f"w: expected Rows8, got {type(w).__name__}")
-    device = x.values.device if isinstance(x, Rows8) else getattr(x, "device", None)
-    # weights, output and offsets are looked at before anything is launched
-    wv = w._checked("w", 2 + pair + (offsets is not None))
-    if pair and wv.shape[-3] != 2:
-        raise SpmmError(SPMM_INVALID, f"w: shape {tuple(wv.shape)}, expected [..., 2, N, K]")
-    given = x.width if isinstance(x, Rows8) else x.shape[-1] if isinstance(x, torch.Tensor) \
-        and x.dim() else None
-    if given != w.width:
-        raise SpmmError(SPMM_INVALID, f"w: rows of {w.width} for x of {given}")
     if dtype is not None and dtype not in _TYPES:
         raise SpmmError(SPMM_INVALID, f"dtype: {dtype}, expected one of {list(_TYPES)}")
-    G, at = _groups(offsets, wv.shape, 2 + pair, wv.device)
-    N = wv.shape[-2]
-    with _on(stream, wv.device):
-        q, dtype = _quantised(x, dtype, None)
-        S, depth = q.values.shape
-        if q.values.device != wv.device:
-            raise SpmmError(SPMM_INVALID, f"x: on {device}, expected {wv.device}")
-        _counts(S, N, depth, G)
-        out = _out(out, "out", dtype, (S, N), wv.device)
-        L, s = lib(), _stream(wv.device)
+    # all is looked at before anything is launched
+    wv = w._checked("w", 2 + pair + (offsets is not None))
+    device = wv.device
+    if pair and wv.shape[-3] != 2:
+        raise SpmmError(SPMM_INVALID, f"w: shape {tuple(wv.shape)}, expected [..., 2, N, K]")
+    quantised = isinstance(x, Rows8)
+    if quantised:
+        S, width = x._checked("x", 2, device).shape[0], x.width
+    else:
+        _operand(x, "x", _TYPES, 2, device)
+        S, width = x.shape
+    if width != w.width:
+        raise SpmmError(SPMM_INVALID, f"w: rows of {w.width} for x of {width}")
+    if dtype is None:
+        dtype = torch.bfloat16 if quantised else x.dtype
+    G, at = _groups(offsets, wv.shape, device)
+    N, depth = wv.shape[-2:]
+    _counts(S, N, depth, G)
+    L = lib()
+    with _on(stream, device):
+        out = _out(out, "out", dtype, (S, N), device)
+        q = x if quantised else quantize_rows(x)
+        args = (q.values.data_ptr(), q.scales.data_ptr(), wv.data_ptr(), w.scales.data_ptr(), at, G,
+                S, N, depth)
         if pair:
-            _check(L.spmm_c_gated_int8_mm(q.values.data_ptr(), q.scales.data_ptr(), wv.data_ptr(),
-                                          w.scales.data_ptr(), at, G, S, N, depth, act,
-                                          _TYPES[dtype], out.data_ptr(), s))
+            _check(L.spmm_c_gated_int8_mm(*args, act, _TYPES[dtype], out.data_ptr(), _stream(device)))
         else:
-            _check(L.spmm_c_int8_mm(q.values.data_ptr(), q.scales.data_ptr(), wv.data_ptr(),
-                                    w.scales.data_ptr(), at, G, S, N, depth, _TYPES[dtype],
-                                    out.data_ptr(), s))
+            _check(L.spmm_c_int8_mm(*args, _TYPES[dtype], out.data_ptr(), _stream(device)))
     return out
 
 
@@ -253,7 +242,7 @@ def _pairs(w, dtype, K: int, offsets, device):
     _operand(w, "w", (dtype,), 3 + (offsets is not None), device)
     if w.shape[-3] != 2 or w.shape[-1] != K:
         raise SpmmError(SPMM_INVALID, f"w: shape {tuple(w.shape)}, expected [..., 2, N, {K}]")
-    G, at = _groups(offsets, w.shape, 3, device)
+    G, at = _groups(offsets, w.shape, device)
     N = w.shape[-2]
     _counts(G, 2 * N)
     return G, N, at
