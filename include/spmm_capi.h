@@ -462,9 +462,9 @@ int spmm_c_adapter_mm(const void* d_x, const void* d_w, const void* d_a, const v
  *   NaN all its values, for a block with an infinity or NaN.  fp32, fp16 or bf16.
  * unpack8: the values, rounded to the output's type (exact in bf16).
  * quantize_rows: d_values int8 [rows, width rounded up to 16], zero past width, and fp32
- *   d_scales [rows]: scale = max / 127 and q = x (127 / max) rounded to the nearest integer,
- *   max a row's largest magnitude, at least 2^-100; scale 0 for a row of zeros, NaN for
- *   one with an infinity or NaN.
+ *   d_scales [rows]: scale = max (1 / 127) and q = x (127 (1 / max)), x's product rounded once
+ *   to the nearest integer, the others to fp32, max a row's largest magnitude, at least
+ *   2^-100; scale 0 for a row of zeros, NaN for one with an infinity or NaN.
  * int8_mm: d_out[s, c] = x_scales[s] w_scales[c] sum_k x[s, k] w[c, k] for quantised rows
  *   d_x [rows, depth], d_w [groups, width, depth], d_w_scales [groups, width]; depth as
  *   padded, a multiple of 16 up to 131056, values 16-byte aligned.  The sum is exact,

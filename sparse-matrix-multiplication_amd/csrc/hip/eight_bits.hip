@@ -4,7 +4,9 @@
 //                  that are kept for a backward pass
 //   unpack8        the values that they stand for
 //   quantize_rows  rows with one fp32 scale, for products in 8-bit integers:
-//                  scale = max|x| / 127, q = the integer next to x (127 / max|x|)
+//                  scale = max|x| / 127, q = the integer next to x * (127 / max|x|),
+//                  both by reciprocals rounded to fp32; the last product is exact until
+//                  it is rounded to an integer
 //
 // All are bound by memory.
 
@@ -74,7 +76,7 @@ __device__ __forceinline__ unsigned group_max(unsigned v) {
 
 // A workgroup takes a row: its first kHeld eights a thread stay in registers between the
 // maximum and the rounding, the rest is read again.
-//   Rows below 2^-100 take that as their largest value, so that 127 / max stays finite.
+//   Rows below 2^-100 take that as their largest value, so that 1 / max stays finite.
 //   A row with an infinity or a NaN has the scale NaN, which its products become, and zeros.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void quantize(const T* __restrict__ x, int width, int padded,
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(WAVES * 64) void quantize(const T* __restrict__ x, 
     most = group_max<WAVES>(most);
     const bool fine = most < 0x7f800000u;
     const float largest = fmaxf(__uint_as_float(most), 0x1p-100f);
-    const float up = fine ? 127.0f / largest : 0.0f;
+    const float up = fine ? 1.0f / largest * 127.0f : 0.0f;
     auto put = [&](int c, const float (&g)[8]) {
         unsigned q[8];
 #pragma unroll
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(WAVES * 64) void quantize(const T* __restrict__ x, 
         put(c, g);
     }
     if (threadIdx.x == 0) {
-        scales[blockIdx.x] = !fine ? __builtin_nanf("") : most == 0 ? 0.0f : largest / 127.0f;
+        scales[blockIdx.x] = !fine ? __builtin_nanf("") : most == 0 ? 0.0f : largest * (1.0f / 127.0f);
     }
 }
 

@@ -90,13 +90,8 @@ Error launch_gated_mm(const void* x, const void* w, ElementType type, const int*
     a.rows_end = static_cast<const char*>(x) + 2LL * total * depth;
     a.cols_end = static_cast<const char*>(w) + 4LL * groups * width * depth;
     const Lie lie = lie_of(a, depth, depth);
-    const Form form = choose_finished(a, 2 * width, lie, kept_scales != nullptr);
     return with_half(type, "gated_mm", [&](auto zero) {
-        using T = decltype(zero);
-        if (form == Form::FewRows) {
-            return launch_few_finished<T, Ends::Gated>(a, lie == Lie::Pieces, stream, "gated_mm");
-        }
-        return launch_tiles<T, false, false, Ends::Gated>(a, form, lie, stream, "gated_mm");
+        return launch_finished<decltype(zero), Ends::Gated>(a, lie, stream, "gated_mm");
     });
 }
 
@@ -109,11 +104,7 @@ Error launch_gated_int8_mm(const void* x, const float* x_scales, const void* w, 
                        "gated_int8_mm", a));
     if (total == 0) return Error{};
     a.act = act;
-    const Form form = choose_finished(a, 2 * width, Lie::Pieces, false);
-    if (form == Form::FewRows) {
-        return launch_few_finished<Int8Pair, Ends::Gated>(a, true, stream, "gated_int8_mm");
-    }
-    return launch_tiles<Int8Pair, false, false, Ends::Gated>(a, form, Lie::Pieces, stream, "gated_int8_mm");
+    return launch_finished<Int8Pair, Ends::Gated>(a, Lie::Pieces, stream, "gated_int8_mm");
 }
 
 Error launch_gated_grad(const void* dh, ElementType type, const void* kept, const void* kept_scales,

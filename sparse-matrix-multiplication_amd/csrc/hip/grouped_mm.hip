@@ -157,7 +157,7 @@ Error launch_few_rows(const TileArgs& a, bool pieces, hipStream_t stream, const 
 //   Rows of whole words that are no pieces: in tiles as those of pieces, or one of 128 x 128 a
 //     CU in a ring (3001 rows in seven groups, 2002 x 1030, W [k][c]: 29 us, 36 in
 //     tile_product).  All have the same sums in the same order as through registers.
-Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie) {
+Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie, double* least = nullptr) {
     const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     const double mean = a.total / groups;
     const double weights = 2.0 * groups * a.width * a.depth;
@@ -197,8 +197,16 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie) {
         best = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
         if (time(Form::Wide) < time(best)) best = Form::Wide;
     }
+    // a single group, whose rows all know: the ring where there are few tiles of a long
+    // contraction
+    if (a.ids == nullptr && a.offsets == nullptr && lie != Lie::Odd) {
+        if (time(Form::Ring128) < 0.9 * time(best)) best = Form::Ring128;
+        if (time(Form::Ring64) < 0.9 * time(best)) best = Form::Ring64;
+    }
     if (time(Form::Shared) < time(best)) best = Form::Shared;
-    return few_allowed && few <= time(best) ? Form::FewRows : best;
+    if (few_allowed && few <= time(best)) best = Form::FewRows;
+    if (least != nullptr) *least = best == Form::FewRows ? few : time(best);
+    return best;
 }
 
 }  // namespace
@@ -225,12 +233,30 @@ Error launch_grouped_mm(const void* x, const void* w, ElementType type, const in
     a.cols_end = static_cast<const char*>(w) + 2LL * groups * width * depth;
     const Lie lie = lie_of(a, depth, w_in_rows ? width : depth);
     const Form form = choose_form(a, pieces, !w_in_rows, lie);
-    return with_half(type, "grouped_mm", [&](auto zero) {
-        using T = decltype(zero);
-        if (form == Form::FewRows) return launch_few_rows<T, Ends::Plain>(a, pieces, stream, "grouped_mm");
-        return w_in_rows ? launch_tiles<T, false, true, Ends::Plain>(a, form, lie, stream, "grouped_mm")
-                         : launch_tiles<T, false, false, Ends::Plain>(a, form, lie, stream, "grouped_mm");
-    });
+    auto launch = [&](const TileArgs& part, Form form) {
+        return with_half(type, "grouped_mm", [&](auto zero) {
+            using T = decltype(zero);
+            if (form == Form::FewRows) return launch_few_rows<T, Ends::Plain>(part, pieces, stream, "grouped_mm");
+            return w_in_rows ? launch_tiles<T, false, true, Ends::Plain>(part, form, lie, stream, "grouped_mm")
+                             : launch_tiles<T, false, false, Ends::Plain>(part, form, lie, stream, "grouped_mm");
+        });
+    };
+    if (offsets == nullptr && lie != Lie::Odd) {
+        const int head = whole_rounds(total, 1, width, [&](int rows, bool wide) {
+            TileArgs part = a;
+            part.total = rows;
+            double time;
+            choose_form(part, pieces, !w_in_rows, lie, &time);
+            auto tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge); };
+            return wide ? tile_time(Form::Wide, tiles, width, depth, 0) : time;
+        });
+        if (head > 0) {
+            SPMM_TRY(launch(rows_alone(a, 0, head, 2), Form::Wide));
+            const TileArgs rest = rows_alone(a, head, total - head, 2);
+            return launch(rest, choose_form(rest, pieces, !w_in_rows, lie));
+        }
+    }
+    return launch(a, form);
 }
 
 Error launch_grouped_outer(const void* p, const void* q, ElementType type, const int* offsets,
@@ -250,24 +276,43 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
     a.height = height;
     a.width = width;
     const bool pieces = height % 8 == 0 && width % 8 == 0 && aligned16(p) && aligned16(q);
-    auto row_tiles = [&](int edge) { return std::ceil(static_cast<double>(height) / edge) * groups; };
-    auto time = [&](Form f) {
-        return tile_time(f, row_tiles, width, static_cast<double>(total) / groups, 0);
-    };
     a.rows_end = static_cast<const char*>(p) + 2LL * total * height;
     a.cols_end = static_cast<const char*>(q) + 2LL * total * width;
     const Lie lie = lie_of(a, height, width);
-    Form form = !pieces ? Form::Any
-                : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
-    if (lie == Lie::Words) {
-        form = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
-        if (time(Form::Wide) < time(form)) form = Form::Wide;
-    }
-    if (time(Form::Shared) < time(form)) form = Form::Shared;
-    return with_half(type, "grouped_outer", [&](auto zero) {
-        using T = decltype(zero);
-        return launch_tiles<T, true, true, Ends::Plain>(a, form, lie, stream, "grouped_outer");
+    // the form with the least time for `rows` of the output's
+    auto choose = [&](int rows, double* least) {
+        auto row_tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge) * groups; };
+        auto time = [&](Form f) {
+            return tile_time(f, row_tiles, width, static_cast<double>(total) / groups, 0);
+        };
+        Form form = !pieces ? Form::Any
+                    : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
+        if (lie == Lie::Words) {
+            form = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
+            if (time(Form::Wide) < time(form)) form = Form::Wide;
+        }
+        if (time(Form::Shared) < time(form)) form = Form::Shared;
+        *least = time(form);
+        return form;
+    };
+    auto launch = [&](int from, int upto, Form form) {
+        TileArgs part = a;
+        part.from = from;
+        part.upto = upto;
+        return with_half(type, "grouped_outer", [&](auto zero) {
+            return launch_tiles<decltype(zero), true, true, Ends::Plain>(part, form, lie, stream, "grouped_outer");
+        });
+    };
+    double least;
+    const int head = lie == Lie::Odd ? 0 : whole_rounds(height, groups, width, [&](int rows, bool wide) {
+        auto row_tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge) * groups; };
+        if (wide) return tile_time(Form::Wide, row_tiles, width, static_cast<double>(total) / groups, 0);
+        choose(rows, &least);
+        return least;
     });
+    if (head > 0) SPMM_TRY(launch(0, head, Form::Wide));
+    const Form form = choose(height - head, &least);
+    return launch(head, height, form);
 }
 
 long long adapter_workspace(long long total, int rank) {

@@ -21,9 +21,7 @@ Error launch_int8_mm(const void* x, const float* x_scales, const void* w, const 
     SPMM_TRY(int8_args(x, x_scales, w, w_scales, offsets, groups, total, width, depth, out_type, out,
                        "int8_mm", a));
     if (total == 0) return Error{};
-    const Form form = choose_finished(a, width, Lie::Pieces, false);
-    if (form == Form::FewRows) return launch_few_finished<Int8Pair, Ends::Plain>(a, true, stream, "int8_mm");
-    return launch_tiles<Int8Pair, false, false, Ends::Plain>(a, form, Lie::Pieces, stream, "int8_mm");
+    return launch_finished<Int8Pair, Ends::Plain>(a, Lie::Pieces, stream, "int8_mm");
 }
 
 }  // namespace engine

@@ -111,6 +111,7 @@ struct TileArgs {
     int         groups;
     int         total;    // rows of X, P, Q
     int         height;   // gradient: rows of each group's output
+    int         from, upto; // gradient: those of them that this launch takes
     int         width;    // columns of the output
     int         depth;    // product: contraction
     // adapters (ids null: none)
@@ -374,11 +375,11 @@ __device__ __forceinline__ bool take_tile(const TileArgs& a, Tile<T>& t) {
     int ct;
     if constexpr (GRAD) {
         int rt;
-        const int row_tiles = (a.height + BR - 1) / BR;
+        const int row_tiles = (a.upto - a.from + BR - 1) / BR;
         if (!tile_of_block(a.groups * row_tiles, col_tiles, rt, ct)) return false;
         const int g = rt / row_tiles;
-        t.row0 = (rt % row_tiles) * BR;
-        t.rows_here = min(BR, a.height - t.row0);
+        t.row0 = a.from + (rt % row_tiles) * BR;
+        t.rows_here = min(BR, a.upto - t.row0);
         t.c0 = ct * BC;
         const int lo = row_bound(a, g), hi = max(row_bound(a, g + 1), lo);
         t.depth   = hi - lo;
@@ -2002,6 +2003,9 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
     if (form == Form::Ring128) {
         return std::max(std::ceil(tiles / 256) * (3 + 0.62 * rounds), weights);
     }
+    if (form == Form::Ring64) {  // row_tiles counts its rows
+        return std::max(std::ceil(row_tiles(64) * std::ceil(width / 128.0) / 256) * (3 + 0.48 * rounds), weights);
+    }
     const double two = form == Form::Any ? 1.5 : 0.95, one = form == Form::Any ? 1 : 0.62;
     const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
     const double time = whole * (3 + two * rounds) +
@@ -2028,7 +2032,7 @@ inline Lie lie_of(const TileArgs& a, long long ld_rows, long long ld_cols) {
 //   tile_product: 0.85 us with one tile a CU, 1.15 with two, through registers 1.2 and 1.5;
 //     tile_product_wide 1.55 (2 x 8192 x 4096: 512 rows 79 us in tile_product, 88 in the ring,
 //     1024 rows 113 wide, 154 and 167).
-inline Form choose_finished(const TileArgs& a, int width, Lie lie, bool packs) {
+inline Form choose_finished(const TileArgs& a, int width, Lie lie, bool packs, double* time) {
     const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     const double mean = a.total / groups, weights = 2.0 * groups * width * a.depth;
     // groups of all lengths end, on average, in the middle of a tile
@@ -2069,7 +2073,38 @@ inline Form choose_finished(const TileArgs& a, int width, Lie lie, bool packs) {
         take(Form::FewRows, (4 + std::max(reading, std::ceil(workgroups / 512) * chain)) *
                                 (lie == Lie::Pieces ? 1 : lie == Lie::Words ? 1.1 : 2));
     }
+    *time = best;
     return form;
+}
+
+// How many of `rows` output rows (a group's, of `groups` as high as each other) go to 256 x
+// 256 tiles in whole rounds of a tile a CU, the rest to what is fastest for it: 0 for none, or
+// where one launch takes no longer.  time(rows, form): the best form's estimate, or with a
+// form that one's (8192 rows for 11264 x 2048, 352 tiles: 256 and 384 of 128 x 128 346 us,
+// 356 in one launch; 9000 for 2 x 1024 x 4096, gated: 139 us, 180).
+template <typename F>
+int whole_rounds(int rows, int groups, int width, F time) {
+    const long long col_tiles = (width + 255) / 256, tiles = groups * ((rows + 255) / 256) * col_tiles;
+    const long long high = tiles / 256 * 256 / (groups * col_tiles);  // row tiles a group
+    const int head = static_cast<int>(high * 256);
+    if (high < 1 || head >= rows) return 0;
+    return time(head, true) + time(rows - head, false) + 2 < 0.96 * time(rows, false) ? head : 0;
+}
+
+// A product's rows [first, first + rows) by themselves, of one group that has all.
+inline TileArgs rows_alone(const TileArgs& all, int first, int rows, int out_bytes) {
+    TileArgs a = all;
+    auto later = [&](const void* p, long long bytes) { return static_cast<const char*>(p) + first * bytes; };
+    a.total = rows;
+    a.rows = later(all.rows, 2LL * all.depth);
+    a.out = const_cast<char*>(later(all.out, static_cast<long long>(all.width) * out_bytes));
+    if (all.row_scales != nullptr) a.row_scales = all.row_scales + first;
+    if (all.kept != nullptr) {
+        const bool packed = all.kept_scales != nullptr;
+        a.kept = const_cast<char*>(later(all.kept, 2LL * all.width * (packed ? 1 : 2)));
+        if (packed) a.kept_scales = all.kept_scales + first * (2LL * ((all.width + kPackBlock - 1) / kPackBlock));
+    }
+    return a;
 }
 
 template <typename T, bool GRAD, bool COLS_MAJOR, Ends E, Lie L, int RF>
@@ -2084,7 +2119,7 @@ Error launch_tiles(const TileArgs& a, Form form, Lie lie, hipStream_t stream, co
     const int edge = edge_of(form), out = E == Ends::Gated ? edge / 2 : edge, rows = rows_of(form);
     // every group may end in a part-filled tile, and so may the rows before and behind them
     const long long row_tiles =
-        GRAD ? static_cast<long long>(a.groups) * ((a.height + rows - 1) / rows)
+        GRAD ? static_cast<long long>(a.groups) * ((a.upto - a.from + rows - 1) / rows)
         : a.offsets == nullptr ? (a.total + rows - 1) / rows
                                : a.total / rows + std::min<long long>(a.groups + 2LL, a.total);
     // a whole number of workgroups for each XCD
@@ -2120,6 +2155,16 @@ Error launch_tiles(const TileArgs& a, Form form, Lie lie, hipStream_t stream, co
         }
     } else {
         if constexpr (E == Ends::Plain) {
+            if constexpr (!GRAD) {
+                if (form == Form::Ring64) {
+                    return lie == Lie::Words
+                        ? launch_ring<T, GRAD, COLS_MAJOR, E, Lie::Words, 2>(a, blocks, stream, name)
+                        : launch_ring<T, GRAD, COLS_MAJOR, E, Lie::Pieces, 2>(a, blocks, stream, name);
+                }
+                if (form == Form::Ring128 && lie == Lie::Pieces) {
+                    return launch_ring<T, GRAD, COLS_MAJOR, E, Lie::Pieces, 4>(a, blocks, stream, name);
+                }
+            }
             if (form == Form::Ring128) {
                 return launch_ring<T, GRAD, COLS_MAJOR, E, Lie::Words, 4>(a, blocks, stream, name);
             }
@@ -2140,6 +2185,36 @@ Error launch_tiles(const TileArgs& a, Form form, Lie lie, hipStream_t stream, co
     }
     SPMM_TRY_HIP(hipGetLastError(), name);
     return Error{};
+}
+
+// Launches a gated product or one in 8-bit integers, in one or two parts.
+template <typename T, Ends E>
+Error launch_finished(const TileArgs& a, Lie lie, hipStream_t stream, const char* name) {
+    const int width = E == Ends::Gated ? 2 * a.width : a.width;
+    const bool packs = a.kept_scales != nullptr;
+    auto launch = [&](const TileArgs& part, Form form) {
+        if (form == Form::FewRows) return launch_few_finished<T, E>(part, lie == Lie::Pieces, stream, name);
+        return launch_tiles<T, false, false, E>(part, form, lie, stream, name);
+    };
+    double best;
+    const Form form = choose_finished(a, width, lie, packs, &best);
+    if (a.offsets == nullptr && lie != Lie::Odd) {
+        const int bytes = std::is_same_v<T, Int8Pair> && a.out_type == ElementType::F32 ? 4 : 2;
+        const int head = whole_rounds(a.total, 1, width, [&](int rows, bool wide) {
+            TileArgs part = a;
+            part.total = rows;
+            double time;
+            choose_finished(part, width, lie, packs, &time);
+            auto tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge); };
+            return wide ? tile_time(Form::Wide, tiles, width, a.depth, 0) : time;
+        });
+        if (head > 0) {
+            SPMM_TRY(launch(rows_alone(a, 0, head, bytes), Form::Wide));
+            const TileArgs rest = rows_alone(a, head, a.total - head, bytes);
+            return launch(rest, choose_finished(rest, width, lie, packs, &best));
+        }
+    }
+    return launch(a, form);
 }
 
 // The operands of a product in 8-bit integers, checked: depth bytes a row, in pairs.

@@ -128,8 +128,8 @@ def unpack8(packed: Packed8, dtype=torch.bfloat16, out=None, stream=None):
 
 def quantize_rows(x, stream=None) -> Rows8:
     """Rows of x [..., K] (float32, float16 or bfloat16) as 8-bit integers: scale = max|x| /
-    127, and the integers next to x * (127 / max|x|), ties to even.  A row with an infinity
-    or a NaN has the scale NaN."""
+    127, and the integers next to x * (127 / max|x|), ties to even (the quotients by
+    reciprocals in float32).  A row with an infinity or a NaN has the scale NaN."""
     rows, width = _flat(x, "x")
     device = x.device
     with _on(stream, device):
@@ -178,13 +178,20 @@ def _int8(x, w, offsets, pair: bool, act: int, dtype, out, stream):
     L = lib()
     with _on(stream, device):
         out = _out(out, "out", dtype, (S, N), device)
-        q = x if quantised else quantize_rows(x)
-        args = (q.values.data_ptr(), q.scales.data_ptr(), wv.data_ptr(), w.scales.data_ptr(), at, G,
-                S, N, depth)
-        if pair:
-            _check(L.spmm_c_gated_int8_mm(*args, act, _TYPES[dtype], out.data_ptr(), _stream(device)))
+        s = _stream(device)
+        if quantised:
+            values, scales = x.values.data_ptr(), x.scales.data_ptr()
         else:
-            _check(L.spmm_c_int8_mm(*args, _TYPES[dtype], out.data_ptr(), _stream(device)))
+            # rows of integers and behind them their scales
+            room = torch.empty(S * (depth + 4), dtype=torch.int8, device=device)
+            values = room.data_ptr()
+            scales = values + S * depth
+            _check(L.spmm_c_quantize_rows(x.data_ptr(), _TYPES[x.dtype], S, width, values, scales, s))
+        args = (values, scales, wv.data_ptr(), w.scales.data_ptr(), at, G, S, N, depth)
+        if pair:
+            _check(L.spmm_c_gated_int8_mm(*args, act, _TYPES[dtype], out.data_ptr(), s))
+        else:
+            _check(L.spmm_c_int8_mm(*args, _TYPES[dtype], out.data_ptr(), s))
     return out
 
 

@@ -102,9 +102,9 @@ def quantise(x: np.ndarray):
         most = np.abs(x).view(np.uint32).max(-1).view(np.float32)
         fine = np.isfinite(most)
         largest = np.maximum(most, np.float32(2.0 ** -100))
-        up = np.where(fine, np.float32(127) / largest, np.float32(0)).astype(np.float32)
+        up = np.where(fine, np.float32(1) / largest * np.float32(127), np.float32(0)).astype(np.float32)
         q = np.rint(x.astype(np.float64) * up.astype(np.float64)[..., None])
-        scale = np.where(fine, np.where(most == 0, np.float32(0), largest / np.float32(127)),
+        scale = np.where(fine, np.where(most == 0, np.float32(0), largest * (np.float32(1) / np.float32(127))),
                          np.float32(np.nan)).astype(np.float32)
     q = np.where(fine[..., None], q, 0)
     out = np.zeros(x.shape[:-1] + (-(-K // 16) * 16,), np.int8)
