@@ -32,6 +32,16 @@ __device__ __forceinline__ float gate_value(Act act, float g) {
     g = g < lowest ? lowest : g;
     return g * gate_share(act, g);
 }
+// act of eight, the choice made once.
+__device__ __forceinline__ void gate_values(Act act, const float (&g)[8], float (&value)[8]) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) value[i] = f(g[i]);
+    };
+    if (act == Act::Silu) each([](float x) { return gate_value(Act::Silu, x); });
+    else if (act == Act::Gelu) each([](float x) { return gate_value(Act::Gelu, x); });
+    else each([](float x) { return gate_value(Act::GeluTanh, x); });
+}
 // act(g) and act'(g).  Past 128 on either side p' is 0 in fp32, whatever g multiplies it by.
 __device__ __forceinline__ void gate_slope(Act act, float g, float& value, float& slope) {
     const float lowest = -3.4028235e38f;

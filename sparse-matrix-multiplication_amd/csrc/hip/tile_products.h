@@ -635,8 +635,9 @@ __device__ __forceinline__ void finish_row(const TileArgs& a, long long row, int
     if (count <= 0) return;
     if constexpr (GATED) {
         float h[8];
+        gate_values(a.act, f[0], h);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = gate_value(a.act, f[0][e]) * f[1][e];
+        for (int e = 0; e < 8; ++e) h[e] *= f[1][e];
         store(a.out, row * a.width + c, h);
     } else {
         store(a.out, row * a.width + c, f[0]);
@@ -697,26 +698,27 @@ __device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, 
     });
 }
 
-// The gated and the scaled stores of a wave's tile, sixteen rows at a time through its own
-// part of LDS as StoreTile's.  Gated, the first half of a row's sums are the gates and the
-// second half what they multiply, of the same kCols columns; a lane takes eight columns of
-// both, four lanes a block of 32 for packing.
-template <typename T, int RF, int CF, bool GATED>
+// The gated and the scaled stores of a wave's tile, B sixteens of rows at a time through its
+// own part of LDS (one at a time, each waits for its own way through LDS and for its own
+// functions: 20800 rows x 2 x 3776 x
+// 128 in 256 x 256 tiles 208 us, 136 so).  Gated, the first half of a row's
+// sums are the gates and the second half what they multiply, of the same kCols columns; a
+// lane takes eight columns of both, four lanes a block of 32 for packing.
+template <typename T, int CF, bool GATED, int B>
 struct FinishTile {
     static constexpr bool kScaled = std::is_same_v<T, Int8Pair>;
     static constexpr int  kPitch = CF * 16 + 4, kCols = GATED ? CF * 8 : CF * 16;
-    static constexpr int  kLanes = kCols / 8, kRows = 64 / kLanes < 16 ? 64 / kLanes : 16;
+    static constexpr int  kLanes = kCols / 8, kRows = 64 / kLanes;
     static constexpr int  kParts = GATED ? 2 : 1;
     const TileArgs& a;
     const Tile<T>&  t;
-    int    r0, c, count;  // the lane's first column, and how many of its eight there are
+    int    c, count;  // the lane's first column, and how many of its eight there are
     float* sums;
     float  scale[kScaled ? kParts : 1][8];  // of the lane's columns
 
-    __device__ __forceinline__ FinishTile(const TileArgs& args, const Tile<T>& tile, int row,
-                                          int col, float* lds)
-        : a(args), t(tile), r0(row), c(col + (threadIdx.x & 63) % kLanes * 8),
-          count(min(8, a.width - c)), sums(lds) {
+    __device__ __forceinline__ FinishTile(const TileArgs& args, const Tile<T>& tile, int col, float* lds)
+        : a(args), t(tile), c(col + (threadIdx.x & 63) % kLanes * 8), count(min(8, a.width - c)),
+          sums(lds) {
         if constexpr (kScaled) {
             const float* from = a.col_scales + static_cast<long long>(t.group) * kParts * a.width;
 #pragma unroll
@@ -727,28 +729,20 @@ struct FinishTile {
                 }
         }
     }
-    template <int I>
-    __device__ __forceinline__ void put(const Sums<T> (&acc)[CF][RF]) const {
+    // A sixteen's sums into place k.
+    __device__ __forceinline__ void put(int k, int j, Sums<T> x) const {
         const int lane = threadIdx.x & 63;
+        f32x4 v;
 #pragma unroll
-        for (int j = 0; j < CF; ++j) {
-            // the sixteens' bodies differ by this statement: merged into one with a variable
-            // place, some of the sums would leave their registers
-            Sums<T> x = acc[j][I];
-            asm volatile("; rows %1" : "+v"(x) : "n"(I));
-            f32x4 v;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) v[n] = static_cast<float>(x[n]);
-            *reinterpret_cast<f32x4*>(sums + (lane & 15) * kPitch + j * 16 + 4 * (lane >> 4)) = v;
-        }
+        for (int n = 0; n < 4; ++n) v[n] = static_cast<float>(x[n]);
+        *reinterpret_cast<f32x4*>(sums + (k * 16 + (lane & 15)) * kPitch + j * 16 + 4 * (lane >> 4)) = v;
     }
-    __device__ __forceinline__ void store(int i) const {
+    // Rows row0 .. of the tile, from the first place on.
+    __device__ __forceinline__ void store(int row0) const {
         const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int n = 0; n < 16 / kRows; ++n) {
-            const int r = n * kRows + lane / kLanes;  // past 16 in lanes without a part
-            if (r >= 16) break;
-            const int row = r0 + i * 16 + r;
+#pragma unroll 2
+        for (int n = 0; n < B * 16 / kRows; ++n) {
+            const int r = n * kRows + lane / kLanes, row = row0 + r;
             const float* from = sums + r * kPitch + lane % kLanes * 8;
             float f[kParts][8];
 #pragma unroll
@@ -766,18 +760,19 @@ struct FinishTile {
         }
     }
 };
-template <typename T, int RF, int CF, bool GATED>
+template <typename T, int RF, int CF, bool GATED, int B>
 __device__ __forceinline__ void finish_tile(const TileArgs& a, const Tile<T>& t, int r0, int c0,
                                             const Sums<T> (&acc)[CF][RF], float* sums) {
-    const FinishTile<T, RF, CF, GATED> tile(a, t, r0, c0, sums);
-    // one body for all sixteens of rows, as for the adapters
-#pragma unroll 1
-    for (int i = 0; i < RF && r0 + i * 16 < t.rows_here; ++i) {
-        unrolled(std::make_integer_sequence<int, RF>{}, [&](auto at) {
-            if (at.value == i) tile.template put<at.value>(acc);
-        });
-        tile.store(i);
-    }
+    const FinishTile<T, CF, GATED, B> tile(a, t, c0, sums);
+    unrolled(std::make_integer_sequence<int, RF / B>{}, [&](auto at) {
+        constexpr int first = at.value * B;
+        if (r0 + first * 16 < t.rows_here) {
+            unrolled(std::make_integer_sequence<int, B * CF>{}, [&](auto m) {
+                tile.put(m.value / CF, m.value % CF, acc[m.value % CF][first + m.value / CF]);
+            });
+            tile.store(r0 + first * 16);
+        }
+    });
 }
 
 // How 128 rows (or columns) of an operand's staged tile reach LDS in 16-byte
@@ -892,11 +887,16 @@ __device__ __forceinline__ u32x4 operand_words(const void* at, const void* end) 
 template <typename T, Ends E>
 constexpr bool kPlainEnds = E != Ends::Gated && !std::is_same_v<T, Int8Pair>;
 
-template <typename T, int RF, int CF, Ends E>
+// Floats of LDS that a wave's end takes.  B: sixteens of rows that gated and scaled sums leave in.
+template <typename T, int CF, Ends E, int B>
+constexpr int kLeaveFloats = kStoreFloats<CF> * (kPlainEnds<T, E> ? 1 : B);
+
+template <typename T, int RF, int CF, Ends E, int B>
 __device__ __forceinline__ void leave(const TileArgs& a, const Tile<T>& t, int r0, int c0,
-                                      const Sums<T> (&acc)[CF][RF], float* sums) {
+                                      const Sums<T> (&acc)[CF][RF], char* lds, int wave) {
+    float* sums = reinterpret_cast<float*>(lds) + wave * kLeaveFloats<T, CF, E, B>;
     if constexpr (!kPlainEnds<T, E>) {
-        finish_tile<T, RF, CF, E == Ends::Gated>(a, t, r0, c0, acc, sums);
+        finish_tile<T, RF, CF, E == Ends::Gated, B>(a, t, r0, c0, acc, sums);
     } else if constexpr (E == Ends::Adapters) {
         store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
     } else {
@@ -1040,8 +1040,8 @@ __global__ __launch_bounds__(256, L == Lie::Odd ? 2 : 1) void tile_product(TileA
         }
     }
     lds_barrier();  // the operands' LDS is free
-    float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
-    leave<T, RF, CF, E>(a, t, r0, c0, acc, sums);
+    static_assert(WC * 2 * kLeaveFloats<T, CF, E, 2> * sizeof(float) <= sizeof(s_tiles), "LDS of the ends");
+    leave<T, RF, CF, E, 2>(a, t, r0, c0, acc, reinterpret_cast<char*>(s_tiles), wave);
 }
 
 // The 64 x 64 tile of products with few tiles and a long contraction: sixteen waves in
@@ -1139,8 +1139,7 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
             for (int g = 1; g < GROUPS; ++g) acc[j][i] = acc[j][i] + parts[g][wave][j][i][lane];
         }
     // behind the shares: the other waves may still read theirs
-    float* sums = reinterpret_cast<float*>(s_tiles + sizeof(*parts) * GROUPS) + wave * kStoreFloats<CF>;
-    leave<T, RF, CF, E>(a, t, r0, c0, acc, sums);
+    leave<T, RF, CF, E, 1>(a, t, r0, c0, acc, s_tiles + sizeof(*parts) * GROUPS, wave);
 }
 
 // The 256 x 256 tile of large products, for operands whose rows are whole 16-byte
@@ -1346,8 +1345,8 @@ __global__ __launch_bounds__(256, 1) void tile_product_wide(TileArgs a) {
         wait_vmcnt<0>();
         lds_barrier();  // the ring is free
     }
-    float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
-    leave<T, RF, CF, E>(a, t, r0, c0, acc, sums);
+    static_assert(4 * kLeaveFloats<T, CF, E, 4> * sizeof(float) <= kRingLds, "LDS of the ends");
+    leave<T, RF, CF, E, 4>(a, t, r0, c0, acc, s_tiles, wave);
 }
 
 // The tile of 32 RF x 128 of products that the 256 x 256 tiles are too few of, and of rows
@@ -1573,8 +1572,8 @@ __global__ __launch_bounds__(256, 1) void tile_product_ring(TileArgs a) {
         wait_vmcnt<0>();
         lds_barrier();  // the ring is free
     }
-    float* sums = reinterpret_cast<float*>(s_tiles) + wave * kStoreFloats<CF>;
-    leave<T, RF, CF, E>(a, t, r0, c0, acc, sums);
+    static_assert(4 * kLeaveFloats<T, CF, E, RF> * sizeof(float) <= kRingLds, "LDS of the ends");
+    leave<T, RF, CF, E, RF>(a, t, r0, c0, acc, s_tiles, wave);
 }
 
 // Sums of a wave's share of the contraction for CF x 16 columns (rows of `cols`,
@@ -1973,6 +1972,9 @@ Error launch_few_finished(const TileArgs& a, bool pieces, hipStream_t stream, co
     } else {
         if (rows <= 16) return launch_few_rows_of<T, 1, 2, 4, kTwo, E>(a, pieces, stream, name);
         if (rows <= 32) return launch_few_rows_of<T, 2, 2, 4, kTwo, E>(a, pieces, stream, name);
+        if (a.groups * static_cast<long long>((a.width + 31) / 32) <= 256) {
+            return launch_few_rows_of<T, 4, 2, 4, kAll, E>(a, pieces, stream, name);
+        }
         return launch_few_rows_of<T, 4, 2, 4, kTwo, E>(a, pieces, stream, name);
     }
 }
@@ -2019,20 +2021,27 @@ inline Lie lie_of(const TileArgs& a, long long ld_rows, long long ld_cols) {
     return ld % 8 == 0 && at % 16 == 0 ? Lie::Pieces : ld % 2 == 0 && at % 4 == 0 ? Lie::Words : Lie::Odd;
 }
 
+// Microseconds of `tiles` tiles of 256 x 256 with `rounds` x 64 steps that end gated or scaled.
+inline double finished_wide(double tiles, double rounds) {
+    return 4 + std::ceil(tiles / 256) * (11 + 1.45 * rounds);
+}
 // The form of a gated product or one in 8-bit integers (whose depth is in pairs), by its
-// estimated time; width: rows of a group's weights, of both projections of a gated one.
+// estimated time, from measured rates; width: rows of a group's weights, of both projections
+// of a gated one; gated: 16 columns of either a workgroup of few_rows_product.
 //   few_rows_product: weights at 6.3 TB/s, more slowly as the rows' own reading counts and
-//     where a second tile of rows reads them again; 512 workgroups at a time go through a
-//     contraction of 1000 steps in 1.4 us with 16 rows, in 2.6 with 64 (2 x 8192 x 4096: 16
-//     rows 27 us, 64 36, 128 59; 2 x 1024 x 2048: 16 rows 5.0, 256 8.6).  1.1 times as long
-//     for rows that are no whole pieces, twice where they begin between two words.
+//     where a second tile of rows reads them again; 512 workgroups at a time, which take 3 us
+//     and for 1000 steps 1.4 us with 16 rows, 2.6 with 64, 4.2 where those leave no stages
+//     ahead (2 x 8192 x 4096: 16 rows 27 us, 64 36, 128 59; 2 x 1024 x 2048: 16 rows 5.0, 256
+//     8.6; 8 groups of 2 x 7552 x 304 in integers, 21 rows: 24, 16 in tile_product).  1.1 times
+//     as long for rows that are no whole pieces, twice where they begin between two words.
 //   tile_product_ring: 64 steps of a 64 x 128 tile take 0.42 us, of 128 x 128 0.57, more where
 //     rows are cut or shifted, one tile a CU; weights at 3.5 TB/s (2 x 8192 x 4096: 128 rows
 //     39 and 49 us, 256 68 and 49; tile_product 62, 68).
 //   tile_product: 0.85 us with one tile a CU, 1.15 with two, through registers 1.2 and 1.5;
-//     tile_product_wide 1.55 (2 x 8192 x 4096: 512 rows 79 us in tile_product, 88 in the ring,
-//     1024 rows 113 wide, 154 and 167).
-inline Form choose_finished(const TileArgs& a, int width, Lie lie, bool packs, double* time) {
+//     tile_product_wide 1.45 and 11 us for a tile's beginning and end (2 x 8192 x 4096: 512
+//     rows 79 us in tile_product, 88 in the ring, 1024 rows 113 wide, 154 and 167; 24771 rows x
+//     2 x 2430 x 160: 97 in tile_product, 125 wide).
+inline Form choose_finished(const TileArgs& a, int width, bool gated, Lie lie, bool packs, double* time) {
     const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     const double mean = a.total / groups, weights = 2.0 * groups * width * a.depth;
     // groups of all lengths end, on average, in the middle of a tile
@@ -2041,13 +2050,15 @@ inline Form choose_finished(const TileArgs& a, int width, Lie lie, bool packs, d
     };
     const int l = static_cast<int>(lie);
     const double rounds = std::ceil(static_cast<double>(a.depth) / kStep);
-    auto ring = [&](Form f, double stage) {
-        const double tiles = row_tiles(rows_of(f)) * std::ceil(width / 128.0);
+    auto ring = [&](Form f, double begin, double stage) {
+        const double high = row_tiles(rows_of(f));
+        // a few tiles more than groups have on average may be another round
+        const double tiles = high * std::ceil(width / 128.0) * (1 + (groups == 1 ? 0 : std::min(0.1, 0.3 * groups / high)));
         if (tiles * 256 > kLaunchThreads) return HUGE_VAL;
-        return std::max(std::ceil(tiles / 256) * (3 + stage * rounds), weights / 3.5e6);
+        return std::max(2 + std::ceil(tiles / 256) * (begin + stage * rounds), weights / 3.5e6);
     };
     constexpr double stage64[] = {0.42, 0.48, 0.75}, stage128[] = {0.57, 0.62, 0.9};
-    double best = ring(Form::Ring64, stage64[l]);
+    double best = ring(Form::Ring64, 3, stage64[l]);
     Form form = Form::Ring64;
     auto take = [&](Form f, double time) {
         if (time < best) {
@@ -2055,23 +2066,29 @@ inline Form choose_finished(const TileArgs& a, int width, Lie lie, bool packs, d
             form = f;
         }
     };
-    take(Form::Ring128, ring(Form::Ring128, stage128[l]));
+    take(Form::Ring128, ring(Form::Ring128, 4.5, stage128[l]));
     const double tiles = row_tiles(128) * std::ceil(width / 128.0);
     if (tiles * 256 <= kLaunchThreads) {
         const double one = lie != Lie::Odd ? 0.85 : 1.2, two = lie != Lie::Odd ? 1.15 : 1.5;
         const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
         take(lie != Lie::Odd ? Form::Pieces : Form::Any,
-             std::max(whole * (3 + two * rounds) + (rest == 0 ? 0 : 3 + (rest <= 256 ? one : two) * rounds),
+             std::max(2 + whole * (4 + two * rounds) + (rest == 0 ? 0 : 3.5 + (rest <= 256 ? one : two) * rounds),
                       weights / 3.5e6));
     }
-    if (lie != Lie::Odd) take(Form::Wide, tile_time(Form::Wide, row_tiles, width, a.depth, weights / 3.5e6));
+    if (lie != Lie::Odd) {
+        const double wide = row_tiles(256) * std::ceil(width / 256.0);
+        if (wide * 256 <= kLaunchThreads) {
+            take(Form::Wide, std::max(finished_wide(wide, rounds), weights / 3.5e6));
+        }
+    }
     if (!packs) {
-        const double again = row_tiles(64) / groups;
+        const double again = row_tiles(64) / groups, rows = std::min<double>(few_rows(a), 64.0);
         const double reading = weights / 6.3e6 * std::max(1 + mean / 160, again > 1 ? 1.15 * again : 0.0);
-        const double workgroups = row_tiles(64) * std::ceil(width / 32.0);
-        const double chain = a.depth / 1000.0 * (1 + std::min(mean, 64.0) / 40);
-        take(Form::FewRows, (4 + std::max(reading, std::ceil(workgroups / 512) * chain)) *
-                                (lie == Lie::Pieces ? 1 : lie == Lie::Words ? 1.1 : 2));
+        const double workgroups = row_tiles(64) * std::ceil(width / (gated || groups > 1 ? 32.0 : 16.0));
+        const double ahead = rows <= 32 || workgroups <= 256 ? 1 + rows / 40 : 4.2;
+        take(Form::FewRows,
+             (1.3 + std::max(2 + reading, std::ceil(workgroups / 512) * (3 + a.depth / 1000.0 * ahead))) *
+                 (lie == Lie::Pieces ? 1 : lie == Lie::Words ? 1.1 : 2));
     }
     *time = best;
     return form;
@@ -2197,21 +2214,22 @@ Error launch_finished(const TileArgs& a, Lie lie, hipStream_t stream, const char
         return launch_tiles<T, false, false, E>(part, form, lie, stream, name);
     };
     double best;
-    const Form form = choose_finished(a, width, lie, packs, &best);
+    constexpr bool gated = E == Ends::Gated;
+    const Form form = choose_finished(a, width, gated, lie, packs, &best);
     if (a.offsets == nullptr && lie != Lie::Odd) {
         const int bytes = std::is_same_v<T, Int8Pair> && a.out_type == ElementType::F32 ? 4 : 2;
         const int head = whole_rounds(a.total, 1, width, [&](int rows, bool wide) {
             TileArgs part = a;
             part.total = rows;
             double time;
-            choose_finished(part, width, lie, packs, &time);
-            auto tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge); };
-            return wide ? tile_time(Form::Wide, tiles, width, a.depth, 0) : time;
+            choose_finished(part, width, gated, lie, packs, &time);
+            return wide ? finished_wide(std::ceil(rows / 256.0) * std::ceil(width / 256.0),
+                                        std::ceil(static_cast<double>(a.depth) / kStep)) : time;
         });
         if (head > 0) {
             SPMM_TRY(launch(rows_alone(a, 0, head, bytes), Form::Wide));
             const TileArgs rest = rows_alone(a, head, a.total - head, bytes);
-            return launch(rest, choose_finished(rest, width, lie, packs, &best));
+            return launch(rest, choose_finished(rest, width, gated, lie, packs, &best));
         }
     }
     return launch(a, form);

@@ -109,20 +109,18 @@ def test_layer_and_gradients(S, T, D, H, E, k, over, name, act):
 @pytest.mark.parametrize("T,D,H,E,k,over", SIZES)
 @pytest.mark.parametrize("name", ["f16", "bf16"])
 def test_kept_in_eight_bits(S, T, D, H, E, k, over, name):
-    """The same result, and the gradients that the operators give for what 8 bits hold."""
+    """The result and the gradients that the operators give for what 8 bits hold."""
     dtype = R.TYPES[name]
-    full, x, dy = _layer(T, D, H, E, k, over, dtype, "silu")
-    layer, _, _ = _layer(T, D, H, E, k, over, dtype, "silu", "8bit")
-    for a, b in zip(full.parameters(), layer.parameters()):
-        assert torch.equal(a, b)
+    layer, x, dy = _layer(T, D, H, E, k, over, dtype, "silu", "8bit")
     y = layer(x)
-    assert torch.equal(y, full(x))
     got = torch.autograd.grad(y, [x, layer.router, layer.w_in, layer.w_out], dy)
     with torch.no_grad():
         logits = x.float() @ layer.router.t()
         r = S.route(logits, k, over)
         h, kept = S.gated_mm(S.dispatch(x, r), layer.w_in, r.offsets, keep="8bit")
-        ys = S.unpack8(S.pack8(S.grouped_mm(h, layer.w_out, r.offsets)), dtype)
+        ys = S.grouped_mm(h, layer.w_out, r.offsets)
+        assert torch.equal(y, S.combine(ys, r))
+        ys = S.unpack8(S.pack8(ys), dtype)
         xs = S.dispatch(S.unpack8(S.pack8(x), dtype), r)
         dys, dweights = S.combine_backward(dy, ys, r)
         dlogits = S.route_backward(logits, r, dweights)
