@@ -2029,8 +2029,9 @@ inline double finished_wide(double tiles, double rounds) {
 // estimated time, from measured rates; width: rows of a group's weights, of both projections
 // of a gated one; gated: 16 columns of either a workgroup of few_rows_product.
 //   few_rows_product: weights at 6.3 TB/s, more slowly as the rows' own reading counts and
-//     where a second tile of rows reads them again; 512 workgroups at a time, which take 3 us
-//     and for 1000 steps 1.4 us with 16 rows, 2.6 with 64, 4.2 where those leave no stages
+//     where a second tile of rows reads them again, the rows themselves, which each of its
+//     workgroups reads, at 12; 512 workgroups at a time, which take 3 us
+//     and for 1000 steps 1.4 us with 16 rows, 2.6 with 64, 5.5 where those leave no stages
 //     ahead (2 x 8192 x 4096: 16 rows 27 us, 64 36, 128 59; 2 x 1024 x 2048: 16 rows 5.0, 256
 //     8.6; 8 groups of 2 x 7552 x 304 in integers, 21 rows: 24, 16 in tile_product).  1.1 times
 //     as long for rows that are no whole pieces, twice where they begin between two words.
@@ -2083,9 +2084,10 @@ inline Form choose_finished(const TileArgs& a, int width, bool gated, Lie lie, b
     }
     if (!packs) {
         const double again = row_tiles(64) / groups, rows = std::min<double>(few_rows(a), 64.0);
-        const double reading = weights / 6.3e6 * std::max(1 + mean / 160, again > 1 ? 1.15 * again : 0.0);
+        const double reading = std::max(weights / 6.3e6 * std::max(1 + mean / 160, again > 1 ? 1.15 * again : 0.0),
+                                        a.total / 6e6 * a.depth * (width / 32.0));
         const double workgroups = row_tiles(64) * std::ceil(width / (gated || groups > 1 ? 32.0 : 16.0));
-        const double ahead = rows <= 32 || workgroups <= 256 ? 1 + rows / 40 : 4.2;
+        const double ahead = rows <= 32 || workgroups <= 256 ? 1 + rows / 40 : 5.5;
         take(Form::FewRows,
              (1.3 + std::max(2 + reading, std::ceil(workgroups / 512) * (3 + a.depth / 1000.0 * ahead))) *
                  (lie == Lie::Pieces ? 1 : lie == Lie::Words ? 1.1 : 2));
@@ -2105,7 +2107,7 @@ int whole_rounds(int rows, int groups, int width, F time) {
     const long long high = tiles / 256 * 256 / (groups * col_tiles);  // row tiles a group
     const int head = static_cast<int>(high * 256);
     if (high < 1 || head >= rows) return 0;
-    return time(head, true) + time(rows - head, false) + 2 < 0.96 * time(rows, false) ? head : 0;
+    return time(head, true) + time(rows - head, false) + 2 < 0.93 * time(rows, false) ? head : 0;
 }
 
 // A product's rows [first, first + rows) by themselves, of one group that has all.
