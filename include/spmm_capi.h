@@ -452,9 +452,9 @@ int spmm_c_adapter_mm(const void* d_x, const void* d_w, const void* d_a, const v
  *   d_kept: null, or g and u [rows, 2, width] for the gradients, of the operands' type or,
  *   with d_kept_scales, packed as by pack8 from their fp32 sums.
  * gated_grad: from d_dh [rows, width] and what was kept, d_dkept [rows, 2, width], the
- *   gradients of g and u, and h again in d_h where that is not null.  The gradients of x
- *   and of the weights are grouped_mm (w_in_rows) and grouped_outer of d_dkept as rows of
- *   2 width.
+ *   gradients of g and u, and h again in d_h where that is not null.
+ * gated_mm_backward: from d_dkept the gradients of x, d_dx [rows, depth], and of the weights,
+ *   d_dw as d_w; one that is null is not computed (nor are d_w or d_x read for it).
  * pack8: blocks of 32 values along a row (the last may be shorter) as int8 d_values
  *   [rows, width] and a scale byte each, d_scales [rows, width / 32 rounded up]: the value
  *   is q 2^(scale - 133), scale the exponent byte of the block's largest magnitude in fp32
@@ -476,6 +476,9 @@ int spmm_c_gated_mm(const void* d_x, const void* d_w, int type, const int* d_off
                     void* d_kept_scales, void* stream);
 int spmm_c_gated_grad(const void* d_dh, int type, const void* d_kept, const void* d_kept_scales,
                       int rows, int width, int act, void* d_dkept, void* d_h, void* stream);
+int spmm_c_gated_mm_backward(const void* d_dkept, const void* d_x, const void* d_w, int type,
+                             const int* d_offsets, int groups, int rows, int width, int depth,
+                             void* d_dx, void* d_dw, void* stream);
 int spmm_c_pack8(const void* d_x, int type, long long rows, int width, void* d_values,
                  void* d_scales, void* stream);
 int spmm_c_unpack8(const void* d_values, const void* d_scales, int type, long long rows, int width,

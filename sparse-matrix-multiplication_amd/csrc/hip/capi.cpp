@@ -1134,6 +1134,18 @@ int spmm_c_gated_grad(const void* d_dh, int type, const void* d_kept, const void
     });
 }
 
+int spmm_c_gated_mm_backward(const void* d_dkept, const void* d_x, const void* d_w, int type,
+                             const int* d_offsets, int groups, int rows, int width, int depth,
+                             void* d_dx, void* d_dw, void* stream) {
+    return guarded([&] {
+        spmm::engine::ElementType t;
+        if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
+        return from_engine(spmm::engine::launch_gated_backward(d_dkept, d_x, d_w, t, d_offsets, groups,
+                                                               rows, width, depth, d_dx, d_dw,
+                                                               as_stream(stream)));
+    });
+}
+
 int spmm_c_pack8(const void* d_x, int type, long long rows, int width, void* d_values, void* d_scales,
                  void* stream) {
     return guarded([&] {

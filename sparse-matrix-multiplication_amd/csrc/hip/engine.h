@@ -326,6 +326,12 @@ Error launch_gated_mm(const void* x, const void* w, ElementType type, const int*
 Error launch_gated_grad(const void* dh, ElementType type, const void* kept, const void* kept_scales,
                         int total, int width, Act act, void* dkept, void* h, hipStream_t stream);
 
+// The gradients of x [total, depth] and of W (each null: not computed) from dkept [total, 2,
+// width].
+Error launch_gated_backward(const void* dkept, const void* x, const void* w, ElementType type,
+                            const int* offsets, int groups, int total, int width, int depth, void* dx,
+                            void* dw, hipStream_t stream);
+
 // ---- values in eight bits (eight_bits.hip, int8_mm.hip) -----------------
 // Blocks of 32 along rows with a power-of-two scale (eight_bits.h): values int8 [rows, width]
 // and scales uint8 [rows, width / 32 rounded up].

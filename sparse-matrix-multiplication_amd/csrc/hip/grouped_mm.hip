@@ -156,8 +156,13 @@ Error launch_few_rows(const TileArgs& a, bool pieces, hipStream_t stream, const 
 //     4000 x 4097 30, few_rows_product 43; 12 rows x 1504 x 2057 15, few_rows_product 8.
 //   Rows of whole words that are no pieces: in tiles as those of pieces, or one of 128 x 128 a
 //     CU in a ring (3001 rows in seven groups, 2002 x 1030, W [k][c]: 29 us, 36 in
-//     tile_product).  All have the same sums in the same order as through registers.
-Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie, double* least = nullptr) {
+//     tile_product).  A single group whose rows all know: the ring where there are few tiles of
+//     a long contraction (2000 rows x 1024 x 16384, W [k][c]: 107 us, 150 in tile_product).
+//   These, and tiles through registers, all add a sum's products in one order; few_rows_product
+//     and tile_product_shared have others.  kept: the choice between those three orders is
+//     the one of tile_product, so that a product's sums do not change with what else is built.
+Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie, bool kept,
+                 double* least = nullptr) {
     const double groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     const double mean = a.total / groups;
     const double weights = 2.0 * groups * a.width * a.depth;
@@ -193,31 +198,34 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie, doub
     };
     Form best = pieces ? Form::Pieces : Form::Any;
     if (pieces && time(Form::Wide) < time(best)) best = Form::Wide;
+    Form same = best;  // the fastest of the same order
     if (a.ids == nullptr && lie == Lie::Words) {
-        best = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
-        if (time(Form::Wide) < time(best)) best = Form::Wide;
+        same = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
+        if (time(Form::Wide) < time(same)) same = Form::Wide;
     }
-    // a single group, whose rows all know: the ring where there are few tiles of a long
-    // contraction
     if (a.ids == nullptr && a.offsets == nullptr && lie != Lie::Odd) {
-        if (time(Form::Ring128) < 0.9 * time(best)) best = Form::Ring128;
-        if (time(Form::Ring64) < 0.9 * time(best)) best = Form::Ring64;
+        if (time(Form::Ring128) < 0.9 * time(same)) same = Form::Ring128;
+        if (time(Form::Ring64) < 0.9 * time(same)) same = Form::Ring64;
     }
-    if (time(Form::Shared) < time(best)) best = Form::Shared;
-    if (few_allowed && few <= time(best)) best = Form::FewRows;
-    if (least != nullptr) *least = best == Form::FewRows ? few : time(best);
-    return best;
+    const double tiles = time(kept ? best : same);
+    Form form = time(Form::Shared) < tiles ? Form::Shared : same;
+    if (few_allowed && few <= std::min(tiles, time(Form::Shared))) form = Form::FewRows;
+    if (least != nullptr) *least = form == Form::FewRows ? few : time(form);
+    return form;
 }
 
 }  // namespace
 
-Error launch_grouped_mm(const void* x, const void* w, ElementType type, const int* offsets,
-                        int groups, int total, int width, int depth, bool w_in_rows, void* out,
-                        hipStream_t stream) {
-    SPMM_TRY(check_product(total, groups, width, depth, "grouped_mm"));
+namespace {
+
+// launch_grouped_mm, with the sums in an order that is kept or free.
+Error product(const void* x, const void* w, ElementType type, const int* offsets, int groups, int total,
+              int width, int depth, bool w_in_rows, bool kept, void* out, hipStream_t stream,
+              const char* name) {
+    SPMM_TRY(check_product(total, groups, width, depth, name));
     if (total == 0) return Error{};
     if (x == nullptr || w == nullptr || (offsets == nullptr && groups != 1) || out == nullptr) {
-        return Error{kInvalid, "grouped_mm: null pointer"};
+        return Error{kInvalid, std::string(name) + ": null pointer"};
     }
     TileArgs a{};
     a.rows = x;
@@ -232,39 +240,38 @@ Error launch_grouped_mm(const void* x, const void* w, ElementType type, const in
     a.rows_end = static_cast<const char*>(x) + 2LL * total * depth;
     a.cols_end = static_cast<const char*>(w) + 2LL * groups * width * depth;
     const Lie lie = lie_of(a, depth, w_in_rows ? width : depth);
-    const Form form = choose_form(a, pieces, !w_in_rows, lie);
     auto launch = [&](const TileArgs& part, Form form) {
-        return with_half(type, "grouped_mm", [&](auto zero) {
+        return with_half(type, name, [&](auto zero) {
             using T = decltype(zero);
-            if (form == Form::FewRows) return launch_few_rows<T, Ends::Plain>(part, pieces, stream, "grouped_mm");
-            return w_in_rows ? launch_tiles<T, false, true, Ends::Plain>(part, form, lie, stream, "grouped_mm")
-                             : launch_tiles<T, false, false, Ends::Plain>(part, form, lie, stream, "grouped_mm");
+            if (form == Form::FewRows) return launch_few_rows<T, Ends::Plain>(part, pieces, stream, name);
+            return w_in_rows ? launch_tiles<T, false, true, Ends::Plain>(part, form, lie, stream, name)
+                             : launch_tiles<T, false, false, Ends::Plain>(part, form, lie, stream, name);
         });
     };
-    if (offsets == nullptr && lie != Lie::Odd) {
+    if (!kept && offsets == nullptr && lie != Lie::Odd) {
         const int head = whole_rounds(total, 1, width, [&](int rows, bool wide) {
             TileArgs part = a;
             part.total = rows;
             double time;
-            choose_form(part, pieces, !w_in_rows, lie, &time);
+            choose_form(part, pieces, !w_in_rows, lie, kept, &time);
             auto tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge); };
             return wide ? tile_time(Form::Wide, tiles, width, depth, 0) : time;
         });
         if (head > 0) {
             SPMM_TRY(launch(rows_alone(a, 0, head, 2), Form::Wide));
             const TileArgs rest = rows_alone(a, head, total - head, 2);
-            return launch(rest, choose_form(rest, pieces, !w_in_rows, lie));
+            return launch(rest, choose_form(rest, pieces, !w_in_rows, lie, kept));
         }
     }
-    return launch(a, form);
+    return launch(a, choose_form(a, pieces, !w_in_rows, lie, kept));
 }
 
-Error launch_grouped_outer(const void* p, const void* q, ElementType type, const int* offsets,
-                           int groups, int total, int height, int width, void* out,
-                           hipStream_t stream) {
-    SPMM_TRY(check_product(total, groups, width, height, "grouped_outer"));
+// launch_grouped_outer, likewise.
+Error outer(const void* p, const void* q, ElementType type, const int* offsets, int groups, int total,
+            int height, int width, bool kept, void* out, hipStream_t stream, const char* name) {
+    SPMM_TRY(check_product(total, groups, width, height, name));
     if ((offsets == nullptr && groups != 1) || out == nullptr || (total > 0 && (p == nullptr || q == nullptr))) {
-        return Error{kInvalid, "grouped_outer: null pointer"};
+        return Error{kInvalid, std::string(name) + ": null pointer"};
     }
     TileArgs a{};
     a.rows = p;
@@ -279,19 +286,21 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
     a.rows_end = static_cast<const char*>(p) + 2LL * total * height;
     a.cols_end = static_cast<const char*>(q) + 2LL * total * width;
     const Lie lie = lie_of(a, height, width);
-    // the form with the least time for `rows` of the output's
-    auto choose = [&](int rows, double* least) {
+    // the form with the least time for `rows` of the output's; part: of those that add in one
+    // order, so that an element's sum does not hang on the row it is in
+    auto choose = [&](int rows, bool part, double* least) {
         auto row_tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge) * groups; };
         auto time = [&](Form f) {
             return tile_time(f, row_tiles, width, static_cast<double>(total) / groups, 0);
         };
-        Form form = !pieces ? Form::Any
-                    : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
+        const Form best = !pieces ? Form::Any
+                          : time(Form::Wide) <= time(Form::Pieces) ? Form::Wide : Form::Pieces;
+        Form same = best;
         if (lie == Lie::Words) {
-            form = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
-            if (time(Form::Wide) < time(form)) form = Form::Wide;
+            same = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
+            if (time(Form::Wide) < time(same)) same = Form::Wide;
         }
-        if (time(Form::Shared) < time(form)) form = Form::Shared;
+        const Form form = !part && time(Form::Shared) < time(kept ? best : same) ? Form::Shared : same;
         *least = time(form);
         return form;
     };
@@ -299,20 +308,55 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
         TileArgs part = a;
         part.from = from;
         part.upto = upto;
-        return with_half(type, "grouped_outer", [&](auto zero) {
-            return launch_tiles<decltype(zero), true, true, Ends::Plain>(part, form, lie, stream, "grouped_outer");
+        return with_half(type, name, [&](auto zero) {
+            return launch_tiles<decltype(zero), true, true, Ends::Plain>(part, form, lie, stream, name);
         });
     };
     double least;
-    const int head = lie == Lie::Odd ? 0 : whole_rounds(height, groups, width, [&](int rows, bool wide) {
-        auto row_tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge) * groups; };
-        if (wide) return tile_time(Form::Wide, row_tiles, width, static_cast<double>(total) / groups, 0);
-        choose(rows, &least);
-        return least;
-    });
-    if (head > 0) SPMM_TRY(launch(0, head, Form::Wide));
-    const Form form = choose(height - head, &least);
+    Form form = choose(height, false, &least);
+    int head = 0;
+    if (lie != Lie::Odd && form != Form::Shared) {
+        head = whole_rounds(height, groups, width, [&](int rows, bool wide) {
+            auto row_tiles = [&](int edge) { return std::ceil(static_cast<double>(rows) / edge) * groups; };
+            if (wide) return tile_time(Form::Wide, row_tiles, width, static_cast<double>(total) / groups, 0);
+            choose(rows, true, &least);
+            return least;
+        });
+    }
+    if (head > 0) {
+        SPMM_TRY(launch(0, head, Form::Wide));
+        form = choose(height - head, true, &least);
+    }
     return launch(head, height, form);
+}
+
+}  // namespace
+
+Error launch_grouped_mm(const void* x, const void* w, ElementType type, const int* offsets,
+                        int groups, int total, int width, int depth, bool w_in_rows, void* out,
+                        hipStream_t stream) {
+    return product(x, w, type, offsets, groups, total, width, depth, w_in_rows, true, out, stream,
+                   "grouped_mm");
+}
+
+Error launch_grouped_outer(const void* p, const void* q, ElementType type, const int* offsets,
+                           int groups, int total, int height, int width, void* out,
+                           hipStream_t stream) {
+    return outer(p, q, type, offsets, groups, total, height, width, true, out, stream, "grouped_outer");
+}
+
+Error launch_gated_backward(const void* dkept, const void* x, const void* w, ElementType type,
+                            const int* offsets, int groups, int total, int width, int depth, void* dx,
+                            void* dw, hipStream_t stream) {
+    const char* name = "gated_mm_backward";
+    if (width > 0x3fffffff) return Error{kUnsupported, std::string(name) + ": rows over 2^22 elements"};
+    if (dx != nullptr) {
+        SPMM_TRY(product(dkept, w, type, offsets, groups, total, depth, 2 * width, true, false, dx, stream, name));
+    }
+    if (dw != nullptr) {
+        SPMM_TRY(outer(dkept, x, type, offsets, groups, total, 2 * width, depth, false, dw, stream, name));
+    }
+    return Error{};
 }
 
 long long adapter_workspace(long long total, int rank) {
@@ -348,7 +392,7 @@ Error launch_adapter_mm(const void* x, const void* w, const void* down, const vo
     a.rank16 = (rank + 15) / 16 * 16;
     const bool pieces = depth % 8 == 0 && aligned16(x) && aligned16(w);
     a.b_pieces = rank % 8 == 0 && aligned16(up);
-    const Form form = choose_form(a, pieces, true, Lie::Pieces);
+    const Form form = choose_form(a, pieces, true, Lie::Pieces, true);
     return with_half(type, "adapter_mm", [&](auto zero) {
         using T = decltype(zero);
         const bool whole = pieces && aligned16(down);

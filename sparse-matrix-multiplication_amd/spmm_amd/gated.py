@@ -21,7 +21,7 @@ import torch
 
 from . import SPMM_INVALID, SPMM_UNSUPPORTED, SpmmError, _check, lib
 from .experts import (_FLOAT, _INT, _TYPES, _counts, _half, _on, _operand, _out, _refuse,
-                      _stream, grouped_mm)
+                      _stream)
 
 _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 _BYTES = (torch.int8,)
@@ -292,15 +292,13 @@ def gated_mm_backward(dh, x, w, kept, offsets=None, act: str = "silu", stream=No
         _check(L.spmm_c_gated_grad(dh.data_ptr(), _TYPES[dtype], values.data_ptr(),
                                    kept.scales.data_ptr() if packed else None, S, N, act_id,
                                    dkept.data_ptr(), None if h is None else h.data_ptr(), s))
-        dx = dw = None
-        if rows:
-            dx = torch.empty((S, K), dtype=dtype, device=device)
-            _check(L.spmm_c_grouped_mm(dkept.data_ptr(), w.data_ptr(), _TYPES[dtype], at, G, S, K,
-                                       2 * N, 1, dx.data_ptr(), s))
-        if weights:
-            if isinstance(x, Packed8):
-                x = unpack8(x, dtype)
-            dw = torch.empty_like(w)
-            _check(L.spmm_c_grouped_outer(dkept.data_ptr(), x.data_ptr(), _TYPES[dtype], at, G, S,
-                                          2 * N, K, dw.data_ptr(), s))
+        dx = torch.empty((S, K), dtype=dtype, device=device) if rows else None
+        dw = torch.empty_like(w) if weights else None
+        if weights and isinstance(x, Packed8):
+            x = unpack8(x, dtype)
+        if rows or weights:
+            _check(L.spmm_c_gated_mm_backward(dkept.data_ptr(), x.data_ptr() if weights else None,
+                                              w.data_ptr(), _TYPES[dtype], at, G, S, N, K,
+                                              dx.data_ptr() if rows else None,
+                                              dw.data_ptr() if weights else None, s))
     return (dx, dw, h) if hidden else (dx, dw)

@@ -323,6 +323,14 @@ def test_c_entries_refuse_bad_arguments(S):
     assert grad(dh=None) == grad(kept=None) == grad(dkept=None) == grad(act=9) == grad(type=3) == bad
     assert grad(rows=-1) == grad(width=0) == bad
     assert grad(type=0) == grad(width=1 << 23) == not_here
+    back = lambda **k: L.spmm_c_gated_mm_backward(*{**dict(  # noqa: E731
+        dkept=some, x=some, w=some, type=1, offsets=some, groups=2, rows=4, width=8, depth=8, dx=some,
+        dw=some, stream=None), **k}.values())
+    assert back(dkept=None) == back(w=None) == back(offsets=None) == back(type=9) == bad
+    assert back(dx=None, x=None) == back(rows=-1) == back(width=0) == back(groups=0) == bad
+    assert back(type=0) == back(depth=1 << 23) == back(width=top) == back(width=1 << 22) == not_here
+    assert back(groups=many, rows=many) == back(groups=many, rows=many, dx=None) == not_here
+    assert back(dx=None, dw=None) == S.SPMM_OK
     for f in (lambda **k: L.spmm_c_pack8(*{**dict(x=some, type=0, rows=4, width=8, values=some,
                                                  scales=some, stream=None), **k}.values()),
               lambda **k: L.spmm_c_unpack8(*{**dict(values=some, scales=some, type=0, rows=4, width=8,
