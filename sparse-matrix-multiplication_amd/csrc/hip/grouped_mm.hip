@@ -203,7 +203,7 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie, bool
         same = time(Form::Pieces) < 0.9 * time(Form::Ring128) ? Form::Pieces : Form::Ring128;
         if (time(Form::Wide) < time(same)) same = Form::Wide;
     }
-    if (a.ids == nullptr && a.offsets == nullptr && lie != Lie::Odd) {
+    if (!kept && a.offsets == nullptr && lie != Lie::Odd) {  // W [k][c]
         if (time(Form::Ring128) < 0.9 * time(same)) same = Form::Ring128;
         if (time(Form::Ring64) < 0.9 * time(same)) same = Form::Ring64;
     }
@@ -218,7 +218,7 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie, bool
 
 namespace {
 
-// launch_grouped_mm, with the sums in an order that is kept or free.
+// launch_grouped_mm, with the sums in an order that is kept, or free (W [k][c] alone).
 Error product(const void* x, const void* w, ElementType type, const int* offsets, int groups, int total,
               int width, int depth, bool w_in_rows, bool kept, void* out, hipStream_t stream,
               const char* name) {

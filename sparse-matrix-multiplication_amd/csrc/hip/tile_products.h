@@ -2174,7 +2174,7 @@ Error launch_tiles(const TileArgs& a, Form form, Lie lie, hipStream_t stream, co
         }
     } else {
         if constexpr (E == Ends::Plain) {
-            if constexpr (!GRAD) {
+            if constexpr (!GRAD && COLS_MAJOR) {
                 if (form == Form::Ring64) {
                     return lie == Lie::Words
                         ? launch_ring<T, GRAD, COLS_MAJOR, E, Lie::Words, 2>(a, blocks, stream, name)
