@@ -204,7 +204,8 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie, bool
         if (time(Form::Wide) < time(same)) same = Form::Wide;
     }
     if (!kept && a.offsets == nullptr && lie != Lie::Odd) {  // W [k][c]
-        if (time(Form::Ring128) < 0.9 * time(same)) same = Form::Ring128;
+        // as many rounds of tiles in the ring, which is further ahead of memory
+        if (same == Form::Pieces && time(Form::Ring128) < 1.05 * time(same)) same = Form::Ring128;
         if (time(Form::Ring64) < 0.9 * time(same)) same = Form::Ring64;
     }
     const double tiles = time(kept ? best : same);

@@ -9,7 +9,7 @@ import expert_reference as R  # noqa: E402
 import gated_reference as G  # noqa: E402
 
 SHAPES = [(1, 1), (1, 8), (3, 7), (2, 31), (5, 32), (4, 33), (7, 64), (3, 100), (2, 5, 48), (61, 1000),
-          (9, 2047), (6, 2050), (4, 8192), (2, 8200), (1, 40000), (1000, 17), (64,)]
+          (9, 2047), (6, 2050), (4, 8192), (2, 8200), (1, 40000), (1000, 17), (64,), (600, 2056)]
 
 
 def _values(shape, dtype, seed, scale=1.0):
