@@ -271,7 +271,8 @@ Error product(const void* x, const void* w, ElementType type, const int* offsets
 Error outer(const void* p, const void* q, ElementType type, const int* offsets, int groups, int total,
             int height, int width, bool kept, void* out, hipStream_t stream, const char* name) {
     SPMM_TRY(check_product(total, groups, width, height, name));
-    if ((offsets == nullptr && groups != 1) || out == nullptr || (total > 0 && (p == nullptr || q == nullptr))) {
+    if ((offsets == nullptr && groups != 1) || out == nullptr ||
+        (total > 0 && (p == nullptr || q == nullptr))) {
         return Error{kInvalid, std::string(name) + ": null pointer"};
     }
     TileArgs a{};
@@ -352,7 +353,8 @@ Error launch_gated_backward(const void* dkept, const void* x, const void* w, Ele
     const char* name = "gated_mm_backward";
     if (width > 0x3fffffff) return Error{kUnsupported, std::string(name) + ": rows over 2^22 elements"};
     if (dx != nullptr) {
-        SPMM_TRY(product(dkept, w, type, offsets, groups, total, depth, 2 * width, true, false, dx, stream, name));
+        SPMM_TRY(product(dkept, w, type, offsets, groups, total, depth, 2 * width, true, false, dx,
+                         stream, name));
     }
     if (dw != nullptr) {
         SPMM_TRY(outer(dkept, x, type, offsets, groups, total, 2 * width, depth, false, dw, stream, name));

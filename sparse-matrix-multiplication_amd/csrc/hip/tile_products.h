@@ -700,10 +700,10 @@ __device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, 
 
 // The gated and the scaled stores of a wave's tile, B sixteens of rows at a time through its
 // own part of LDS (one at a time, each waits for its own way through LDS and for its own
-// functions: 20800 rows x 2 x 3776 x
-// 128 in 256 x 256 tiles 208 us, 136 so).  Gated, the first half of a row's
-// sums are the gates and the second half what they multiply, of the same kCols columns; a
-// lane takes eight columns of both, four lanes a block of 32 for packing.
+// functions: 20800 rows x 2 x 3776 x 128 in 256 x 256 tiles 208 us, 136 with four).  Gated,
+// the first half of a row's sums are the gates and the second half what they multiply, of
+// the same kCols columns; a lane takes eight columns of both, four lanes a block of 32 for
+// packing.
 template <typename T, int CF, bool GATED, int B>
 struct FinishTile {
     static constexpr bool kScaled = std::is_same_v<T, Int8Pair>;
@@ -1053,10 +1053,10 @@ __global__ __launch_bounds__(256, L == Lie::Odd ? 2 : 1) void tile_product(TileA
 // rows 136, 287.
 template <typename T, bool GRAD, bool COLS_MAJOR, Ends E>
 __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
-    constexpr bool GATED = E == Ends::Gated;
-    constexpr int BR = 64, BC = 64, WC = 2, RF = 2, CF = 2, GROUPS = 4, OUT = GATED ? BC / 2 : BC;
+    static_assert(kPlainEnds<T, E>);
+    constexpr int BR = 64, BC = 64, WC = 2, RF = 2, CF = 2, GROUPS = 4;
     using Rows = Operands<T, BR, GRAD, 256>;
-    using Cols = Operands<T, BC, GRAD || COLS_MAJOR, 256, GATED ? 2 : 1>;
+    using Cols = Operands<T, BC, GRAD || COLS_MAJOR, 256>;
     extern __shared__ __attribute__((aligned(16))) char s_tiles[];
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int wave  = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
@@ -1065,31 +1065,26 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
     auto cols_at = [&](int it) { return rows_at(it) + BR * kStep; };
     const int wr = wave / WC, wc = wave % WC;
     Tile<T> t;
-    if (!take_tile<T, BR, OUT, GRAD, COLS_MAJOR, GATED>(a, t)) return;
-    if constexpr (!kPlainEnds<T, E>) {
-        if (t.depth == 0) return finish_zeros<OUT, T, GATED>(a, t);
-    }
+    if (!take_tile<T, BR, BC, GRAD, COLS_MAJOR>(a, t)) return;
 
     Sums<T> acc[CF][RF];
 #pragma unroll
     for (int j = 0; j < CF; ++j)
 #pragma unroll
         for (int i = 0; i < RF; ++i) acc[j][i] = Sums<T>(0);
-    const int r0 = wr * RF * 16, c0 = t.c0 + wc * (OUT / WC);
-    auto column = [&](int j) { return GATED ? j * (BC / 2) + wc * 16 : (wc * CF + j) * 16; };
+    const int r0 = wr * RF * 16, c0 = t.c0 + wc * (BC / WC);
     // all groups go through as many turns: past the end there are zeros
     const int turns = (t.depth + GROUPS * kStep - 1) / (GROUPS * kStep);
     Rows pr;
     Cols pc;
     pr.place(t.rows, t.ld_rows, t.rows_here);
-    pc.place(t.cols, t.ld_cols, a.width - t.c0, GATED ? t.second : nullptr);
+    pc.place(t.cols, t.ld_cols, a.width - t.c0);
     WordPiece vr[Rows::kPieces], vc[Cols::kPieces];
     auto run = [&](auto odd) {
         auto load = [&](int it) {
             const int n = it * GROUPS + group, left = t.depth - n * kStep;
             pr.template load<odd.value>(t.rows + n * t.step_rows, left, vr);
-            pc.template load<odd.value>(t.cols + n * t.step_cols, left, vc,
-                                            GATED ? t.second + n * t.step_cols : nullptr);
+            pc.template load<odd.value>(t.cols + n * t.step_cols, left, vc);
         };
         auto store = [&](int it) {
             const int left = t.depth - (it * GROUPS + group) * kStep;
@@ -1107,7 +1102,7 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
 #pragma unroll
                 for (int i = 0; i < RF; ++i) fr[i] = Rows::read(rows_at(it), (wr * RF + i) * 16, half);
 #pragma unroll
-                for (int j = 0; j < CF; ++j) fc[j] = Cols::read(cols_at(it), column(j), half);
+                for (int j = 0; j < CF; ++j) fc[j] = Cols::read(cols_at(it), (wc * CF + j) * 16, half);
 #pragma unroll
                 for (int j = 0; j < CF; ++j)
 #pragma unroll
@@ -1117,7 +1112,6 @@ __global__ __launch_bounds__(1024) void tile_product_shared(TileArgs a) {
         }
     };
     const uintptr_t ends = reinterpret_cast<uintptr_t>(t.rows) | reinterpret_cast<uintptr_t>(t.cols) |
-                           (GATED ? reinterpret_cast<uintptr_t>(t.second) : 0) |
                            static_cast<uintptr_t>(t.ld_rows | t.ld_cols) * 2;
     if (turns > 0) {
         if ((ends & 2) != 0) run(std::true_type{});
@@ -1947,12 +1941,12 @@ long long few_rows(const TileArgs& a) {
     const long long groups = a.offsets == nullptr ? 1 : std::min(a.groups, a.total);
     return groups == 1 ? a.total : 2LL * a.total / groups;
 }
-// How few_rows_product is launched for gated products and for those in 8-bit integers: four waves and two workgroups a
-// CU with sixteen columns of either projection, or 32 (rows of integers are half as long, and
-// the rows' own reading counts twice as much: 64 groups of 2048 x 4096, 256 rows 93 us, 107
-// with sixteen columns; a single group has the workgroups to hide that: 8192 x 8192, 16 rows
-// 15.4, 19.9 with 32).  All of the LDS where a gated product has one workgroup a CU and its
-// rows leave no stages else (2 x 1024 x 4096, 64 rows: 15 us, 20).
+// How few_rows_product is launched for gated products and for those in 8-bit integers: four
+// waves and two workgroups a CU with sixteen columns of either projection, or 32 (rows of
+// integers are half as long, and the rows' own reading counts twice as much: 64 groups of
+// 2048 x 4096, 256 rows 93 us, 107 with sixteen columns; a single group has the workgroups to
+// hide that: 8192 x 8192, 16 rows 15.4, 19.9 with 32).  All of the LDS where there is one
+// workgroup a CU and its rows leave no stages else (gated, 2 x 1024 x 4096, 64 rows: 15 us, 20).
 template <typename T, Ends E>
 Error launch_few_finished(const TileArgs& a, bool pieces, hipStream_t stream, const char* name) {
     constexpr int kTwo = 80 * 1024, kAll = 160 * 1024;
@@ -1989,7 +1983,9 @@ constexpr int rows_of(Form form) { return form == Form::Ring64 ? 64 : edge_of(fo
 // Estimated microseconds of a form for `row_tiles(edge)` x width tiles of `steps`
 // steps, from measured rates: 64 steps of a 128 x 128 tile take 0.62 us where a CU has
 // one and 0.95 us where it has two (through registers 1 and 1.5 us), of a 256 x 256 tile
-// 1.55 us, one a CU, and 256 steps of a 64 x 64 tile 1.1 us, one a CU; `weights` microseconds is what reading the weights takes.
+// 1.55 us, one a CU, and 256 steps of a 64 x 64 tile 1.1 us, one a CU; of the ring's tiles,
+// one a CU, 64 steps of 64 x 128 take 0.48 us and of 128 x 128 0.62; `weights` microseconds is
+// what reading the weights takes.
 template <typename F>
 double tile_time(Form form, F row_tiles, int width, double steps, double weights) {
     const int edge = edge_of(form);
@@ -2006,7 +2002,8 @@ double tile_time(Form form, F row_tiles, int width, double steps, double weights
         return std::max(std::ceil(tiles / 256) * (3 + 0.62 * rounds), weights);
     }
     if (form == Form::Ring64) {  // row_tiles counts its rows
-        return std::max(std::ceil(row_tiles(64) * std::ceil(width / 128.0) / 256) * (3 + 0.48 * rounds), weights);
+        const double low = row_tiles(64) * std::ceil(width / 128.0);
+        return std::max(std::ceil(low / 256) * (3 + 0.48 * rounds), weights);
     }
     const double two = form == Form::Any ? 1.5 : 0.95, one = form == Form::Any ? 1 : 0.62;
     const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
@@ -2054,7 +2051,8 @@ inline Form choose_finished(const TileArgs& a, int width, bool gated, Lie lie, b
     auto ring = [&](Form f, double begin, double stage) {
         const double high = row_tiles(rows_of(f));
         // a few tiles more than groups have on average may be another round
-        const double tiles = high * std::ceil(width / 128.0) * (1 + (groups == 1 ? 0 : std::min(0.1, 0.3 * groups / high)));
+        const double more = groups == 1 ? 0 : std::min(0.1, 0.3 * groups / high);
+        const double tiles = high * std::ceil(width / 128.0) * (1 + more);
         if (tiles * 256 > kLaunchThreads) return HUGE_VAL;
         return std::max(2 + std::ceil(tiles / 256) * (begin + stage * rounds), weights / 3.5e6);
     };
@@ -2073,7 +2071,8 @@ inline Form choose_finished(const TileArgs& a, int width, bool gated, Lie lie, b
         const double one = lie != Lie::Odd ? 0.85 : 1.2, two = lie != Lie::Odd ? 1.15 : 1.5;
         const double whole = std::floor(tiles / 512), rest = tiles - 512 * whole;
         take(lie != Lie::Odd ? Form::Pieces : Form::Any,
-             std::max(2 + whole * (4 + two * rounds) + (rest == 0 ? 0 : 3.5 + (rest <= 256 ? one : two) * rounds),
+             std::max(2 + whole * (4 + two * rounds) +
+                          (rest == 0 ? 0 : 3.5 + (rest <= 256 ? one : two) * rounds),
                       weights / 3.5e6));
     }
     if (lie != Lie::Odd) {
@@ -2084,8 +2083,8 @@ inline Form choose_finished(const TileArgs& a, int width, bool gated, Lie lie, b
     }
     if (!packs) {
         const double again = row_tiles(64) / groups, rows = std::min<double>(few_rows(a), 64.0);
-        const double reading = std::max(weights / 6.3e6 * std::max(1 + mean / 160, again > 1 ? 1.15 * again : 0.0),
-                                        a.total / 6e6 * a.depth * (width / 32.0));
+        const double slower = std::max(1 + mean / 160, again > 1 ? 1.15 * again : 0.0);
+        const double reading = std::max(weights / 6.3e6 * slower, a.total / 6e6 * a.depth * (width / 32.0));
         const double workgroups = row_tiles(64) * std::ceil(width / (gated || groups > 1 ? 32.0 : 16.0));
         const double ahead = rows <= 32 || workgroups <= 256 ? 1 + rows / 40 : 5.5;
         take(Form::FewRows,
@@ -2121,7 +2120,8 @@ inline TileArgs rows_alone(const TileArgs& all, int first, int rows, int out_byt
     if (all.kept != nullptr) {
         const bool packed = all.kept_scales != nullptr;
         a.kept = const_cast<char*>(later(all.kept, 2LL * all.width * (packed ? 1 : 2)));
-        if (packed) a.kept_scales = all.kept_scales + first * (2LL * ((all.width + kPackBlock - 1) / kPackBlock));
+        const long long line = 2LL * ((all.width + kPackBlock - 1) / kPackBlock);
+        if (packed) a.kept_scales = all.kept_scales + first * line;
     }
     return a;
 }
