@@ -166,7 +166,7 @@ class ExpertLayer(torch.nn.Module):
     def __init__(self, width: int, hidden: int, experts: int, k: int, over: str = "chosen",
                  dtype=torch.bfloat16, device="cuda", gated=None, keep: str = "full"):
         super().__init__()
-        if gated is not None and gated not in _ACTS:
+        if gated is not None and (not isinstance(gated, str) or gated not in _ACTS):
             raise SpmmError(SPMM_INVALID, f"gated: {gated!r}, expected None or one of {sorted(_ACTS)}")
         if keep not in ("full", "8bit"):
             raise SpmmError(SPMM_INVALID, f"keep: {keep!r}, expected 'full' or '8bit'")

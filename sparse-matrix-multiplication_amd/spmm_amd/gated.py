@@ -75,7 +75,7 @@ def _padded(width: int) -> int:
 
 
 def _act_id(act) -> int:
-    if act not in _ACTS:
+    if not isinstance(act, str) or act not in _ACTS:
         raise SpmmError(SPMM_INVALID, f"act: {act!r}, expected one of {sorted(_ACTS)}")
     return _ACTS[act]
 

@@ -249,7 +249,8 @@ def test_refusals(S):
     p8 = S.pack8(kept)
     q, qw, qp = S.quantize_rows(x), S.quantize_rows(w[0]), S.quantize_rows(pair)
     byte = torch.empty(6 * 16 + 1, dtype=torch.int8, device="cuda")[1:].view(6, 16)
-    bad = [lambda: S.gated_mm(x, w, act="relu"), lambda: S.gated_mm(x, w, keep="4bit"),
+    bad = [lambda: S.gated_mm(x, w, act="relu"), lambda: S.gated_mm(x, w, act=["silu"]),
+           lambda: S.gated_mm(x, w, keep="4bit"),
            lambda: S.gated_mm(x, w[0]), lambda: S.gated_mm(x, pair), lambda: S.gated_mm(x, w, offsets),
            lambda: S.gated_mm(x, pair, offsets[:2]), lambda: S.gated_mm(x, pair, offsets.long()),
            lambda: S.gated_mm(x, h(3, 4, 8)), lambda: S.gated_mm(x, h(2, 4, 9)),

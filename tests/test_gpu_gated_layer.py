@@ -214,6 +214,6 @@ def test_command_line_refuses():
 
 def test_layer_refuses(S):
     from spmm_amd.expert_layer import ExpertLayer
-    for bad in ({"gated": "relu"}, {"gated": "silu", "keep": "none"}, {"keep": "8bit"}):
+    for bad in ({"gated": "relu"}, {"gated": ["silu"]}, {"gated": "silu", "keep": "none"}, {"keep": "8bit"}):
         with pytest.raises(S.SpmmError):
             ExpertLayer(8, 8, 2, 1, device="cpu", **bad)
