@@ -455,6 +455,11 @@ int spmm_c_adapter_mm(const void* d_x, const void* d_w, const void* d_a, const v
  *   gradients of g and u, and h again in d_h where that is not null.
  * gated_mm_backward: from d_dkept the gradients of x, d_dx [rows, depth], and of the weights,
  *   d_dw as d_w; one that is null is not computed (nor are d_w or d_x read for it).
+ * gated_grad_scaled, gated_mm_backward_scaled: both for fp16, whose range products of two and
+ *   three numbers pass where the sums of them need not.  d_row_scales [rows], out and in: row s
+ *   of d_dkept is the gradients times 1 / d_row_scales[s], a power of two for the row's
+ *   largest magnitude.  d_dw brings rows to one scale a group: d_dkept is overwritten, and
+ *   d_workspace holds as many floats as groups (null without d_dw).
  * pack8: blocks of 32 values along a row (the last may be shorter) as int8 d_values
  *   [rows, width] and a scale byte each, d_scales [rows, width / 32 rounded up]: the value
  *   is q 2^(scale - 133), scale the exponent byte of the block's largest magnitude in fp32
@@ -479,6 +484,13 @@ int spmm_c_gated_grad(const void* d_dh, int type, const void* d_kept, const void
 int spmm_c_gated_mm_backward(const void* d_dkept, const void* d_x, const void* d_w, int type,
                              const int* d_offsets, int groups, int rows, int width, int depth,
                              void* d_dx, void* d_dw, void* stream);
+int spmm_c_gated_grad_scaled(const void* d_dh, const void* d_kept, const void* d_kept_scales,
+                             int rows, int width, int act, void* d_dkept, float* d_row_scales,
+                             void* d_h, void* stream);
+int spmm_c_gated_mm_backward_scaled(void* d_dkept, const float* d_row_scales, const void* d_x,
+                                    const void* d_w, const int* d_offsets, int groups, int rows,
+                                    int width, int depth, void* d_dx, void* d_dw,
+                                    float* d_workspace, void* stream);
 int spmm_c_pack8(const void* d_x, int type, long long rows, int width, void* d_values,
                  void* d_scales, void* stream);
 int spmm_c_unpack8(const void* d_values, const void* d_scales, int type, long long rows, int width,

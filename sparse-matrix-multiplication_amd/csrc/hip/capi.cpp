@@ -1140,9 +1140,34 @@ int spmm_c_gated_mm_backward(const void* d_dkept, const void* d_x, const void* d
     return guarded([&] {
         spmm::engine::ElementType t;
         if (!element_type(type, &t)) return set_error(SPMM_INVALID, "unknown element type");
-        return from_engine(spmm::engine::launch_gated_backward(d_dkept, d_x, d_w, t, d_offsets, groups,
-                                                               rows, width, depth, d_dx, d_dw,
-                                                               as_stream(stream)));
+        // without scales dkept is only read
+        return from_engine(spmm::engine::launch_gated_backward(const_cast<void*>(d_dkept), nullptr, d_x, d_w,
+                                                               t, d_offsets, groups, rows, width, depth,
+                                                               d_dx, d_dw, nullptr, as_stream(stream)));
+    });
+}
+
+int spmm_c_gated_grad_scaled(const void* d_dh, const void* d_kept, const void* d_kept_scales, int rows,
+                             int width, int act, void* d_dkept, float* d_row_scales, void* d_h,
+                             void* stream) {
+    return guarded([&] {
+        return from_engine(spmm::engine::launch_gated_grad_scaled(
+            d_dh, d_kept, d_kept_scales, rows, width, static_cast<spmm::engine::Act>(act), d_dkept,
+            d_row_scales, d_h, as_stream(stream)));
+    });
+}
+
+int spmm_c_gated_mm_backward_scaled(void* d_dkept, const float* d_row_scales, const void* d_x,
+                                    const void* d_w, const int* d_offsets, int groups, int rows,
+                                    int width, int depth, void* d_dx, void* d_dw, float* d_workspace,
+                                    void* stream) {
+    return guarded([&] {
+        if (rows > 0 && d_row_scales == nullptr) {
+            return set_error(SPMM_INVALID, "gated_mm_backward: null pointer");
+        }
+        return from_engine(spmm::engine::launch_gated_backward(
+            d_dkept, d_row_scales, d_x, d_w, spmm::engine::ElementType::F16, d_offsets, groups, rows, width,
+            depth, d_dx, d_dw, d_workspace, as_stream(stream)));
     });
 }
 

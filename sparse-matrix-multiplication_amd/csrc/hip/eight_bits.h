@@ -33,6 +33,20 @@ __device__ __forceinline__ unsigned quad_max(unsigned v) {
     v = max(v, dpp<0xB1>(0u, v));  // lanes 1 0 3 2
     return max(v, dpp<0x4E>(0u, v));  // lanes 2 3 0 1
 }
+// The largest magnitude's bits over a workgroup of WAVES waves.
+template <int WAVES>
+__device__ __forceinline__ unsigned group_max(unsigned v) {
+    v = wave_max(v);
+    if constexpr (WAVES > 1) {
+        __shared__ unsigned s_most[WAVES];
+        if ((threadIdx.x & 63) == 0) s_most[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = s_most[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v = max(v, s_most[w]);
+    }
+    return v;
+}
 __device__ __forceinline__ unsigned pack_scale(unsigned largest) {
     return largest >= 0x7f800000u ? kPackNone : max(largest >> 23, kPackLeast);
 }

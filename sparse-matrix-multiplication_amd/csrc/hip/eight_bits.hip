@@ -59,21 +59,6 @@ __global__ __launch_bounds__(256) void unpack_blocks(const signed char* __restri
     store_eight(out + at, f, count);
 }
 
-// The largest magnitude's bits over a workgroup of WAVES waves.
-template <int WAVES>
-__device__ __forceinline__ unsigned group_max(unsigned v) {
-    v = wave_max(v);
-    if constexpr (WAVES > 1) {
-        __shared__ unsigned s_most[WAVES];
-        if ((threadIdx.x & 63) == 0) s_most[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = s_most[0];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) v = max(v, s_most[w]);
-    }
-    return v;
-}
-
 // A workgroup takes a row: its first kHeld eights a thread stay in registers between the
 // maximum and the rounding, the rest is read again.  16 rows of 8192 2.7 us with sixteen
 // waves, 4.2 with four; 8192 rows 31, 6.5 TB/s; 65536 rows of 256 18, bound by the chain of a

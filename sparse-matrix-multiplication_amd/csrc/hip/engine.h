@@ -326,11 +326,21 @@ Error launch_gated_mm(const void* x, const void* w, ElementType type, const int*
 Error launch_gated_grad(const void* dh, ElementType type, const void* kept, const void* kept_scales,
                         int total, int width, Act act, void* dkept, void* h, hipStream_t stream);
 
+// The same in fp16 with row s of the gradients times 1 / row_scales[s], a power of two that
+// brings them into fp16's range.
+Error launch_gated_grad_scaled(const void* dh, const void* kept, const void* kept_scales, int total,
+                               int width, Act act, void* dkept, float* row_scales, void* h,
+                               hipStream_t stream);
+
 // The gradients of x [total, depth] and of W (each null: not computed) from dkept [total, 2,
-// width].
-Error launch_gated_backward(const void* dkept, const void* x, const void* w, ElementType type,
-                            const int* offsets, int groups, int total, int width, int depth, void* dx,
-                            void* dw, hipStream_t stream);
+// width].  row_scales: dkept's, or null; with them for the gradient of W the rows of dkept are
+// brought to one scale a group, in place, and workspace holds as many floats as groups.
+Error launch_gated_backward(void* dkept, const float* row_scales, const void* x, const void* w,
+                            ElementType type, const int* offsets, int groups, int total, int width,
+                            int depth, void* dx, void* dw, float* workspace, hipStream_t stream);
+// That step, for rows of `elements`.
+Error launch_common_scales(void* rows, const float* row_scales, const int* offsets, int groups, int total,
+                           long long elements, float* group_scales, hipStream_t stream);
 
 // ---- values in eight bits (eight_bits.hip, int8_mm.hip) -----------------
 // Blocks of 32 along rows with a power-of-two scale (eight_bits.h): values int8 [rows, width]

@@ -220,9 +220,10 @@ Form choose_form(const TileArgs& a, bool pieces, bool few_allowed, Lie lie, bool
 namespace {
 
 // launch_grouped_mm, with the sums in an order that is kept, or free (W [k][c] alone).
+// row_scales: null, or what the rows of fp16 sums are multiplied by (W [k][c] alone).
 Error product(const void* x, const void* w, ElementType type, const int* offsets, int groups, int total,
               int width, int depth, bool w_in_rows, bool kept, void* out, hipStream_t stream,
-              const char* name) {
+              const char* name, const float* row_scales = nullptr) {
     SPMM_TRY(check_product(total, groups, width, depth, name));
     if (total == 0) return Error{};
     if (x == nullptr || w == nullptr || (offsets == nullptr && groups != 1) || out == nullptr) {
@@ -237,6 +238,7 @@ Error product(const void* x, const void* w, ElementType type, const int* offsets
     a.total = total;
     a.width = width;
     a.depth = depth;
+    a.row_scales = row_scales;
     const bool pieces = depth % 8 == 0 && (!w_in_rows || width % 8 == 0) && aligned16(x) && aligned16(w);
     a.rows_end = static_cast<const char*>(x) + 2LL * total * depth;
     a.cols_end = static_cast<const char*>(w) + 2LL * groups * width * depth;
@@ -245,6 +247,11 @@ Error product(const void* x, const void* w, ElementType type, const int* offsets
         return with_half(type, name, [&](auto zero) {
             using T = decltype(zero);
             if (form == Form::FewRows) return launch_few_rows<T, Ends::Plain>(part, pieces, stream, name);
+            if constexpr (std::is_same_v<T, _Float16>) {
+                if (row_scales != nullptr) {
+                    return launch_tiles<T, false, true, Ends::Scaled>(part, form, lie, stream, name);
+                }
+            }
             return w_in_rows ? launch_tiles<T, false, true, Ends::Plain>(part, form, lie, stream, name)
                              : launch_tiles<T, false, false, Ends::Plain>(part, form, lie, stream, name);
         });
@@ -267,9 +274,10 @@ Error product(const void* x, const void* w, ElementType type, const int* offsets
     return launch(a, choose_form(a, pieces, !w_in_rows, lie, kept));
 }
 
-// launch_grouped_outer, likewise.
+// launch_grouped_outer, likewise; group_scales: what the groups' fp16 sums are multiplied by.
 Error outer(const void* p, const void* q, ElementType type, const int* offsets, int groups, int total,
-            int height, int width, bool kept, void* out, hipStream_t stream, const char* name) {
+            int height, int width, bool kept, void* out, hipStream_t stream, const char* name,
+            const float* group_scales = nullptr) {
     SPMM_TRY(check_product(total, groups, width, height, name));
     if ((offsets == nullptr && groups != 1) || out == nullptr ||
         (total > 0 && (p == nullptr || q == nullptr))) {
@@ -284,6 +292,7 @@ Error outer(const void* p, const void* q, ElementType type, const int* offsets, 
     a.total = total;
     a.height = height;
     a.width = width;
+    a.group_scales = group_scales;
     const bool pieces = height % 8 == 0 && width % 8 == 0 && aligned16(p) && aligned16(q);
     a.rows_end = static_cast<const char*>(p) + 2LL * total * height;
     a.cols_end = static_cast<const char*>(q) + 2LL * total * width;
@@ -311,7 +320,13 @@ Error outer(const void* p, const void* q, ElementType type, const int* offsets, 
         part.from = from;
         part.upto = upto;
         return with_half(type, name, [&](auto zero) {
-            return launch_tiles<decltype(zero), true, true, Ends::Plain>(part, form, lie, stream, name);
+            using T = decltype(zero);
+            if constexpr (std::is_same_v<T, _Float16>) {
+                if (group_scales != nullptr) {
+                    return launch_tiles<T, true, true, Ends::Scaled>(part, form, lie, stream, name);
+                }
+            }
+            return launch_tiles<T, true, true, Ends::Plain>(part, form, lie, stream, name);
         });
     };
     double least;
@@ -347,17 +362,33 @@ Error launch_grouped_outer(const void* p, const void* q, ElementType type, const
     return outer(p, q, type, offsets, groups, total, height, width, true, out, stream, "grouped_outer");
 }
 
-Error launch_gated_backward(const void* dkept, const void* x, const void* w, ElementType type,
-                            const int* offsets, int groups, int total, int width, int depth, void* dx,
-                            void* dw, hipStream_t stream) {
+Error launch_gated_backward(void* dkept, const float* row_scales, const void* x, const void* w,
+                            ElementType type, const int* offsets, int groups, int total, int width,
+                            int depth, void* dx, void* dw, float* workspace, hipStream_t stream) {
     const char* name = "gated_mm_backward";
     if (width > 0x3fffffff) return Error{kUnsupported, std::string(name) + ": rows over 2^22 elements"};
+    if (dx == nullptr && dw == nullptr) return Error{};
+    // all is looked at before anything is launched
+    SPMM_TRY(check_product(total, groups, depth, 2 * width, name));
+    if (dw != nullptr) SPMM_TRY(check_threads(groups, 256, name));
+    if ((offsets == nullptr && groups != 1) ||
+        (total > 0 && (dkept == nullptr || (dx != nullptr && w == nullptr) ||
+                       (dw != nullptr && (x == nullptr || (row_scales != nullptr && workspace == nullptr)))))) {
+        return Error{kInvalid, std::string(name) + ": null pointer"};
+    }
     if (dx != nullptr) {
         SPMM_TRY(product(dkept, w, type, offsets, groups, total, depth, 2 * width, true, false, dx,
-                         stream, name));
+                         stream, name, row_scales));
     }
     if (dw != nullptr) {
-        SPMM_TRY(outer(dkept, x, type, offsets, groups, total, 2 * width, depth, false, dw, stream, name));
+        const float* group_scales = nullptr;
+        if (row_scales != nullptr && total > 0) {
+            SPMM_TRY(launch_common_scales(dkept, row_scales, offsets, groups, total, 2LL * width, workspace,
+                                          stream));
+            group_scales = workspace;
+        }
+        SPMM_TRY(outer(dkept, x, type, offsets, groups, total, 2 * width, depth, false, dw, stream, name,
+                       group_scales));
     }
     return Error{};
 }

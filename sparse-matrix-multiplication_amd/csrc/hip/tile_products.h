@@ -100,8 +100,9 @@ template <typename T>
 using Sums = std::conditional_t<std::is_same_v<T, Int8Pair>, i32x4, f32x4>;
 
 // What becomes of a tile's sums: they leave as they are (8-bit integers': scaled), with
-// their rows' adapters added, or as act(g) * u, two columns' sums each.
-enum class Ends { Plain, Adapters, Gated };
+// their rows' adapters added, as act(g) * u, two columns' sums each, or multiplied by their
+// row's or their group's power of two (operands that were held in range by it).
+enum class Ends { Plain, Adapters, Gated, Scaled };
 
 struct TileArgs {
     const void* rows;     // X [total, depth], or P [total, height]
@@ -130,6 +131,8 @@ struct TileArgs {
     const float* row_scales;  // total
     const float* col_scales;  // [groups, width], gated [groups, 2, width]
     ElementType out_type;
+    // scaled: row_scales, or in a gradient
+    const float* group_scales; // groups
     // where the operands end, for rows that are no whole pieces
     const void* rows_end;
     const void* cols_end;
@@ -378,6 +381,7 @@ __device__ __forceinline__ bool take_tile(const TileArgs& a, Tile<T>& t) {
         const int row_tiles = (a.upto - a.from + BR - 1) / BR;
         if (!tile_of_block(a.groups * row_tiles, col_tiles, rt, ct)) return false;
         const int g = rt / row_tiles;
+        t.group = g;
         t.row0 = a.from + (rt % row_tiles) * BR;
         t.rows_here = min(BR, a.upto - t.row0);
         t.c0 = ct * BC;
@@ -667,7 +671,9 @@ struct StoreTile {
             *reinterpret_cast<f32x4*>(sums + (lane & 15) * kPitch + j * 16 + 4 * (lane >> 4)) = acc[j][I];
         }
     }
-    __device__ __forceinline__ void store(int i) const {
+    // SCALED: lane l < 16 holds what row l's sums are multiplied by.
+    template <bool SCALED = false>
+    __device__ __forceinline__ void store(int i, float scale = 1.0f) const {
         const int lane = threadIdx.x & 63;
         const int c = c0 + lane % kLanes * 8;
         const int count = min(8, a.width - c);
@@ -677,6 +683,11 @@ struct StoreTile {
             const float* from = sums + r * kPitch + lane % kLanes * 8;
             float f[8];
             __builtin_memcpy(f, __builtin_assume_aligned(from, 16), 32);
+            if constexpr (SCALED) {
+                const float by = __shfl(scale, r);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= by;
+            }
             const uint4 v = piece_from_float<T>(f);
             if (r0 + i * 16 + r < t.rows_here && count > 0) {
                 T* p = t.out + static_cast<long long>(r0 + i * 16 + r) * a.width + c;
@@ -686,14 +697,24 @@ struct StoreTile {
         }
     }
 };
-template <typename T, int RF, int CF>
+template <typename T, int RF, int CF, bool SCALED>
 __device__ __forceinline__ void store_tile(const TileArgs& a, const Tile<T>& t, int r0, int c0,
                                            const f32x4 (&acc)[CF][RF], float* sums) {
     const StoreTile<T, RF, CF> tile{a, t, r0, c0, sums};
+    float scale[RF];  // all rows' loads before the first store
+    if constexpr (SCALED) {
+#pragma unroll
+        for (int i = 0; i < RF; ++i) {
+            const int row = r0 + i * 16 + (threadIdx.x & 15);
+            scale[i] = a.group_scales != nullptr ? a.group_scales[t.group]
+                       : row < t.rows_here ? a.row_scales[t.row0 + row] : 0.0f;
+        }
+    }
     unrolled(std::make_integer_sequence<int, RF>{}, [&](auto at) {
         if (r0 + at.value * 16 < t.rows_here) {
             tile.template put<at.value>(acc);
-            tile.store(at.value);
+            if constexpr (SCALED) tile.template store<true>(at.value, scale[at.value]);
+            else tile.store(at.value);
         }
     });
 }
@@ -883,7 +904,7 @@ __device__ __forceinline__ u32x4 operand_words(const void* at, const void* end) 
     return buffer_words(reinterpret_cast<const void*>(from), 0, static_cast<int>(records));
 }
 
-// Whether a tile's sums leave as they are, through store_tile (or with adapters).
+// Whether a tile's sums leave through store_tile (or with adapters).
 template <typename T, Ends E>
 constexpr bool kPlainEnds = E != Ends::Gated && !std::is_same_v<T, Int8Pair>;
 
@@ -900,7 +921,7 @@ __device__ __forceinline__ void leave(const TileArgs& a, const Tile<T>& t, int r
     } else if constexpr (E == Ends::Adapters) {
         store_adapted<T, RF, CF>(a, t, r0, c0, acc, sums);
     } else {
-        store_tile<T, RF, CF>(a, t, r0, c0, acc, sums);
+        store_tile<T, RF, CF, E == Ends::Scaled>(a, t, r0, c0, acc, sums);
     }
 }
 
@@ -2173,7 +2194,7 @@ Error launch_tiles(const TileArgs& a, Form form, Lie lie, hipStream_t stream, co
                        : launch_ring<T, false, false, E, Lie::Pieces, 4>(a, blocks, stream, name);
         }
     } else {
-        if constexpr (E == Ends::Plain) {
+        if constexpr (E != Ends::Adapters) {
             if constexpr (!GRAD && COLS_MAJOR) {
                 if (form == Form::Ring64) {
                     return lie == Lie::Words

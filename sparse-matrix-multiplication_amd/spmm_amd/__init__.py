@@ -170,6 +170,8 @@ _SIGNATURES = {
     "spmm_c_gated_mm": (_int, [_vp, _vp, _int, _vp] + [_int] * 5 + [_vp] * 4),
     "spmm_c_gated_grad": (_int, [_vp, _int, _vp, _vp] + [_int] * 3 + [_vp] * 3),
     "spmm_c_gated_mm_backward": (_int, [_vp] * 3 + [_int, _vp] + [_int] * 4 + [_vp] * 3),
+    "spmm_c_gated_grad_scaled": (_int, [_vp] * 3 + [_int] * 3 + [_vp] * 4),
+    "spmm_c_gated_mm_backward_scaled": (_int, [_vp] * 5 + [_int] * 4 + [_vp] * 4),
     "spmm_c_pack8": (_int, [_vp, _int, ctypes.c_longlong, _int] + [_vp] * 3),
     "spmm_c_unpack8": (_int, [_vp, _vp, _int, ctypes.c_longlong, _int] + [_vp] * 2),
     "spmm_c_quantize_rows": (_int, [_vp, _int, ctypes.c_longlong, _int] + [_vp] * 3),

@@ -260,6 +260,9 @@ def gated_mm_backward(dh, x, w, kept, offsets=None, act: str = "silu", stream=No
     """The gradients of ``gated_mm`` for dh [S, N]: (dx [S, K], dw like w), and with hidden
     the product act(g) * u again [S, N], for the gradient of what it was multiplied by.
 
+    The gradients of g and u go into the products in dh's type, which rounds them once; in
+    float16 a row's are multiplied by a power of two on their way, so that products of dh, u and
+    act'(g) past float16's range at either end do not matter.
     kept is what ``gated_mm`` kept, in full or packed; x the operand, or packed by ``pack8``
     (only needed for weights).  A gradient that is not asked for (rows=False,
     weights=False) is not computed and None."""
@@ -289,16 +292,29 @@ def gated_mm_backward(dh, x, w, kept, offsets=None, act: str = "silu", stream=No
         L, s = lib(), _stream(device)
         h = torch.empty((S, N), dtype=dtype, device=device) if hidden else None
         dkept = torch.empty((S, 2, N), dtype=dtype, device=device)
-        _check(L.spmm_c_gated_grad(dh.data_ptr(), _TYPES[dtype], values.data_ptr(),
-                                   kept.scales.data_ptr() if packed else None, S, N, act_id,
-                                   dkept.data_ptr(), None if h is None else h.data_ptr(), s))
+        held = values.data_ptr(), kept.scales.data_ptr() if packed else None
+        again = None if h is None else h.data_ptr()
+        # float16's range: rows times a power of two each, and behind those the groups'
+        scales = None
+        if dtype == torch.float16:
+            scales = torch.empty(S + G, dtype=torch.float32, device=device)
+            _check(L.spmm_c_gated_grad_scaled(dh.data_ptr(), *held, S, N, act_id, dkept.data_ptr(),
+                                              scales.data_ptr(), again, s))
+        else:
+            _check(L.spmm_c_gated_grad(dh.data_ptr(), _TYPES[dtype], *held, S, N, act_id,
+                                       dkept.data_ptr(), again, s))
         dx = torch.empty((S, K), dtype=dtype, device=device) if rows else None
         dw = torch.empty_like(w) if weights else None
         if weights and isinstance(x, Packed8):
             x = unpack8(x, dtype)
         if rows or weights:
-            _check(L.spmm_c_gated_mm_backward(dkept.data_ptr(), x.data_ptr() if weights else None,
-                                              w.data_ptr(), _TYPES[dtype], at, G, S, N, K,
-                                              dx.data_ptr() if rows else None,
-                                              dw.data_ptr() if weights else None, s))
+            operands = x.data_ptr() if weights else None, w.data_ptr()
+            results = dx.data_ptr() if rows else None, dw.data_ptr() if weights else None
+            if scales is None:
+                _check(L.spmm_c_gated_mm_backward(dkept.data_ptr(), *operands, _TYPES[dtype], at, G, S, N,
+                                                  K, *results, s))
+            else:
+                _check(L.spmm_c_gated_mm_backward_scaled(dkept.data_ptr(), scales.data_ptr(), *operands, at,
+                                                         G, S, N, K, *results,
+                                                         scales.data_ptr() + 4 * S, s))
     return (dx, dw, h) if hidden else (dx, dw)
