@@ -206,12 +206,13 @@ class ExpertLayer(torch.nn.Module):
 
 
 class Int8Experts:
-    """A layer's experts in 8-bit integers with a scale a channel, made from it once; tokens
-    and what is between the layers get a scale a row.  The router stays in float32."""
+    """A layer's experts in 8-bit integers with a scale a channel, made from it once: changing
+    the layer later does not change them.  Tokens and what is between the layers get a scale a
+    row.  The router stays in float32."""
 
     @torch.no_grad()
     def __init__(self, layer: ExpertLayer):
-        self.router = layer.router.detach()
+        self.router = layer.router.detach().clone()
         self.w_in = quantize_rows(layer.w_in.detach())
         self.w_out = quantize_rows(layer.w_out.detach())
         self.k, self.over, self.gated = layer.k, layer.over, layer.gated
