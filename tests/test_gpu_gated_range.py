@@ -20,6 +20,7 @@ SIZES = [(None, 1, 1, 1), (None, 5, 9, 33), (None, 300, 264, 520), (None, 301, 2
          (None, 40, 2056, 64), (None, 17, 9001, 40), (None, 2, 8200, 24), (None, 300, 3000, 130),
          (None, 3000, 1024, 520), (None, 3000, 1024, 522), (None, 8200, 600, 2048), (None, 8200, 600, 2050),
          (None, 1000, 1501, 514), (None, 9000, 2300, 300), (None, 70, 1000, 1000), (None, 20000, 16, 16),
+         (None, 3000, 4500, 2048), (None, 3000, 4500, 2050),
          ([3, 0, 5], 11, 100, 72), ([7] * 70, 493, 33, 65), ([900, 0, 1, 700], 1604, 1000, 776),
          ([2500, 1400], 4000, 1001, 519), ([2500, 4400], 7000, 1020, 1032), ([600, 300], 905, 1001, 1030)]
 
