@@ -127,9 +127,11 @@ def unpack8(packed: Packed8, dtype=torch.bfloat16, out=None, stream=None):
 
 
 def quantize_rows(x, stream=None) -> Rows8:
-    """Rows of x [..., K] (float32, float16 or bfloat16) as 8-bit integers: scale = max|x| /
-    127, and the integers next to x * (127 / max|x|), ties to even (the quotients by
-    reciprocals in float32).  A row with an infinity or a NaN has the scale NaN."""
+    """Rows of x [..., K] (float32, float16 or bfloat16) as 8-bit integers: scale = max|x| *
+    (1 / 127), and the integers next to x * (1 / max|x| * 127), ties to even; these factors are
+    rounded to float32 at each step, so they are up to two roundings from the quotients.  A
+    largest value below 2^-100 is taken as that, so rows below 2^-108 are zeros.  A row with an
+    infinity or a NaN has the scale NaN."""
     rows, width = _flat(x, "x")
     device = x.device
     with _on(stream, device):
