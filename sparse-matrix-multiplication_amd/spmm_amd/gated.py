@@ -27,6 +27,7 @@ _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 _BYTES = (torch.int8,)
 _SCALES = (torch.uint8,)
 BLOCK = 32  # values that share a scale
+_WIDEST_GRADIENT = 1 << 21  # columns: both projections' gradients are a product's row of 2^22
 
 
 @dataclass
@@ -266,7 +267,7 @@ def gated_mm_backward(dh, x, w, kept, offsets=None, act: str = "silu", stream=No
     float16 a row's are multiplied by a power of two on their way, so that products of dh, u and
     act'(g) past float16's range at either end do not matter.
     kept is what ``gated_mm`` kept, in full or packed; x the operand, or packed by ``pack8``
-    (only needed for weights).  A gradient that is not asked for (rows=False,
+    (only needed for weights).  N goes up to 2^21, ``gated_mm``'s to 2^22.  A gradient that is not asked for (rows=False,
     weights=False) is not computed and None."""
     act_id = _act_id(act)
     _half(dh, "dh")
@@ -290,6 +291,9 @@ def gated_mm_backward(dh, x, w, kept, offsets=None, act: str = "silu", stream=No
         else:
             _operand(x, "x", (dtype,), (S, K), device)
     _counts(S, K, 2 * N)
+    if (rows or weights) and (N > _WIDEST_GRADIENT or K > 2 * _WIDEST_GRADIENT):
+        raise SpmmError(SPMM_UNSUPPORTED, f"gradients for weights {tuple(w.shape)}: N over 2^21, whose "
+                        "rows hold both projections', or K over 2^22")
     with _on(stream, device):
         L, s = lib(), _stream(device)
         h = torch.empty((S, N), dtype=dtype, device=device) if hidden else None

@@ -7,8 +7,13 @@ LIES = ("pieces", "words", "odd")
 
 
 def kernels(call):
-    """The kernels of a call in order, each with what its template says of the operands: a name
+    """The tile kernels of a call in order, each with what its template says of the operands: a name
     and, for tiles, how the operands' rows lie ("ring64 words", "wide pieces", "tile odd", "few")."""
+    return [n for n in map(_kind, launches(call)) if n]
+
+
+def launches(call):
+    """The names of all kernels of a call in order, the second time that it is made."""
     from torch.profiler import ProfilerActivity, profile
     call()
     torch.cuda.synchronize()
@@ -16,7 +21,7 @@ def kernels(call):
         call()
         torch.cuda.synchronize()
     events = [e for e in p.events() if e.device_type == torch.autograd.DeviceType.CUDA]
-    return [n for n in map(_kind, [e.name for e in sorted(events, key=lambda e: e.time_range.start)]) if n]
+    return [e.name for e in sorted(events, key=lambda e: e.time_range.start)]
 
 
 def _kind(name: str):
