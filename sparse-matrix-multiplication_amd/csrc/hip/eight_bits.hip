@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void unpack_blocks(const signed char* __restri
 // A workgroup takes a row: its first kHeld eights a thread stay in registers between the
 // maximum and the rounding, the rest is read again.  16 rows of 8192 2.7 us with sixteen
 // waves, 4.2 with four; 8192 rows 31 us again and again (the last cache holds them: 6.5 TB/s),
-// 37 between products that take it, 5.4 TB/s; 65536 rows of 256 18, bound by the chain of a
+// 41 between products that take it, 5.0 TB/s; 65536 rows of 256 18, bound by the chain of a
 // row's load, maximum and store (four rows a workgroup 17, and 16384 of 2048 17.4 for 16.8).
 //   Rows below 2^-100 take that as their largest value: 127 / max (finite down to 2^-121) and
 //   max / 127 stay far from fp32's ends, where a product's scales are multiplied one after the
