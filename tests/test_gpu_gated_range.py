@@ -218,3 +218,26 @@ def test_c_entries_refuse_bad_arguments(S):
         assert f(depth=1 << 23) == f(width=top) == f(width=1 << 22) == not_here
         assert f(groups=1 << 24, rows=1 << 24) == not_here
     assert back(dx=None, dw=None, workspace=None) == S.SPMM_OK
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_takes(S):
+    """Rows past 2^22, whose workgroups of a row each are another launch's."""
+    rows, N, K, tail = (1 << 22) + 1000, 8, 8, 2000
+    o = [0, rows - tail, rows]
+    offsets = torch.tensor(o, dtype=torch.int32, device="cuda")
+    dh = torch.zeros((rows, N), dtype=HALF, device="cuda")
+    kept = torch.zeros((rows, 2, N), dtype=HALF, device="cuda")
+    x = torch.zeros((rows, K), dtype=HALF, device="cuda")
+    d, x1, w, k1, *_ = _operands(None, tail, N, K, 300.0, 2.0 ** -13, 2.0 ** -15)
+    w = torch.cat([w, w])
+    dh[-tail:], kept[-tail:], x[-tail:] = d, k1, x1
+    dx, dw = S.gated_mm_backward(dh, x, w, kept, offsets)
+    only = torch.tensor([0, tail], dtype=torch.int32, device="cuda")
+    dx1, dw1, terms = _check(S, d, x1, w[1:].contiguous(), k1, [0, tail], only)
+    assert torch.equal(dx[-tail:], dx1) and (dx[:-tail] == 0).all()
+    assert (dw[0] == 0).all()
+    # the same rounded terms in another order: fp32 sums apart, then a rounding each
+    sums = tail * 2.0 ** -24 * (terms.abs().t() @ x1.double().abs()).view(2, N, K) * (1 + 2.0 ** -10)
+    assert ((dw[1].double() - dw1[0].double()).abs()
+            <= 2 * sums + 2 * R.ROUNDOFF[HALF] * (dw1[0].double().abs() + 2 * sums)).all()
