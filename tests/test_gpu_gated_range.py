@@ -241,3 +241,34 @@ def test_more_rows_than_one_launch_takes(S):
     sums = tail * 2.0 ** -24 * (terms.abs().t() @ x1.double().abs()).view(2, N, K) * (1 + 2.0 ** -10)
     assert ((dw[1].double() - dw1[0].double()).abs()
             <= 2 * sums + 2 * R.ROUNDOFF[HALF] * (dw1[0].double().abs() + 2 * sums)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("rows,N,K", [(300, 264, 520), (65, 97, 65), (9, 9001, 40)])
+def test_the_entries_without_scales(S, rows, N, K, packed):
+    """In fp16 too.  dg and du within their bounds (not the same bits as with scales: without, the
+    last product is rounded to fp16 at once, with them to fp32 first), and from the same dg and du
+    the same bits as with scales of 1."""
+    dh, kept = _normal((rows, N), 1).to(HALF), _normal((rows, 2, N), 2).to(HALF)
+    dh[:, 0], kept[:, :, 0] = 4.0, 4.0
+    x, w = _normal((rows, K), 3).to(HALF), (_normal((2, N, K), 4) * K ** -0.5).to(HALF)
+    p = S.pack8(kept)
+    held = (p.values.data_ptr(), p.scales.data_ptr()) if packed else (kept.data_ptr(), None)
+    dkept, h, dx, dw = (torch.empty_like(t) for t in (kept, dh, x, w))
+    L, stream = S.lib(), torch.cuda.current_stream().cuda_stream
+    assert L.spmm_c_gated_grad(dh.data_ptr(), 1, *held, rows, N, 0, dkept.data_ptr(), h.data_ptr(),
+                               stream) == S.SPMM_OK
+    assert L.spmm_c_gated_mm_backward(dkept.data_ptr(), x.data_ptr(), w.data_ptr(), 1, None, 1, rows, N, K,
+                                      dx.data_ptr(), dw.data_ptr(), stream) == S.SPMM_OK
+    g, u = (S.unpack8(p, HALF) if packed else kept).double().unbind(1)
+    dg, du, eg, eu = G.gradients(dh.double(), g, u, "silu")
+    G.close(dkept[:, 0], dg, eg)
+    G.close(dkept[:, 1], du, eu)
+    *_, again = S.gated_mm_backward(dh, x, w, p if packed else kept, hidden=True)
+    assert torch.equal(h, again)
+    one, dx1, dw1, before = torch.ones(rows + 1, device="cuda"), torch.empty_like(x), torch.empty_like(w), dkept.clone()
+    assert L.spmm_c_gated_mm_backward_scaled(
+        dkept.data_ptr(), one.data_ptr(), x.data_ptr(), w.data_ptr(), None, 1, rows, N, K, dx1.data_ptr(),
+        dw1.data_ptr(), one.data_ptr() + 4 * rows, stream) == S.SPMM_OK
+    assert torch.equal(dx1, dx) and torch.equal(dw1, dw) and torch.equal(dkept, before)
